@@ -193,7 +193,9 @@ def _places(case, pages, table, seq, pos):
     quad, two = torch.arange(2, device=dev)[:, None], torch.arange(2, device=dev)
     k_code = (sub // 2 * 8 * g + 8 * group + 4 * (sub % 2) + byte).reshape(-1)
     k_exp = (512 * g + 4 * group + 2 * quad + two).reshape(-1)
-    v_code = (sub * 8 * g + 8 * group + 4 * (byte // 2) + byte % 2).reshape(-1)
+    pair = (r // 2)[:, None, None, None]
+    v_code = (sub ^ 2 * (pair % 4)) * 8 * g + 8 * group + 4 * (byte // 2) + byte % 2  # chunks swizzled by the pair
+    v_code = v_code.reshape(len(r), 32 * g)
     v_exp = (512 * g + 8 * group + 4 * quad + two).reshape(-1)
     scale = 576 * g + torch.arange(g, device=dev)
     r = r[:, None]
