@@ -102,6 +102,9 @@ __global__ void selftest_wait_kernel(uint64_t limit_ns) {
 #include "glue.cu"
 #include "decode.cu"
 #include "gptq.cu"
+#include "kv_cache.cu"
+#include "paged_attention.cu"
+#include "verify.cu"
 
 extern "C" int faq_version(void) { return 100; }
 

@@ -17,6 +17,7 @@ FAQ_OK = 0
 FAQ_BF16 = 0
 FAQ_F32 = 1
 FAQ_STATUS_TIMEOUT = 1
+FAQ_STATUS_BAD_PAGE = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -71,6 +72,15 @@ SIGNATURES: dict[str, list] = {
                                          _int, _int, _c_void_p, _i64, _i64, _i64, _c_void_p],
     "faq_gptq_hif4_block": [_c_void_p, _i64, _i64, _int, _i64, _c_void_p, _i64, _i64, _int, _c_void_p, _i64,
                             _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p],
+    "faq_hif4_kv_write": [_c_void_p, _c_void_p, _int, _i64, _i64, _int, _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64,
+                          _int, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p],
+    "faq_hif4_kv_read": [_c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
+                         _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _i64, _c_void_p],
+    "faq_hif4_paged_attention": [_c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p,
+                                 _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _i64,
+                                 _i64, _c_void_p, ctypes.c_size_t, _c_void_p],
+    "faq_verify_drafts": [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p,
+                          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "faq_selftest_wait_timeout": [_i64, _c_void_p],
     "faq_selftest_ex2_monotone": [ctypes.POINTER(ctypes.c_uint64), _c_void_p],
     "faq_device_trace": [ctypes.POINTER(ctypes.c_uint), _int, _int],
@@ -102,6 +112,8 @@ def load() -> ctypes.CDLL:
             # size queries return size_t, not a status
             lib.faq_hif4_decode_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i64, _int]
             lib.faq_hif4_decode_workspace_bytes.restype = ctypes.c_size_t
+            lib.faq_hif4_paged_attention_workspace_bytes.argtypes = [_i64, _i64, _i64, _int]
+            lib.faq_hif4_paged_attention_workspace_bytes.restype = ctypes.c_size_t
             _lib = lib
         return _lib
 

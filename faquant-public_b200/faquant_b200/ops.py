@@ -676,3 +676,190 @@ def hif4_decode_attention(
               v.stride(2), scale, lv, int(quantized_normalizer), out.data_ptr(), out.stride(0), out.stride(1),
               out.stride(2), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(device))
     return out
+
+
+def hif4_page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Bytes of one page of the HiF4 K/V cache: K and V of ``page_size`` tokens, 4.625 bits
+    per value (the page format is in ``include/faquant_b200.h``)."""
+    if head_dim not in (64, 128) or page_size < 16 or page_size & (page_size - 1):
+        raise ValueError("head_dim must be 64 or 128 and page_size a power of two from 16")
+    return 2 * kv_heads * (page_size // 16) * 592 * (head_dim // 64)
+
+
+def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, kv_heads: int,
+            head_dim: int, page_size: int) -> None:
+    """Checks of a pool and the arrays that describe a ragged batch on it."""
+    if pages.dtype != torch.uint8 or pages.dim() < 2:
+        raise TypeError("pages must be a uint8 tensor [num_pages, ...]")
+    if pages[0].numel() != hif4_page_bytes(kv_heads, head_dim, page_size) or not pages[0].is_contiguous():
+        raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
+    if pages.dim() == 4 and pages.shape[1:3] != (2, kv_heads):
+        raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
+    for t in (table, cu, lens):
+        if t.dtype != torch.int32:
+            raise TypeError("table, cu and lens must be int32")
+    if table.dim() != 2 or table.shape[1] < 1 or table.stride(1) != 1:
+        raise ValueError("table must be [batch, columns] with unit column stride")
+    if cu.shape != (table.shape[0] + 1,) or lens.shape != (table.shape[0],):
+        raise ValueError("cu must be [batch + 1] and lens [batch]")
+    if not cu.is_contiguous() or not lens.is_contiguous():
+        raise ValueError("cu and lens must be contiguous")
+
+
+def hif4_kv_write(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    levels: tuple[str | int, str | int] = ("123", "123"),
+) -> None:
+    """Quantize the new tokens' ``k``/``v [T, Hkv, D]`` (bf16 or fp32, D 64 or 128, any token
+    and head strides) to HiF4 and write them into their ``pages`` (uint8 ``[num_pages,
+    ...]``, ``hif4_page_bytes`` each, ``faq_hif4_kv_write``).
+
+    ``cu [B + 1]`` bounds each sequence's new tokens, ``lens [B]`` are the lengths that
+    include them, ``table [B, columns]`` the sequences' pages (all int32, on the device):
+    new token i of n goes to position ``lens - n + i``. ``levels`` are K's and V's."""
+    device = _require_cuda(k, v, pages, table, cu, lens)
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one shape and dtype")
+    total, h, d = k.shape
+    _ragged(pages, table, cu, lens, h, d, page_size)
+    k = k if k.stride(2) == 1 else k.contiguous()
+    v = v if v.stride(2) == 1 else v.contiguous()
+    _lib.call("faq_hif4_kv_write", k.data_ptr(), v.data_ptr(), _dtype_code(k), total, h, d, k.stride(0), k.stride(1),
+              v.stride(0), v.stride(1), pages.data_ptr(), pages.shape[0], pages.stride(0), page_size,
+              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), table.shape[0],
+              levels_code(levels[0]), levels_code(levels[1]), _stream(device))
+
+
+def hif4_kv_read(
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    head_dim: int,
+    total: int,
+    dtype: torch.dtype = torch.bfloat16,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The last ``cu[b + 1] - cu[b]`` cached tokens of every sequence, dequantized:
+    ``(k, v)``, each ``[total, Hkv, D]`` bf16 or fp32 (``total = cu[-1]``, known on the host),
+    packed in sequence order; ``out`` takes tensors of that shape with unit channel stride."""
+    device = _require_cuda(pages, table, cu, lens, *(out or ()))
+    bytes_per_head = hif4_page_bytes(1, head_dim, page_size)
+    h = pages[0].numel() // bytes_per_head
+    _ragged(pages, table, cu, lens, h, head_dim, page_size)
+    if out is None:
+        out = (torch.empty((total, h, head_dim), dtype=dtype, device=device),
+               torch.empty((total, h, head_dim), dtype=dtype, device=device))
+    k, v = out
+    if k.shape != (total, h, head_dim) or v.shape != k.shape or k.dtype != v.dtype or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("out must be two [total, kv_heads, head_dim] tensors of one dtype with unit channel stride")
+    _lib.call("faq_hif4_kv_read", pages.data_ptr(), pages.shape[0], pages.stride(0), page_size, h, head_dim,
+              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), table.shape[0],
+              k.data_ptr(), v.data_ptr(), _dtype_code(k), total, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+              _stream(device))
+    return k, v
+
+
+def hif4_paged_attention(
+    q: torch.Tensor,
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    max_new: int,
+    max_len: int | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each sequence's new tokens over its HiF4 pages: ``q [T, H, D]`` bf16,
+    returns ``[T, H, D]`` bf16 (``faq_hif4_paged_attention``). ``table``, ``cu`` and ``lens``
+    as in :func:`hif4_kv_write`, which must have written the tokens before: new token i of
+    n sees the keys ``0 .. lens - n + i``, query head h those of kv head ``h // (H / Hkv)``.
+
+    ``max_new`` and ``max_len`` (the table's capacity by default) bound the sequences' new
+    tokens and lengths from above; they are host numbers, so nothing is copied from the
+    device. ``workspace``: a device buffer to use instead of a new one."""
+    device = _require_cuda(q, pages, table, cu, lens)
+    if q.dtype != torch.bfloat16 or q.dim() != 3:
+        raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
+    total, heads, d = q.shape
+    h = pages[0].numel() // hif4_page_bytes(1, d, page_size)
+    _ragged(pages, table, cu, lens, h, d, page_size)
+    if heads % h:
+        raise ValueError("query heads must be divisible by key/value heads")
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
+        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+    if max_len is None:
+        max_len = table.shape[1] * page_size
+    need = int(_lib.load().faq_hif4_paged_attention_workspace_bytes(heads, h, max_new, d))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, q.stride(0), q.stride(1), pages.data_ptr(),
+              pages.shape[0], pages.stride(0), page_size, h, d, table.data_ptr(), table.stride(0), table.shape[1],
+              cu.data_ptr(), lens.data_ptr(), table.shape[0], max_new, max_len,
+              float(scale if scale is not None else d**-0.5), out.data_ptr(), out.stride(0), out.stride(1),
+              workspace.data_ptr(), need, _stream(device))
+    return out
+
+
+def verify_drafts(
+    draft_tokens: torch.Tensor,
+    target_probs: torch.Tensor,
+    draft_probs: torch.Tensor | None,
+    accept_u: torch.Tensor,
+    sample_u: torch.Tensor,
+    *,
+    num_drafts: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Speculative sampling's check of drafted tokens (``faq_verify_drafts``).
+
+    ``draft_tokens [B, K]`` int64, ``target_probs [B, K + 1, V]`` and ``draft_probs [B, K, V]``
+    (bf16 or fp32; None for drafts without a distribution, such as tokens looked up in the
+    context), uniform random numbers ``accept_u [B, K]`` and ``sample_u [B]`` (fp32),
+    ``num_drafts [B]`` int32 for a ragged batch. Returns ``(tokens [B, K + 1] int64, accepted
+    [B] int32)``: the accepted drafts, one token sampled from the residual or the target,
+    then -1. The result does not depend on the order of summation."""
+    device = _require_cuda(draft_tokens, target_probs, draft_probs, accept_u, sample_u, num_drafts)
+    if target_probs.dim() != 3 or draft_tokens.dim() != 2:
+        raise ValueError("draft_tokens must be [B, K] and target_probs [B, K + 1, V]")
+    b, k1, vocab = target_probs.shape
+    k = k1 - 1
+    if draft_tokens.shape != (b, k) or accept_u.shape != (b, k) or sample_u.shape != (b,):
+        raise ValueError("draft_tokens and accept_u must be [B, K], sample_u [B], target_probs [B, K + 1, V]")
+    if draft_tokens.dtype != torch.int64 or accept_u.dtype != torch.float32 or sample_u.dtype != torch.float32:
+        raise TypeError("draft_tokens must be int64, accept_u and sample_u float32")
+    if target_probs.stride(2) != 1:
+        target_probs = target_probs.contiguous()
+    if draft_probs is not None:
+        if draft_probs.shape != (b, k, vocab) or draft_probs.dtype != target_probs.dtype:
+            raise ValueError("draft_probs must be [B, K, V] of target_probs' dtype")
+        if draft_probs.stride(2) != 1:
+            draft_probs = draft_probs.contiguous()
+    if num_drafts is not None and (num_drafts.shape != (b,) or num_drafts.dtype != torch.int32):
+        raise ValueError("num_drafts must be int32 [B]")
+    draft_tokens, accept_u, sample_u = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
+    num_drafts = None if num_drafts is None else num_drafts.contiguous()
+    tokens = torch.empty((b, k1), dtype=torch.int64, device=device)
+    accepted = torch.empty((b,), dtype=torch.int32, device=device)
+    ds = (0, 0) if draft_probs is None else (draft_probs.stride(0), draft_probs.stride(1))
+    _lib.call("faq_verify_drafts", draft_tokens.data_ptr(), target_probs.data_ptr(), _ptr(draft_probs),
+              _dtype_code(target_probs), b, k, vocab, target_probs.stride(0), target_probs.stride(1), *ds,
+              accept_u.data_ptr(), sample_u.data_ptr(), _ptr(num_drafts), tokens.data_ptr(), accepted.data_ptr(),
+              _stream(device))
+    return tokens, accepted

@@ -46,6 +46,7 @@ extern "C" {
 
 /* device status word bits */
 #define FAQ_STATUS_TIMEOUT 1u
+#define FAQ_STATUS_BAD_PAGE 2u /* a page table entry or a length outside the pool or the table */
 
 /* element types */
 #define FAQ_BF16 0
@@ -384,6 +385,92 @@ int faq_gptq_hif4_block(const float* w, int64_t ldw, int64_t rows, int cols, int
                         const float* hinv, int64_t ldh, int64_t hinv_stride, int levels, float* q,
                         int64_t ldq, float* err, int64_t lde, float* scale, float* rec, int8_t* lv2,
                         int8_t* lv3, int64_t groups_per_row, void* stream);
+
+/*
+ * K8 -- the HiF4 K/V cache in pages (no counterpart in the reference, whose append cache
+ * keeps dequantized bf16: simulated_flash_attention.py:243-289).
+ *
+ * A ragged batch, in every call: `cu` int32 [batch + 1] bounds each sequence's new tokens in
+ * the packed token axis (cu[b] .. cu[b + 1] - 1), `lens` int32 [batch] are the sequences'
+ * lengths with those tokens, so new token i of n stands at position lens[b] - n + i; a token
+ * whose position is negative has no place (it is not written, reads as zeros, attends to
+ * nothing). `table` int32 [batch, table_cols] (row stride table_ld) holds the page of tokens
+ * c * page_size .. of each sequence in column c; entries past a sequence's length are not
+ * read. An entry outside 0 .. num_pages - 1, or a length beyond the table's columns, sets
+ * FAQ_STATUS_BAD_PAGE in the device status word and leaves those tokens out.
+ *
+ * Page format (d = 64 NG channels, NG 1 or 2): `pages` uint8, page p at p * page_stride
+ * bytes (a multiple of 16; layers may interleave): [2: K, V][kv_heads][page_size / 16]
+ * blocks of 16 tokens, 592 NG bytes each (4.625 bits per value), little-endian:
+ *   codes     512 NG bytes: a nibble n = 8 + m or 8 - m (m the element's quarters, 0..7) per
+ *             channel. The eight channels of sub-block s (channels 8 s .. of a group) are a
+ *             quad a (first four) and a quad b.
+ *     K: token r, group g, sub-block s: the 32-bit word at 32 NG r + 8 NG (s / 2) + 8 g +
+ *        4 (s % 2), channel i at bits 4 i;
+ *     V: tokens 2 p, 2 p + 1 (pair p), chunk s ^ 2 (p % 4) of 8 NG bytes at 64 NG p: per
+ *        group a word of quad a and one of quad b, token 2 p in its low half, 2 p + 1 in
+ *        its high half, channel j of the quad at bits 4 j of the half;
+ *   exponents 64 NG bytes: 2 bits (lv2 + lv3) per quad, those of sub-block s at bits 2 s of a
+ *             16-bit half. K: per token and group a word of halves (a, b). V: per pair and
+ *             group a word of quad a's halves (2 p, 2 p + 1) and one of quad b's;
+ *   scales    16 NG bytes: the E6M2 code of [token][group].
+ * value = (n - 8) / 4 * 2^exponent * scale. page_size: a power of two, 16 to 4096.
+ *
+ * faq_hif4_kv_write quantizes k and v [total, kv_heads, d] (bf16 or fp32; token and head
+ * strides in elements, d contiguous) as faq_qk_prep's operand quantization does, the same
+ * values, and writes them at their tokens' places. faq_hif4_kv_read writes the last cu[b + 1] -
+ * cu[b] cached tokens of each sequence, dequantized, to k and v [total, kv_heads, d].
+ */
+int faq_hif4_kv_write(const void* k, const void* v, int dtype, int64_t total, int64_t kv_heads, int d,
+                      int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                      void* pages, int64_t num_pages, int64_t page_stride, int page_size, const int32_t* table,
+                      int64_t table_ld, int64_t table_cols, const int32_t* cu, const int32_t* lens, int64_t batch,
+                      int k_levels, int v_levels, void* stream);
+int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t page_stride, int page_size, int64_t kv_heads, int d,
+                     const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
+                     const int32_t* lens, int64_t batch, void* k, void* v, int dtype, int64_t total,
+                     int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                     void* stream);
+
+/*
+ * K9 -- attention of each sequence's new tokens over its pages: q and out bf16 [total,
+ * heads, d] (token and head strides multiples of 8 elements, 16-byte aligned), query head h
+ * on kv head h / (heads / kv_heads); new token i sees the keys 0 .. lens[b] - n + i (itself
+ * included, so write the tokens first). fp32 scores times `scale` and softmax, P rounded to
+ * bf16 for the products with V, fp32 accumulation; P is not quantized (faq_hif4_attention
+ * and faq_hif4_decode_attention keep the reference's HiF4 P). A row without a key is
+ * zero. Covers one decode step, chunks of drafted tokens and prompt chunks in one batch.
+ * max_new and max_len are upper bounds on the sequences' new tokens and lengths, known on
+ * the host (they choose the kernel and its workspace; nothing is copied from the device).
+ * `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * aligned, not initialized.
+ */
+size_t faq_hif4_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t max_new, int d);
+int faq_hif4_paged_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* pages, int64_t num_pages, int64_t page_stride, int page_size,
+                             int64_t kv_heads, int d, const int32_t* table, int64_t table_ld, int64_t table_cols,
+                             const int32_t* cu, const int32_t* lens, int64_t batch, int64_t max_new, int64_t max_len,
+                             float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * K10 -- verification of drafted tokens (no counterpart in the reference): draft_tokens int64
+ * [batch, k], target_probs [batch, k + 1, vocab] and draft_probs [batch, k, vocab] (bf16 or
+ * fp32, vocab contiguous; draft_probs null: drafts without a distribution, q = 1), uniform
+ * random numbers accept_u fp32 [batch, k] and sample_u fp32 [batch], num_drafts int32
+ * [batch] (null: k each). Draft i is accepted while accept_u * q(x) < p(x); with n accepted,
+ * tokens int64 [batch, k + 1] receives the n drafts, one sampled token and -1 after it, and
+ * accepted int32 [batch] n. The sampled token comes from max(p_n - q_n, 0) after a rejection
+ * (p_n without the draft when draft_probs is null; p_n itself when nothing is left), from p_n
+ * when all were accepted, as the first whose cumulative weight passes sample_u times their
+ * sum; the weights are rounded to 2^-40, so the result does not depend on the order of
+ * summation. A draft outside the vocabulary is rejected; a row without mass gives -1.
+ */
+int faq_verify_drafts(const int64_t* draft_tokens, const void* target_probs, const void* draft_probs, int dtype,
+                      int64_t batch, int64_t k, int64_t vocab, int64_t target_batch_stride,
+                      int64_t target_step_stride, int64_t draft_batch_stride, int64_t draft_step_stride,
+                      const float* accept_u, const float* sample_u, const int32_t* num_drafts, int64_t* tokens,
+                      int32_t* accepted, void* stream);
 
 /* Diagnostics: copy up to max_records records of the waits that gave up (3 words
  * each: site | tile << 8, blockIdx.x | blockIdx.y << 16, blockIdx.z) into `records`

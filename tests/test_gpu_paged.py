@@ -1,0 +1,360 @@
+"""The paged HiF4 K/V cache (faq_hif4_kv_write / _read) and the attention of new tokens over it
+(faq_hif4_paged_attention), against the oracle's quantizer and a 64-bit softmax.
+
+Tolerance of the attention, derived: bf16 has 8 significant bits, so its rounding errs by at
+most 2^-8 of the value. P is rounded to bf16 after its product with V's scale, the output to
+bf16 (|O| <= A, A = sum p |v|); scores are fp32 sums of 128 exact products, which moves p by
+less than 2^-13 relative for the |scores| used here. So every value is within
+(2^-8 + 2^-8 + 2^-12) A of the fp64 result, plus the smallest normal number."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from paged_reference import Pool, attention, quantized
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+BOUND = 2.0**-8 + 2.0**-8 + 2.0**-12
+
+
+def _randn(*shape, seed, dtype=torch.bfloat16, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(DEV)
+
+
+def _close(got, lens, new, q, k, v, scale=None):
+    ref, size = attention(q, k, v, lens, new, scale)
+    err = (got.double().cpu() - ref).abs()
+    assert bool((err <= BOUND * size + 2.0**-126).all()), float((err / size.clamp(min=1e-30)).max())
+
+
+def _no_status():
+    from faquant_b200 import _lib
+
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == 0
+
+
+# ------------------------------------------------------------------ write, read
+@pytest.mark.parametrize("levels", ["123", "12", "13"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_write_then_read_gives_the_oracles_values(d, dtype, levels) -> None:
+    lens = [1, 2, 15, 16, 17, 0, 63, 200]
+    pool = Pool(lens, 3, d, 32, DEV)
+    k = _randn(sum(lens), 3, d, seed=1, dtype=dtype, scale=3.0)
+    v = _randn(sum(lens), 3, d, seed=2, dtype=dtype, scale=0.01)
+    k[::7] *= 1e4
+    v[::5] = 0
+    pool.write(k, v, levels=(levels, "123"))
+    for out_dtype in (torch.bfloat16, torch.float32):
+        rk, rv = pool.read(dtype=out_dtype)
+        assert torch.equal(rk.float().cpu(), quantized(k, levels)) and torch.equal(rv.float().cpu(), quantized(v))
+    _no_status()
+
+
+def test_the_cache_holds_the_operand_preparations_values() -> None:
+    from faquant_b200 import ops
+
+    pool = Pool([70], 2, 128, 16, DEV)
+    k, v = _randn(70, 2, 128, seed=3), _randn(70, 2, 128, seed=4)
+    pool.write(k, v)
+    rk, rv = pool.read()
+    for x, r in ((k, rk), (v, rv)):
+        prep = ops.qk_prep(x.transpose(0, 1)[None], levels="123", rotate=False)[0]
+        assert torch.equal(prep[0].transpose(0, 1), r)
+
+
+@pytest.mark.parametrize("page_size", [16, 64, 256])
+def test_tokens_written_one_by_one_or_in_chunks_give_the_same_pages(page_size) -> None:
+    lens, h, d = [37, 5], 2, 128
+    k, v = _randn(42, h, d, seed=5), _randn(42, h, d, seed=6)
+    whole, steps = (Pool(lens, h, d, page_size, DEV, seed=9) for _ in range(2))
+    whole.write(k, v)
+    for begin, end in [(0, 1), (1, 2), (2, 19), (19, 20), (20, 37)]:  # the other sequence idle, then in the last step
+        new = [end - begin, 5 if end == 37 else 0]
+        parts = [torch.cat((x[begin:end], x[37:] if end == 37 else x[:0])) for x in (k, v)]
+        steps.write(*parts, new=new, lens=[end, 5 if end == 37 else 0])
+    assert torch.equal(whole.store, steps.store)
+
+
+def test_write_touches_only_its_tokens_bytes() -> None:
+    from faquant_b200 import ops
+
+    pool = Pool([40], 2, 64, 16, DEV, gap=16)
+    before = pool.store.clone()
+    k = _randn(3, 2, 64, seed=7)
+    pool.write(k, k, new=[3])
+    changed = (pool.store != before).sum().item()
+    assert 0 < changed <= 3 * 2 * 2 * 37  # three tokens, K and V, two heads, 37 bytes each
+    assert torch.equal(pool.store[:, -16:], before[:, -16:])
+    rk, _ = pool.read(new=[3])
+    assert torch.equal(rk.float().cpu(), quantized(k))
+    assert ops.hif4_page_bytes(2, 64, 16) == 2 * 2 * 592
+
+
+def test_strides_alignment_and_outputs() -> None:
+    lens, h, d = [21, 40], 2, 128
+    total = sum(lens)
+    pool = Pool(lens, h, d, 16, DEV)
+    wide = _randn(total, 3 * h * d + 8, seed=8)  # a fused projection: heads strided, a slice not 16-byte aligned
+    k = wide[:, 1 : 1 + h * d].unflatten(1, (h, d))
+    v = _randn(h, total, d, seed=9).transpose(0, 1)  # heads outermost
+    assert k.data_ptr() % 16
+    pool.write(k, v)
+    want_k, want_v = quantized(k), quantized(v)
+    rk, rv = pool.read()
+    assert torch.equal(rk.float().cpu(), want_k) and torch.equal(rv.float().cpu(), want_v)
+    out_k = torch.empty(total, h, d + 1, device=DEV)[..., 1:]  # unaligned rows
+    out_v = torch.empty(h, total, d, device=DEV).transpose(0, 1)
+    pool.read(out=(out_k, out_v))
+    assert torch.equal(out_k.cpu(), want_k) and torch.equal(out_v.cpu(), want_v)
+
+
+def test_offsets_past_32_bits() -> None:
+    """Pages beyond 2^31 and 2^32 bytes of a pool, written, read and attended to."""
+    from faquant_b200 import ops
+
+    size = ops.hif4_page_bytes(8, 128, 4096)
+    count = (1 << 32) // size + 4
+    pages = torch.empty(count, size, dtype=torch.uint8, device=DEV)
+    table = torch.tensor([[(1 << 31) // size + 1], [count - 1]], dtype=torch.int32, device=DEV)
+    lens, new = [50, 33], [50, 33]
+    cu = torch.tensor([0, 50, 83], dtype=torch.int32, device=DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    k, v = _randn(83, 8, 128, seed=10), _randn(83, 8, 128, seed=11)
+    q = _randn(83, 8, 128, seed=12)
+    ops.hif4_kv_write(k, v, pages, table, cu, lens_d, page_size=4096)
+    rk, rv = ops.hif4_kv_read(pages, table, cu, lens_d, page_size=4096, head_dim=128, total=83)
+    assert torch.equal(rk.float().cpu(), quantized(k)) and torch.equal(rv.float().cpu(), quantized(v))
+    out = ops.hif4_paged_attention(q, pages, table, cu, lens_d, page_size=4096, max_new=50)
+    _close(out, lens, new, q, rk, rv)
+    _no_status()
+
+
+def test_tokens_without_a_place() -> None:
+    """Positions below zero are skipped; bad table entries and lengths are reported."""
+    from faquant_b200 import _lib, ops
+
+    pool = Pool([20], 1, 64, 16, DEV)
+    k = _randn(20, 1, 64, seed=13)
+    pool.write(k, k, new=[20])
+    keep = pool.store.clone()
+    ops.hif4_kv_write(k, k, pool.pages, pool.table, pool.cu([20]), torch.tensor([4], dtype=torch.int32, device=DEV),
+                      page_size=16)  # only the last four tokens have a place
+    pool.lens.fill_(4)
+    assert torch.equal(pool.read(new=[4])[0].float().cpu(), quantized(k[16:]))
+    rk, _ = pool.read(new=[6])
+    assert not rk[:2].any() and torch.equal(rk[2:].float().cpu(), quantized(k[16:]))
+    _no_status()
+    pool.store.copy_(keep)
+    pool.lens.fill_(20)
+    pool.table[0, 1] = 10**6
+    rk, _ = pool.read(new=[20])
+    assert torch.equal(rk[:16].float().cpu(), quantized(k[:16])) and not rk[16:].any()
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_PAGE
+    pool.write(k, k, new=[20])
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_PAGE
+    # the attention leaves that page's keys out
+    q = _randn(1, 2, 64, seed=14)
+    out = pool.attend(q, [1])
+    ref, size = attention(q, quantized(k[:16]), quantized(k[:16]), [16], [1])
+    assert bool(((out.double().cpu() - ref).abs() <= BOUND * size).all())
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_PAGE
+
+
+# ------------------------------------------------------------------ attention
+SHAPES = [  # heads, kv_heads, d, page_size, lens, new
+    (4, 1, 128, 16, [1], [1]),
+    (8, 2, 128, 16, [1, 2, 15, 16, 17, 127, 129, 500], [1] * 8),
+    (32, 8, 128, 64, [3000], [1]),
+    (5, 1, 128, 32, [100, 31], [1, 3]),
+    (7, 1, 64, 16, [90, 300], [2, 1]),
+    (2, 2, 64, 128, [40, 700, 0, 3], [1, 8, 0, 3]),
+    (16, 4, 128, 32, [5, 70, 64, 200], [5, 0, 8, 1]),
+    (16, 2, 64, 16, [33, 260], [33, 17]),
+    (12, 4, 128, 16, [130], [130]),
+    (24, 2, 128, 256, [700, 20], [40, 20]),
+    (3, 3, 128, 16, [0, 0, 9], [0, 0, 1]),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"h{s[0]}_{s[1]}_d{s[2]}_p{s[3]}_b{len(s[4])}_n{max(s[5])}")
+def test_attention_matches_fp64(shape) -> None:
+    heads, h, d, page, lens, new = shape
+    pool = Pool(lens, h, d, page, DEV, fill=0xFF)  # unwritten slots hold the largest scales and codes
+    k, v = _randn(sum(lens), h, d, seed=20), _randn(sum(lens), h, d, seed=21, scale=0.5)
+    pool.write(k, v)
+    q = _randn(sum(new), heads, d, seed=22, scale=2.0)
+    out = pool.attend(q, new)
+    assert out.shape == q.shape and out.dtype == torch.bfloat16
+    _close(out, lens, new, q, quantized(k), quantized(v))
+    _no_status()
+
+
+@pytest.mark.parametrize("n", [1, 2, 4, 9, 40])
+def test_rows_without_a_key_are_zero(n) -> None:
+    """More new tokens than the sequence holds: the first have no position."""
+    lens, new = [max(1, n // 2), 0, 300], [n, n, n]
+    pool = Pool(lens, 2, 128, 16, DEV)
+    k, v = _randn(sum(lens), 2, 128, seed=23), _randn(sum(lens), 2, 128, seed=24)
+    pool.write(k, v)
+    q = _randn(3 * n, 8, 128, seed=25)
+    out = torch.full_like(q, float("nan"))
+    pool.attend(q, new, out=out)
+    none = n - lens[0]
+    assert not out[:none].any() and not out[n : 2 * n].any()
+    _close(out, lens, new, q, quantized(k), quantized(v))
+
+
+def test_a_step_of_queries_equals_each_alone() -> None:
+    """Chunk invariance: the drafts' rows, attended together, are the rows of one-token calls
+    within the bound of both."""
+    pool = Pool([1500], 2, 128, 64, DEV)
+    k, v = _randn(1500, 2, 128, seed=26), _randn(1500, 2, 128, seed=27)
+    pool.write(k, v)
+    q = _randn(8, 16, 128, seed=28, scale=2.0)
+    out = pool.attend(q, [8])
+    _, size = attention(q, quantized(k), quantized(v), [1500], [8])
+    for i in range(8):
+        pool.lens.fill_(1500 - 7 + i)
+        one = pool.attend(q[i : i + 1], [1])
+        assert bool(((one[0] - out[i]).double().abs().cpu() <= 2 * BOUND * size[i]).all())
+
+
+def test_peaked_and_flat_scores_scale_and_ranges() -> None:
+    lens, new = [900], [4]
+    pool = Pool(lens, 1, 128, 16, DEV)
+    k, v = _randn(900, 1, 128, seed=29), _randn(900, 1, 128, seed=30)
+    k[700] *= 30.0  # one key far above the others, found late
+    v[3] *= 1e6     # and a value row of another magnitude
+    v[600:] *= 1e-20
+    pool.write(k, v)
+    q = _randn(4, 4, 128, seed=31)
+    q[1] = 0
+    for scale in (None, 0.002, 0.5):
+        _close(pool.attend(q, new, scale=scale), lens, new, q, quantized(k), quantized(v), scale)
+
+
+def test_not_a_number_stays_in_its_row() -> None:
+    pool = Pool([300], 2, 128, 16, DEV)
+    k, v = _randn(300, 2, 128, seed=32), _randn(300, 2, 128, seed=33)
+    pool.write(k, v)
+    q = _randn(6, 8, 128, seed=34)
+    good = pool.attend(q, [6])
+    q[2, 5, 17] = float("nan")
+    q[4, 0, 0] = float("inf")
+    out = pool.attend(q, [6])
+    assert out[2, 5].isnan().all() and out[4, 0].isnan().any()
+    out[2, 5], out[4, 0] = good[2, 5], good[4, 0]
+    assert torch.equal(out, good)
+
+
+def test_shared_pages_strides_streams_and_repetition() -> None:
+    """Two sequences share a prefix's pages; q and out strided; another stream; the same bits
+    on every call, with one workspace and back to back."""
+    from faquant_b200 import ops
+
+    pool = Pool([64, 0], 2, 128, 16, DEV, spare=4)
+    k, v = _randn(64, 2, 128, seed=35), _randn(64, 2, 128, seed=36)
+    pool.write(k, v)
+    pool.table[1] = pool.table[0]
+    pool.lens_host = [64, 64]
+    pool.lens.fill_(64)
+    wide = _randn(4, 3, 8, 136, seed=37)
+    q = wide[:, 1, :, :128]
+    out = torch.empty(8, 4, 128, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        pool.attend(q, [2, 2], out=out)
+    stream.synchronize()
+    kk, vv = torch.cat((quantized(k),) * 2), torch.cat((quantized(v),) * 2)
+    _close(out, [64, 64], [2, 2], q, kk, vv)
+    big = Pool([4000, 77, 2500], 2, 128, 32, DEV)
+    k, v = _randn(6577, 2, 128, seed=38), _randn(6577, 2, 128, seed=39)
+    big.write(k, v)
+    new = [1, 1, 1]
+    q = _randn(3, 16, 128, seed=40)
+    first = big.attend(q, new)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=DEV)
+    again = [big.attend(q, new, workspace=ws) for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, x) for x in again)
+    assert ops.hif4_page_bytes(2, 128, 32) == 2 * 2 * 2 * 1184
+
+
+def test_captured_in_a_graph_with_growing_lengths() -> None:
+    """A captured step replays with the device's lengths of the moment."""
+    pool = Pool([400], 2, 128, 64, DEV)
+    k, v = _randn(400, 2, 128, seed=41), _randn(400, 2, 128, seed=42)
+    pool.write(k, v)
+    q = _randn(1, 8, 128, seed=43)
+    out, ws = torch.empty_like(q), torch.empty(8 << 20, dtype=torch.uint8, device=DEV)
+    cu = pool.cu([1])
+    from faquant_b200 import ops
+
+    def step():
+        ops.hif4_paged_attention(q, pool.pages, pool.table, cu, pool.lens, page_size=64, max_new=1, max_len=400, out=out,
+                                 workspace=ws)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in (1, 63, 64, 65, 399, 400):
+        pool.lens.fill_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        _close(out, [n], [1], q, quantized(k[:n]), quantized(v[:n]))
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals() -> None:
+    from faquant_b200 import ops
+
+    pool = Pool([20, 20], 2, 128, 16, DEV)
+    cu, kw = pool.cu([1, 1]), dict(page_size=16)
+    k = _randn(2, 2, 128, seed=50)
+    q = _randn(2, 4, 128, seed=51)
+    args = (pool.pages, pool.table, cu, pool.lens)
+    with pytest.raises(ValueError):  # another page size than the pages'
+        ops.hif4_kv_write(k, k, *args, page_size=32)
+    with pytest.raises(ValueError):  # not a power of two
+        ops.hif4_kv_write(k, k, *args, page_size=24)
+    with pytest.raises(ValueError):  # K and V differ
+        ops.hif4_kv_write(k, k[:1], *args, **kw)
+    with pytest.raises(TypeError):
+        ops.hif4_kv_write(k.half(), k.half(), *args, **kw)
+    with pytest.raises(ValueError):
+        ops.hif4_kv_write(k, k, *args, levels=("123", "23"), **kw)
+    with pytest.raises(TypeError):  # 64-bit lengths
+        ops.hif4_kv_write(k, k, pool.pages, pool.table, cu, pool.lens.long(), **kw)
+    with pytest.raises(ValueError):  # cu of another batch
+        ops.hif4_paged_attention(q, pool.pages, pool.table, cu[:2], pool.lens, max_new=1, **kw)
+    with pytest.raises(ValueError):  # heads not a multiple
+        ops.hif4_paged_attention(q[:, :3], *args, max_new=1, **kw)
+    with pytest.raises(TypeError):
+        ops.hif4_paged_attention(q.float(), *args, max_new=1, **kw)
+    with pytest.raises(ValueError):
+        ops.hif4_paged_attention(q, *args, max_new=1, scale=-1.0, **kw)
+    with pytest.raises(ValueError):  # head_dim the pages do not have
+        ops.hif4_paged_attention(_randn(2, 4, 64, seed=52), *args, max_new=1, **kw, out=q)
+    with pytest.raises(RuntimeError):  # host tensors
+        ops.hif4_kv_read(pool.pages.cpu(), pool.table, cu, pool.lens, head_dim=128, total=2, **kw)
+    with pytest.raises(ValueError):
+        ops.hif4_kv_read(*args, head_dim=96, total=2, **kw)
+    with pytest.raises(ValueError):
+        ops.hif4_kv_read(*args, head_dim=128, total=2, out=(k, k[:1]), **kw)
+
+
+def test_no_tokens_is_no_work() -> None:
+    pool = Pool([20], 2, 128, 16, DEV)
+    empty = torch.empty(0, 2, 128, dtype=torch.bfloat16, device=DEV)
+    before = pool.store.clone()
+    pool.write(empty, empty, new=[0])
+    assert torch.equal(before, pool.store)
+    assert pool.read(new=[0])[0].shape == (0, 2, 128)
+    assert pool.attend(torch.empty(0, 4, 128, dtype=torch.bfloat16, device=DEV), [0]).shape == (0, 4, 128)

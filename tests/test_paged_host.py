@@ -1,0 +1,72 @@
+"""Host-side checks of the paged-cache and verification entry points (no GPU): refusals before
+any CUDA call, and the size functions."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+
+def test_page_bytes() -> None:
+    from faquant_b200 import ops
+
+    assert ops.hif4_page_bytes(8, 128, 64) == 2 * 8 * 64 * 74  # 74 bytes per token, head and K or V
+    assert ops.hif4_page_bytes(1, 64, 16) == 2 * 592
+    for bad in ((1, 96, 16), (1, 128, 8), (1, 128, 48)):
+        with pytest.raises(ValueError):
+            ops.hif4_page_bytes(*bad)
+
+
+def test_c_entry_points_refuse_bad_arguments() -> None:
+    from faquant_b200 import _lib
+
+    lib = _lib.load()
+    p = ctypes.c_void_p(16)
+
+    def write(d=128, page=16, stride=1 << 20, pages=p, levels=123, dtype=0):
+        return lib.faq_hif4_kv_write(p, p, dtype, 4, 2, d, 256, 128, 256, 128, pages, 4, stride, page, p, 3, 3, p, p, 1,
+                                     levels, 123, None)
+
+    assert write(pages=None) == 1 and "null" in _lib.last_error()
+    assert write(d=96) == 3 and "head_dim" in _lib.last_error()
+    assert write(page=24) == 3 and "page_size" in _lib.last_error()
+    assert write(stride=1000) == 1 and "aligned" in _lib.last_error()
+    assert write(stride=1024) == 1 and "page stride" in _lib.last_error()
+    assert write(pages=ctypes.c_void_p(8)) == 1
+    assert write(levels=1) == 1 and "levels" in _lib.last_error()
+    assert write(dtype=7) == 1 and "dtype" in _lib.last_error()
+
+    def attend(heads=4, scale=1.0, ws=1 << 30, qs=512, max_new=1):
+        return lib.faq_hif4_paged_attention(p, 4, heads, qs, 128, p, 4, 1 << 20, 16, 2, 128, p, 3, 3, p, p, 1, max_new, 48,
+                                            ctypes.c_float(scale), p, 512, 128, p, ws, None)
+
+    assert attend(heads=3) == 1 and "divisible" in _lib.last_error()
+    assert attend(scale=0.0) == 1 and "scale" in _lib.last_error()
+    assert attend(scale=float("nan")) == 1
+    assert attend(qs=12) == 1 and "strides" in _lib.last_error()
+    assert attend(ws=16) == 1 and "workspace" in _lib.last_error()
+    assert attend(max_new=-1) == 1
+    assert lib.faq_hif4_paged_attention_workspace_bytes(6, 4, 1, 128) == 0
+
+    def verify(batch=1, k=2, vocab=10, dtype=1, target=p):
+        return lib.faq_verify_drafts(p, target, None, dtype, batch, k, vocab, 30, 10, 0, 0, p, p, None, p, p, None)
+
+    assert verify(target=None) == 1 and verify(vocab=0) == 1 and verify(vocab=1 << 23) == 1
+    assert verify(k=-1) == 1 and verify(dtype=3) == 1
+    assert verify(batch=0) == 0
+
+
+def test_operators_refuse_cpu_tensors() -> None:
+    from faquant_b200 import ops
+
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    pages = torch.zeros(1, 1184, dtype=torch.uint8)
+    table, cu, lens = (torch.zeros(*s, dtype=torch.int32) for s in ((1, 1), (2,), (1,)))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.hif4_kv_write(x, x, pages, table, cu, lens, page_size=16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.hif4_paged_attention(x, pages, table, cu, lens, page_size=16, max_new=1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.verify_drafts(torch.zeros(1, 1, dtype=torch.int64), torch.ones(1, 2, 4), None, torch.ones(1, 1), torch.ones(1))
