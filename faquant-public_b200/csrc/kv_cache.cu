@@ -6,6 +6,8 @@
 // places of the page format (include/faquant_b200.h). Every byte of the cache belongs to one
 // token, so tokens are written without reading what is there.
 // Read: the inverse, value = (n - 8) / 4 * 2^e * scale, exact in bf16.
+#include <atomic>
+
 #include "kv_pages.cuh"
 
 namespace faq {
@@ -197,14 +199,15 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams w, bool vec) {
     const uint32_t ve = vx[0] | (static_cast<uint32_t>(vx[2]) << 16);
     const float ks = twice_scale(ksrc[scale_offset(NG) + r * NG + g]);
     const float vs = twice_scale(vsrc[scale_offset(NG) + r * NG + g]);
+    const Expand expand;
     uint32_t y[4];
-    expand_word(kw, exponent_pair(ke, (7 - 2 * s) & 31), y);
+    expand.word(kw, expand.exponents(ke, (7 - 2 * s) & 31), y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       vk[j] = __fmul_rn(__uint_as_float(y[j] << 16), ks);
       vk[4 + j] = __fmul_rn(__uint_as_float(y[j] & 0xFFFF0000u), ks);
     }
-    expand_word(vw, exponent_pair(ve, (7 - 2 * s) & 31), y);
+    expand.word(vw, expand.exponents(ve, (7 - 2 * s) & 31), y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       vv[j] = __fmul_rn(__uint_as_float(y[j] << 16), vs);
@@ -240,6 +243,18 @@ static int make_pages(Pages& p, const void* pages, int64_t num_pages, int64_t pa
   p.cu = cu;
   p.lens = lens;
   p.batch = static_cast<int>(batch);
+  return FAQ_OK;
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device, once per device
+// (`set` holds a bit per device).
+static int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& set) {
+  int dev = 0;
+  FAQ_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (set.load(std::memory_order_acquire) & bit)) return FAQ_OK;
+  FAQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) set.fetch_or(bit, std::memory_order_release);
   return FAQ_OK;
 }
 

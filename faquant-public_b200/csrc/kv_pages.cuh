@@ -76,22 +76,38 @@ __device__ __forceinline__ uint32_t hmul2_bf16(uint32_t a, uint32_t b) {
   return d;
 }
 
-// (2^(e - 3), 2^(e' - 3)) as bf16, from the exponent word's two halves: e is bits
-// 2 s, 2 s + 1 of the half of sub-block s, rotated into the low bits of the exponent
-// field (rot = 7 - 2 s modulo 32; the bits it wraps are masked off). 0x3E00 is 2^-3, whose
-// field ends in 00.
-__device__ __forceinline__ uint32_t exponent_pair(uint32_t ew, int rot) {
-  return (__funnelshift_l(ew, ew, rot) & 0x01800180u) | 0x3E003E00u;
-}
-
-// The eight nibbles of a code word as four bf16 pairs (n - 8) 2^(e - 3): pair j holds
-// nibble j of the word's low and high halves. 0x4300 | n is 128 + n exactly, and one
-// FMA with (E, -136 E) gives (n - 8) E exactly (at most 4 significant bits).
-__device__ __forceinline__ void expand_word(uint32_t w, uint32_t e, uint32_t (&out)[4]) {
-  const uint32_t n = hmul2_bf16(e, 0xC308C308u);  // -136
+// The constants of the expansion, in registers whose values the compiler does not know: it
+// would else split (x & mask) | bits with two constants into two instructions, or make the
+// constants anew at each use (the integer pipe, which bounds the expansion, then does 40 %
+// more).
+struct Expand {
+  uint32_t magic, base, shift;
+  __device__ __forceinline__ Expand() {
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));  // bf16 128, twice
+    asm volatile("mov.b32 %0, 0x3E003E00;" : "=r"(base));   // 2^-3
+    asm volatile("mov.b32 %0, 0xC308C308;" : "=r"(shift));  // -136
+  }
+  // (2^(e - 3), 2^(e' - 3)) as bf16, from the exponent word's two halves: e is bits 2 s,
+  // 2 s + 1 of the half of sub-block s, rotated into the low bits of the exponent field
+  // (rot = 7 - 2 s modulo 32; the bits it wraps are masked off; 2^-3's field ends in 00).
+  __device__ __forceinline__ uint32_t exponents(uint32_t ew, int rot) const {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, 0x01800180, %2, 0xEA;" : "=r"(d) : "r"(__funnelshift_l(ew, ew, rot)), "r"(base));
+    return d;
+  }
+  // The eight nibbles of a code word as four bf16 pairs (n - 8) 2^(e - 3): pair j holds
+  // nibble j of the word's low and high halves. 0x4300 | n is 128 + n exactly, and one
+  // FMA with (E, -136 E) gives (n - 8) E exactly (at most 4 significant bits).
+  __device__ __forceinline__ void word(uint32_t w, uint32_t e, uint32_t (&out)[4]) const {
+    const uint32_t n = hmul2_bf16(e, shift);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] = hfma2_bf16(((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u, e, n);
-}
+    for (int j = 0; j < 4; ++j) {
+      uint32_t x;
+      asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * j)), "r"(magic));
+      out[j] = hfma2_bf16(x, e, n);
+    }
+  }
+};
 
 }  // namespace kvp
 }  // namespace faq

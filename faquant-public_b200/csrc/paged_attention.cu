@@ -25,11 +25,12 @@
 //
 // Work split: the key blocks of all units, in the order (sequence, kv head, rows), are cut
 // into equal runs, one per CTA (a function of the device's cu / lens only, so the host
-// needs no lengths). Within a run the eight warps take blocks in turn, each with its own ring
+// needs no lengths). Within a run the CTA's warps take blocks in turn, each with its own ring
 // of bulk copies and its own O; they meet in shared memory at the unit's end. A unit that lies
 // in one run is written out at once; else each run writes a partial (O, m, l) -- at most two per
 // CTA -- and paged_combine_kernel joins them in run order (the same bits on every call).
 #include <algorithm>
+#include <atomic>
 
 #include "kv_pages.cuh"
 
@@ -38,9 +39,8 @@ namespace pat {
 
 using namespace kvp;
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
 constexpr float RAISE = 8.0f;  // log2 headroom of a row's reference maximum
+constexpr float LOWEST = -3.402823466e38f;  // where it starts: below every finite score
 
 struct Params {
   Pages p;
@@ -50,14 +50,19 @@ struct Params {
   int64_t ot, oh;
   int64_t total;   // rows of q and out
   int group;       // query heads per kv head
+  uint32_t group_magic;  // ceil(2^32 / group), see small_div
   float scale_log2;
   float* parts;    // [2 gridDim][rows x d + 2 rows]: O, m, l
   int32_t* joins;  // [gridDim][8]: the unit that began in an earlier run and ends in this one
 };
 
-// rows r0 .. of a unit; number of key blocks they see
+// x / group for x < 2^32 / group (x is below group + 32 here); a group of 1 has no magic number
+__device__ __forceinline__ int small_div(const Params& P, int x) {
+  return P.group == 1 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), P.group_magic));
+}
+
 struct Seq {
-  int n, len, rows, nrb;
+  int n, len, nrb;  // new tokens, length, row blocks of RB rows
 };
 template <int RB>
 __device__ __forceinline__ Seq sequence(const Params& P, int b) {
@@ -65,22 +70,25 @@ __device__ __forceinline__ Seq sequence(const Params& P, int b) {
   const int c0 = P.p.cu[b], c1 = P.p.cu[b + 1];
   s.n = (c0 >= 0 && c1 > c0 && c1 <= P.total) ? c1 - c0 : 0;
   s.len = length_of(P.p, b);
-  s.rows = s.n * P.group;
-  s.nrb = (s.rows + RB - 1) / RB;
+  s.nrb = (s.n * P.group + RB - 1) / RB;
   return s;
 }
 template <int RB>
 __device__ __forceinline__ int key_blocks(const Params& P, const Seq& s, int rb) {
-  const int last = min(s.n - 1, ((rb + 1) * RB - 1) / P.group);  // the row block's last token
+  // the row block's last token
+  const int last = rb + 1 >= s.nrb ? s.n - 1 : ((rb + 1) * RB - 1) / P.group;
   const int seen = s.len - s.n + last + 1;
   return seen <= 0 ? 0 : (seen + BLOCK - 1) / BLOCK;
 }
+// cost of a sequence's units of one kv head; units without a key cost nothing
 template <int RB>
-__device__ __forceinline__ int64_t sequence_blocks(const Params& P, int b) {
-  const Seq s = sequence<RB>(P, b);
+__device__ __forceinline__ int64_t head_cost(const Params& P, const Seq& s, int unit_cost) {
   int64_t sum = 0;
-  for (int rb = 0; rb < s.nrb; ++rb) sum += key_blocks<RB>(P, s, rb);
-  return sum * P.p.kv_heads;
+  for (int rb = 0; rb < s.nrb; ++rb) {
+    const int blocks = key_blocks<RB>(P, s, rb);
+    sum += blocks ? blocks + unit_cost : 0;
+  }
+  return sum;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -103,181 +111,290 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-template <int NG>
-__host__ __device__ constexpr int stage_bytes() { return 2 * block_bytes(NG); }
+// Warps per CTA (one CTA per SM): with 8 rows a warp needs 128 registers, with more O and Q
+// fill up to 255.
+__host__ __device__ constexpr int warps_of(int nb) { return nb == 1 ? 16 : 8; }
+constexpr int S = 4;  // blocks in flight per warp, 2 x 1184 bytes each at d = 128
+// shared memory: the warps' rings | their O (rows padded) and (m, l) at a unit's end | Q
+// fragments | mbarriers
 template <int NG, int NB>
-__host__ __device__ constexpr int stages() { return NB == 2 ? 6 : 4; }
-// shared memory: the warps' rings | their O and (m, l) at a unit's end | mbarriers
-template <int NG, int NB>
-__host__ __device__ constexpr int smem_bytes() {
-  return WARPS * stages<NG, NB>() * stage_bytes<NG>() + WARPS * (8 * NB) * (64 * NG + 2) * 4 +
-         WARPS * stages<NG, NB>() * 8;
-}
+struct Smem {
+  static constexpr int W = warps_of(NB), RB = 8 * NB, OLD = 64 * NG + 8;
+  static constexpr int stage = 2 * block_bytes(NG);
+  static constexpr int o = W * S * stage;
+  static constexpr int m = o + W * RB * OLD * 4;
+  static constexpr int l = m + W * RB * 4;
+  static constexpr int q = l + W * RB * 4;
+  static constexpr int bar = q + NB * NG * 2 * 32 * 16;
+  static constexpr int bytes = bar + W * S * 8;
+};
+
+// What a unit costs beyond its blocks (filling the rings, joining the warps), in blocks: the
+// runs are cut in this measure. Without it a CTA whose run holds many short units works
+// four times as long as the others (32 sequences of 1 .. 16000 tokens: 129 us against TODO).
+template <int NB>
+__host__ __device__ constexpr int unit_cost() { return warps_of(NB); }
+
+// A run's part of one unit, made by one thread for the CTA.
+struct Segment {
+  int b, head, rb;       // the unit
+  int c0, n, len, nrb;   // of its sequence: first token in q, new tokens, length, row blocks
+  int rows;              // rows of the unit
+  int tok0, rem0;        // its first row is query head rem0 of token tok0
+  int k0, count, blocks; // key blocks k0 .. k0 + count - 1 of `blocks`
+  int64_t at;            // the unit's place in the order of all costs
+};
 
 template <int NG, int NB>
-__global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kernel(Params P) {
-  constexpr int RB = 8 * NB, D = 64 * NG, S = stages<NG, NB>();
-  constexpr int UNIT = block_bytes(NG), STAGE = stage_bytes<NG>();
+__global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(Params P) {
+  using L = Smem<NG, NB>;
+  constexpr int RB = 8 * NB, D = 64 * NG, W = L::W, THREADS = 32 * W, OLD = L::OLD;
+  constexpr int UNIT = block_bytes(NG), STAGE = L::stage, COST = unit_cost<NB>();
   extern __shared__ __align__(128) unsigned char smem[];
-  float* s_o = reinterpret_cast<float*>(smem + WARPS * S * STAGE);  // [WARPS][RB][D]
-  float* s_m = s_o + WARPS * RB * D;                                // [WARPS][RB]
-  float* s_l = s_m + WARPS * RB;
-  uint64_t* s_bar = reinterpret_cast<uint64_t*>(s_l + WARPS * RB);  // [WARPS][S]
-  __shared__ int64_t s_scan[WARPS + 1];
-  __shared__ int s_start_b;
-  __shared__ int64_t s_start_at;
+  float* s_o = reinterpret_cast<float*>(smem + L::o);  // [W][RB][OLD]
+  float* s_m = reinterpret_cast<float*>(smem + L::m);  // [W][RB]
+  float* s_l = reinterpret_cast<float*>(smem + L::l);
+  uint4* s_q = reinterpret_cast<uint4*>(smem + L::q);  // [NB][NG][2 step pairs][32 lanes]
+  uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + L::bar);  // [W][S]
+  __shared__ int64_t s_scan[W], s_per, s_end;
+  __shared__ Segment s_seg[3];  // this one, the next, the one after
+  __shared__ int s_any, s_empty;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const Pages& p = P.p;
-  if (tid < WARPS * S) {
+  if (tid < W * S) {
     mbar_init(smem_addr(&s_bar[tid]), 1);
     fence_barrier_init();
   }
+  if (tid == 0) s_any = s_empty = 0;
   grid_dependency_wait();
   allow_dependent_launch();
 
-  // ---- this CTA's run of key blocks
-  auto scan = [&](int64_t mine, int64_t& before) {  // exclusive prefix over the CTA's threads; returns the sum
-    int64_t x = mine;
+  // Segment x's part in the run [begin, end) of costs, and its unit's rows. A unit's blocks
+  // stand behind its fixed cost.
+  auto fill = [&](Segment& x, const Seq& s, int64_t begin, int64_t end) {
+    x.c0 = p.cu[x.b];
+    x.n = s.n;
+    x.len = s.len;
+    x.nrb = s.nrb;
+    const int64_t first = x.at + COST;
+    x.k0 = static_cast<int>(std::max<int64_t>(begin - first, 0));
+    x.count = static_cast<int>(std::max<int64_t>(std::min<int64_t>(end - first, x.blocks) - x.k0, 0));
+    x.rows = min(RB, s.n * P.group - x.rb * RB);
+    x.tok0 = x.rb * RB / P.group;
+    x.rem0 = x.rb * RB - x.tok0 * P.group;
+  };
+  // x becomes the next unit with keys in the run (count 0: there is none)
+  auto next_unit = [&](Segment& x, int64_t begin, int64_t end) {
+    x.at += x.blocks + COST;
+    x.count = 0;
+    if (x.at + COST >= end) return;
+    Seq s = {x.n, x.len, x.nrb};
+    do {
+      if (++x.rb >= s.nrb) {
+        x.rb = 0;
+        if (++x.head >= p.kv_heads || s.nrb == 0) {
+          x.head = 0;
+          do {
+            if (++x.b >= p.batch) return;
+            s = sequence<RB>(P, x.b);
+          } while (s.nrb == 0);
+        }
+      }
+      x.blocks = key_blocks<RB>(P, s, x.rb);
+    } while (x.blocks == 0);
+    fill(x, s, begin, end);
+  };
+
+  // ---- this CTA's run of key blocks: a prefix sum over the sequences, one per thread (and
+  // round, past THREADS sequences); the thread that holds the run's start makes its segment
+  Seq sq = {0, 0, 0};
+  int64_t mine = 0, upto = 0;
+  auto count_blocks = [&](int b) {  // warps without a sequence do nothing
+    if (b - lane >= p.batch) return;
+    sq = {0, 0, 0};
+    if (b < p.batch) sq = sequence<RB>(P, b);
+    mine = head_cost<RB>(P, sq, COST) * p.kv_heads;
+    if (sq.n > sq.len) s_empty = 1;
+    upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
     }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = x;
-    __syncthreads();
-    int64_t base = 0, all = 0;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) base += s_scan[w];
-      all += s_scan[w];
-    }
-    before = base + x - mine;
-    return all;
+    if (lane == 31) s_scan[warp] = upto;
   };
-  int64_t total = 0, mine = 0, before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
-    mine = b0 + tid < p.batch ? sequence_blocks<RB>(P, b0 + tid) : 0;
-    total += scan(mine, before);
+  const int rounds = (p.batch + THREADS - 1) / THREADS;
+  int64_t total = 0;
+  for (int r = 0; r < rounds; ++r) {
+    if (r > 0) __syncthreads();
+    count_blocks(r * THREADS + tid);
+    __syncthreads();
+    if (rounds > 1 || warp * 32 < p.batch)
+      for (int w = 0; w < W && r * THREADS + w * 32 < p.batch; ++w) total += s_scan[w];
   }
-  // at least one block per warp, so that short problems have few partials to join
-  const int64_t per = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, WARPS);
-  const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(total, begin + per);
-  if (tid == 0) s_start_b = -1;
   int64_t base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
-    if (p.batch > THREADS) mine = b0 + tid < p.batch ? sequence_blocks<RB>(P, b0 + tid) : 0;
-    const int64_t sum = p.batch > THREADS ? scan(mine, before) : total;
-    if (begin < end && begin >= base + before && begin < base + before + mine) {
-      s_start_b = b0 + tid;
-      s_start_at = base + before;
+  for (int r = 0; r < rounds; ++r) {
+    const int b = r * THREADS + tid;
+    if (rounds > 1) {
+      __syncthreads();
+      count_blocks(b);
+      __syncthreads();
     }
-    base += sum;
+    if (b - lane < p.batch) {
+      // at least a round of the warps beyond a unit's cost, so that short problems have few
+      // partials to join
+      const int64_t per = std::max<int64_t>(
+          total < (int64_t(1) << 31) ? (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x
+                                     : (total + gridDim.x - 1) / gridDim.x, W + COST);
+      const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(total, begin + per);
+      int64_t start = base;  // of this thread's sequence, in the order of all costs
+      for (int w = 0; w < warp; ++w) start += s_scan[w];
+      start += upto - mine;
+      if (begin < end && begin >= start && begin < start + mine) {
+        Segment x;
+        x.b = b;
+        const int64_t per_head = mine / p.kv_heads;
+        const int64_t at = begin - start;
+        x.head = static_cast<int>(mine < (int64_t(1) << 31) ? static_cast<uint32_t>(at) / static_cast<uint32_t>(per_head)
+                                                            : at / per_head);
+        x.at = start + x.head * per_head;
+        x.rb = 0;
+        x.blocks = key_blocks<RB>(P, sq, 0);
+        while (begin >= x.at + (x.blocks ? x.blocks + COST : 0)) {
+          x.at += x.blocks ? x.blocks + COST : 0;
+          x.blocks = key_blocks<RB>(P, sq, ++x.rb);
+        }
+        s_per = per;
+        s_end = end;
+        fill(x, sq, begin, end);
+        if (x.count == 0) next_unit(x, begin, end);  // the run starts behind the unit's last block
+        s_seg[0] = x;
+        Segment y = x;
+        if (y.count) next_unit(y, begin, end);
+        s_seg[1] = y;
+        s_any = x.count > 0;
+      }
+    }
+    if (rounds > 1) {
+      for (int w = 0; w < W && r * THREADS + w * 32 < p.batch; ++w) base += s_scan[w];
+    }
   }
   int32_t* join = P.joins + blockIdx.x * 8;
   if (tid == 0) join[0] = 0;
-  // rows that see no key are zero
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    const Seq s = sequence<RB>(P, b);
-    const int none = min(s.n, s.n - s.len);  // tokens at positions below zero
-    for (int64_t i = tid; i < static_cast<int64_t>(std::max(none, 0)) * P.group * p.kv_heads * D; i += THREADS) {
-      const int c = i % D;
-      const int64_t row = i / D;
-      const int head = row % (P.group * p.kv_heads);
-      P.out[(p.cu[b] + row / (P.group * p.kv_heads)) * P.ot + head * P.oh + c] = __float2bfloat16_rn(0.0f);
+  __syncthreads();
+  if (s_empty) {  // rows that see no key are zero: tokens at positions below zero
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      const Seq e = sequence<RB>(P, b);
+      const int none = min(e.n, e.n - e.len), heads = P.group * p.kv_heads;
+      for (int64_t i = tid; i < static_cast<int64_t>(none) * heads * (D / 8); i += THREADS) {
+        const int64_t row = i / (D / 8);
+        *reinterpret_cast<uint4*>(P.out + (p.cu[b] + row / heads) * P.ot + (row % heads) * P.oh + i % (D / 8) * 8) =
+            make_uint4(0, 0, 0, 0);
+      }
     }
   }
-  __syncthreads();
-  if (begin >= end || s_start_b < 0) return;
+  if (!s_any) return;
 
-  // ---- the run's segments, one per unit
-  int b = s_start_b, head, rb;
-  Seq sq = sequence<RB>(P, b);
-  int64_t at = begin - s_start_at;  // within the sequence, then within the unit
-  {
-    int64_t per_head = 0;
-    for (int i = 0; i < sq.nrb; ++i) per_head += key_blocks<RB>(P, sq, i);
-    head = static_cast<int>(at / per_head);
-    at -= head * per_head;
-    rb = 0;
-    while (at >= key_blocks<RB>(P, sq, rb)) at -= key_blocks<RB>(P, sq, rb++);
-  }
-  int64_t left = end - begin;
   unsigned char* ring = smem + warp * S * STAGE;
   uint64_t* bars = s_bar + warp * S;
   int issued = 0, used = 0;  // copies of this warp's ring
-  int64_t first_at = begin - at;  // the current unit's first block, in the order of all blocks
-  bool ok = true;
-
-  while (left > 0) {
-    const int unit_blocks = key_blocks<RB>(P, sq, rb);
-    const int k0 = static_cast<int>(at), count = static_cast<int>(std::min<int64_t>(left, unit_blocks - at));
-    const int kend = k0 + count;
-    // this warp's blocks: k0 + warp, + WARPS, ...; lane l looks up the page of the l-th (of 32 at a time)
-    const int mine_blocks = count > warp ? (count - warp + WARPS - 1) / WARPS : 0;
-    int64_t page_off = -1;
-    auto look_up = [&](int from) {
-      const int i = from + lane;
-      page_off = -1;
-      if (i < mine_blocks) {
-        const int pos = (k0 + warp + i * WARPS) * BLOCK;
-        const int64_t page = page_of(p, b, pos);
-        if (page >= 0) page_off = page * p.page_stride + block_in_page<NG>(p, 0, head, pos);
-      }
-    };
-    const int64_t v_off = static_cast<int64_t>(p.kv_heads) * (1 << (p.page_shift - 4)) * UNIT;
-    auto issue = [&](int64_t off) {  // warp-uniform off
-      if (off < 0) return;
-      if (lane == 0) {
-        const uint32_t bar = smem_addr(&bars[issued % S]);
-        const uint32_t dst = smem_addr(ring + (issued % S) * STAGE);
-        mbar_arrive_expect_tx(bar, STAGE);
-        bulk_copy(dst, p.base + off, UNIT, bar);
-        bulk_copy(dst + UNIT, p.base + off + v_off, UNIT, bar);
-      }
-      ++issued;
-    };
-    look_up(0);
-    int64_t next_off = -1;  // pages of the window after this one are looked up when it starts
-    // the fragments of this unit's rows: query head head * G + r % G of token r / G
-    uint32_t qf[NB][NG][4][2];
-    int lim[NB][2];
-    const int rows = min(RB, sq.rows - rb * RB);
-    const int nbs = (rows + 7) / 8;
-    const int c0 = p.cu[b];
-    for (int i = 0; i < min(mine_blocks, S - 1); ++i) issue(__shfl_sync(0xffffffffu, page_off, i));
-    int lim_min = 0x7fffffff;
+  uint32_t has_page = 0;     // bit of a ring slot: its block has a page
+  int ahead = 0, ahead_blocks = 0;  // the next block to copy, of this warp's blocks of s_seg[ahead_seg]
+  int ahead_seg = 0;
+  const uint8_t* address = nullptr;  // lane l: where the l-th block of the window of 32 starts
+  uint32_t valid = 0;                // which of the window's blocks have a page
+  auto blocks_of = [&](const Segment& x) { return x.count > warp ? (x.count - warp + W - 1) / W : 0; };
+  // A block without a page is copied from page 0 and left out of the softmax.
+  auto look_up = [&](const Segment& x) {
+    const int i = ahead + lane;
+    bool has = false;
+    address = p.base;
+    if (i < ahead_blocks) {
+      const int pos = (x.k0 + warp + i * W) * BLOCK;
+      const int64_t page = page_of(p, x.b, pos);
+      has = page >= 0;
+      address = p.base + (has ? page : 0) * p.page_stride + block_in_page<NG>(p, 0, x.head, pos);
+    }
+    valid = __ballot_sync(0xffffffffu, has);
+  };
+  const uint32_t v_off = static_cast<uint32_t>(p.kv_heads << (p.page_shift - 4)) * UNIT;
+  auto copy_next = [&]() {  // into a free slot of the ring
+    if ((ahead & 31) == 0) look_up(s_seg[ahead_seg]);
+    const uint32_t slot = issued % S;
+    if (lane == (ahead & 31)) {
+      const uint32_t bar = smem_addr(&bars[slot]);
+      const uint32_t dst = smem_addr(ring + slot * STAGE);
+      mbar_arrive_expect_tx(bar, STAGE);
+      bulk_copy(dst, address, UNIT, bar);
+      bulk_copy(dst + UNIT, address + v_off, UNIT, bar);
+    }
+    has_page = (has_page & ~(1u << slot)) | (((valid >> (ahead & 31)) & 1u) << slot);
+    ++issued;
+    ++ahead;
+  };
+  // The fragments of n-block `nb` of a unit's rows, by one warp: a B fragment's column is row
+  // g, and lane t holds channels 16 t .. 16 t + 15 of each group; step ks takes channels
+  // 16 t + ks and + 4 (pair ks of word 2 t), then + 8 and + 12 (of word 2 t + 1).
+  auto make_q = [&](const Segment& x, int nb) {
+    const int r = x.rem0 + nb * 8 + g, tok = small_div(P, r);
+    const bool live = nb * 8 + g < x.rows;
+    const __nv_bfloat16* row = P.q + static_cast<int64_t>(x.c0 + x.tok0 + (live ? tok : 0)) * P.qt +
+                               (x.head * P.group + (live ? r - tok * P.group : 0)) * P.qh;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int r = rb * RB + nb * 8 + g;  // the B fragment's column
-      const bool live = nb * 8 + g < rows;
-      const __nv_bfloat16* row =
-          P.q + static_cast<int64_t>(c0 + (live ? r / P.group : 0)) * P.qt + (head * P.group + (live ? r % P.group : 0)) * P.qh;
+    for (int gr = 0; gr < NG; ++gr) {
+      const uint4* src = reinterpret_cast<const uint4*>(row + 64 * gr + 16 * t);
+      const uint4 u0 = live ? src[0] : make_uint4(0, 0, 0, 0), u1 = live ? src[1] : make_uint4(0, 0, 0, 0);
+      const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        uint32_t w[8];  // channels 16 t .. 16 t + 15 of the group
-        const uint4* src = reinterpret_cast<const uint4*>(row + 64 * gr + 16 * t);
-        const uint4 u0 = live ? src[0] : make_uint4(0, 0, 0, 0), u1 = live ? src[1] : make_uint4(0, 0, 0, 0);
-        w[0] = u0.x; w[1] = u0.y; w[2] = u0.z; w[3] = u0.w;
-        w[4] = u1.x; w[5] = u1.y; w[6] = u1.z; w[7] = u1.w;
-        // step ks: channels 16 t + ks and + 4 (word 2 t's pair ks), then + 8 and + 12
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const uint32_t sel = (ks & 1) ? 0x7632 : 0x5410;
-          qf[nb][gr][ks][0] = __byte_perm(w[ks >> 1], w[2 + (ks >> 1)], sel);
-          qf[nb][gr][ks][1] = __byte_perm(w[4 + (ks >> 1)], w[6 + (ks >> 1)], sel);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // the C fragments' columns: row 2 t + h
-        const int rr = nb * 8 + 2 * t + h;
-        lim[nb][h] = rr < rows ? sq.len - sq.n + (rb * RB + rr) / P.group : 0x7fffffff;
-        lim_min = min(lim_min, lim[nb][h]);
+      for (int i = 0; i < 2; ++i)
+        s_q[((nb * NG + gr) * 2 + i) * 32 + lane] =
+            make_uint4(__byte_perm(w[i], w[2 + i], 0x5410), __byte_perm(w[4 + i], w[6 + i], 0x5410),
+                       __byte_perm(w[i], w[2 + i], 0x7632), __byte_perm(w[4 + i], w[6 + i], 0x7632));
+    }
+  };
+  // fills the ring's free slots, going on with the next unit's blocks when this one's are done
+  auto top_up = [&](int cur, int next, bool more) {
+    while (issued - used < S) {
+      if (ahead < ahead_blocks) {
+        copy_next();
+      } else {
+        if (!more || ahead_seg != cur) break;
+        ahead_seg = next;
+        ahead = 0;
+        ahead_blocks = blocks_of(s_seg[next]);
       }
     }
-    lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
-    lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
+  };
+  const Expand expand;
+  int cur = 0;
+  bool ok = true;
+  ahead_blocks = blocks_of(s_seg[0]);
+  top_up(0, 0, false);
+  if (warp < NB) make_q(s_seg[0], warp);
+  __syncthreads();
+
+  while (true) {
+    const Segment x = s_seg[cur];
+    const int next = cur == 2 ? 0 : cur + 1;
+    const bool more = s_seg[next].count > 0;
+    const int mine_blocks = blocks_of(x);
+    const int nbs = (x.rows + 7) / 8;
+    top_up(cur, next, more);
+    uint4 qr[NB == 1 ? NG * 2 : 1];  // one n-block: Q stays in registers
+    if constexpr (NB == 1) {
+#pragma unroll
+      for (int i = 0; i < NG * 2; ++i) qr[i] = s_q[i * 32 + lane];
+    }
+    // last visible key of the C fragments' columns (rows 2 t, 2 t + 1 of each n-block); the
+    // rows past the unit's are not masked (their scores are 0) and not written
+    const int lim0 = x.len - x.n + x.tok0;
+    int lim[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) lim[nb][h] = lim0 + small_div(P, x.rem0 + nb * 8 + 2 * t + h);
 
     float o[NB][NG * 4][4], m[NB][2], l[NB][2];
 #pragma unroll
@@ -286,32 +403,18 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
       for (int i = 0; i < NG * 4; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[nb][i][c] = 0.0f;
-      m[nb][0] = m[nb][1] = -INFINITY;
+      m[nb][0] = m[nb][1] = LOWEST;
       l[nb][0] = l[nb][1] = 0.0f;
     }
 
     for (int i = 0; i < mine_blocks; ++i) {
-      if ((i & 31) == 0 && i > 0) look_up(i);  // this window's pages
-      const int64_t off = __shfl_sync(0xffffffffu, page_off, i & 31);
-      // the block S - 1 ahead: its page is in this window or read here for the next one
-      const int ahead = i + S - 1;
-      if (ahead < mine_blocks) {
-        if ((ahead >> 5) == (i >> 5)) {
-          next_off = __shfl_sync(0xffffffffu, page_off, ahead & 31);
-        } else {
-          const int pos = (k0 + warp + ahead * WARPS) * BLOCK;
-          const int64_t page = page_of(p, b, pos);
-          next_off = page < 0 ? -1 : page * p.page_stride + block_in_page<NG>(p, 0, head, pos);
-        }
-        issue(next_off);
-      }
-      if (off < 0) continue;  // no such page: its keys are left out
       if (!mbar_wait_warp(smem_addr(&bars[used % S]), (used / S) & 1, 42, used)) {
         ok = false;
         break;
       }
       const unsigned char* kb = ring + (used % S) * STAGE;
       const unsigned char* vb = kb + UNIT;
+      const bool page = (has_page >> (used % S)) & 1;
       ++used;
 
       // ---- S^T = K Q^T
@@ -352,41 +455,52 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int wd = 0; wd < 2; ++wd)
-            expand_word(kw[h][2 * gr + wd], exponent_pair(ke[h][gr], (7 - 4 * t - 2 * wd) & 31), a[h][wd]);
+            expand.word(kw[h][2 * gr + wd], expand.exponents(ke[h][gr], (7 - 4 * t - 2 * wd) & 31), a[h][wd]);
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const uint32_t fa[4] = {a[0][0][st], a[1][0][st], a[0][1][st], a[1][1][st]};
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const uint32_t f0[4] = {a[0][0][2 * i2], a[1][0][2 * i2], a[0][1][2 * i2], a[1][1][2 * i2]};
+          const uint32_t f1[4] = {a[0][0][2 * i2 + 1], a[1][0][2 * i2 + 1], a[0][1][2 * i2 + 1], a[1][1][2 * i2 + 1]};
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            if (nb < nbs) mma_bf16_16816(acc[nb][gr], fa, qf[nb][gr][st][0], qf[nb][gr][st][1]);
+          for (int nb = 0; nb < NB; ++nb) {
+            if (NB > 1 && nb >= nbs) continue;
+            const uint4 qf = NB == 1 ? qr[gr * 2 + i2] : s_q[((nb * NG + gr) * 2 + i2) * 32 + lane];
+            mma_bf16_16816(acc[nb][gr], f0, qf.x, qf.y);
+            mma_bf16_16816(acc[nb][gr], f1, qf.z, qf.w);
+          }
         }
       }
       // ---- softmax; c of the fragment: key g + 8 (c / 2), row 2 t + c % 2
-      const int key0 = (k0 + warp + i * WARPS) * BLOCK + g;
-      const bool edge = key0 - g + BLOCK - 1 > lim_min;
+      const int first_key = (x.k0 + warp + i * W) * BLOCK, key0 = first_key + g;
+      const bool edge = first_key + BLOCK - 1 > lim0 || !page;  // lim0: the unit's first row's
       uint32_t pf[NB][NG][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        if (nb >= nbs) continue;
+        if (NB > 1 && nb >= nbs) continue;
         float s[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           s[c] = __fmul_rn(acc[nb][0][c], ks[c >> 1][0]);
           if constexpr (NG == 2) s[c] = __fmaf_rn(acc[nb][1][c], ks[c >> 1][1], s[c]);
-          if (edge && key0 + 8 * (c >> 1) > lim[nb][c & 1]) s[c] = -INFINITY;
         }
-        const float top0 = __fmul_rn(fmaxf(s[0], s[2]), P.scale_log2), top1 = __fmul_rn(fmaxf(s[1], s[3]), P.scale_log2);
-        if (__any_sync(0xffffffffu, top0 > m[nb][0] + RAISE || top1 > m[nb][1] + RAISE)) {
-          float n0 = top0, n1 = top1;
+        if (edge) {
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+          for (int c = 0; c < 4; ++c)
+            if (key0 + 8 * (c >> 1) > lim[nb][c & 1] || !page) s[c] = -INFINITY;
+        }
+        // log2 p against the reference maxima (finite from the start, so no case of its own)
+        float e[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[nb][c & 1]);
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > RAISE)) {
+          float n0 = __fmul_rn(fmaxf(s[0], s[2]), P.scale_log2), n1 = __fmul_rn(fmaxf(s[1], s[3]), P.scale_log2);
+#pragma unroll
+          for (int y = 4; y < 32; y <<= 1) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, y));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, y));
           }
           n0 = fmaxf(n0, m[nb][0]);
           n1 = fmaxf(n1, m[nb][1]);
-          const float a0 = m[nb][0] == -INFINITY ? 0.0f : ex2(m[nb][0] - n0);
-          const float a1 = m[nb][1] == -INFINITY ? 0.0f : ex2(m[nb][1] - n1);
+          const float a0 = ex2(m[nb][0] - n0), a1 = ex2(m[nb][1] - n1);
           m[nb][0] = n0;
           m[nb][1] = n1;
           l[nb][0] *= a0;
@@ -398,11 +512,11 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
             o[nb][j][2] *= a0;
             o[nb][j][3] *= a1;
           }
-        }
-        const float u0 = m[nb][0] == -INFINITY ? 0.0f : m[nb][0], u1 = m[nb][1] == -INFINITY ? 0.0f : m[nb][1];
-        float e[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) e[c] = ex2(__fmaf_rn(s[c], P.scale_log2, (c & 1) ? -u1 : -u0));
+          for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[nb][c & 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) e[c] = ex2(e[c]);
         l[nb][0] += e[0] + e[2];
         l[nb][1] += e[1] + e[3];
 #pragma unroll
@@ -435,57 +549,77 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int qd = 0; qd < 2; ++qd)
-            expand_word(vw[h][2 * gr + qd], exponent_pair(ve[h][2 * gr + qd], (7 - 2 * g) & 31), a[h][qd]);
+            expand.word(vw[h][2 * gr + qd], expand.exponents(ve[h][2 * gr + qd], (7 - 2 * g) & 31), a[h][qd]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t fa[4] = {a[0][0][j], a[0][1][j], a[1][0][j], a[1][1][j]};
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            if (nb < nbs) mma_bf16_16816(o[nb][gr * 4 + j], fa, pf[nb][gr][0], pf[nb][gr][1]);
+            if (NB == 1 || nb < nbs) mma_bf16_16816(o[nb][gr * 4 + j], fa, pf[nb][gr][0], pf[nb][gr][1]);
         }
       }
-      __syncwarp();  // the stage may be refilled: every lane has read it
+      __syncwarp();  // the slot may be refilled: every lane has read it
+      if (ahead < ahead_blocks) copy_next();
+      else if (more && ahead_seg == cur) top_up(cur, next, more);
     }
 
     // ---- the warps' results meet
-    __syncthreads();  // the previous unit's s_o has been read
+    const bool worked = warp < x.count;  // warps without a block hold nothing
+    if (worked) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      if (nb >= nbs) continue;
+      for (int nb = 0; nb < NB; ++nb) {
+        if (nb >= nbs) continue;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], x);
-        const int r = nb * 8 + 2 * t + h;
-        float* dst = s_o + (warp * RB + r) * D + 8 * g;
+          for (int y = 4; y < 32; y <<= 1) l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], y);
+          const int r = nb * 8 + 2 * t + h;
+          if (r < x.rows) {
+            float* dst = s_o + (warp * RB + r) * OLD + 8 * g;
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          *reinterpret_cast<float4*>(dst + 64 * gr) =
-              make_float4(o[nb][4 * gr][h], o[nb][4 * gr + 1][h], o[nb][4 * gr + 2][h], o[nb][4 * gr + 3][h]);
-          *reinterpret_cast<float4*>(dst + 64 * gr + 4) =
-              make_float4(o[nb][4 * gr][2 + h], o[nb][4 * gr + 1][2 + h], o[nb][4 * gr + 2][2 + h], o[nb][4 * gr + 3][2 + h]);
-        }
-        if (g == 0) {
-          s_m[warp * RB + r] = m[nb][h];
-          s_l[warp * RB + r] = l[nb][h];
+            for (int gr = 0; gr < NG; ++gr) {
+              *reinterpret_cast<float4*>(dst + 64 * gr) =
+                  make_float4(o[nb][4 * gr][h], o[nb][4 * gr + 1][h], o[nb][4 * gr + 2][h], o[nb][4 * gr + 3][h]);
+              *reinterpret_cast<float4*>(dst + 64 * gr + 4) =
+                  make_float4(o[nb][4 * gr][2 + h], o[nb][4 * gr + 1][2 + h], o[nb][4 * gr + 2][2 + h], o[nb][4 * gr + 3][2 + h]);
+            }
+            if (g == 0) {
+              s_m[warp * RB + r] = m[nb][h];
+              s_l[warp * RB + r] = l[nb][h];
+            }
+          }
         }
       }
     }
-    const bool whole = k0 == 0 && kend == unit_blocks;
+    const bool whole = x.count == x.blocks;
+    if (tid == 0) {
+      if (x.k0 > 0 && x.k0 + x.count == x.blocks) {  // the unit ends here and began in an earlier run
+        join[1] = x.c0 + x.tok0;
+        join[2] = x.head;
+        join[3] = x.rem0;
+        join[4] = x.rows;
+        join[5] = static_cast<int>((x.at + COST) / s_per);  // the run that holds the unit's first block
+        join[0] = 1;
+      }
+      if (more) {  // the unit after the next one
+        Segment y = s_seg[next];
+        next_unit(y, blockIdx.x * s_per, s_end);
+        s_seg[next == 2 ? 0 : next + 1] = y;
+      }
+    }
     if (!__syncthreads_and(ok)) break;  // a copy never landed: recorded; this unit is not written
-    float* part = P.parts + (2 * static_cast<int64_t>(blockIdx.x) + (kend < unit_blocks && k0 == 0)) * (RB * D + 2 * RB);
-    for (int i = tid; i < rows * (D / 4); i += THREADS) {
+    float* part = P.parts + (2 * static_cast<int64_t>(blockIdx.x) + (x.k0 == 0)) * (RB * D + 2 * RB);
+    const int parts = min(W, x.count);
+    for (int i = tid; i < x.rows * (D / 4); i += THREADS) {
       const int r = i / (D / 4), c = i % (D / 4) * 4;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w * RB + r]);
-      const float use = top == -INFINITY ? 0.0f : top;
+      float top = LOWEST;
+      for (int w = 0; w < parts; ++w) top = fmaxf(top, s_m[w * RB + r]);
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       float den = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = ex2(s_m[w * RB + r] - use);
-        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * D + c);
+#pragma unroll 4
+      for (int w = 0; w < parts; ++w) {
+        const float f = ex2(s_m[w * RB + r] - top);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * OLD + c);
         sum.x += f * v.x;
         sum.y += f * v.y;
         sum.z += f * v.z;
@@ -493,13 +627,13 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
         den += f * s_l[w * RB + r];
       }
       if (whole) {
-        const int row = rb * RB + r;
+        const int tok = small_div(P, x.rem0 + r);
         const float inv = den > 0.0f ? __fdiv_rn(1.0f, den) : (den == 0.0f ? 0.0f : den);  // NaN stays
         uint2 w2;
         w2.x = pack_bf16(sum.x * inv, sum.y * inv);
         w2.y = pack_bf16(sum.z * inv, sum.w * inv);
-        *reinterpret_cast<uint2*>(P.out + static_cast<int64_t>(c0 + row / P.group) * P.ot +
-                                  (head * P.group + row % P.group) * P.oh + c) = w2;
+        *reinterpret_cast<uint2*>(P.out + static_cast<int64_t>(x.c0 + x.tok0 + tok) * P.ot +
+                                  (x.head * P.group + x.rem0 + r - tok * P.group) * P.oh + c) = w2;
       } else {
         *reinterpret_cast<float4*>(part + r * D + c) = sum;
         if (c == 0) {
@@ -508,30 +642,10 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
         }
       }
     }
-    if (!whole && k0 > 0 && kend == unit_blocks && tid == 0) {
-      join[1] = c0;
-      join[2] = head;
-      join[3] = rb;
-      join[4] = rows;
-      join[5] = static_cast<int>(first_at / per);  // the run that holds the unit's first block
-      join[0] = 1;
-    }
-    // ---- the next unit with keys
-    left -= count;
-    if (left > 0) {
-      first_at += unit_blocks;
-      at = 0;
-      do {
-        if (++rb >= sq.nrb) {
-          rb = 0;
-          if (++head >= p.kv_heads || sq.nrb == 0) {
-            head = 0;
-            do sq = sequence<RB>(P, ++b);
-            while (sq.nrb == 0 && b + 1 < p.batch);
-          }
-        }
-      } while (key_blocks<RB>(P, sq, rb) == 0);
-    }
+    if (!more) break;
+    cur = next;
+    if (warp < NB) make_q(s_seg[cur], warp);
+    __syncthreads();  // s_o has been read, Q is there
   }
   // a timeout leaves copies in flight: wait for them (bounded) before the CTA's memory goes
   if (lane == 0)
@@ -540,62 +654,87 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) paged_attention_kern
 }
 
 // Joins the partials of the unit that ended in run blockIdx.x: its first run's (slot 2 c + 1),
-// then those of the runs up to this one (slot 2 c). One warp per row.
+// then those of the runs up to this one (slot 2 c). One CTA per row: eight warps take the
+// partials in turn, four channels (two at d = 64) per lane, and meet in shared memory.
 template <int D, int RB>
-__global__ void __launch_bounds__(128) paged_combine_kernel(Params P) {
+__global__ void __launch_bounds__(256) paged_combine_kernel(Params P) {
+  constexpr int V = D / 32;
+  constexpr int64_t SIZE = RB * D + 2 * RB;
+  __shared__ float s_sum[8][D], s_top[8], s_den[8];
   grid_dependency_wait();
   allow_dependent_launch();
   const int32_t* join = P.joins + blockIdx.x * 8;
-  if (join[0] == 0) return;
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (r >= join[4]) return;
+  const int r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (join[0] == 0 || r >= join[4]) return;
   const int first = join[5], last = blockIdx.x;
-  constexpr int64_t SIZE = RB * D + 2 * RB;
-  auto part = [&](int c) { return P.parts + (2 * static_cast<int64_t>(c) + (c == first)) * SIZE; };
-  float top = -INFINITY;
-  for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, part(c)[RB * D + r]);
+  float sum[V], den = 0.0f, top = LOWEST;
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  const float use = top == -INFINITY ? 0.0f : top;
-  constexpr int W = D / 32;  // channels per lane
-  float sum[W], den = 0.0f;
-#pragma unroll
-  for (int i = 0; i < W; ++i) sum[i] = 0.0f;
+  for (int i = 0; i < V; ++i) sum[i] = 0.0f;
 #pragma unroll 4
-  for (int c = first; c <= last; ++c) {
-    const float* src = part(c);
-    const float f = ex2(src[RB * D + r] - use);
-    den += f * src[RB * D + RB + r];
+  for (int c = first + warp; c <= last; c += 8) {
+    const float* src = P.parts + (2 * static_cast<int64_t>(c) + (c == first)) * SIZE;
+    float v[V];
+    if constexpr (V == 4) {
+      const float4 u = *reinterpret_cast<const float4*>(src + r * D + lane * 4);
+      v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    } else {
+      const float2 u = *reinterpret_cast<const float2*>(src + r * D + lane * 2);
+      v[0] = u.x; v[1] = u.y;
+    }
+    const float m = src[RB * D + r], l = src[RB * D + RB + r];
+    const float next = fmaxf(top, m);
+    const float f = ex2(top - next), e = ex2(m - next);
 #pragma unroll
-    for (int i = 0; i < W; ++i) sum[i] += f * src[r * D + lane * W + i];
+    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f + v[i] * e;
+    den = den * f + l * e;
+    top = next;
   }
-  const float inv = den > 0.0f ? __fdiv_rn(1.0f, den) : (den == 0.0f ? 0.0f : den);
-  const int row = join[3] * RB + r;
-  __nv_bfloat16* dst = P.out + static_cast<int64_t>(join[1] + row / P.group) * P.ot +
-                       (join[2] * P.group + row % P.group) * P.oh + lane * W;
 #pragma unroll
-  for (int i = 0; i < W; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16(sum[i] * inv, sum[i + 1] * inv);
+  for (int i = 0; i < V; ++i) s_sum[warp][lane * V + i] = sum[i];
+  if (lane == 0) {
+    s_top[warp] = top;
+    s_den[warp] = den;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  const int c = threadIdx.x * 2;
+  float all = LOWEST, o0 = 0.0f, o1 = 0.0f, d = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) all = fmaxf(all, s_top[w]);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float f = ex2(s_top[w] - all);
+    o0 += f * s_sum[w][c];
+    o1 += f * s_sum[w][c + 1];
+    d += f * s_den[w];
+  }
+  const float inv = d > 0.0f ? __fdiv_rn(1.0f, d) : (d == 0.0f ? 0.0f : d);
+  const int row = join[3] + r, tok = small_div(P, row);
+  *reinterpret_cast<uint32_t*>(P.out + static_cast<int64_t>(join[1] + tok) * P.ot +
+                               (join[2] * P.group + row - tok * P.group) * P.oh + c) = pack_bf16(o0 * inv, o1 * inv);
 }
 
 constexpr int JOIN_BYTES_PER_CTA = 32;
-inline int ctas(int nb) { return num_sms() * (nb == 1 ? 2 : 1); }
+inline int ctas() { return num_sms(); }
 inline int n_blocks(int64_t max_rows) { return max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4; }
 inline size_t workspace(int nb, int d) {
   const int64_t rows = 8 * nb;
-  return static_cast<size_t>(ctas(nb)) * (JOIN_BYTES_PER_CTA + 2 * (rows * d + 2 * rows) * 4);
+  return static_cast<size_t>(ctas()) * (JOIN_BYTES_PER_CTA + 2 * (rows * d + 2 * rows) * 4);
 }
 
 template <int NG, int NB>
 static int launch(Params& P, void* ws, void* stream) {
-  const int grid = ctas(NB);
+  const int grid = ctas();
   P.joins = static_cast<int32_t*>(ws);
   P.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + static_cast<size_t>(grid) * JOIN_BYTES_PER_CTA);
-  constexpr int bytes = smem_bytes<NG, NB>();
+  constexpr int bytes = Smem<NG, NB>::bytes;
   auto kern = paged_attention_kernel<NG, NB>;
-  FAQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(grid)), THREADS, bytes, stream, P));
-  FAQ_CUDA(launch_early(paged_combine_kernel<64 * NG, 8 * NB>, dim3(static_cast<unsigned>(grid), 2 * NB), 128, 0, stream, P));
-  return launch_status("paged attention kernels");
+  static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
+  int rc = allow_smem(reinterpret_cast<const void*>(kern), bytes, set);
+  if (rc) return rc;
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(grid)), 32 * warps_of(NB), bytes, stream, P));
+  FAQ_CUDA(launch_early(paged_combine_kernel<64 * NG, 8 * NB>, dim3(static_cast<unsigned>(grid), 8 * NB), 256, 0, stream, P));
+  return FAQ_OK;
 }
 
 }  // namespace pat
@@ -640,6 +779,8 @@ extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t he
   P.oh = out_head_stride;
   P.total = total;
   P.group = static_cast<int>(heads / kv_heads);
+  FAQ_CHECK_ARG(P.group < 4096, "more than 4095 query heads per key/value head");
+  P.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + P.group - 1) / P.group);
   P.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   if (d == 64) return nb == 1 ? launch<1, 1>(P, workspace, stream) : nb == 2 ? launch<1, 2>(P, workspace, stream) : launch<1, 4>(P, workspace, stream);
   return nb == 1 ? launch<2, 1>(P, workspace, stream) : nb == 2 ? launch<2, 2>(P, workspace, stream) : launch<2, 4>(P, workspace, stream);
