@@ -49,6 +49,7 @@ struct Params {
   __nv_bfloat16* out;
   int64_t ot, oh;
   int64_t total;   // rows of q and out
+  int max_rows;    // sequences with more rows are the prompt kernel's
   int group;       // query heads per kv head
   uint32_t group_magic;  // ceil(2^32 / group), see small_div
   float scale_log2;
@@ -69,6 +70,7 @@ __device__ __forceinline__ Seq sequence(const Params& P, int b) {
   Seq s;
   const int c0 = P.p.cu[b], c1 = P.p.cu[b + 1];
   s.n = (c0 >= 0 && c1 > c0 && c1 <= P.total) ? c1 - c0 : 0;
+  if (static_cast<int64_t>(s.n) * P.group > P.max_rows) s.n = 0;
   s.len = length_of(P.p, b);
   s.nrb = (s.n * P.group + RB - 1) / RB;
   return s;
@@ -740,48 +742,3 @@ static int launch(Params& P, void* ws, void* stream) {
 }  // namespace pat
 }  // namespace faq
 
-extern "C" size_t faq_hif4_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t max_new, int d) {
-  using namespace faq::pat;
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_new < 0 || (d != 64 && d != 128)) return 0;
-  return workspace(n_blocks(heads / kv_heads * max_new), d);
-}
-
-extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride,
-                                        int64_t q_head_stride, const void* pages, int64_t num_pages,
-                                        int64_t page_stride, int page_size, int64_t kv_heads, int d,
-                                        const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
-                                        const int32_t* lens, int64_t batch, int64_t max_new, int64_t max_len, float scale,
-                                        void* out, int64_t out_token_stride, int64_t out_head_stride, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
-  using namespace faq;
-  using namespace faq::pat;
-  Params P;
-  const int rc = make_pages(P.p, pages, num_pages, page_stride, page_size, kv_heads, d, table, table_ld, table_cols, cu,
-                            lens, batch);
-  if (rc) return rc;
-  FAQ_CHECK_ARG(heads > 0 && heads % kv_heads == 0, "query heads must be divisible by key/value heads");
-  FAQ_CHECK_ARG(total >= 0 && max_new >= 0 && max_len >= 0 && total * heads < (int64_t(1) << 31), "bad token count");
-  if (total == 0) return FAQ_OK;
-  FAQ_CHECK_ARG(q && out, "null pointer");
-  FAQ_CHECK_ARG(scale > 0.0f && scale < 3.0e38f, "scale must be positive and finite");
-  FAQ_CHECK_ARG(aligned16(q) && aligned16(out) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
-                    out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
-                "q and out must be 16-byte aligned with strides multiple of 8");
-  const int nb = n_blocks(heads / kv_heads * max_new);
-  FAQ_CHECK_ARG(workspace != nullptr && aligned16(workspace), "workspace must be a 16-byte aligned device buffer");
-  FAQ_CHECK_ARG(workspace_bytes >= pat::workspace(nb, d),
-                "workspace too small: faq_hif4_paged_attention_workspace_bytes() bytes needed");
-  P.q = static_cast<const __nv_bfloat16*>(q);
-  P.qt = q_token_stride;
-  P.qh = q_head_stride;
-  P.out = static_cast<__nv_bfloat16*>(out);
-  P.ot = out_token_stride;
-  P.oh = out_head_stride;
-  P.total = total;
-  P.group = static_cast<int>(heads / kv_heads);
-  FAQ_CHECK_ARG(P.group < 4096, "more than 4095 query heads per key/value head");
-  P.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + P.group - 1) / P.group);
-  P.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  if (d == 64) return nb == 1 ? launch<1, 1>(P, workspace, stream) : nb == 2 ? launch<1, 2>(P, workspace, stream) : launch<1, 4>(P, workspace, stream);
-  return nb == 1 ? launch<2, 1>(P, workspace, stream) : nb == 2 ? launch<2, 2>(P, workspace, stream) : launch<2, 4>(P, workspace, stream);
-}

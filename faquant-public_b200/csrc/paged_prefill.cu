@@ -1,0 +1,880 @@
+// K9 for chunks of many new tokens: the prompt kernel on tcgen05 tensor cores.
+//
+// Same operation as paged_attention.cu. With hundreds of rows per kv head the products bound
+// the time (4 d FLOPs per visible key and row), and expanding the codes once costs little
+// beside them, so a chunk takes three kernels:
+//   expand   the long sequences' K and V, page by page, to bf16 [tokens][kv heads][d] in the
+//            workspace (each sequence from a multiple of 128 tokens, zeros to its end), and the
+//            plan of the next kernel's work (one CTA);
+//   prefill  a persistent kernel, one CTA per SM. A unit is (sequence, kv head, 2 x T tokens, T =
+//            128 / group whole tokens): two tiles A and B of 128 rows, row = token * group + query
+//            head, so the keys are read once for the group. Key tiles of 128. The key tiles
+//            of all units are cut into equal runs, one per CTA, as in paged_attention.cu;
+//   combine  joins the partials of units that lie in several runs.
+// In the prefill kernel (384 threads): warps 0-3 the softmax of tile A, 4-7 of tile B, one
+// row per thread; warp 8 loads Q and K by TMA, warp 9 V; warp 10 issues the MMAs. S_t = Q_t K^T
+// goes to 128 columns of tensor memory; the softmax writes P (bf16) over it, from where the
+// tensor core reads it as the A operand of O_t += P_t V (shared memory, which the two
+// products' operands nearly saturate, does not see P). S_t of the next key tile overwrites P_t,
+// so it is issued when that product has completed; the issuing thread takes whichever tile
+// is ready, and the other tile's products fill the wait.
+// Softmax: a row's reference maximum is raised only when a score passes it by more than 2^8
+// (then O is rescaled in tensor memory), so a step mostly has no rescaling.
+#include <algorithm>
+#include <atomic>
+
+#include "kv_pages.cuh"
+#include "tma.h"
+
+namespace faq {
+namespace pre {
+
+using namespace kvp;
+using pat::ex2;
+using pat::LOWEST;
+using pat::pack_bf16;
+using pat::RAISE;
+
+constexpr int TILE = 128;            // rows of a tile, keys of a key tile
+constexpr int CHUNK = TILE * 128;    // 128 rows of 64 channels
+constexpr int THREADS = 384;
+constexpr int COST = 3;              // of a unit beyond its key tiles (filling, joining), in key tiles
+constexpr int ROWS = 2 * TILE;
+
+struct Segment {  // a run's part of one unit
+  int c0, head, tok0;       // first token of the sequence in q; kv head; first token of the unit
+  int n, len;               // of the sequence
+  int key_row;              // of the sequence's first key in the workspace
+  int k0, count;            // key tiles
+  int slot;                 // -1: the whole unit; else where its partial goes
+  int pad[7];
+};
+struct Join {  // the unit that ends in a run and began in an earlier one
+  int first;  // run, -1: none
+  int c0, head, tok0, n;
+  int pad[3];
+};
+
+struct Params {
+  Pages p;
+  int64_t total;
+  int group, tile_tokens;  // query heads per kv head, whole tokens of a tile
+  int min_rows;            // sequences with fewer rows are not ours
+  float scale_log2;
+  __nv_bfloat16* out;
+  int64_t ot, oh;
+  __nv_bfloat16 *k, *v;    // [cap][kv_heads][d]
+  int64_t cap;             // tokens
+  Segment* segments;       // [runs + units]
+  int2* run;               // [runs]: first segment, segments
+  Join* joins;             // [runs]
+  float* parts;            // [2 runs][ROWS x d + 2 ROWS]
+  int runs;
+  int64_t max_units;
+};
+
+struct Seq {
+  int n, len;  // n = 0: not ours
+};
+__device__ __forceinline__ Seq sequence(const Params& P, int b) {
+  const int c0 = P.p.cu[b], c1 = P.p.cu[b + 1];
+  Seq s;
+  s.n = (c0 >= 0 && c1 > c0 && c1 <= P.total) ? c1 - c0 : 0;
+  s.len = length_of(P.p, b);
+  if (static_cast<int64_t>(s.n) * P.group < P.min_rows) s.n = 0;
+  return s;
+}
+__device__ __forceinline__ int padded(const Seq& s) { return s.n ? (s.len + TILE - 1) / TILE * TILE : 0; }
+// key tiles that unit u of a sequence sees
+__device__ __forceinline__ int key_tiles(const Params& P, const Seq& s, int u) {
+  const int last = min(s.n, (u + 1) * 2 * P.tile_tokens) - 1;
+  const int seen = s.len - s.n + last + 1;
+  return seen <= 0 ? 0 : (seen + TILE - 1) / TILE;
+}
+__device__ __forceinline__ int units_of(const Params& P, const Seq& s) {
+  return (s.n + 2 * P.tile_tokens - 1) / (2 * P.tile_tokens);
+}
+
+// Exclusive prefix of `mine` over the CTA's threads; *sum receives the total.
+template <int WARPS>
+__device__ __forceinline__ int64_t block_scan(int64_t mine, int64_t* scratch, int64_t* sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  int64_t before = x - mine, all = 0;
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += scratch[w];
+    all += scratch[w];
+  }
+  *sum = all;
+  return before;
+}
+
+// ---------------------------------------------------------------- plan
+// One CTA: the segments of every run. Units in the order (sequence, token block, kv head);
+// segment of unit u in run c at index c + u.
+__device__ void make_plan(const Params& P) {
+  __shared__ int64_t s_scratch[8];
+  __shared__ int64_t s_cost, s_units, s_keys;  // before the sequence (and round of units) at hand
+  const int tid = threadIdx.x;
+  const int h = P.p.kv_heads;
+  for (int c = tid; c < P.runs; c += 256) {
+    P.run[c] = make_int2(0x7fffffff, 0);
+    P.joins[c].first = -1;
+  }
+  // totals
+  int64_t cost = 0;
+  for (int b = tid; b < P.p.batch; b += 256) {
+    const Seq s = sequence(P, b);
+    for (int u = 0; u < (s.n ? units_of(P, s) : 0); ++u) {
+      const int kt = key_tiles(P, s, u);
+      cost += kt ? static_cast<int64_t>(kt + COST) * h : 0;
+    }
+  }
+  int64_t total;
+  block_scan<8>(cost, s_scratch, &total);
+  const int64_t per = std::max<int64_t>((total + P.runs - 1) / P.runs, COST + 2);
+  if (tid == 0) s_cost = s_units = s_keys = 0;
+  __syncthreads();
+  for (int b = 0; b < P.p.batch; ++b) {  // every thread the same sequence, units over the threads
+    const Seq s = sequence(P, b);
+    if (s.n == 0) continue;
+    const int nu = units_of(P, s);
+    const int64_t key_row = s_keys;
+    const bool fits = key_row + padded(s) <= P.cap && s_units + static_cast<int64_t>(nu) * h <= P.max_units;
+    if (!fits && tid == 0) atomicOr(&g_status, FAQ_STATUS_BAD_BOUND);
+    for (int u0 = 0; u0 < nu; u0 += 256) {
+      const int u = u0 + tid;
+      const int kt = u < nu && fits ? key_tiles(P, s, u) : 0;
+      int64_t cost_sum, unit_sum;
+      const int64_t at0 = s_cost + block_scan<8>(kt ? static_cast<int64_t>(kt + COST) * h : 0, s_scratch, &cost_sum);
+      const int64_t id0 = s_units + block_scan<8>(kt ? h : 0, s_scratch, &unit_sum);
+      for (int hk = 0; kt && hk < h; ++hk) {
+        const int64_t at = at0 + static_cast<int64_t>(hk) * (kt + COST), first = at + COST, end = first + kt;
+        const int64_t id = id0 + hk;
+        const int r0 = static_cast<int>(first / per), r1 = static_cast<int>((end - 1) / per);
+        for (int c = r0; c <= r1; ++c) {
+          Segment g;
+          g.c0 = P.p.cu[b];
+          g.head = hk;
+          g.tok0 = u * 2 * P.tile_tokens;
+          g.n = s.n;
+          g.len = s.len;
+          g.key_row = static_cast<int>(key_row);
+          g.k0 = static_cast<int>(std::max<int64_t>(c * per - first, 0));
+          g.count = static_cast<int>(std::min<int64_t>((c + 1) * per - first, kt)) - g.k0;
+          g.slot = r0 == r1 ? -1 : 2 * c + (c == r0);
+          P.segments[c + id] = g;
+          atomicMin(&P.run[c].x, static_cast<int>(c + id));  // a run's segments have consecutive indexes
+          atomicAdd(&P.run[c].y, 1);
+        }
+        if (r1 > r0) {
+          Join j;
+          j.first = r0;
+          j.c0 = P.p.cu[b];
+          j.head = hk;
+          j.tok0 = u * 2 * P.tile_tokens;
+          j.n = s.n;
+          P.joins[r1] = j;
+        }
+      }
+      __syncthreads();
+      if (tid == 0) {
+        s_cost += cost_sum;
+        s_units += unit_sum;
+      }
+      __syncthreads();
+    }
+    if (tid == 0) s_keys += padded(s);
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- expand
+// The sixteen tokens of a block of one head, K or V, as bf16 rows of `stride` elements, by one
+// warp: K a quarter row (16 channels of each group) per lane and half, V a sub-block of both
+// tokens of a pair. y = (n - 8) 2^(e - 3) times twice the scale is exact in bf16 (six
+// significant bits), so a pair costs one packed product.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
+  const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
+  return s | (s << 16);
+}
+template <int NG>
+__device__ __forceinline__ void expand_block_k(const Expand& expand, const uint8_t* src, __nv_bfloat16* dst, int64_t stride,
+                                               int from, int to, int lane) {
+  const int t = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+    if (r < from || r >= to) continue;
+    uint32_t w[2 * NG];
+    if constexpr (NG == 2) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * r + 16 * t);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + 32 * r + 8 * t);
+      w[0] = u.x; w[1] = u.y;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t e = *reinterpret_cast<const uint32_t*>(src + exp_offset(NG) + (r * NG + g) * 4);
+      const uint32_t sc = scale_pair(src[scale_offset(NG) + r * NG + g]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
+        uint32_t y[4];
+        expand.word(w[2 * g + i], expand.exponents(e, (7 - 4 * t - 2 * i) & 31), y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], sc);
+        *reinterpret_cast<uint4*>(dst + r * stride + 64 * g + 16 * t + 8 * i) =
+            make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                       __byte_perm(y[2], y[3], 0x7632));
+      }
+    }
+  }
+}
+template <int NG>
+__device__ __forceinline__ void expand_block_v(const Expand& expand, const uint8_t* src, __nv_bfloat16* dst, int64_t stride,
+                                               int from, int to, int lane) {
+  const int s = lane & 7;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int p = (lane >> 3) + 4 * h;  // tokens 2 p, 2 p + 1
+    if (2 * p + 1 < from || 2 * p >= to) continue;
+    uint32_t w[2 * NG], e[2 * NG];
+    if constexpr (NG == 2) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + 128 * p + 16 * (s ^ (2 * (p & 3))));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+      const uint4 x = *reinterpret_cast<const uint4*>(src + exp_offset(NG) + 16 * p);
+      e[0] = x.x; e[1] = x.y; e[2] = x.z; e[3] = x.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + 64 * p + 8 * (s ^ (2 * (p & 3))));
+      w[0] = u.x; w[1] = u.y;
+      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * p);
+      e[0] = x.x; e[1] = x.y;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t s0 = scale_pair(src[scale_offset(NG) + 2 * p * NG + g]);
+      const uint32_t s1 = scale_pair(src[scale_offset(NG) + (2 * p + 1) * NG + g]);
+      const uint32_t sc = __byte_perm(s0, s1, 0x5410);
+      uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        expand.word(w[2 * g + q], expand.exponents(e[2 * g + q], (7 - 2 * s) & 31), y[q]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], sc);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t sel = k ? 0x7632 : 0x5410;
+        if (2 * p + k >= from && 2 * p + k < to)
+          *reinterpret_cast<uint4*>(dst + (2 * p + k) * stride + 64 * g + 8 * s) =
+              make_uint4(__byte_perm(y[0][0], y[0][1], sel), __byte_perm(y[0][2], y[0][3], sel),
+                         __byte_perm(y[1][0], y[1][1], sel), __byte_perm(y[1][2], y[1][3], sel));
+      }
+    }
+  }
+}
+
+// Work items: (key tile of 128 tokens, kv head), a block of 16 tokens per warp. The last CTA
+// makes the plan.
+template <int NG>
+__global__ void __launch_bounds__(256) paged_expand_kernel(Params P) {
+  constexpr int D = 64 * NG;
+  grid_dependency_wait();
+  allow_dependent_launch();
+  if (blockIdx.x == gridDim.x - 1) {
+    make_plan(P);
+    return;
+  }
+  __shared__ int64_t s_scratch[8];
+  __shared__ int64_t s_tiles[257];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = P.p.kv_heads, ctas = gridDim.x - 1;
+  const Expand expand;
+  int64_t base = 0, next = blockIdx.x;  // tiles before these sequences; this CTA's next item
+  for (int b0 = 0; b0 < P.p.batch; b0 += 256) {
+    Seq mine = {0, 0};
+    if (b0 + tid < P.p.batch) mine = sequence(P, b0 + tid);
+    int64_t sum;
+    const int64_t before = block_scan<8>(padded(mine) / TILE, s_scratch, &sum);
+    __syncthreads();
+    s_tiles[tid] = before;
+    if (tid == 0) s_tiles[256] = sum;
+    __syncthreads();
+    for (; next < (base + sum) * h; next += ctas) {
+      const int64_t q = next / h - base;
+      const int head = static_cast<int>(next % h);
+      int lo = 0, hi = 256;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_tiles[mid] <= q) lo = mid; else hi = mid;
+      }
+      const int b = b0 + lo;
+      const Seq s = sequence(P, b);
+      const int pos = static_cast<int>(q - s_tiles[lo]) * TILE + warp * BLOCK;
+      const int64_t row = (base + q) * TILE + warp * BLOCK;
+      if (row + BLOCK > P.cap) continue;  // recorded by the plan
+      const int64_t page = pos < s.len ? page_of(P.p, b, pos) : -1;
+      const int have = page < 0 ? 0 : min(BLOCK, s.len - pos);
+      const int64_t stride = static_cast<int64_t>(h) * D;
+      __nv_bfloat16* k = P.k + row * stride + head * D;
+      __nv_bfloat16* v = P.v + row * stride + head * D;
+      if (have) {
+        const uint8_t* unit = P.p.base + page * P.p.page_stride;
+        expand_block_k<NG>(expand, unit + block_in_page<NG>(P.p, 0, head, pos), k, stride, 0, have, lane);
+        expand_block_v<NG>(expand, unit + block_in_page<NG>(P.p, 1, head, pos), v, stride, 0, have, lane);
+      }
+      for (int i = have * (D / 8) + lane; i < BLOCK * (D / 8); i += 32) {  // zeros behind the end
+        *reinterpret_cast<uint4*>(k + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(v + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    base += sum;
+    // rows of these sequences that see no key are zero
+    for (int i = 0; i < 256 && b0 + i < P.p.batch; ++i) {
+      if ((b0 + i) % ctas != blockIdx.x) continue;
+      const Seq s = sequence(P, b0 + i);
+      const int none = min(s.n, s.n - s.len), heads = P.group * h;
+      for (int64_t x = tid; x < static_cast<int64_t>(none) * heads * (D / 8); x += 256) {
+        const int64_t r = x / (D / 8);
+        *reinterpret_cast<uint4*>(P.out + (P.p.cu[b0 + i] + r / heads) * P.ot + (r % heads) * P.oh + x % (D / 8) * 8) =
+            make_uint4(0, 0, 0, 0);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- attention
+template <int NG>
+struct Smem {
+  static constexpr int tile = NG * CHUNK;  // bytes of a Q, K or V tile
+  static constexpr int q = 0;
+  static constexpr int k = q + 2 * tile;
+  static constexpr int v = k + 2 * tile;
+  static constexpr int bar = v + 2 * tile;
+  static constexpr int bytes = 1024 + bar + 256;
+};
+constexpr int TMEM_COLS = 512;
+__device__ __forceinline__ uint32_t s_col(int t) { return 128u * t; }        // S_t, then P_t in its first 64
+__device__ __forceinline__ uint32_t o_col(int t) { return 256u + 128u * t; }
+constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, TILE, false, false);
+constexpr uint32_t idesc_pv(int d) { return idesc_bf16_f32(TILE, d, false, true); }
+
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+template <int NG>
+__global__ void __launch_bounds__(THREADS, 1)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                         const __grid_constant__ CUtensorMap tmap_v, Params P) {
+  using L = Smem<NG>;
+  constexpr int D = 64 * NG;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::bar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;   // [2 stages]
+  uint64_t* k_empty = bars + 4;  // both tiles' products have read the stage
+  uint64_t* v_full = bars + 6;
+  uint64_t* v_empty = bars + 8;
+  uint64_t* s_full = bars + 10;  // [2 tiles] S_t computed
+  uint64_t* p_full = bars + 12;  // P_t written (and O_t rescaled) by the tile's four warps
+  uint64_t* pv_done = bars + 14; // O_t += P_t V completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_addr(q_full), 1);
+    mbar_init(smem_addr(q_empty), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&k_full[i]), 1);
+      mbar_init(smem_addr(&k_empty[i]), 2);
+      mbar_init(smem_addr(&v_full[i]), 1);
+      mbar_init(smem_addr(&v_empty[i]), 2);
+      mbar_init(smem_addr(&s_full[i]), 1);
+      mbar_init(smem_addr(&p_full[i]), 4);
+      mbar_init(smem_addr(&pv_done[i]), 1);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 10) {
+    tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const int2 run = P.run[blockIdx.x];
+  const Segment* segments = P.segments + run.x;
+  const int nseg = run.y;
+  // whether tile B has rows
+  auto two_tiles = [&](const Segment& g) { return g.tok0 + P.tile_tokens < g.n; };
+
+  // Registers: 384 x 168 at launch = 256 x 208 + 128 x 88.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::: "memory");
+    if (warp == 8) {
+      if (lane == 0) {
+        bool ok = true;
+        int step = 0;
+        const uint32_t q_bytes = static_cast<uint32_t>(P.group * P.tile_tokens) * 128;
+        for (int i = 0; i < nseg && ok; ++i) {
+          const Segment g = segments[i];
+          const int tiles = two_tiles(g) ? 2 : 1;
+          if (i > 0 && !mbar_wait_site(smem_addr(q_empty), (i - 1) & 1, 50, i)) break;
+          mbar_arrive_expect_tx(smem_addr(q_full), tiles * NG * q_bytes);
+          for (int t = 0; t < tiles; ++t)
+            for (int c = 0; c < NG; ++c)
+              tma_load_3d(smem_addr(base + L::q + t * L::tile + c * CHUNK), &tmap_q, smem_addr(q_full), c * 64,
+                          g.head * P.group, g.c0 + g.tok0 + t * P.tile_tokens);
+          for (int j = 0; j < g.count; ++j, ++step) {
+            const int st = step & 1;
+            if (!mbar_wait_site(smem_addr(&k_empty[st]), ((step >> 1) & 1) ^ 1, 51, step)) { ok = false; break; }
+            mbar_arrive_expect_tx(smem_addr(&k_full[st]), L::tile);
+            for (int c = 0; c < NG; ++c)
+              tma_load_3d(smem_addr(base + L::k + st * L::tile + c * CHUNK), &tmap_k, smem_addr(&k_full[st]), c * 64,
+                          g.head, g.key_row + (g.k0 + j) * TILE);
+          }
+        }
+        // drain (bounded): the last loads were consumed before the CTA exits
+        for (int x = std::max(0, step - 2); x < step; ++x)
+          if (!mbar_wait_site(smem_addr(&k_empty[x & 1]), (x >> 1) & 1, 53, x)) break;
+      }
+    } else if (warp == 9) {
+      if (lane == 0) {
+        bool ok = true;
+        int step = 0;
+        for (int i = 0; i < nseg && ok; ++i) {
+          const Segment g = segments[i];
+          for (int j = 0; j < g.count; ++j, ++step) {
+            const int st = step & 1;
+            if (!mbar_wait_site(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 52, step)) { ok = false; break; }
+            mbar_arrive_expect_tx(smem_addr(&v_full[st]), L::tile);
+            for (int c = 0; c < NG; ++c)
+              tma_load_3d(smem_addr(base + L::v + st * L::tile + c * CHUNK), &tmap_v, smem_addr(&v_full[st]), c * 64,
+                          g.head, g.key_row + (g.k0 + j) * TILE);
+          }
+        }
+        for (int x = std::max(0, step - 2); x < step; ++x)
+          if (!mbar_wait_site(smem_addr(&v_empty[x & 1]), (x >> 1) & 1, 54, x)) break;
+      }
+    } else if (warp == 10) {
+      if (lane == 0) {
+        const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
+        const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
+        const uint32_t v_desc = sw128_desc_lo(smem_addr(base + L::v), CHUNK);
+        constexpr uint32_t TILE_D = L::tile >> 4;
+        int ring = 0;                // key tiles before this segment
+        uint32_t done[2] = {0, 0};   // steps of each tile so far
+        bool ok = true;
+        for (int i = 0; i < nseg && ok; ++i) {
+          const int n = segments[i].count;
+          const int tiles = two_tiles(segments[i]) ? 2 : 1;
+          if (!mbar_wait_site(smem_addr(q_full), i & 1, 55, i)) break;
+          int qk[2] = {0, 0}, pv[2] = {0, 0};  // issued
+          bool q_read = false;
+          uint64_t since = 0;
+          uint32_t misses = 0;
+          while (pv[0] < n || (tiles == 2 && pv[1] < n)) {
+            bool moved = false;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (t >= tiles) continue;
+              if (qk[t] == pv[t] && qk[t] < n) {  // S_t = Q_t K^T: over P_t, once its product is done
+                const int step = ring + qk[t], st = step & 1;
+                if (mbar_test(smem_addr(&k_full[st]), (step >> 1) & 1) &&
+                    (done[t] == 0 || mbar_test(smem_addr(&pv_done[t]), (done[t] - 1) & 1))) {
+                  tc_fence_after();
+                  const uint32_t a = q_desc + t * TILE_D, b = k_desc + st * TILE_D, d = tmem + s_col(t);
+#pragma unroll
+                  for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
+                    tc_mma_f16_lo(d, a + off, b + off, IDESC_QK, kk != 0);
+                  }
+                  tc_commit(smem_addr(&s_full[t]));
+                  tc_commit(smem_addr(&k_empty[st]));
+                  if (tiles == 1) tc_commit(smem_addr(&k_empty[st]));  // for the tile that is not there
+                  ++qk[t];
+                  moved = true;
+                }
+              } else if (qk[t] > pv[t]) {  // O_t += P_t V
+                const int step = ring + pv[t], st = step & 1;
+                if (mbar_test(smem_addr(&p_full[t]), done[t] & 1) && mbar_test(smem_addr(&v_full[st]), (step >> 1) & 1)) {
+                  tc_fence_after();
+                  const uint32_t b = v_desc + st * TILE_D, d = tmem + o_col(t), a = tmem + s_col(t);
+#pragma unroll
+                  for (int kk = 0; kk < TILE / 16; ++kk)
+                    tc_mma_f16_ts_lo(d, a + kk * 8, b + ((kk * 2048) >> 4), idesc_pv(D), (pv[t] | kk) != 0);
+                  tc_commit(smem_addr(&pv_done[t]));
+                  tc_commit(smem_addr(&v_empty[st]));
+                  if (tiles == 1) tc_commit(smem_addr(&v_empty[st]));
+                  ++pv[t];
+                  ++done[t];
+                  moved = true;
+                }
+              }
+            }
+            if (!q_read && qk[0] == n && (tiles == 1 || qk[1] == n)) {
+              tc_commit(smem_addr(q_empty));  // the next unit's Q may come
+              q_read = true;
+            }
+            if (moved) {
+              misses = 0;
+            } else if (++misses == 256) {
+              since = globaltimer();
+            } else if ((misses & 255) == 0 && globaltimer() - since > kWaitLimitNs) {
+              report_timeout();
+              trace_timeout(56, ring + pv[0]);
+              ok = false;
+              break;
+            }
+          }
+          ring += n;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::: "memory");
+    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + s_col(t), o_addr = tmem + lanes + o_col(t);
+    const float2 c2 = make_float2(P.scale_log2, P.scale_log2);
+    const int row_tok = row / P.group, row_head = row - row_tok * P.group;
+    uint32_t done = 0;  // steps of this tile so far
+    bool ok = true;
+    for (int i = 0; i < nseg && ok; ++i) {
+      const Segment g = segments[i];
+      if (t == 1 && !two_tiles(g)) continue;
+      const int tok = g.tok0 + t * P.tile_tokens + row_tok;
+      const bool live = row_tok < P.tile_tokens && tok < g.n;
+      const int lim = live ? g.len - g.n + tok : 0x7fffffff;  // last visible key; rows that are not there see all
+      float m = LOWEST, l = 0.0f;
+      for (int j = 0; j < g.count; ++j, ++done) {
+        if (!mbar_wait_warp(smem_addr(&s_full[t]), done & 1, 57 + t, j)) { ok = false; break; }
+        tc_fence_after();
+        float f[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32f(s_addr + 32 * c, f + 32 * c);
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) reg_fence32f(f + 32 * c);
+        const int rel = lim - (g.k0 + j) * TILE;
+        if (__any_sync(0xffffffffu, rel < TILE - 1)) {
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x > rel) f[x] = -INFINITY;
+        }
+        float mx[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          mx[c] = fmaxf(f[16 * c], f[16 * c + 1]);
+#pragma unroll
+          for (int x = 2; x < 16; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
+        }
+        const float top = __fmul_rn(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])),
+                                    P.scale_log2);
+        if (__any_sync(0xffffffffu, top > m + RAISE)) {
+          const float next = fmaxf(top, m);
+          const float a = ex2(m - next);
+          m = next;
+          l *= a;
+          if (j > 0) {  // O_t of the steps before is complete, then rescaled
+            if (!mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 59 + t, j)) { ok = false; break; }
+            tc_fence_after();
+            const float2 a2 = make_float2(a, a);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32f(o_addr + 32 * c, o);
+              tc_wait_ld();
+              reg_fence32f(o);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
+                o[2 * x] = v.x;
+                o[2 * x + 1] = v.y;
+              }
+              tmem_st32f(o_addr + 32 * c, o);
+            }
+          }
+        }
+        const float2 mneg = make_float2(-m, -m);
+        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float w[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const float2 d = __ffma2_rn(make_float2(f[64 * c + 2 * x], f[64 * c + 2 * x + 1]), c2, mneg);
+            const float2 e = make_float2(ex2(d.x), ex2(d.y));
+            sum[x & 3] = __fadd2_rn(sum[x & 3], e);
+            w[x] = __uint_as_float(pack_bf16(e.x, e.y));
+          }
+          tmem_st32f(s_addr + 32 * c, w);
+        }
+        const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+        l += s4.x + s4.y;
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&p_full[t]));
+      }
+      if (!ok || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) { ok = false; break; }
+      tc_fence_after();
+      const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
+      float* part = g.slot < 0 ? nullptr : P.parts + static_cast<int64_t>(g.slot) * (ROWS * D + 2 * ROWS);
+      __nv_bfloat16* dst = P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        tmem_ld32f(o_addr + 32 * c, o);
+        tc_wait_ld();
+        reg_fence32f(o);
+        if (live && part) {
+          float4* d4 = reinterpret_cast<float4*>(part + (t * TILE + row) * D + 32 * c);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) d4[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        } else if (live) {
+          uint4* d4 = reinterpret_cast<uint4*>(dst + 32 * c);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            d4[x] = make_uint4(pack_bf16(o[8 * x] * inv, o[8 * x + 1] * inv), pack_bf16(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                               pack_bf16(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                               pack_bf16(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+        }
+        __syncwarp();  // the loads above are made by whole warps
+      }
+      if (part && live) {
+        part[ROWS * D + t * TILE + row] = m;
+        part[ROWS * D + ROWS + t * TILE + row] = l;
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Joins the partials of the unit that ended in run blockIdx.x, a warp per row, in run order.
+template <int D>
+__global__ void __launch_bounds__(256) prefill_combine_kernel(Params P) {
+  constexpr int V = D / 32;
+  constexpr int64_t SIZE = ROWS * D + 2 * ROWS;
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const Join j = P.joins[blockIdx.x];
+  if (j.first < 0) return;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = r / TILE, in_tile = r % TILE, tok_in = in_tile / P.group;
+  const int tok = j.tok0 + t * P.tile_tokens + tok_in;
+  if (tok_in >= P.tile_tokens || tok >= j.n) return;
+  float sum[V], den = 0.0f, top = LOWEST;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+  for (int c = j.first; c <= static_cast<int>(blockIdx.x); ++c) {
+    const float* src = P.parts + (2 * static_cast<int64_t>(c) + (c == j.first)) * SIZE;
+    const float m = src[ROWS * D + r], l = src[ROWS * D + ROWS + r];
+    const float next = fmaxf(top, m), f = ex2(top - next), e = ex2(m - next);
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f + src[r * D + lane * V + i] * e;
+    den = den * f + l * e;
+    top = next;
+  }
+  const float inv = den > 0.0f ? __fdiv_rn(1.0f, den) : (den == 0.0f ? 0.0f : den);
+  __nv_bfloat16* dst = P.out + static_cast<int64_t>(j.c0 + tok) * P.ot +
+                       (j.head * P.group + in_tile - tok_in * P.group) * P.oh + lane * V;
+#pragma unroll
+  for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16(sum[i] * inv, sum[i + 1] * inv);
+}
+
+// Sections of the workspace, each 256-byte aligned.
+struct Layout {
+  int64_t cap, max_units;
+  size_t k, v, segments, run, joins, parts, bytes;
+};
+inline Layout layout(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch, int64_t max_len, int64_t total_len,
+                     int min_rows, int d) {
+  const int64_t group = heads / kv_heads, tokens = TILE / group;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  Layout a;
+  // sequences that can have min_rows rows, and the keys they can have
+  const int64_t most = std::min<int64_t>(batch, total * group / min_rows);
+  const int64_t len = (max_len + TILE - 1) / TILE * TILE;
+  a.cap = std::min(most * len, total_len + most * TILE);
+  a.cap = std::max<int64_t>((a.cap + TILE - 1) / TILE * TILE, TILE);
+  a.max_units = kv_heads * (total / (2 * tokens) + most);
+  const int runs = num_sms();
+  a.k = 0;
+  a.v = a.k + up(static_cast<size_t>(a.cap) * kv_heads * d * 2);
+  a.segments = a.v + up(static_cast<size_t>(a.cap) * kv_heads * d * 2);
+  a.run = a.segments + up(static_cast<size_t>(a.max_units + runs) * sizeof(Segment));
+  a.joins = a.run + up(runs * sizeof(int2));
+  a.parts = a.joins + up(runs * sizeof(Join));
+  a.bytes = a.parts + up(static_cast<size_t>(2) * runs * (ROWS * d + 2 * ROWS) * 4);
+  return a;
+}
+
+template <int NG>
+static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, int64_t qh, const Layout& a, char* ws,
+                  void* stream) {
+  constexpr int D = 64 * NG;
+  P.k = reinterpret_cast<__nv_bfloat16*>(ws + a.k);
+  P.v = reinterpret_cast<__nv_bfloat16*>(ws + a.v);
+  P.cap = a.cap;
+  P.max_units = a.max_units;
+  P.segments = reinterpret_cast<Segment*>(ws + a.segments);
+  P.run = reinterpret_cast<int2*>(ws + a.run);
+  P.joins = reinterpret_cast<Join*>(ws + a.joins);
+  P.parts = reinterpret_cast<float*>(ws + a.parts);
+  P.runs = num_sms();
+  CUtensorMap mq, mk, mv;
+  {
+    const uint64_t dims[3] = {D, static_cast<uint64_t>(heads), static_cast<uint64_t>(P.total)};
+    const uint64_t str[2] = {static_cast<uint64_t>(qh) * 2, static_cast<uint64_t>(qt) * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(P.tile_tokens)};
+    const int rc = make_tmap(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  const uint64_t dims[3] = {D, static_cast<uint64_t>(P.p.kv_heads), static_cast<uint64_t>(P.cap)};
+  const uint64_t str[2] = {D * 2, static_cast<uint64_t>(P.p.kv_heads) * D * 2};
+  const uint32_t box[3] = {64, 1, TILE};
+  int rc = make_tmap(&mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.k, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = make_tmap(&mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.v, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  auto kern = paged_prefill_kernel<NG>;
+  static std::atomic<uint64_t> set{0};
+  rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
+  if (rc) return rc;
+  const int64_t items = P.cap / TILE * P.p.kv_heads;
+  const unsigned ctas = static_cast<unsigned>(std::min<int64_t>(items, num_sms() * 6)) + 1;
+  FAQ_CUDA(launch_early(paged_expand_kernel<NG>, dim3(ctas), 256, 0, stream, P));
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(P.runs)), THREADS, Smem<NG>::bytes, stream, mq, mk, mv, P));
+  FAQ_CUDA(launch_early(prefill_combine_kernel<D>, dim3(static_cast<unsigned>(P.runs), ROWS / 8), 256, 0, stream, P));
+  return FAQ_OK;
+}
+
+}  // namespace pre
+}  // namespace faq
+
+namespace faq {
+namespace pre {
+// From this many rows (new tokens x query heads of a kv head) a sequence is the prompt kernel's.
+constexpr int MIN_ROWS = 65;
+// Whether a call may have such a sequence, and whether all of its sequences are.
+inline bool any_prompt(int64_t group, int64_t max_new, int64_t total) {
+  return group <= TILE && group * std::min(max_new, total) >= MIN_ROWS;
+}
+inline bool all_prompts(int64_t group, int64_t max_new, int64_t total, int64_t batch) {
+  return any_prompt(group, max_new, total) && total == batch * max_new;
+}
+}  // namespace pre
+}  // namespace faq
+
+extern "C" size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch,
+                                                           int64_t max_new, int64_t max_len, int64_t total_len, int d) {
+  using namespace faq;
+  if (total < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || batch <= 0 || max_new < 0 || max_len < 0 ||
+      total_len < 0 || (d != 64 && d != 128))
+    return 0;
+  const int64_t group = heads / kv_heads;
+  const size_t few = pat::workspace(pat::n_blocks(std::min<int64_t>(max_new, 4096) * group), d);
+  if (!pre::any_prompt(group, max_new, total)) return few;
+  return std::max(few, pre::layout(total, heads, kv_heads, batch, max_len, total_len, pre::MIN_ROWS, d).bytes);
+}
+
+extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride,
+                                        int64_t q_head_stride, const void* pages, int64_t num_pages,
+                                        int64_t page_stride, int page_size, int64_t kv_heads, int d,
+                                        const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
+                                        const int32_t* lens, int64_t batch, int64_t max_new, int64_t max_len,
+                                        int64_t total_len, float scale, void* out, int64_t out_token_stride,
+                                        int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace faq;
+  kvp::Pages pages_;
+  int rc = kvp::make_pages(pages_, pages, num_pages, page_stride, page_size, kv_heads, d, table, table_ld, table_cols, cu,
+                           lens, batch);
+  if (rc) return rc;
+  FAQ_CHECK_ARG(heads > 0 && heads % kv_heads == 0, "query heads must be divisible by key/value heads");
+  const int64_t group = heads / kv_heads;
+  FAQ_CHECK_ARG(group < 4096, "more than 4095 query heads per key/value head");
+  FAQ_CHECK_ARG(total >= 0 && max_new >= 0 && max_len >= 0 && total_len >= 0 && total * heads < (int64_t(1) << 31) &&
+                    max_len < (int64_t(1) << 31) && total_len < (int64_t(1) << 40), "bad token count");
+  if (total == 0) return FAQ_OK;
+  FAQ_CHECK_ARG(q && out, "null pointer");
+  FAQ_CHECK_ARG(scale > 0.0f && scale < 3.0e38f, "scale must be positive and finite");
+  FAQ_CHECK_ARG(aligned16(q) && aligned16(out) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+                    out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
+                "q and out must be 16-byte aligned with strides multiple of 8");
+  FAQ_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+                "workspace must be a 256-byte aligned device buffer");
+  FAQ_CHECK_ARG(workspace_bytes >= faq_hif4_paged_attention_workspace_bytes(total, heads, kv_heads, batch, max_new, max_len,
+                                                                            total_len, d),
+                "workspace too small: faq_hif4_paged_attention_workspace_bytes() bytes needed");
+  const float scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  const bool prompts = pre::any_prompt(group, max_new, total);
+  if (!prompts || !pre::all_prompts(group, max_new, total, batch)) {
+    pat::Params P;
+    P.p = pages_;
+    P.q = static_cast<const __nv_bfloat16*>(q);
+    P.qt = q_token_stride;
+    P.qh = q_head_stride;
+    P.out = static_cast<__nv_bfloat16*>(out);
+    P.ot = out_token_stride;
+    P.oh = out_head_stride;
+    P.total = total;
+    P.max_rows = prompts ? pre::MIN_ROWS - 1 : 0x7fffffff;
+    P.group = static_cast<int>(group);
+    P.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + group - 1) / group);
+    P.scale_log2 = scale_log2;
+    const int nb = pat::n_blocks(std::min<int64_t>(max_new, 4096) * group);
+    if (d == 64)
+      rc = nb == 1 ? pat::launch<1, 1>(P, workspace, stream) : nb == 2 ? pat::launch<1, 2>(P, workspace, stream)
+                                                                       : pat::launch<1, 4>(P, workspace, stream);
+    else
+      rc = nb == 1 ? pat::launch<2, 1>(P, workspace, stream) : nb == 2 ? pat::launch<2, 2>(P, workspace, stream)
+                                                                       : pat::launch<2, 4>(P, workspace, stream);
+    if (rc || !prompts) return rc;
+  }
+  pre::Params P;
+  P.p = pages_;
+  P.total = total;
+  P.group = static_cast<int>(group);
+  P.tile_tokens = static_cast<int>(pre::TILE / group);
+  P.min_rows = pre::MIN_ROWS;
+  P.scale_log2 = scale_log2;
+  P.out = static_cast<__nv_bfloat16*>(out);
+  P.ot = out_token_stride;
+  P.oh = out_head_stride;
+  const pre::Layout a = pre::layout(total, heads, kv_heads, batch, max_len, total_len, pre::MIN_ROWS, d);
+  return d == 64 ? pre::launch<1>(P, static_cast<const __nv_bfloat16*>(q), heads, q_token_stride, q_head_stride, a,
+                                  static_cast<char*>(workspace), stream)
+                 : pre::launch<2>(P, static_cast<const __nv_bfloat16*>(q), heads, q_token_stride, q_head_stride, a,
+                                  static_cast<char*>(workspace), stream);
+}

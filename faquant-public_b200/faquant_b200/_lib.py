@@ -18,6 +18,7 @@ FAQ_BF16 = 0
 FAQ_F32 = 1
 FAQ_STATUS_TIMEOUT = 1
 FAQ_STATUS_BAD_PAGE = 2
+FAQ_STATUS_BAD_BOUND = 4
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -77,7 +78,7 @@ SIGNATURES: dict[str, list] = {
     "faq_hif4_kv_read": [_c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
                          _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _i64, _c_void_p],
     "faq_hif4_paged_attention": [_c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p,
-                                 _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _i64,
+                                 _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _i64,
                                  _i64, _c_void_p, ctypes.c_size_t, _c_void_p],
     "faq_verify_drafts": [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p,
                           _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
@@ -112,7 +113,7 @@ def load() -> ctypes.CDLL:
             # size queries return size_t, not a status
             lib.faq_hif4_decode_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64, _i64, _int]
             lib.faq_hif4_decode_workspace_bytes.restype = ctypes.c_size_t
-            lib.faq_hif4_paged_attention_workspace_bytes.argtypes = [_i64, _i64, _i64, _int]
+            lib.faq_hif4_paged_attention_workspace_bytes.argtypes = [_i64] * 7 + [_int]
             lib.faq_hif4_paged_attention_workspace_bytes.restype = ctypes.c_size_t
             _lib = lib
         return _lib

@@ -779,6 +779,7 @@ def hif4_paged_attention(
     page_size: int,
     max_new: int,
     max_len: int | None = None,
+    total_len: int | None = None,
     scale: float | None = None,
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
@@ -788,9 +789,11 @@ def hif4_paged_attention(
     as in :func:`hif4_kv_write`, which must have written the tokens before: new token i of
     n sees the keys ``0 .. lens - n + i``, query head h those of kv head ``h // (H / Hkv)``.
 
-    ``max_new`` and ``max_len`` (the table's capacity by default) bound the sequences' new
-    tokens and lengths from above; they are host numbers, so nothing is copied from the
-    device. ``workspace``: a device buffer to use instead of a new one."""
+    ``max_new``, ``max_len`` (the table's capacity by default) and ``total_len`` (batch x
+    ``max_len`` by default) bound the sequences' new tokens, their lengths and the sum of
+    the lengths from above; they are host numbers, so nothing is copied from the device, and
+    with prompt chunks in the batch they size the workspace. ``workspace``: a 256-byte
+    aligned device buffer to use instead of a new one."""
     device = _require_cuda(q, pages, table, cu, lens)
     if q.dtype != torch.bfloat16 or q.dim() != 3:
         raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
@@ -807,12 +810,15 @@ def hif4_paged_attention(
         raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
     if max_len is None:
         max_len = table.shape[1] * page_size
-    need = int(_lib.load().faq_hif4_paged_attention_workspace_bytes(heads, h, max_new, d))
+    batch = table.shape[0]
+    if total_len is None:
+        total_len = batch * max_len
+    need = int(_lib.load().faq_hif4_paged_attention_workspace_bytes(total, heads, h, batch, max_new, max_len, total_len, d))
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, q.stride(0), q.stride(1), pages.data_ptr(),
               pages.shape[0], pages.stride(0), page_size, h, d, table.data_ptr(), table.stride(0), table.shape[1],
-              cu.data_ptr(), lens.data_ptr(), table.shape[0], max_new, max_len,
+              cu.data_ptr(), lens.data_ptr(), batch, max_new, max_len, total_len,
               float(scale if scale is not None else d**-0.5), out.data_ptr(), out.stride(0), out.stride(1),
               workspace.data_ptr(), need, _stream(device))
     return out

@@ -46,7 +46,8 @@ extern "C" {
 
 /* device status word bits */
 #define FAQ_STATUS_TIMEOUT 1u
-#define FAQ_STATUS_BAD_PAGE 2u /* a page table entry or a length outside the pool or the table */
+#define FAQ_STATUS_BAD_PAGE 2u  /* a page table entry or a length outside the pool or the table */
+#define FAQ_STATUS_BAD_BOUND 4u /* a ragged batch beyond the bounds the host gave (max_len, total_len) */
 
 /* element types */
 #define FAQ_BF16 0
@@ -397,7 +398,8 @@ int faq_gptq_hif4_block(const float* w, int64_t ldw, int64_t rows, int cols, int
  * nothing). `table` int32 [batch, table_cols] (row stride table_ld) holds the page of tokens
  * c * page_size .. of each sequence in column c; entries past a sequence's length are not
  * read. An entry outside 0 .. num_pages - 1, or a length beyond the table's columns, sets
- * FAQ_STATUS_BAD_PAGE in the device status word and leaves those tokens out.
+ * FAQ_STATUS_BAD_PAGE in the device status word: those tokens are not written and read as
+ * zeros, and the attention of that sequence is not defined.
  *
  * Page format (d = 64 NG channels, NG 1 or 2): `pages` uint8, page p at p * page_stride
  * bytes (a multiple of 16; layers may interleave): [2: K, V][kv_heads][page_size / 16]
@@ -440,17 +442,21 @@ int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t page_stride, 
  * bf16 for the products with V, fp32 accumulation; P is not quantized (faq_hif4_attention
  * and faq_hif4_decode_attention keep the reference's HiF4 P). A row without a key is
  * zero. Covers one decode step, chunks of drafted tokens and prompt chunks in one batch.
- * max_new and max_len are upper bounds on the sequences' new tokens and lengths, known on
- * the host (they choose the kernel and its workspace; nothing is copied from the device).
- * `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * max_new, max_len and total_len are upper bounds on the sequences' new tokens, their lengths
+ * and the sum of the lengths, known on the host (nothing is copied from the device): they
+ * choose the kernels and size the workspace, which for sequences of 65 or more rows (new
+ * tokens x query heads of a kv head) also holds the keys and values of those in bf16. A batch
+ * beyond max_len or total_len sets FAQ_STATUS_BAD_BOUND and leaves those sequences' rows as
+ * they are. `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 256-byte
  * aligned, not initialized.
  */
-size_t faq_hif4_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t max_new, int d);
+size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch,
+                                                int64_t max_new, int64_t max_len, int64_t total_len, int d);
 int faq_hif4_paged_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
                              const void* pages, int64_t num_pages, int64_t page_stride, int page_size,
                              int64_t kv_heads, int d, const int32_t* table, int64_t table_ld, int64_t table_cols,
                              const int32_t* cu, const int32_t* lens, int64_t batch, int64_t max_new, int64_t max_len,
-                             float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                             int64_t total_len, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
                              void* workspace, size_t workspace_bytes, void* stream);
 
 /*

@@ -177,6 +177,15 @@ SHAPES = [  # heads, kv_heads, d, page_size, lens, new
     (12, 4, 128, 16, [130], [130]),
     (24, 2, 128, 256, [700, 20], [40, 20]),
     (3, 3, 128, 16, [0, 0, 9], [0, 0, 1]),
+    # from 65 rows (tokens x query heads of a kv head) a sequence is the prompt kernel's
+    (4, 1, 128, 16, [17], [17]),
+    (4, 1, 128, 16, [200, 16, 17], [17, 16, 16]),
+    (8, 8, 128, 64, [65, 128, 129, 300], [65, 128, 129, 256]),
+    (10, 2, 128, 16, [400, 1, 90], [150, 1, 90]),
+    (14, 2, 64, 32, [300, 80], [60, 11]),
+    (32, 2, 64, 16, [513, 0, 40], [9, 0, 40]),
+    (128, 1, 128, 16, [70], [3]),
+    (48, 2, 128, 128, [1300], [45]),
 ]
 
 
@@ -193,7 +202,7 @@ def test_attention_matches_fp64(shape) -> None:
     _no_status()
 
 
-@pytest.mark.parametrize("n", [1, 2, 4, 9, 40])
+@pytest.mark.parametrize("n", [1, 2, 4, 9, 40, 150])
 def test_rows_without_a_key_are_zero(n) -> None:
     """More new tokens than the sequence holds: the first have no position."""
     lens, new = [max(1, n // 2), 0, 300], [n, n, n]
@@ -309,6 +318,55 @@ def test_captured_in_a_graph_with_growing_lengths() -> None:
         graph.replay()
         torch.cuda.synchronize()
         _close(out, [n], [1], q, quantized(k[:n]), quantized(v[:n]))
+
+
+def test_prompt_kernel_over_many_runs_and_its_ranges() -> None:
+    """A chunk whose units are cut over many CTAs, one query row far above the others, values
+    of very different sizes; strided q; the same bits again."""
+    lens, new = [5000, 260], [70, 200]
+    pool = Pool(lens, 1, 128, 64, DEV)
+    k, v = _randn(sum(lens), 1, 128, seed=60), _randn(sum(lens), 1, 128, seed=61)
+    k[4000] *= 30.0
+    v[3] *= 1e6
+    pool.write(k, v)
+    wide = _randn(sum(new), 3, 2, 136, seed=62)
+    q = wide[:, 1, :, :128]
+    q[20] *= 8.0
+    q[21] = 0
+    out = pool.attend(q, new)
+    _close(out, lens, new, q, quantized(k), quantized(v))
+    assert all(torch.equal(out, pool.attend(q, new, total_len=sum(lens))) for _ in range(3))
+    _no_status()
+
+
+def test_prompt_kernel_keeps_not_a_number_in_its_row() -> None:
+    pool = Pool([300], 2, 128, 16, DEV, fill=0xFF)
+    k, v = _randn(300, 2, 128, seed=63), _randn(300, 2, 128, seed=64)
+    pool.write(k, v)
+    q = _randn(90, 4, 128, seed=65)
+    good = pool.attend(q, [90])
+    q[12, 3, 17] = float("nan")
+    q[40, 0, 0] = float("inf")
+    out = pool.attend(q, [90])
+    assert out[12, 3].isnan().all() and out[40, 0].isnan().any()
+    out[12, 3], out[40, 0] = good[12, 3], good[40, 0]
+    assert torch.equal(out, good)
+
+
+def test_batches_beyond_their_bounds_are_reported() -> None:
+    from faquant_b200 import _lib, ops
+
+    lens, new = [400, 400], [50, 50]
+    pool = Pool(lens, 2, 128, 16, DEV)
+    k, v = _randn(800, 2, 128, seed=66), _randn(800, 2, 128, seed=67)
+    pool.write(k, v)
+    q = _randn(100, 8, 128, seed=68)
+    out = torch.zeros_like(q)
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=50, max_len=400,
+                             total_len=300, out=out)
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
+    ref, size = attention(q, quantized(k), quantized(v), lens, new)  # the first one fits
+    assert bool(((out.double().cpu() - ref).abs() <= BOUND * size)[:50].all()) and not out[50:].any()
 
 
 # ------------------------------------------------------------------ refusals

@@ -23,7 +23,7 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
     from faquant_b200 import _lib
 
     lib = _lib.load()
-    p = ctypes.c_void_p(16)
+    p = ctypes.c_void_p(256)
 
     def write(d=128, page=16, stride=1 << 20, pages=p, levels=123, dtype=0):
         return lib.faq_hif4_kv_write(p, p, dtype, 4, 2, d, 256, 128, 256, 128, pages, 4, stride, page, p, 3, 3, p, p, 1,
@@ -40,7 +40,7 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
 
     def attend(heads=4, scale=1.0, ws=1 << 30, qs=512, max_new=1):
         return lib.faq_hif4_paged_attention(p, 4, heads, qs, 128, p, 4, 1 << 20, 16, 2, 128, p, 3, 3, p, p, 1, max_new, 48,
-                                            ctypes.c_float(scale), p, 512, 128, p, ws, None)
+                                            48, ctypes.c_float(scale), p, 512, 128, p, ws, None)
 
     assert attend(heads=3) == 1 and "divisible" in _lib.last_error()
     assert attend(scale=0.0) == 1 and "scale" in _lib.last_error()
@@ -48,7 +48,7 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
     assert attend(qs=12) == 1 and "strides" in _lib.last_error()
     assert attend(ws=16) == 1 and "workspace" in _lib.last_error()
     assert attend(max_new=-1) == 1
-    assert lib.faq_hif4_paged_attention_workspace_bytes(6, 4, 1, 128) == 0
+    assert lib.faq_hif4_paged_attention_workspace_bytes(4, 6, 4, 1, 1, 48, 48, 128) == 0
 
     def verify(batch=1, k=2, vocab=10, dtype=1, target=p):
         return lib.faq_verify_drafts(p, target, None, dtype, batch, k, vocab, 30, 10, 0, 0, p, p, None, p, p, None)
