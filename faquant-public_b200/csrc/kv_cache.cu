@@ -6,6 +6,11 @@
 // places of the page format (include/faquant_b200.h). Every byte of the cache belongs to one
 // token, so tokens are written without reading what is there.
 // Read: the inverse, value = (n - 8) / 4 * 2^e * scale, exact in bf16.
+// Both give a warp a block of 16 tokens of one head, so that a lane holds both tokens of a pair
+// (V's words interleave them) and stores 8 or 16 bytes. The packed tokens of a ragged batch
+// are found without a prefix sum over its blocks: sequence b's blocks get the slots from
+// cu[b] / 16 + 2 b on, always enough of them (n tokens touch at most n / 16 + 2 blocks).
+#include <algorithm>
 #include <atomic>
 
 #include "kv_pages.cuh"
@@ -79,59 +84,132 @@ __device__ __forceinline__ void load8(const float* src, bool vec, float (&v)[8])
   }
 }
 
+
+// Slot -> (sequence, first position of a block, the live tokens [from, to) of the block, the
+// packed token of the block's first position, the number of new tokens at positions below
+// zero); false if the slot holds nothing. A sequence whose new tokens all have no position
+// has its first slot, with to = 0.
+struct Slot {
+  int b, pos, from, to;
+  int64_t token, none;
+};
+__device__ __forceinline__ int64_t first_slot(const Pages& p, int b) { return (p.cu[b] >> 4) + 2 * static_cast<int64_t>(b); }
+__host__ __device__ inline int64_t slots_of(int64_t total, int64_t batch) { return total / 16 + 2 * batch; }
+__device__ __forceinline__ bool find_slot(const Pages& p, int64_t slot, int64_t total, Slot& s) {
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first_slot(p, mid) <= slot) lo = mid; else hi = mid;
+  }
+  s.b = lo;
+  const int c0 = p.cu[lo], c1 = p.cu[lo + 1];
+  if (c0 < 0 || c1 <= c0 || c1 > total || slot < first_slot(p, lo)) return false;
+  const int64_t first = static_cast<int64_t>(p.lens[lo]) - (c1 - c0);  // position of the first new token
+  // positions below zero have no block; the first block is that of position max(first, 0)
+  const int64_t block = (first > 0 ? first >> 4 : 0) + (slot - first_slot(p, lo));
+  const int64_t pos = block * BLOCK;
+  s.none = first < 0 ? std::min<int64_t>(-first, c1 - c0) : 0;
+  if (pos >= p.lens[lo] && !(pos == 0 && s.none)) return false;
+  s.pos = static_cast<int>(pos);
+  s.from = static_cast<int>(first > pos ? first - pos : 0);
+  s.to = static_cast<int>(std::max<int64_t>(std::min<int64_t>(p.lens[lo] - pos, BLOCK), 0));
+  s.token = c0 + (pos - first);
+  return true;
+}
+
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) kv_write_kernel(WriteParams w, bool vec) {
   grid_dependency_wait();
   allow_dependent_launch();
   const Pages& p = w.p;
-  constexpr int LANES = 8 * NG;  // of a token's row of one head
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = idx / LANES;
-  const int64_t t = row / p.kv_heads;
-  const int head = static_cast<int>(row - t * p.kv_heads);
-  const int c = static_cast<int>(idx % LANES), g = c >> 3, s = c & 7;
-  bool live = t < w.total;
-  int pos = -1;
-  int64_t page = -1;
-  if (live) {
-    const int b = sequence_of(p, t);
-    if (b >= 0) pos = p.lens[b] - p.cu[b + 1] + static_cast<int>(t);
-    if (pos >= 0) page = page_of(p, b, pos);
-  }
-  live = page >= 0;
-  float vk[8], vv[8];
+  const int lane = threadIdx.x & 31, s = lane & 7;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t slot = item / p.kv_heads;
+  const int head = static_cast<int>(item - slot * p.kv_heads);
+  Slot x;
+  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x) || x.to == 0) return;  // warp-uniform
+  const int64_t page = page_of(p, x.b, x.pos);
+  if (page < 0) return;
+  uint8_t* kdst = p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, x.pos);
+  uint8_t* vdst = p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, x.pos);
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    if (x.from >= 8 * (h + 1) || x.to <= 8 * h) continue;  // warp-uniform
+    const int pr = (lane >> 3) + 4 * h;  // tokens 2 pr, 2 pr + 1 of the block
+    const bool live[2] = {2 * pr >= x.from && 2 * pr < x.to, 2 * pr + 1 >= x.from && 2 * pr + 1 < x.to};
+    uint32_t kw[2][NG], vw[2][NG], ve[2][NG];  // [token]; the exponents of all sub-blocks, (a, b) halves
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vk[i] = vv[i] = 0.0f;
-  if (live) {
-    load8<T>(static_cast<const T*>(w.k) + t * w.kt + head * w.kh + 8 * c, vec, vk);
-    load8<T>(static_cast<const T*>(w.v) + t * w.vt + head * w.vh + 8 * c, vec, vv);
-  }
-  uint32_t ka, kb, ks, va, vb, vs;
-  const uint32_t kw = quantize8(vk, w.k_levels, ka, kb, ks);
-  const uint32_t vw = quantize8(vv, w.v_levels, va, vb, vs);
-  // the group's exponent words: quarter a in the low half, b in the high half
-  uint32_t ke = (ka | (kb << 16)) << (2 * s), ve = (va | (vb << 16)) << (2 * s);
+    for (int k = 0; k < 2; ++k) {
+      const int r = 2 * pr + k;
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    ke |= __shfl_xor_sync(0xffffffffu, ke, o);
-    ve |= __shfl_xor_sync(0xffffffffu, ve, o);
-  }
-  if (!live) return;
-  const int r = pos & 15, pair = r >> 1, par = r & 1;
-  uint8_t* kdst = p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, pos);
-  uint8_t* vdst = p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, pos);
-  *reinterpret_cast<uint32_t*>(kdst + 32 * NG * r + (s >> 1) * 8 * NG + 8 * g + 4 * (s & 1)) = kw;
-  uint16_t* vq = reinterpret_cast<uint16_t*>(vdst + 64 * NG * pair + (s ^ (2 * (pair & 3))) * 8 * NG + 8 * g + 2 * par);
-  vq[0] = static_cast<uint16_t>(vw);
-  vq[2] = static_cast<uint16_t>(vw >> 16);
-  if (s == 0) {
-    *reinterpret_cast<uint32_t*>(kdst + exp_offset(NG) + (r * NG + g) * 4) = ke;
-    kdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(ks);
-  } else if (s == 1) {
-    uint16_t* vx = reinterpret_cast<uint16_t*>(vdst + exp_offset(NG) + (pair * NG + g) * 8 + 2 * par);
-    vx[0] = static_cast<uint16_t>(ve);
-    vx[2] = static_cast<uint16_t>(ve >> 16);
-    vdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(vs);
+      for (int g = 0; g < NG; ++g) {
+        float vk[8], vv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vk[i] = vv[i] = 0.0f;
+        if (live[k]) {
+          load8<T>(static_cast<const T*>(w.k) + (x.token + r) * w.kt + head * w.kh + 64 * g + 8 * s, vec, vk);
+          load8<T>(static_cast<const T*>(w.v) + (x.token + r) * w.vt + head * w.vh + 64 * g + 8 * s, vec, vv);
+        }
+        uint32_t ka, kb, ks, va, vb, vs;
+        kw[k][g] = quantize8(vk, w.k_levels, ka, kb, ks);
+        vw[k][g] = quantize8(vv, w.v_levels, va, vb, vs);
+        uint32_t ke = (ka | (kb << 16)) << (2 * s), ve1 = (va | (vb << 16)) << (2 * s);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          ke |= __shfl_xor_sync(0xffffffffu, ke, o);
+          ve1 |= __shfl_xor_sync(0xffffffffu, ve1, o);
+        }
+        ve[k][g] = ve1;
+        if (live[k] && s == 0) {
+          *reinterpret_cast<uint32_t*>(kdst + exp_offset(NG) + (r * NG + g) * 4) = ke;
+          kdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(ks);
+          vdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(vs);
+        }
+      }
+      // K: the even lane of two stores both lanes' words of group 0, the odd one of group 1
+      uint8_t* krow = kdst + 32 * NG * r + (s >> 1) * 8 * NG;
+      if constexpr (NG == 2) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, (s & 1) ? kw[k][0] : kw[k][1], 1);
+        if (live[k])
+          *reinterpret_cast<uint2*>(krow + 8 * (s & 1)) = (s & 1) ? make_uint2(other, kw[k][1]) : make_uint2(kw[k][0], other);
+      } else if (live[k]) {
+        *reinterpret_cast<uint32_t*>(krow + 4 * (s & 1)) = kw[k][0];
+      }
+    }
+    // V: words of a quad's halves (token 2 pr, 2 pr + 1)
+    uint8_t* vrow = vdst + 64 * NG * pr + (s ^ (2 * (pr & 3))) * 8 * NG;
+    uint8_t* vexp = vdst + exp_offset(NG) + pr * NG * 8;
+    if (live[0] && live[1]) {
+      uint32_t q[2 * NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        q[2 * g] = __byte_perm(vw[0][g], vw[1][g], 0x5410);
+        q[2 * g + 1] = __byte_perm(vw[0][g], vw[1][g], 0x7632);
+      }
+      if constexpr (NG == 2)
+        *reinterpret_cast<uint4*>(vrow) = make_uint4(q[0], q[1], q[2], q[3]);
+      else
+        *reinterpret_cast<uint2*>(vrow) = make_uint2(q[0], q[1]);
+      if (s < NG)
+        *reinterpret_cast<uint2*>(vexp + 8 * s) = make_uint2(__byte_perm(ve[0][s ? NG - 1 : 0], ve[1][s ? NG - 1 : 0], 0x5410),
+                                                             __byte_perm(ve[0][s ? NG - 1 : 0], ve[1][s ? NG - 1 : 0], 0x7632));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (!live[k]) continue;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint16_t* q = reinterpret_cast<uint16_t*>(vrow + 8 * g + 2 * k);
+          q[0] = static_cast<uint16_t>(vw[k][g]);
+          q[2] = static_cast<uint16_t>(vw[k][g] >> 16);
+          if (s == 0) {
+            uint16_t* e = reinterpret_cast<uint16_t*>(vexp + 8 * g + 2 * k);
+            e[0] = static_cast<uint16_t>(ve[k][g]);
+            e[2] = static_cast<uint16_t>(ve[k][g] >> 16);
+          }
+        }
+      }
+    }
   }
 }
 
@@ -141,22 +219,19 @@ struct ReadParams {
   int64_t total, kt, kh, vt, vh;
 };
 
-template <typename T>
-__device__ __forceinline__ void store8(T* dst, bool vec, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void store8(__nv_bfloat16* dst, bool vec, const float (&v)[8]) {
+// Eight consecutive channels as four bf16 pairs, to bf16 or fp32.
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, bool vec, const uint32_t (&w)[4]) {
   if (vec) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = exact_bf16_bits(v[2 * i]) | (__float_as_uint(v[2 * i + 1]) & 0xFFFF0000u);
     *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(dst)[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
   }
 }
-template <>
-__device__ __forceinline__ void store8(float* dst, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void store_pairs(float* dst, bool vec, const uint32_t (&w)[4]) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float((i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
   if (vec) {
     *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -166,56 +241,129 @@ __device__ __forceinline__ void store8(float* dst, bool vec, const float (&v)[8]
   }
 }
 
+// The tokens [from, to) of a block of one head, K or V, as rows of `stride` elements from dst
+// (the block's first token), by one warp: K sixteen channels of each group per lane and half, V
+// a sub-block of both tokens of a pair. y = (n - 8) 2^(e - 3) times twice the scale is exact
+// in bf16 (six significant bits), so a pair costs one packed product.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
+  const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
+  return s | (s << 16);
+}
+template <typename T, int NG>
+__device__ __forceinline__ void expand_block_k(const Expand& expand, const uint8_t* src, T* dst, int64_t stride, int from,
+                                               int to, int lane, bool vec = true) {
+  const int t = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+    if (r < from || r >= to) continue;
+    uint32_t w[2 * NG], e[NG], sc[NG];
+    if constexpr (NG == 2) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * r + 16 * t);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * r);
+      e[0] = x.x; e[1] = x.y;
+      const uint32_t c = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * r);
+      sc[0] = scale_pair(c & 255); sc[1] = scale_pair(c >> 8);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + 32 * r + 8 * t);
+      w[0] = u.x; w[1] = u.y;
+      e[0] = *reinterpret_cast<const uint32_t*>(src + exp_offset(NG) + 4 * r);
+      sc[0] = scale_pair(src[scale_offset(NG) + r]);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
+        uint32_t y[4];
+        expand.word(w[2 * g + i], expand.exponents(e[g], (7 - 4 * t - 2 * i) & 31), y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], sc[g]);
+        const uint32_t row[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                                 __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)};
+        store_pairs(dst + r * stride + 64 * g + 16 * t + 8 * i, vec, row);
+      }
+    }
+  }
+}
+template <typename T, int NG>
+__device__ __forceinline__ void expand_block_v(const Expand& expand, const uint8_t* src, T* dst, int64_t stride, int from,
+                                               int to, int lane, bool vec = true) {
+  const int s = lane & 7;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int p = (lane >> 3) + 4 * h;  // tokens 2 p, 2 p + 1
+    if (2 * p + 1 < from || 2 * p >= to) continue;
+    uint32_t w[2 * NG], e[2 * NG], sc[NG];
+    if constexpr (NG == 2) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + 128 * p + 16 * (s ^ (2 * (p & 3))));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+      const uint4 x = *reinterpret_cast<const uint4*>(src + exp_offset(NG) + 16 * p);
+      e[0] = x.x; e[1] = x.y; e[2] = x.z; e[3] = x.w;
+      const uint32_t c = *reinterpret_cast<const uint32_t*>(src + scale_offset(NG) + 4 * p);  // [token][group]
+      sc[0] = __byte_perm(scale_pair(c & 255), scale_pair((c >> 16) & 255), 0x5410);
+      sc[1] = __byte_perm(scale_pair((c >> 8) & 255), scale_pair(c >> 24), 0x5410);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + 64 * p + 8 * (s ^ (2 * (p & 3))));
+      w[0] = u.x; w[1] = u.y;
+      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * p);
+      e[0] = x.x; e[1] = x.y;
+      const uint32_t c = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * p);
+      sc[0] = __byte_perm(scale_pair(c & 255), scale_pair(c >> 8), 0x5410);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        expand.word(w[2 * g + q], expand.exponents(e[2 * g + q], (7 - 2 * s) & 31), y[q]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], sc[g]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t sel = k ? 0x7632 : 0x5410;
+        const uint32_t row[4] = {__byte_perm(y[0][0], y[0][1], sel), __byte_perm(y[0][2], y[0][3], sel),
+                                 __byte_perm(y[1][0], y[1][1], sel), __byte_perm(y[1][2], y[1][3], sel)};
+        if (2 * p + k >= from && 2 * p + k < to) store_pairs(dst + (2 * p + k) * stride + 64 * g + 8 * s, vec, row);
+      }
+    }
+  }
+}
+
+// Zeros for `count` tokens from `token` on, which have no place in the cache.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const ReadParams& w, int64_t token, int64_t count, int head, int d, int lane) {
+  for (int64_t i = token; i < token + count; ++i)
+    for (int c = lane; c < d; c += 32) {
+      static_cast<T*>(w.k)[i * w.kt + head * w.kh + c] = T(0.0f);
+      static_cast<T*>(w.v)[i * w.vt + head * w.vh + c] = T(0.0f);
+    }
+}
+
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams w, bool vec) {
   grid_dependency_wait();
   allow_dependent_launch();
   const Pages& p = w.p;
-  constexpr int LANES = 8 * NG;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = idx / LANES;
-  const int64_t t = row / p.kv_heads;
-  if (t >= w.total) return;
-  const int head = static_cast<int>(row - t * p.kv_heads);
-  const int c = static_cast<int>(idx % LANES), g = c >> 3, s = c & 7;
-  int pos = -1;
-  int64_t page = -1;
-  const int b = sequence_of(p, t);
-  if (b >= 0) pos = p.lens[b] - p.cu[b + 1] + static_cast<int>(t);
-  if (pos >= 0) page = page_of(p, b, pos);
-  float vk[8], vv[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) vk[i] = vv[i] = 0.0f;  // a token without a place reads as zeros
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t slot = item / p.kv_heads;
+  const int head = static_cast<int>(item - slot * p.kv_heads);
+  Slot x;
+  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;
+  T* k = static_cast<T*>(w.k) + x.token * w.kt + head * w.kh;
+  T* v = static_cast<T*>(w.v) + x.token * w.vt + head * w.vh;
+  const int64_t page = x.to ? page_of(p, x.b, x.pos) : -1;
   if (page >= 0) {
-    const int r = pos & 15, pair = r >> 1, par = r & 1;
-    const uint8_t* ksrc = p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, pos);
-    const uint8_t* vsrc = p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, pos);
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(ksrc + 32 * NG * r + (s >> 1) * 8 * NG + 8 * g + 4 * (s & 1));
-    const uint16_t* vq =
-        reinterpret_cast<const uint16_t*>(vsrc + 64 * NG * pair + (s ^ (2 * (pair & 3))) * 8 * NG + 8 * g + 2 * par);
-    const uint32_t vw = vq[0] | (static_cast<uint32_t>(vq[2]) << 16);
-    const uint32_t ke = *reinterpret_cast<const uint32_t*>(ksrc + exp_offset(NG) + (r * NG + g) * 4);
-    const uint16_t* vx = reinterpret_cast<const uint16_t*>(vsrc + exp_offset(NG) + (pair * NG + g) * 8 + 2 * par);
-    const uint32_t ve = vx[0] | (static_cast<uint32_t>(vx[2]) << 16);
-    const float ks = twice_scale(ksrc[scale_offset(NG) + r * NG + g]);
-    const float vs = twice_scale(vsrc[scale_offset(NG) + r * NG + g]);
     const Expand expand;
-    uint32_t y[4];
-    expand.word(kw, expand.exponents(ke, (7 - 2 * s) & 31), y);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      vk[j] = __fmul_rn(__uint_as_float(y[j] << 16), ks);
-      vk[4 + j] = __fmul_rn(__uint_as_float(y[j] & 0xFFFF0000u), ks);
-    }
-    expand.word(vw, expand.exponents(ve, (7 - 2 * s) & 31), y);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      vv[j] = __fmul_rn(__uint_as_float(y[j] << 16), vs);
-      vv[4 + j] = __fmul_rn(__uint_as_float(y[j] & 0xFFFF0000u), vs);
-    }
+    const uint8_t* src = p.base + page * p.page_stride;
+    expand_block_k<T, NG>(expand, src + block_in_page<NG>(p, 0, head, x.pos), k, w.kt, x.from, x.to, lane, vec);
+    expand_block_v<T, NG>(expand, src + block_in_page<NG>(p, 1, head, x.pos), v, w.vt, x.from, x.to, lane, vec);
+  } else {
+    zero_rows<T>(w, x.token + x.from, x.to - x.from, head, 64 * NG, lane);
   }
-  store8<T>(static_cast<T*>(w.k) + t * w.kt + head * w.kh + 8 * c, vec, vk);
-  store8<T>(static_cast<T*>(w.v) + t * w.vt + head * w.vh + 8 * c, vec, vv);
+  if (x.pos == 0) zero_rows<T>(w, p.cu[x.b], x.none, head, 64 * NG, lane);
 }
 
 // The checks every entry point over pages makes; fills `p`.
@@ -309,7 +457,7 @@ extern "C" int faq_hif4_kv_write(const void* k, const void* v, int dtype, int64_
   const bool vec = aligned16(k) && aligned16(v) && k_token_stride % unit == 0 && k_head_stride % unit == 0 &&
                    v_token_stride % unit == 0 && v_head_stride % unit == 0;
   const int ng = d / 64;
-  const int64_t blocks = (total * kv_heads * 8 * ng + 255) / 256;
+  const int64_t blocks = (slots_of(total, batch) * kv_heads + 7) / 8;
   FAQ_CHECK_ARG(blocks < (int64_t(1) << 31), "too many tokens for one call");
   auto kern = dtype == FAQ_BF16 ? (ng == 1 ? kv_write_kernel<__nv_bfloat16, 1> : kv_write_kernel<__nv_bfloat16, 2>)
                                 : (ng == 1 ? kv_write_kernel<float, 1> : kv_write_kernel<float, 2>);
@@ -343,7 +491,7 @@ extern "C" int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t pa
   const bool vec = aligned16(k) && aligned16(v) && k_token_stride % unit == 0 && k_head_stride % unit == 0 &&
                    v_token_stride % unit == 0 && v_head_stride % unit == 0;
   const int ng = d / 64;
-  const int64_t blocks = (total * kv_heads * 8 * ng + 255) / 256;
+  const int64_t blocks = (slots_of(total, batch) * kv_heads + 7) / 8;
   FAQ_CHECK_ARG(blocks < (int64_t(1) << 31), "too many tokens for one call");
   auto kern = dtype == FAQ_BF16 ? (ng == 1 ? kv_read_kernel<__nv_bfloat16, 1> : kv_read_kernel<__nv_bfloat16, 2>)
                                 : (ng == 1 ? kv_read_kernel<float, 1> : kv_read_kernel<float, 2>);

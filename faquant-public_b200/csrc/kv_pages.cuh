@@ -56,17 +56,6 @@ __device__ __forceinline__ int length_of(const Pages& p, int b) {
   return min(max(len, 0), most);
 }
 
-// Sequence of packed token t: the b with cu[b] <= t < cu[b + 1], or -1.
-__device__ __forceinline__ int sequence_of(const Pages& p, int64_t t) {
-  int lo = 0, hi = p.batch;  // cu[lo] <= t < cu[hi]
-  if (t < p.cu[0] || t >= p.cu[hi]) return -1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
 // twice the scale of a scale byte: the expansion below yields half the value over it
 __device__ __forceinline__ float twice_scale(uint32_t code) { return __uint_as_float((code << 21) + (80u << 23)); }
 

@@ -198,91 +198,6 @@ __device__ void make_plan(const Params& P) {
 }
 
 // ---------------------------------------------------------------- expand
-// The sixteen tokens of a block of one head, K or V, as bf16 rows of `stride` elements, by one
-// warp: K a quarter row (16 channels of each group) per lane and half, V a sub-block of both
-// tokens of a pair. y = (n - 8) 2^(e - 3) times twice the scale is exact in bf16 (six
-// significant bits), so a pair costs one packed product.
-__device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
-  const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
-  return s | (s << 16);
-}
-template <int NG>
-__device__ __forceinline__ void expand_block_k(const Expand& expand, const uint8_t* src, __nv_bfloat16* dst, int64_t stride,
-                                               int from, int to, int lane) {
-  const int t = lane & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = (lane >> 2) + 8 * h;
-    if (r < from || r >= to) continue;
-    uint32_t w[2 * NG];
-    if constexpr (NG == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * r + 16 * t);
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + 32 * r + 8 * t);
-      w[0] = u.x; w[1] = u.y;
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const uint32_t e = *reinterpret_cast<const uint32_t*>(src + exp_offset(NG) + (r * NG + g) * 4);
-      const uint32_t sc = scale_pair(src[scale_offset(NG) + r * NG + g]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
-        uint32_t y[4];
-        expand.word(w[2 * g + i], expand.exponents(e, (7 - 4 * t - 2 * i) & 31), y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], sc);
-        *reinterpret_cast<uint4*>(dst + r * stride + 64 * g + 16 * t + 8 * i) =
-            make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
-                       __byte_perm(y[2], y[3], 0x7632));
-      }
-    }
-  }
-}
-template <int NG>
-__device__ __forceinline__ void expand_block_v(const Expand& expand, const uint8_t* src, __nv_bfloat16* dst, int64_t stride,
-                                               int from, int to, int lane) {
-  const int s = lane & 7;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int p = (lane >> 3) + 4 * h;  // tokens 2 p, 2 p + 1
-    if (2 * p + 1 < from || 2 * p >= to) continue;
-    uint32_t w[2 * NG], e[2 * NG];
-    if constexpr (NG == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + 128 * p + 16 * (s ^ (2 * (p & 3))));
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-      const uint4 x = *reinterpret_cast<const uint4*>(src + exp_offset(NG) + 16 * p);
-      e[0] = x.x; e[1] = x.y; e[2] = x.z; e[3] = x.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + 64 * p + 8 * (s ^ (2 * (p & 3))));
-      w[0] = u.x; w[1] = u.y;
-      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * p);
-      e[0] = x.x; e[1] = x.y;
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const uint32_t s0 = scale_pair(src[scale_offset(NG) + 2 * p * NG + g]);
-      const uint32_t s1 = scale_pair(src[scale_offset(NG) + (2 * p + 1) * NG + g]);
-      const uint32_t sc = __byte_perm(s0, s1, 0x5410);
-      uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        expand.word(w[2 * g + q], expand.exponents(e[2 * g + q], (7 - 2 * s) & 31), y[q]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], sc);
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t sel = k ? 0x7632 : 0x5410;
-        if (2 * p + k >= from && 2 * p + k < to)
-          *reinterpret_cast<uint4*>(dst + (2 * p + k) * stride + 64 * g + 8 * s) =
-              make_uint4(__byte_perm(y[0][0], y[0][1], sel), __byte_perm(y[0][2], y[0][3], sel),
-                         __byte_perm(y[1][0], y[1][1], sel), __byte_perm(y[1][2], y[1][3], sel));
-      }
-    }
-  }
-}
-
 // Work items: (key tile of 128 tokens, kv head), a block of 16 tokens per warp. The last CTA
 // makes the plan.
 template <int NG>
@@ -329,8 +244,8 @@ __global__ void __launch_bounds__(256) paged_expand_kernel(Params P) {
       __nv_bfloat16* v = P.v + row * stride + head * D;
       if (have) {
         const uint8_t* unit = P.p.base + page * P.p.page_stride;
-        expand_block_k<NG>(expand, unit + block_in_page<NG>(P.p, 0, head, pos), k, stride, 0, have, lane);
-        expand_block_v<NG>(expand, unit + block_in_page<NG>(P.p, 1, head, pos), v, stride, 0, have, lane);
+        expand_block_k<__nv_bfloat16, NG>(expand, unit + block_in_page<NG>(P.p, 0, head, pos), k, stride, 0, have, lane);
+        expand_block_v<__nv_bfloat16, NG>(expand, unit + block_in_page<NG>(P.p, 1, head, pos), v, stride, 0, have, lane);
       }
       for (int i = have * (D / 8) + lane; i < BLOCK * (D / 8); i += 32) {  // zeros behind the end
         *reinterpret_cast<uint4*>(k + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);

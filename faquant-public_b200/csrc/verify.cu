@@ -9,9 +9,10 @@
 // weights fit 64 bits. The threshold u sum w is one fp64 product.
 //
 // Bound by reading one row of p and q per sequence; a small batch by its round trips. A
-// cluster of eight CTAs takes a sequence: every warp sums its own contiguous piece, the
-// CTAs' sums meet through distributed shared memory, and the one warp whose piece holds the
-// threshold reads it again (from L2) to find the token.
+// cluster of eight CTAs takes a sequence: every warp sums its own contiguous piece (the loads
+// of four steps in flight), the CTAs' sums meet through distributed shared memory, and the CTA
+// whose part holds the threshold reads that warp's piece again (from L2), a step per warp,
+// to find the token. The target's own weights are summed only when nothing is left over.
 #include "common.cuh"
 
 namespace faq {
@@ -65,23 +66,67 @@ struct Rows {
   const T *p, *q;  // q null: no subtraction
   int64_t vocab, dropped;  // the token whose weight is 0 (-1: none)
   bool vec;
-  // the residual weights of entries at .. at + 3 and the target's own
-  __device__ __forceinline__ void get(int64_t at, float (&left)[4], float (&whole)[4]) const {
+  // the weights of entries at .. at + 3
+  __device__ __forceinline__ void get(int64_t at, float (&r)[4]) const {
     float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (vec && at + 4 <= vocab) {
-      load4(p + at, whole);
+      load4(p + at, r);
       if (q) load4(q + at, b);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        whole[i] = at + i < vocab ? load1(p, at + i) : 0.0f;
+        r[i] = at + i < vocab ? load1(p, at + i) : 0.0f;
         if (q && at + i < vocab) b[i] = load1(q, at + i);
       }
     }
+    take(at, r, b);
+  }
+  __device__ __forceinline__ void take(int64_t at, float (&r)[4], const float (&b)[4]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) left[i] = at + i == dropped ? 0.0f : __fsub_rn(whole[i], b[i]);
+    for (int i = 0; i < 4; ++i) r[i] = at + i == dropped ? 0.0f : __fsub_rn(r[i], b[i]);
   }
 };
+
+__device__ __forceinline__ uint64_t sum4(const float (&r)[4]) {
+  uint32_t hi = 0, lo = 0;  // four weights of at most 2^20 each
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Weight w = weight(r[i]);
+    hi += w.hi;
+    lo += w.lo;
+  }
+  return join({hi, lo});
+}
+
+// This lane's part of the sum over steps s0 .. s1 - 1 of the row. Q: there is a draft row.
+template <typename T, bool Q>
+__device__ __forceinline__ uint64_t sum_steps(const Rows<T>& rows, int64_t s0, int64_t s1, int lane) {
+  constexpr int AHEAD = 4;
+  uint64_t sum = 0;
+  int64_t s = s0;
+  if (rows.vec) {
+    for (; s + AHEAD <= s1 && (s + AHEAD) * STEP <= rows.vocab; s += AHEAD) {
+      float r[AHEAD][4], b[AHEAD][4];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        load4(rows.p + (s + i) * STEP + lane * 4, r[i]);
+        if constexpr (Q) load4(rows.q + (s + i) * STEP + lane * 4, b[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if constexpr (!Q) b[i][0] = b[i][1] = b[i][2] = b[i][3] = 0.0f;
+        rows.take((s + i) * STEP + lane * 4, r[i], b[i]);
+        sum += sum4(r[i]);
+      }
+    }
+  }
+  for (; s < s1; ++s) {
+    float r[4];
+    rows.get(s * STEP + lane * 4, r);
+    sum += sum4(r);
+  }
+  return sum;
+}
 
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
@@ -90,9 +135,9 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) __cluster_dims__(CLUSTER, 1, 1) verify_kernel(Params P) {
-  __shared__ uint64_t s_warp[2][WARPS];  // residual, whole
-  __shared__ uint64_t s_cta[2];
+__global__ void __launch_bounds__(THREADS, 2) __cluster_dims__(CLUSTER, 1, 1) verify_kernel(Params P) {
+  __shared__ uint64_t s_warp[WARPS], s_step[WARPS];
+  __shared__ uint64_t s_cta[2];  // of the residual, then of the target's row
   __shared__ int s_first;
   grid_dependency_wait();
   allow_dependent_launch();
@@ -126,93 +171,95 @@ __global__ void __launch_bounds__(THREADS) __cluster_dims__(CLUSTER, 1, 1) verif
   const int64_t steps = (P.vocab + STEP - 1) / STEP;
   const int64_t each = (steps + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
   const int64_t s0 = (rank * WARPS + warp) * each, s1 = min(steps, s0 + each);
-  uint64_t left = 0, whole = 0;
-#pragma unroll 4
-  for (int64_t s = s0; s < s1; ++s) {
-    float r[4], w[4];
-    rows.get(s * STEP + lane * 4, r, w);
-    uint32_t lh = 0, ll = 0, wh = 0, wl = 0;  // four weights at most 2^20 each
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const Weight a = weight(r[i]), c = weight(w[i]);
-      lh += a.hi;
-      ll += a.lo;
-      wh += c.hi;
-      wl += c.lo;
+  uint64_t total = 0, before = 0;
+  auto sum_row = [&](int use) {  // the row's total, and what stands before this CTA's part
+    const uint64_t mine = warp_sum(rows.q ? sum_steps<T, true>(rows, s0, s1, lane) : sum_steps<T, false>(rows, s0, s1, lane));
+    if (lane == 0) s_warp[warp] = mine;
+    __syncthreads();
+    if (tid == 0) {
+      uint64_t sum = 0;
+      for (int w = 0; w < WARPS; ++w) sum += s_warp[w];
+      s_cta[use] = sum;
     }
-    left += join({lh, ll});
-    whole += join({wh, wl});
-  }
-  left = warp_sum(left);
-  whole = warp_sum(whole);
-  if (lane == 0) {
-    s_warp[0][warp] = left;
-    s_warp[1][warp] = whole;
-  }
-  __syncthreads();
-  if (tid < 2) {
-    uint64_t sum = 0;
-    for (int w = 0; w < WARPS; ++w) sum += s_warp[tid][w];
-    s_cta[tid] = sum;
-  }
-  __syncthreads();
-  cluster_sync();
-  uint64_t total[2] = {0, 0}, before[2] = {0, 0};
+    __syncthreads();
+    cluster_sync();
+    total = before = 0;
 #pragma unroll
-  for (int r = 0; r < CLUSTER; ++r) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int r = 0; r < CLUSTER; ++r) {
       uint64_t v;
-      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_addr(&s_cta[k]), r)));
-      total[k] += v;
-      if (r < rank) before[k] += v;
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_addr(&s_cta[use]), r)));
+      total += v;
+      if (r < rank) before += v;
     }
+  };
+  sum_row(0);
+  if (total == 0) {  // nothing left over: the target's own row
+    rows.q = nullptr;
+    rows.dropped = -1;
+    sum_row(1);
   }
   cluster_sync();  // no CTA leaves while its sums are read
-  const int use = total[0] > 0 ? 0 : 1;  // nothing left over: the target's own row
   int64_t* tokens = P.tokens + static_cast<int64_t>(b) * (P.k + 1);
   if (rank == 0) {
     for (int i = tid; i <= P.k; i += THREADS)
       if (i != n) tokens[i] = i < n ? draft[i] : -1;
     if (tid == 0) {
       P.accepted[b] = n;
-      if (total[use] == 0) tokens[n] = -1;  // no mass at all
+      if (total == 0) tokens[n] = -1;  // no mass at all
     }
   }
-  if (total[use] == 0) return;
+  if (total == 0) return;
   // u in [0, 1): below it by construction; anything else is brought there (NaN to 0)
   const float u = fminf(fmaxf(P.sample_u[b], 0.0f), 0.99999994f);
-  const double at = __dmul_rn(static_cast<double>(u), __ull2double_rn(total[use]));
-  uint64_t start = before[use];
-  for (int w = 0; w < warp; ++w) start += s_warp[use][w];
-  const uint64_t stop = start + s_warp[use][warp];
-  if (!(__ull2double_rn(start) <= at && __ull2double_rn(stop) > at)) return;  // warp-uniform
-  for (int64_t s = s0; s < s1; ++s) {
-    float r[4], w[4];
-    rows.get(s * STEP + lane * 4, r, w);
+  const double at = __dmul_rn(static_cast<double>(u), __ull2double_rn(total));
+  auto past = [&](uint64_t sum) { return __ull2double_rn(sum) > at; };
+  // the warp of this CTA whose piece passes the threshold (the same for all threads)
+  uint64_t start = before;
+  int owner = -1;
+  if (!past(start)) {
+    for (int w = 0; w < WARPS; ++w) {
+      if (past(start + s_warp[w])) {
+        owner = w;
+        break;
+      }
+      start += s_warp[w];
+    }
+  }
+  if (owner < 0) return;
+  const int64_t f0 = (rank * WARPS + owner) * each, f1 = min(steps, f0 + each);
+  for (int64_t s = f0; s < f1; s += WARPS) {  // a step per warp
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t at4 = (s + warp) * STEP + lane * 4;
+    if (s + warp < f1) rows.get(at4, r);
     uint64_t v[4], mine = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mine += v[i] = join(weight(use ? w[i] : r[i]));
+    for (int i = 0; i < 4; ++i) mine += v[i] = join(weight(r[i]));
     uint64_t x = mine;  // inclusive prefix over the lanes
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, __ull2double_rn(start + x) > at);
-    if (past) {
-      if (lane == __ffs(past) - 1) {
-        uint64_t c = start + x - mine;
-        int i = 0;
-        for (; i < 3; ++i) {
-          c += v[i];
-          if (__ull2double_rn(c) > at) break;
-        }
-        tokens[n] = s * STEP + lane * 4 + i;
-      }
-      return;
+    if (lane == 31) s_step[warp] = x;
+    __syncthreads();
+    uint64_t mine0 = start;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) mine0 += s_step[w];
+      start += s_step[w];
     }
-    start += __shfl_sync(0xffffffffu, x, 31);
+    // past() grows along the row: the first lane of the first warp that passes
+    const uint32_t here = __ballot_sync(0xffffffffu, past(mine0 + x));
+    if (!past(mine0) && here && lane == __ffs(here) - 1) {
+      uint64_t c = mine0 + x - mine;
+      int i = 0;
+      for (; i < 3; ++i) {
+        c += v[i];
+        if (past(c)) break;
+      }
+      tokens[n] = at4 + i;
+    }
+    if (past(start)) return;  // CTA-uniform
+    __syncthreads();
   }
 }
 

@@ -135,7 +135,9 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc:
+        check(rc, name)
 
 
 def device_trace(reset: bool = False) -> list[tuple[int, int, int, int, int]]:

@@ -6,6 +6,7 @@ Each function validates its torch arguments, allocates the outputs with torch
 
 from __future__ import annotations
 
+import functools
 import os
 
 import torch
@@ -75,7 +76,13 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without making a Stream object (2 us less per call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -687,23 +694,49 @@ def hif4_page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
 
 
 def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, kv_heads: int,
-            head_dim: int, page_size: int) -> None:
-    """Checks of a pool and the arrays that describe a ragged batch on it."""
-    if pages.dtype != torch.uint8 or pages.dim() < 2:
+            head_dim: int, page_size: int) -> int:
+    """Checks of a pool and the arrays that describe a ragged batch on it; the batch size."""
+    size = hif4_page_bytes(kv_heads, head_dim, page_size)
+    shape, stride = pages.shape, pages.stride()
+    if pages.dtype is not torch.uint8 or len(shape) < 2:
         raise TypeError("pages must be a uint8 tensor [num_pages, ...]")
-    if pages[0].numel() != hif4_page_bytes(kv_heads, head_dim, page_size) or not pages[0].is_contiguous():
-        raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
-    if pages.dim() == 4 and pages.shape[1:3] != (2, kv_heads):
+    if len(shape) == 4 and shape[1:3] != (2, kv_heads):
         raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
-    for t in (table, cu, lens):
-        if t.dtype != torch.int32:
-            raise TypeError("table, cu and lens must be int32")
-    if table.dim() != 2 or table.shape[1] < 1 or table.stride(1) != 1:
+    inner = 1
+    for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if st != inner and n != 1:
+            raise ValueError("a page must be contiguous bytes")
+        inner *= n
+    if inner != size:
+        raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) bytes")
+    if table.dtype is not torch.int32 or cu.dtype is not torch.int32 or lens.dtype is not torch.int32:
+        raise TypeError("table, cu and lens must be int32")
+    columns = table.shape
+    if len(columns) != 2 or columns[1] < 1 or table.stride(1) != 1:
         raise ValueError("table must be [batch, columns] with unit column stride")
-    if cu.shape != (table.shape[0] + 1,) or lens.shape != (table.shape[0],):
+    batch = columns[0]
+    if cu.shape != (batch + 1,) or lens.shape != (batch,):
         raise ValueError("cu must be [batch + 1] and lens [batch]")
     if not cu.is_contiguous() or not lens.is_contiguous():
         raise ValueError("cu and lens must be contiguous")
+    return batch
+
+
+def _kv_heads(pages: torch.Tensor, head_dim: int, page_size: int) -> int:
+    """The kv heads that a pool of such pages holds."""
+    shape = pages.shape
+    if len(shape) == 4:
+        return shape[2]
+    size = 1
+    for n in shape[1:]:
+        size *= n
+    return max(1, size // hif4_page_bytes(1, head_dim, page_size))
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(device: int, *sizes: int) -> int:
+    with torch.cuda.device(device):
+        return int(_lib.load().faq_hif4_paged_attention_workspace_bytes(*sizes))
 
 
 def hif4_kv_write(
@@ -728,13 +761,18 @@ def hif4_kv_write(
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one shape and dtype")
     total, h, d = k.shape
-    _ragged(pages, table, cu, lens, h, d, page_size)
-    k = k if k.stride(2) == 1 else k.contiguous()
-    v = v if v.stride(2) == 1 else v.contiguous()
-    _lib.call("faq_hif4_kv_write", k.data_ptr(), v.data_ptr(), _dtype_code(k), total, h, d, k.stride(0), k.stride(1),
-              v.stride(0), v.stride(1), pages.data_ptr(), pages.shape[0], pages.stride(0), page_size,
-              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), table.shape[0],
-              levels_code(levels[0]), levels_code(levels[1]), _stream(device))
+    batch = _ragged(pages, table, cu, lens, h, d, page_size)
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1:
+        k = k.contiguous()
+        ks = k.stride()
+    if vs[2] != 1:
+        v = v.contiguous()
+        vs = v.stride()
+    _lib.call("faq_hif4_kv_write", k.data_ptr(), v.data_ptr(), _dtype_code(k), total, h, d, ks[0], ks[1], vs[0], vs[1],
+              pages.data_ptr(), pages.shape[0], pages.stride(0), page_size, table.data_ptr(), table.stride(0),
+              table.shape[1], cu.data_ptr(), lens.data_ptr(), batch, levels_code(levels[0]), levels_code(levels[1]),
+              _stream(device))
 
 
 def hif4_kv_read(
@@ -753,19 +791,23 @@ def hif4_kv_read(
     ``(k, v)``, each ``[total, Hkv, D]`` bf16 or fp32 (``total = cu[-1]``, known on the host),
     packed in sequence order; ``out`` takes tensors of that shape with unit channel stride."""
     device = _require_cuda(pages, table, cu, lens, *(out or ()))
-    bytes_per_head = hif4_page_bytes(1, head_dim, page_size)
-    h = pages[0].numel() // bytes_per_head
-    _ragged(pages, table, cu, lens, h, head_dim, page_size)
+    h = _kv_heads(pages, head_dim, page_size)
+    batch = _ragged(pages, table, cu, lens, h, head_dim, page_size)
+    if total < 0:
+        raise ValueError("total must not be negative")
     if out is None:
-        out = (torch.empty((total, h, head_dim), dtype=dtype, device=device),
-               torch.empty((total, h, head_dim), dtype=dtype, device=device))
-    k, v = out
-    if k.shape != (total, h, head_dim) or v.shape != k.shape or k.dtype != v.dtype or k.stride(2) != 1 or v.stride(2) != 1:
-        raise ValueError("out must be two [total, kv_heads, head_dim] tensors of one dtype with unit channel stride")
+        k = torch.empty((total, h, head_dim), dtype=dtype, device=device)
+        v = torch.empty_like(k)
+        ks = vs = (h * head_dim, head_dim)
+    else:
+        k, v = out
+        if (k.shape != (total, h, head_dim) or v.shape != k.shape or k.dtype != v.dtype or k.stride(2) != 1
+                or v.stride(2) != 1):
+            raise ValueError("out must be two [total, kv_heads, head_dim] tensors of one dtype with unit channel stride")
+        ks, vs = k.stride(), v.stride()
     _lib.call("faq_hif4_kv_read", pages.data_ptr(), pages.shape[0], pages.stride(0), page_size, h, head_dim,
-              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), table.shape[0],
-              k.data_ptr(), v.data_ptr(), _dtype_code(k), total, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-              _stream(device))
+              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), batch,
+              k.data_ptr(), v.data_ptr(), _dtype_code(k), total, ks[0], ks[1], vs[0], vs[1], _stream(device))
     return k, v
 
 
@@ -794,33 +836,37 @@ def hif4_paged_attention(
     the lengths from above; they are host numbers, so nothing is copied from the device, and
     with prompt chunks in the batch they size the workspace. ``workspace``: a 256-byte
     aligned device buffer to use instead of a new one."""
-    device = _require_cuda(q, pages, table, cu, lens)
-    if q.dtype != torch.bfloat16 or q.dim() != 3:
+    device = _require_cuda(q, pages, table, cu, lens, out, workspace)
+    if q.dtype is not torch.bfloat16 or q.dim() != 3:
         raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
     total, heads, d = q.shape
-    h = pages[0].numel() // hif4_page_bytes(1, d, page_size)
-    _ragged(pages, table, cu, lens, h, d, page_size)
+    h = _kv_heads(pages, d, page_size)
+    batch = _ragged(pages, table, cu, lens, h, d, page_size)
     if heads % h:
         raise ValueError("query heads must be divisible by key/value heads")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    qs = q.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] < 8 or qs[1] < 8 or q.data_ptr() % 16:
         q = q.contiguous()
+        qs = (heads * d, d)
     if out is None:
-        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
-        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+        out = q.new_empty((total, heads, d))
+        os_ = (heads * d, d)
+    else:
+        if out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+            raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+        os_ = out.stride()
+    columns = table.shape[1]
     if max_len is None:
-        max_len = table.shape[1] * page_size
-    batch = table.shape[0]
+        max_len = columns * page_size
     if total_len is None:
         total_len = batch * max_len
-    need = int(_lib.load().faq_hif4_paged_attention_workspace_bytes(total, heads, h, batch, max_new, max_len, total_len, d))
+    need = _attention_workspace(device.index, total, heads, h, batch, max_new, max_len, total_len, d)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, q.stride(0), q.stride(1), pages.data_ptr(),
-              pages.shape[0], pages.stride(0), page_size, h, d, table.data_ptr(), table.stride(0), table.shape[1],
-              cu.data_ptr(), lens.data_ptr(), batch, max_new, max_len, total_len,
-              float(scale if scale is not None else d**-0.5), out.data_ptr(), out.stride(0), out.stride(1),
-              workspace.data_ptr(), need, _stream(device))
+        workspace = pages.new_empty(need)
+    _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, qs[0], qs[1], pages.data_ptr(), pages.shape[0],
+              pages.stride(0), page_size, h, d, table.data_ptr(), table.stride(0), columns, cu.data_ptr(),
+              lens.data_ptr(), batch, max_new, max_len, total_len, d**-0.5 if scale is None else float(scale),
+              out.data_ptr(), os_[0], os_[1], workspace.data_ptr(), need, _stream(device))
     return out
 
 
@@ -848,24 +894,28 @@ def verify_drafts(
     k = k1 - 1
     if draft_tokens.shape != (b, k) or accept_u.shape != (b, k) or sample_u.shape != (b,):
         raise ValueError("draft_tokens and accept_u must be [B, K], sample_u [B], target_probs [B, K + 1, V]")
-    if draft_tokens.dtype != torch.int64 or accept_u.dtype != torch.float32 or sample_u.dtype != torch.float32:
+    if draft_tokens.dtype is not torch.int64 or accept_u.dtype is not torch.float32 or sample_u.dtype is not torch.float32:
         raise TypeError("draft_tokens must be int64, accept_u and sample_u float32")
-    if target_probs.stride(2) != 1:
+    ts = target_probs.stride()
+    if ts[2] != 1:
         target_probs = target_probs.contiguous()
+        ts = target_probs.stride()
+    ds = (0, 0)
     if draft_probs is not None:
         if draft_probs.shape != (b, k, vocab) or draft_probs.dtype != target_probs.dtype:
             raise ValueError("draft_probs must be [B, K, V] of target_probs' dtype")
-        if draft_probs.stride(2) != 1:
+        ds = draft_probs.stride()
+        if ds[2] != 1:
             draft_probs = draft_probs.contiguous()
-    if num_drafts is not None and (num_drafts.shape != (b,) or num_drafts.dtype != torch.int32):
-        raise ValueError("num_drafts must be int32 [B]")
+            ds = draft_probs.stride()
+    if num_drafts is not None:
+        if num_drafts.shape != (b,) or num_drafts.dtype is not torch.int32:
+            raise ValueError("num_drafts must be int32 [B]")
+        num_drafts = num_drafts.contiguous()
     draft_tokens, accept_u, sample_u = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
-    num_drafts = None if num_drafts is None else num_drafts.contiguous()
-    tokens = torch.empty((b, k1), dtype=torch.int64, device=device)
+    tokens = draft_tokens.new_empty((b, k1))
     accepted = torch.empty((b,), dtype=torch.int32, device=device)
-    ds = (0, 0) if draft_probs is None else (draft_probs.stride(0), draft_probs.stride(1))
     _lib.call("faq_verify_drafts", draft_tokens.data_ptr(), target_probs.data_ptr(), _ptr(draft_probs),
-              _dtype_code(target_probs), b, k, vocab, target_probs.stride(0), target_probs.stride(1), *ds,
-              accept_u.data_ptr(), sample_u.data_ptr(), _ptr(num_drafts), tokens.data_ptr(), accepted.data_ptr(),
-              _stream(device))
+              _dtype_code(target_probs), b, k, vocab, ts[0], ts[1], ds[0], ds[1], accept_u.data_ptr(),
+              sample_u.data_ptr(), _ptr(num_drafts), tokens.data_ptr(), accepted.data_ptr(), _stream(device))
     return tokens, accepted
