@@ -26,14 +26,15 @@ struct WriteParams {
 };
 
 // HiF4 of eight values: the code word (nibble i = 8 + signed code of value i), the two
-// quarters' exponents and the group's scale byte. All lanes of the warp take part.
+// quarters' exponents and the group's scale byte. All lanes of the warp take part. The
+// arithmetic of hif4.cuh on FP32x2 pairs: t = min(fl(fl(|x| 4qm) + 0.5), 7.5), whose floor is
+// t + 2^23 rounded toward zero; with the sign of x put back, the four codes of a quarter are
+// digits of base 16 that three exact FMAs add up (2^23 + 0x8888 makes them n = 8 + code, and
+// the sum's low 16 bits are the quarter's nibbles).
 __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], int levels, uint32_t& ea, uint32_t& eb,
                                               uint32_t& scale) {
-  float a[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = fabsf(v[i]);
-  const float ma = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-  const float mb = fmaxf(fmaxf(a[4], a[5]), fmaxf(a[6], a[7]));
+  const float ma = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  const float mb = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
   float m1 = fmaxf(ma, mb);
   m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
   m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
@@ -45,45 +46,73 @@ __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], int levels, u
   const float qa = __uint_as_float(rec_q - ea), qb = __uint_as_float(rec_q - eb);  // 4 qm
   ea >>= 23;
   eb >>= 23;
-  uint32_t word = 0;
+  uint32_t quarter[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float m = hif4_code4(a[i], i < 4 ? qa : qb);
-    const float n = __fadd_rn(v[i] < 0.0f ? -m : m, 8388616.0f);  // 2^23 + 8 + signed code
-    word |= (__float_as_uint(n) & 15u) << (4 * i);
+  for (int h = 0; h < 2; ++h) {
+    float c[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x0 = v[4 * h + 2 * i], x1 = v[4 * h + 2 * i + 1], q = h ? qb : qa;
+      float2 t = __fadd2_rn(__fmul2_rn(make_float2(fabsf(x0), fabsf(x1)), make_float2(q, q)), make_float2(0.5f, 0.5f));
+      t = make_float2(fminf(t.x, 7.5f), fminf(t.y, 7.5f));
+      const float2 r = __fadd2_rn(__fadd2_rz(t, make_float2(8388608.0f, 8388608.0f)), make_float2(-8388608.0f, -8388608.0f));
+      c[2 * i] = __uint_as_float(__float_as_uint(r.x) | (__float_as_uint(x0) & 0x80000000u));
+      c[2 * i + 1] = __uint_as_float(__float_as_uint(r.y) | (__float_as_uint(x1) & 0x80000000u));
+    }
+    const float n = __fmaf_rn(c[3], 4096.0f, __fmaf_rn(c[2], 256.0f, __fmaf_rn(c[1], 16.0f, __fadd_rn(c[0], 8423560.0f))));
+    quarter[h] = __float_as_uint(n);
   }
-  return word;
+  return __byte_perm(quarter[0], quarter[1], 0x5410);
 }
 
+// Eight consecutive values as loaded, so that a lane's loads are all in flight before the
+// first of them is quantized.
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, bool vec, float (&v)[8]);
+struct Raw;
 template <>
-__device__ __forceinline__ void load8(const __nv_bfloat16* src, bool vec, float (&v)[8]) {
-  if (vec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+  __device__ __forceinline__ void load(const __nv_bfloat16* src, bool vec) {
+    if (vec) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = __uint_as_float(w[i] << 16);
       v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(src[i]);
   }
-}
+};
 template <>
-__device__ __forceinline__ void load8(const float* src, bool vec, float (&v)[8]) {
-  if (vec) {
-    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
+struct Raw<float> {
+  float f[8];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = src[i];
+    for (int i = 0; i < 8; ++i) f[i] = 0.0f;
   }
-}
-
+  __device__ __forceinline__ void load(const float* src, bool vec) {
+    if (vec) {
+      const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = src[i];
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f[i];
+  }
+};
 
 // Slot -> (sequence, first position of a block, the live tokens [from, to) of the block, the
 // packed token of the block's first position, the number of new tokens at positions below
@@ -117,96 +146,115 @@ __device__ __forceinline__ bool find_slot(const Pages& p, int64_t slot, int64_t 
   return true;
 }
 
+// A warp takes half a block (8 tokens): its loads are then all in flight at once.
+constexpr int WRITE_WARPS = 4;
 template <typename T, int NG>
-__global__ void __launch_bounds__(256) kv_write_kernel(WriteParams w, bool vec) {
+__global__ void __launch_bounds__(32 * WRITE_WARPS, sizeof(T) == 2 ? 8 : 4) kv_write_kernel(WriteParams w, bool vec) {
   grid_dependency_wait();
   allow_dependent_launch();
   const Pages& p = w.p;
   const int lane = threadIdx.x & 31, s = lane & 7;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t slot = item / p.kv_heads;
-  const int head = static_cast<int>(item - slot * p.kv_heads);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * WRITE_WARPS + (threadIdx.x >> 5);
+  const int h = static_cast<int>(item & 1);
+  const int64_t slot = (item >> 1) / p.kv_heads;
+  const int head = static_cast<int>((item >> 1) - slot * p.kv_heads);
   Slot x;
-  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x) || x.to == 0) return;  // warp-uniform
+  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;  // warp-uniform
+  if (x.from >= 8 * (h + 1) || x.to <= 8 * h) return;
   const int64_t page = page_of(p, x.b, x.pos);
   if (page < 0) return;
   uint8_t* kdst = p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, x.pos);
   uint8_t* vdst = p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, x.pos);
-#pragma unroll 1
-  for (int h = 0; h < 2; ++h) {
-    if (x.from >= 8 * (h + 1) || x.to <= 8 * h) continue;  // warp-uniform
-    const int pr = (lane >> 3) + 4 * h;  // tokens 2 pr, 2 pr + 1 of the block
-    const bool live[2] = {2 * pr >= x.from && 2 * pr < x.to, 2 * pr + 1 >= x.from && 2 * pr + 1 < x.to};
-    uint32_t kw[2][NG], vw[2][NG], ve[2][NG];  // [token]; the exponents of all sub-blocks, (a, b) halves
+  const T* ksrc = static_cast<const T*>(w.k) + x.token * w.kt + head * w.kh + 8 * s;
+  const T* vsrc = static_cast<const T*>(w.v) + x.token * w.vt + head * w.vh + 8 * s;
+  const int pr = (lane >> 3) + 4 * h;  // tokens 2 pr, 2 pr + 1 of the block
+  const bool live[2] = {2 * pr >= x.from && 2 * pr < x.to, 2 * pr + 1 >= x.from && 2 * pr + 1 < x.to};
+  Raw<T> rk[2][NG], rv[2][NG];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = 2 * pr + k;
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float vk[8], vv[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vk[i] = vv[i] = 0.0f;
-        if (live[k]) {
-          load8<T>(static_cast<const T*>(w.k) + (x.token + r) * w.kt + head * w.kh + 64 * g + 8 * s, vec, vk);
-          load8<T>(static_cast<const T*>(w.v) + (x.token + r) * w.vt + head * w.vh + 64 * g + 8 * s, vec, vv);
-        }
-        uint32_t ka, kb, ks, va, vb, vs;
-        kw[k][g] = quantize8(vk, w.k_levels, ka, kb, ks);
-        vw[k][g] = quantize8(vv, w.v_levels, va, vb, vs);
-        uint32_t ke = (ka | (kb << 16)) << (2 * s), ve1 = (va | (vb << 16)) << (2 * s);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          ke |= __shfl_xor_sync(0xffffffffu, ke, o);
-          ve1 |= __shfl_xor_sync(0xffffffffu, ve1, o);
-        }
-        ve[k][g] = ve1;
-        if (live[k] && s == 0) {
-          *reinterpret_cast<uint32_t*>(kdst + exp_offset(NG) + (r * NG + g) * 4) = ke;
-          kdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(ks);
-          vdst[scale_offset(NG) + r * NG + g] = static_cast<uint8_t>(vs);
-        }
-      }
-      // K: the even lane of two stores both lanes' words of group 0, the odd one of group 1
-      uint8_t* krow = kdst + 32 * NG * r + (s >> 1) * 8 * NG;
-      if constexpr (NG == 2) {
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, (s & 1) ? kw[k][0] : kw[k][1], 1);
-        if (live[k])
-          *reinterpret_cast<uint2*>(krow + 8 * (s & 1)) = (s & 1) ? make_uint2(other, kw[k][1]) : make_uint2(kw[k][0], other);
-      } else if (live[k]) {
-        *reinterpret_cast<uint32_t*>(krow + 4 * (s & 1)) = kw[k][0];
+    for (int g = 0; g < NG; ++g) {
+      if (live[k]) {
+        rk[k][g].load(ksrc + (2 * pr + k) * w.kt + 64 * g, vec);
+        rv[k][g].load(vsrc + (2 * pr + k) * w.vt + 64 * g, vec);
+      } else {
+        rk[k][g].zero();
+        rv[k][g].zero();
       }
     }
-    // V: words of a quad's halves (token 2 pr, 2 pr + 1)
-    uint8_t* vrow = vdst + 64 * NG * pr + (s ^ (2 * (pr & 3))) * 8 * NG;
-    uint8_t* vexp = vdst + exp_offset(NG) + pr * NG * 8;
-    if (live[0] && live[1]) {
-      uint32_t q[2 * NG];
+  uint32_t vw[2][NG], ve[2][NG];  // [token]; the exponents of all sub-blocks, (a, b) halves
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = 2 * pr + k;
+    if (!__any_sync(0xffffffffu, live[k])) continue;  // a step of one token per sequence
+    uint32_t kw[NG], kx[NG], kscale = 0, vscale = 0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float v[8];
+      uint32_t ea, eb, sc;
+      rk[k][g].values(v);
+      kw[g] = quantize8(v, w.k_levels, ea, eb, sc);
+      kx[g] = (ea | (eb << 16)) << (2 * s);
+      kscale |= sc << (8 * g);
+      rv[k][g].values(v);
+      vw[k][g] = quantize8(v, w.v_levels, ea, eb, sc);
+      ve[k][g] = (ea | (eb << 16)) << (2 * s);
+      vscale |= sc << (8 * g);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        kx[g] |= __shfl_xor_sync(0xffffffffu, kx[g], o);
+        ve[k][g] |= __shfl_xor_sync(0xffffffffu, ve[k][g], o);
+      }
+    }
+    // K: the even lane of two stores both lanes' words of group 0, the odd one of group 1
+    uint8_t* krow = kdst + 32 * NG * r + (s >> 1) * 8 * NG;
+    if constexpr (NG == 2) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, (s & 1) ? kw[0] : kw[1], 1);
+      if (live[k]) {
+        *reinterpret_cast<uint2*>(krow + 8 * (s & 1)) = (s & 1) ? make_uint2(other, kw[1]) : make_uint2(kw[0], other);
+        if (s == 0) *reinterpret_cast<uint2*>(kdst + exp_offset(NG) + r * 8) = make_uint2(kx[0], kx[1]);
+        if (s == 1) *reinterpret_cast<uint16_t*>(kdst + scale_offset(NG) + r * 2) = static_cast<uint16_t>(kscale);
+        if (s == 2) *reinterpret_cast<uint16_t*>(vdst + scale_offset(NG) + r * 2) = static_cast<uint16_t>(vscale);
+      }
+    } else if (live[k]) {
+      *reinterpret_cast<uint32_t*>(krow + 4 * (s & 1)) = kw[0];
+      if (s == 0) *reinterpret_cast<uint32_t*>(kdst + exp_offset(NG) + r * 4) = kx[0];
+      if (s == 1) kdst[scale_offset(NG) + r] = static_cast<uint8_t>(kscale);
+      if (s == 2) vdst[scale_offset(NG) + r] = static_cast<uint8_t>(vscale);
+    }
+  }
+  // V: words of a quad's halves (token 2 pr, 2 pr + 1)
+  uint8_t* vrow = vdst + 64 * NG * pr + (s ^ (2 * (pr & 3))) * 8 * NG;
+  uint8_t* vexp = vdst + exp_offset(NG) + pr * NG * 8;
+  if (live[0] && live[1]) {
+    uint32_t q[2 * NG], e[2 * NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      q[2 * g] = __byte_perm(vw[0][g], vw[1][g], 0x5410);
+      q[2 * g + 1] = __byte_perm(vw[0][g], vw[1][g], 0x7632);
+      e[2 * g] = __byte_perm(ve[0][g], ve[1][g], 0x5410);
+      e[2 * g + 1] = __byte_perm(ve[0][g], ve[1][g], 0x7632);
+    }
+    if constexpr (NG == 2) {
+      *reinterpret_cast<uint4*>(vrow) = make_uint4(q[0], q[1], q[2], q[3]);
+      if (s == 3) *reinterpret_cast<uint4*>(vexp) = make_uint4(e[0], e[1], e[2], e[3]);
+    } else {
+      *reinterpret_cast<uint2*>(vrow) = make_uint2(q[0], q[1]);
+      if (s == 3) *reinterpret_cast<uint2*>(vexp) = make_uint2(e[0], e[1]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!live[k]) continue;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        q[2 * g] = __byte_perm(vw[0][g], vw[1][g], 0x5410);
-        q[2 * g + 1] = __byte_perm(vw[0][g], vw[1][g], 0x7632);
-      }
-      if constexpr (NG == 2)
-        *reinterpret_cast<uint4*>(vrow) = make_uint4(q[0], q[1], q[2], q[3]);
-      else
-        *reinterpret_cast<uint2*>(vrow) = make_uint2(q[0], q[1]);
-      if (s < NG)
-        *reinterpret_cast<uint2*>(vexp + 8 * s) = make_uint2(__byte_perm(ve[0][s ? NG - 1 : 0], ve[1][s ? NG - 1 : 0], 0x5410),
-                                                             __byte_perm(ve[0][s ? NG - 1 : 0], ve[1][s ? NG - 1 : 0], 0x7632));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (!live[k]) continue;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          uint16_t* q = reinterpret_cast<uint16_t*>(vrow + 8 * g + 2 * k);
-          q[0] = static_cast<uint16_t>(vw[k][g]);
-          q[2] = static_cast<uint16_t>(vw[k][g] >> 16);
-          if (s == 0) {
-            uint16_t* e = reinterpret_cast<uint16_t*>(vexp + 8 * g + 2 * k);
-            e[0] = static_cast<uint16_t>(ve[k][g]);
-            e[2] = static_cast<uint16_t>(ve[k][g] >> 16);
-          }
+        uint16_t* q = reinterpret_cast<uint16_t*>(vrow + 8 * g + 2 * k);
+        q[0] = static_cast<uint16_t>(vw[k][g]);
+        q[2] = static_cast<uint16_t>(vw[k][g] >> 16);
+        if (s == 0) {
+          uint16_t* e = reinterpret_cast<uint16_t*>(vexp + 8 * g + 2 * k);
+          e[0] = static_cast<uint16_t>(ve[k][g]);
+          e[2] = static_cast<uint16_t>(ve[k][g] >> 16);
         }
       }
     }
@@ -331,39 +379,41 @@ __device__ __forceinline__ void expand_block_v(const Expand& expand, const uint8
   }
 }
 
-// Zeros for `count` tokens from `token` on, which have no place in the cache.
+// Zeros for `count` tokens' rows, which have no place in the cache.
 template <typename T>
-__device__ __forceinline__ void zero_rows(const ReadParams& w, int64_t token, int64_t count, int head, int d, int lane) {
-  for (int64_t i = token; i < token + count; ++i)
-    for (int c = lane; c < d; c += 32) {
-      static_cast<T*>(w.k)[i * w.kt + head * w.kh + c] = T(0.0f);
-      static_cast<T*>(w.v)[i * w.vt + head * w.vh + c] = T(0.0f);
-    }
+__device__ __forceinline__ void zero_rows(T* rows, int64_t stride, int64_t count, int d, int lane) {
+  for (int64_t i = 0; i < count; ++i)
+    for (int c = lane; c < d; c += 32) rows[i * stride + c] = T(0.0f);
 }
 
+// A warp takes a block of K or of V.
+constexpr int READ_WARPS = 4;
 template <typename T, int NG>
-__global__ void __launch_bounds__(256) kv_read_kernel(ReadParams w, bool vec) {
+__global__ void __launch_bounds__(32 * READ_WARPS) kv_read_kernel(ReadParams w, bool vec) {
   grid_dependency_wait();
   allow_dependent_launch();
   const Pages& p = w.p;
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t slot = item / p.kv_heads;
-  const int head = static_cast<int>(item - slot * p.kv_heads);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * READ_WARPS + (threadIdx.x >> 5);
+  const int which = static_cast<int>(item & 1);
+  const int64_t slot = (item >> 1) / p.kv_heads;
+  const int head = static_cast<int>((item >> 1) - slot * p.kv_heads);
   Slot x;
   if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;
-  T* k = static_cast<T*>(w.k) + x.token * w.kt + head * w.kh;
-  T* v = static_cast<T*>(w.v) + x.token * w.vt + head * w.vh;
+  const int64_t stride = which ? w.vt : w.kt;
+  T* rows = which ? static_cast<T*>(w.v) + head * w.vh : static_cast<T*>(w.k) + head * w.kh;
   const int64_t page = x.to ? page_of(p, x.b, x.pos) : -1;
   if (page >= 0) {
     const Expand expand;
-    const uint8_t* src = p.base + page * p.page_stride;
-    expand_block_k<T, NG>(expand, src + block_in_page<NG>(p, 0, head, x.pos), k, w.kt, x.from, x.to, lane, vec);
-    expand_block_v<T, NG>(expand, src + block_in_page<NG>(p, 1, head, x.pos), v, w.vt, x.from, x.to, lane, vec);
+    const uint8_t* src = p.base + page * p.page_stride + block_in_page<NG>(p, which, head, x.pos);
+    if (which)
+      expand_block_v<T, NG>(expand, src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
+    else
+      expand_block_k<T, NG>(expand, src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
   } else {
-    zero_rows<T>(w, x.token + x.from, x.to - x.from, head, 64 * NG, lane);
+    zero_rows<T>(rows + (x.token + x.from) * stride, stride, x.to - x.from, 64 * NG, lane);
   }
-  if (x.pos == 0) zero_rows<T>(w, p.cu[x.b], x.none, head, 64 * NG, lane);
+  if (x.pos == 0) zero_rows<T>(rows + p.cu[x.b] * stride, stride, x.none, 64 * NG, lane);
 }
 
 // The checks every entry point over pages makes; fills `p`.
@@ -457,11 +507,11 @@ extern "C" int faq_hif4_kv_write(const void* k, const void* v, int dtype, int64_
   const bool vec = aligned16(k) && aligned16(v) && k_token_stride % unit == 0 && k_head_stride % unit == 0 &&
                    v_token_stride % unit == 0 && v_head_stride % unit == 0;
   const int ng = d / 64;
-  const int64_t blocks = (slots_of(total, batch) * kv_heads + 7) / 8;
+  const int64_t blocks = (2 * slots_of(total, batch) * kv_heads + WRITE_WARPS - 1) / WRITE_WARPS;
   FAQ_CHECK_ARG(blocks < (int64_t(1) << 31), "too many tokens for one call");
   auto kern = dtype == FAQ_BF16 ? (ng == 1 ? kv_write_kernel<__nv_bfloat16, 1> : kv_write_kernel<__nv_bfloat16, 2>)
                                 : (ng == 1 ? kv_write_kernel<float, 1> : kv_write_kernel<float, 2>);
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, w, vec));
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(blocks)), 32 * WRITE_WARPS, 0, stream, w, vec));
   return launch_status("kv_write_kernel");
 }
 
@@ -491,10 +541,10 @@ extern "C" int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t pa
   const bool vec = aligned16(k) && aligned16(v) && k_token_stride % unit == 0 && k_head_stride % unit == 0 &&
                    v_token_stride % unit == 0 && v_head_stride % unit == 0;
   const int ng = d / 64;
-  const int64_t blocks = (slots_of(total, batch) * kv_heads + 7) / 8;
+  const int64_t blocks = (2 * slots_of(total, batch) * kv_heads + READ_WARPS - 1) / READ_WARPS;
   FAQ_CHECK_ARG(blocks < (int64_t(1) << 31), "too many tokens for one call");
   auto kern = dtype == FAQ_BF16 ? (ng == 1 ? kv_read_kernel<__nv_bfloat16, 1> : kv_read_kernel<__nv_bfloat16, 2>)
                                 : (ng == 1 ? kv_read_kernel<float, 1> : kv_read_kernel<float, 2>);
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, w, vec));
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(blocks)), 32 * READ_WARPS, 0, stream, w, vec));
   return launch_status("kv_read_kernel");
 }

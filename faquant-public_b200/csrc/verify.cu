@@ -9,7 +9,7 @@
 // weights fit 64 bits. The threshold u sum w is one fp64 product.
 //
 // Bound by reading one row of p and q per sequence; a small batch by its round trips. A
-// cluster of eight CTAs takes a sequence: every warp sums its own contiguous piece (the loads
+// cluster of one to eight CTAs takes a sequence: every warp sums its own contiguous piece (the loads
 // of four steps in flight), the CTAs' sums meet through distributed shared memory, and the CTA
 // whose part holds the threshold reads that warp's piece again (from L2), a step per warp,
 // to find the token. The target's own weights are summed only when nothing is left over.
@@ -18,7 +18,7 @@
 namespace faq {
 namespace ver {
 
-constexpr int CLUSTER = 8, WARPS = 16, THREADS = WARPS * 32;
+constexpr int WARPS = 16, THREADS = WARPS * 32;
 constexpr int STEP = 128;  // weights a warp takes at a time, four per lane
 
 struct Params {
@@ -32,7 +32,17 @@ struct Params {
   int k;
   int64_t vocab;
   bool vec;
+  int cluster;  // CTAs per sequence
 };
+
+// CTAs per sequence: as many (up to 8) as fill the GPU's two CTAs per SM once. More than that
+// run in waves whose gathers and joins leave the memory idle: 128 sequences of 151936 fp32
+// weights took 43 us with clusters of 8 against TODO with 2.
+inline int cluster_of(int64_t batch) {
+  int c = 8;
+  while (c > 1 && batch * c > 2 * num_sms()) c /= 2;
+  return c;
+}
 
 __device__ __forceinline__ float load1(const float* p, int64_t i) { return p[i]; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p, int64_t i) { return __bfloat162float(p[i]); }
@@ -135,13 +145,13 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) __cluster_dims__(CLUSTER, 1, 1) verify_kernel(Params P) {
+__global__ void __launch_bounds__(THREADS, 2) verify_kernel(Params P) {
   __shared__ uint64_t s_warp[WARPS], s_step[WARPS];
   __shared__ uint64_t s_cta[2];  // of the residual, then of the target's row
   __shared__ int s_first;
   grid_dependency_wait();
   allow_dependent_launch();
-  const int b = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
+  const int b = blockIdx.x / P.cluster, rank = blockIdx.x % P.cluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* target = static_cast<const T*>(P.target) + b * P.tb;
   const T* drafter = P.drafter ? static_cast<const T*>(P.drafter) + b * P.qb : nullptr;
@@ -169,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 2) __cluster_dims__(CLUSTER, 1, 1) ve
 
   // each warp's piece: whole steps, in the order (rank, warp)
   const int64_t steps = (P.vocab + STEP - 1) / STEP;
-  const int64_t each = (steps + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
+  const int64_t each = (steps + P.cluster * WARPS - 1) / (P.cluster * WARPS);
   const int64_t s0 = (rank * WARPS + warp) * each, s1 = min(steps, s0 + each);
   uint64_t total = 0, before = 0;
   auto sum_row = [&](int use) {  // the row's total, and what stands before this CTA's part
@@ -184,8 +194,8 @@ __global__ void __launch_bounds__(THREADS, 2) __cluster_dims__(CLUSTER, 1, 1) ve
     __syncthreads();
     cluster_sync();
     total = before = 0;
-#pragma unroll
-    for (int r = 0; r < CLUSTER; ++r) {
+#pragma unroll 1
+    for (int r = 0; r < P.cluster; ++r) {
       uint64_t v;
       asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_addr(&s_cta[use]), r)));
       total += v;
@@ -295,8 +305,19 @@ extern "C" int faq_verify_drafts(const int64_t* draft_tokens, const void* target
   P.vocab = vocab;
   P.vec = aligned16(target_probs) && aligned16(draft_probs) && target_batch_stride % 4 == 0 &&
           target_step_stride % 4 == 0 && draft_batch_stride % 4 == 0 && draft_step_stride % 4 == 0;
-  const dim3 grid(static_cast<unsigned>(batch * CLUSTER));
-  FAQ_CUDA(kvp::launch_early(dtype == FAQ_BF16 ? verify_kernel<__nv_bfloat16> : verify_kernel<float>, grid, THREADS, 0,
-                             stream, P));
+  P.cluster = cluster_of(batch);
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = static_cast<unsigned>(P.cluster);
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(batch * P.cluster));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = attrs;
+  cfg.numAttrs = 2;
+  FAQ_CUDA(cudaLaunchKernelEx(&cfg, dtype == FAQ_BF16 ? verify_kernel<__nv_bfloat16> : verify_kernel<float>, P));
   return launch_status("verify_kernel");
 }
