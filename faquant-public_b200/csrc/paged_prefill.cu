@@ -11,17 +11,20 @@
 //            head, so the keys are read once for the group. Key tiles of 128. The key tiles
 //            of all units are cut into equal runs, one per CTA, as in paged_attention.cu;
 //   combine  joins the partials of units that lie in several runs.
-// In the prefill kernel (384 threads): warps 0-3 the softmax of tile A, 4-7 of tile B, one
-// row per thread; warp 8 loads Q and K by TMA, warp 9 V; warp 10 issues the MMAs. S_t = Q_t K^T
-// goes to 128 columns of tensor memory; the softmax writes P (bf16) over it, from where the
-// tensor core reads it as the A operand of O_t += P_t V (shared memory, which the two
-// products' operands nearly saturate, does not see P). S_t of the next key tile overwrites P_t,
+// In the prefill kernel (640 threads): warps 0-7 the softmax of tile A, 8-15 of tile B, a row's
+// 128 keys split over two threads (four warps per scheduler keep the exponentials busy; with
+// one row per thread and half the warps a step took twice as long); warp 16 loads Q and K by
+// TMA, warp 17 V; warp 18 issues the MMAs. S_t = Q_t K^T goes to 128 columns of tensor memory;
+// the softmax writes P (bf16) over it, from where the tensor core reads it as the A operand
+// of O_t += P_t V (shared memory, which the two products' operands nearly saturate, does not
+// see P). S_t of the next key tile overwrites P_t,
 // so it is issued when that product has completed; the issuing thread takes whichever tile
 // is ready, and the other tile's products fill the wait.
 // Softmax: a row's reference maximum is raised only when a score passes it by more than 2^8
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv_pages.cuh"
 #include "tma.h"
@@ -37,7 +40,7 @@ using pat::RAISE;
 
 constexpr int TILE = 128;            // rows of a tile, keys of a key tile
 constexpr int CHUNK = TILE * 128;    // 128 rows of 64 channels
-constexpr int THREADS = 384;
+constexpr int THREADS = 640;
 constexpr int COST = 3;              // of a unit beyond its key tiles (filling, joining), in key tiles
 constexpr int ROWS = 2 * TILE;
 
@@ -275,7 +278,8 @@ struct Smem {
   static constexpr int q = 0;
   static constexpr int k = q + 2 * tile;
   static constexpr int v = k + 2 * tile;
-  static constexpr int bar = v + 2 * tile;
+  static constexpr int x = v + 2 * tile;  // what the halves of a row exchange: [2][2 tiles][2 halves][128] fp32
+  static constexpr int bar = x + 4096;
   static constexpr int bytes = 1024 + bar + 256;
 };
 constexpr int TMEM_COLS = 512;
@@ -292,7 +296,37 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// MMAs and commits by one elected lane of a warp that executes them as a whole.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p, e; .reg .b64 ad, bd; setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 ad, {%1, %5}; mov.b64 bd, {%2, %5};\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p; }" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(SW128_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p, e; .reg .b64 bd; setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 bd, {%2, %5};\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p; }" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(SW128_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred e; elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar)
+      : "memory");
+}
 
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -312,7 +346,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_full = bars + 10;  // [2 tiles] S_t computed
   uint64_t* p_full = bars + 12;  // P_t written (and O_t rescaled) by the tile's four warps
   uint64_t* pv_done = bars + 14; // O_t += P_t V completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  uint64_t* met = bars + 16;     // [2 tiles][4 quarters] both halves' warps have read S_t
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  float* s_x = reinterpret_cast<float*>(base + L::x);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(q_full), 1);
@@ -323,15 +359,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(smem_addr(&v_full[i]), 1);
       mbar_init(smem_addr(&v_empty[i]), 2);
       mbar_init(smem_addr(&s_full[i]), 1);
-      mbar_init(smem_addr(&p_full[i]), 4);
+      mbar_init(smem_addr(&p_full[i]), 8);
       mbar_init(smem_addr(&pv_done[i]), 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(smem_addr(&met[i]), 2);
     fence_barrier_init();
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
-  if (warp == 10) {
+  if (warp == 18) {
     tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
@@ -347,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   // whether tile B has rows
   auto two_tiles = [&](const Segment& g) { return g.tok0 + P.tile_tokens < g.n; };
 
-  // Registers: 384 x 168 at launch = 256 x 208 + 128 x 88.
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::: "memory");
-    if (warp == 8) {
+  // Registers: 640 x 96 at launch = 512 x 104 + 128 x 64.
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::: "memory");
+    if (warp == 16) {
       if (lane == 0) {
         bool ok = true;
         int step = 0;
@@ -377,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int x = std::max(0, step - 2); x < step; ++x)
           if (!mbar_wait_site(smem_addr(&k_empty[x & 1]), (x >> 1) & 1, 53, x)) break;
       }
-    } else if (warp == 9) {
+    } else if (warp == 17) {
       if (lane == 0) {
         bool ok = true;
         int step = 0;
@@ -395,87 +432,120 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int x = std::max(0, step - 2); x < step; ++x)
           if (!mbar_wait_site(smem_addr(&v_empty[x & 1]), (x >> 1) & 1, 54, x)) break;
       }
-    } else if (warp == 10) {
-      if (lane == 0) {
-        const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
-        const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
-        const uint32_t v_desc = sw128_desc_lo(smem_addr(base + L::v), CHUNK);
-        constexpr uint32_t TILE_D = L::tile >> 4;
-        int ring = 0;                // key tiles before this segment
-        uint32_t done[2] = {0, 0};   // steps of each tile so far
-        bool ok = true;
-        for (int i = 0; i < nseg && ok; ++i) {
-          const int n = segments[i].count;
-          const int tiles = two_tiles(segments[i]) ? 2 : 1;
-          if (!mbar_wait_site(smem_addr(q_full), i & 1, 55, i)) break;
-          int qk[2] = {0, 0}, pv[2] = {0, 0};  // issued
-          bool q_read = false;
-          uint64_t since = 0;
-          uint32_t misses = 0;
-          while (pv[0] < n || (tiles == 2 && pv[1] < n)) {
-            bool moved = false;
+    } else if (warp == 18) {
+      // The whole warp walks this loop and one elected lane issues each instruction, so that
+      // addresses and descriptors stay in uniform registers: with one lane in the loop an MMA
+      // took 85 cycles to issue (64 to run), beside warps that want the same issue slots.
+      const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
+      const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
+      const uint32_t v_desc = sw128_desc_lo(smem_addr(base + L::v), CHUNK);
+      constexpr uint32_t TILE_D = L::tile >> 4;
+      auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(smem_addr(bar), parity)); };
+      // S_t = Q_t K^T with K in stage st; t and st are constants
+      auto issue_qk = [&](auto tile, auto stage) {
+        constexpr int t = decltype(tile)::value, st = decltype(stage)::value;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (t >= tiles) continue;
-              if (qk[t] == pv[t] && qk[t] < n) {  // S_t = Q_t K^T: over P_t, once its product is done
-                const int step = ring + qk[t], st = step & 1;
-                if (mbar_test(smem_addr(&k_full[st]), (step >> 1) & 1) &&
-                    (done[t] == 0 || mbar_test(smem_addr(&pv_done[t]), (done[t] - 1) & 1))) {
-                  tc_fence_after();
-                  const uint32_t a = q_desc + t * TILE_D, b = k_desc + st * TILE_D, d = tmem + s_col(t);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          constexpr uint32_t a0 = t * TILE_D, b0 = st * TILE_D;
+          const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + s_col(t), q_desc + a0 + off, k_desc + b0 + off, IDESC_QK, kk != 0);
+        }
+        commit(smem_addr(&s_full[t]));
+        commit(smem_addr(&k_empty[st]));
+      };
+      // O_t += P_t V with V in stage st
+      auto issue_pv = [&](auto tile, auto stage, bool add) {
+        constexpr int t = decltype(tile)::value, st = decltype(stage)::value;
 #pragma unroll
-                  for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
-                    tc_mma_f16_lo(d, a + off, b + off, IDESC_QK, kk != 0);
-                  }
-                  tc_commit(smem_addr(&s_full[t]));
-                  tc_commit(smem_addr(&k_empty[st]));
-                  if (tiles == 1) tc_commit(smem_addr(&k_empty[st]));  // for the tile that is not there
-                  ++qk[t];
-                  moved = true;
-                }
-              } else if (qk[t] > pv[t]) {  // O_t += P_t V
-                const int step = ring + pv[t], st = step & 1;
-                if (mbar_test(smem_addr(&p_full[t]), done[t] & 1) && mbar_test(smem_addr(&v_full[st]), (step >> 1) & 1)) {
-                  tc_fence_after();
-                  const uint32_t b = v_desc + st * TILE_D, d = tmem + o_col(t), a = tmem + s_col(t);
-#pragma unroll
-                  for (int kk = 0; kk < TILE / 16; ++kk)
-                    tc_mma_f16_ts_lo(d, a + kk * 8, b + ((kk * 2048) >> 4), idesc_pv(D), (pv[t] | kk) != 0);
-                  tc_commit(smem_addr(&pv_done[t]));
-                  tc_commit(smem_addr(&v_empty[st]));
-                  if (tiles == 1) tc_commit(smem_addr(&v_empty[st]));
-                  ++pv[t];
-                  ++done[t];
-                  moved = true;
-                }
+        for (int kk = 0; kk < TILE / 16; ++kk)
+          mma_ts(tmem + o_col(t), tmem + s_col(t) + kk * 8, v_desc + st * TILE_D + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
+        commit(smem_addr(&pv_done[t]));
+        commit(smem_addr(&v_empty[st]));
+      };
+      const std::integral_constant<int, 0> c0;
+      const std::integral_constant<int, 1> c1;
+      int ring = 0;                 // key tiles before this segment
+      uint32_t done0 = 0, done1 = 0;  // steps of each tile so far
+      bool ok = true;
+      for (int i = 0; i < nseg && ok; ++i) {
+        const int n = __shfl_sync(0xffffffffu, segments[i].count, 0);
+        const bool two = __all_sync(0xffffffffu, two_tiles(segments[i]));
+        if (!mbar_wait_warp(smem_addr(q_full), i & 1, 55, i)) break;
+        int qk0 = 0, pv0 = 0, qk1 = two ? 0 : n, pv1 = two ? 0 : n;  // issued
+        bool q_read = false;
+        uint64_t since = 0;
+        uint32_t misses = 0;
+        while (pv0 < n || pv1 < n) {
+          bool moved = false;
+          // tile t's next product, if its operands are there: S_t over P_t once P_t's is done, else O_t
+          auto advance = [&](auto tile, int& qk, int& pv, uint32_t& done) {
+            constexpr int t = decltype(tile)::value;
+            if (qk == pv && qk < n) {
+              const int step = ring + qk;
+              if ((done == 0 || ready(&pv_done[t], (done - 1) & 1)) && ready(&k_full[step & 1], (step >> 1) & 1)) {
+                tc_fence_after();
+                if (step & 1) issue_qk(tile, c1); else issue_qk(tile, c0);
+                if (!two) commit(smem_addr(&k_empty[step & 1]));  // for the tile that is not there
+                ++qk;
+                moved = true;
+              }
+            } else if (qk > pv) {
+              const int step = ring + pv;
+              if (ready(&p_full[t], done & 1) && ready(&v_full[step & 1], (step >> 1) & 1)) {
+                tc_fence_after();
+                if (step & 1) issue_pv(tile, c1, pv != 0); else issue_pv(tile, c0, pv != 0);
+                if (!two) commit(smem_addr(&v_empty[step & 1]));
+                ++pv;
+                ++done;
+                moved = true;
               }
             }
-            if (!q_read && qk[0] == n && (tiles == 1 || qk[1] == n)) {
-              tc_commit(smem_addr(q_empty));  // the next unit's Q may come
-              q_read = true;
-            }
-            if (moved) {
-              misses = 0;
-            } else if (++misses == 256) {
-              since = globaltimer();
-            } else if ((misses & 255) == 0 && globaltimer() - since > kWaitLimitNs) {
-              report_timeout();
-              trace_timeout(56, ring + pv[0]);
-              ok = false;
-              break;
-            }
+          };
+          advance(c0, qk0, pv0, done0);
+          advance(c1, qk1, pv1, done1);
+          if (!q_read && qk0 == n && qk1 == n) {
+            commit(smem_addr(q_empty));  // the next unit's Q may come
+            q_read = true;
           }
-          ring += n;
+          if (moved) {
+            misses = 0;
+          } else if (++misses == 256) {
+            since = globaltimer();
+          } else if ((misses & 255) == 0 && __any_sync(0xffffffffu, globaltimer() - since > kWaitLimitNs)) {
+            if (lane == 0) {
+              report_timeout();
+              trace_timeout(56, ring + pv0);
+            }
+            ok = false;
+            break;
+          }
         }
+        ring += n;
       }
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::: "memory");
-    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
+    const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + s_col(t), o_addr = tmem + lanes + o_col(t);
+    const uint32_t s_addr = tmem + lanes + s_col(t) + 64 * half;   // this half's 64 keys
+    const uint32_t p_addr = tmem + lanes + s_col(t) + 32 * half;   // and their P, two to a column
+    const uint32_t o_addr = tmem + lanes + o_col(t) + D / 2 * half;  // this half's channels
+    const uint32_t met_bar = smem_addr(&met[t * 4 + quarter]);
+    float* x_mine = s_x + (t * 2 + half) * TILE + row;         // + 512 floats on odd meetings
+    const float* x_other = s_x + (t * 2 + (half ^ 1)) * TILE + row;
+    uint32_t meetings = 0;
+    // this thread's value for the row's other half's
+    auto exchange = [&](float mine, float& other, int site) {
+      const int buffer = (meetings & 1) * 4 * TILE;
+      x_mine[buffer] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(met_bar);
+      const bool there = mbar_wait_warp(met_bar, meetings & 1, site, meetings);
+      other = x_other[buffer];
+      ++meetings;
+      return there;
+    };
     const float2 c2 = make_float2(P.scale_log2, P.scale_log2);
     const int row_tok = row / P.group, row_head = row - row_tok * P.group;
     uint32_t done = 0;  // steps of this tile so far
@@ -490,28 +560,33 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int j = 0; j < g.count; ++j, ++done) {
         if (!mbar_wait_warp(smem_addr(&s_full[t]), done & 1, 57 + t, j)) { ok = false; break; }
         tc_fence_after();
-        float f[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32f(s_addr + 32 * c, f + 32 * c);
+        float f[64];
+        tmem_ld32f(s_addr, f);
+        tmem_ld32f(s_addr + 32, f + 32);
         tc_wait_ld();
+        reg_fence32f(f);
+        reg_fence32f(f + 32);
+        const int rel = lim - (g.k0 + j) * TILE - 64 * half;
+        if (__any_sync(0xffffffffu, rel < 63)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) reg_fence32f(f + 32 * c);
-        const int rel = lim - (g.k0 + j) * TILE;
-        if (__any_sync(0xffffffffu, rel < TILE - 1)) {
-#pragma unroll
-          for (int x = 0; x < 128; ++x)
+          for (int x = 0; x < 64; ++x)
             if (x > rel) f[x] = -INFINITY;
         }
-        float mx[8];
+        float mx[4];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          mx[c] = fmaxf(f[16 * c], f[16 * c + 1]);
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = max3(f[16 * c], f[16 * c + 1], f[16 * c + 2]);
 #pragma unroll
-          for (int x = 2; x < 16; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
+          for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
         }
-        const float top = __fmul_rn(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])),
-                                    P.scale_log2);
-        if (__any_sync(0xffffffffu, top > m + RAISE)) {
+        const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
+        float other;
+        // also: both halves have read S_t, so P_t may be written over it
+        tc_fence_before();
+        if (!exchange(mine, other, 63 + t)) { ok = false; break; }
+        tc_fence_after();
+        const float top = __fmul_rn(fmaxf(mine, other), P.scale_log2);
+        if (__any_sync(0xffffffffu, top > m + RAISE)) {  // the same rows in both halves' warps
           const float next = fmaxf(top, m);
           const float a = ex2(m - next);
           m = next;
@@ -521,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_after();
             const float2 a2 = make_float2(a, a);
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 64; ++c) {
               float o[32];
               tmem_ld32f(o_addr + 32 * c, o);
               tc_wait_ld();
@@ -538,18 +613,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const float2 mneg = make_float2(-m, -m);
         float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float w[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float w[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const float2 d = __ffma2_rn(make_float2(f[64 * c + 2 * x], f[64 * c + 2 * x + 1]), c2, mneg);
-            const float2 e = make_float2(ex2(d.x), ex2(d.y));
-            sum[x & 3] = __fadd2_rn(sum[x & 3], e);
-            w[x] = __uint_as_float(pack_bf16(e.x, e.y));
-          }
-          tmem_st32f(s_addr + 32 * c, w);
+        for (int x = 0; x < 32; ++x) {
+          const float2 d = __ffma2_rn(make_float2(f[2 * x], f[2 * x + 1]), c2, mneg);
+          const float2 e = make_float2(ex2(d.x), ex2(d.y));
+          sum[x & 3] = __fadd2_rn(sum[x & 3], e);
+          w[x] = __uint_as_float(pack_bf16(e.x, e.y));
         }
+        tmem_st32f(p_addr, w);
         const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
         l += s4.x + s4.y;
         tc_wait_st();
@@ -557,19 +629,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&p_full[t]));
       }
-      if (!ok || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) { ok = false; break; }
+      float other;
+      if (!ok || !exchange(l, other, 65 + t) || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
+      l = half ? other + l : l + other;  // the same sum in both halves
       const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
       float* part = g.slot < 0 ? nullptr : P.parts + static_cast<int64_t>(g.slot) * (ROWS * D + 2 * ROWS);
-      __nv_bfloat16* dst = P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh;
+      __nv_bfloat16* dst =
+          P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh + D / 2 * half;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
         float o[32];
         tmem_ld32f(o_addr + 32 * c, o);
         tc_wait_ld();
         reg_fence32f(o);
         if (live && part) {
-          float4* d4 = reinterpret_cast<float4*>(part + (t * TILE + row) * D + 32 * c);
+          float4* d4 = reinterpret_cast<float4*>(part + (t * TILE + row) * D + D / 2 * half + 32 * c);
 #pragma unroll
           for (int x = 0; x < 8; ++x) d4[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
         } else if (live) {
@@ -582,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         __syncwarp();  // the loads above are made by whole warps
       }
-      if (part && live) {
+      if (part && live && half == 0) {
         part[ROWS * D + t * TILE + row] = m;
         part[ROWS * D + ROWS + t * TILE + row] = l;
       }
@@ -590,7 +668,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 18) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
