@@ -12,14 +12,13 @@
 //            of all units are cut into equal runs, one per CTA, as in paged_attention.cu;
 //   combine  joins the partials of units that lie in several runs.
 // In the prefill kernel (640 threads): warps 0-7 the softmax of tile A, 8-15 of tile B, a row's
-// 128 keys split over two threads (four warps per scheduler keep the exponentials busy; with
-// one row per thread and half the warps a step took twice as long); warp 16 loads Q and K by
-// TMA, warp 17 V; warp 18 issues the MMAs. S_t = Q_t K^T goes to 128 columns of tensor memory;
-// the softmax writes P (bf16) over it, from where the tensor core reads it as the A operand
-// of O_t += P_t V (shared memory, which the two products' operands nearly saturate, does not
-// see P). S_t of the next key tile overwrites P_t,
-// so it is issued when that product has completed; the issuing thread takes whichever tile
-// is ready, and the other tile's products fill the wait.
+// 128 keys split over two threads (each reads the other's scores too, for the maximum); warp
+// 16 loads Q and K by TMA, warp 17 V; warp 18 issues the MMAs. S_t = Q_t K^T and O_t take 128
+// columns of tensor memory each, all there is at d = 128. The softmax warps release S_t as
+// soon as it is in their registers, so the next S_t is computed under their exponentials, and
+// write P_t (bf16) to shared memory as the A operand of O_t += P_t V. (P_t in tensor memory,
+// over S_t, saves shared-memory traffic but chains the next S_t behind this product: 4700
+// cycles per key tile against TODO.)
 // Softmax: a row's reference maximum is raised only when a score passes it by more than 2^8
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
 #include <algorithm>
@@ -43,6 +42,7 @@ constexpr int CHUNK = TILE * 128;    // 128 rows of 64 channels
 constexpr int THREADS = 640;
 constexpr int COST = 3;              // of a unit beyond its key tiles (filling, joining), in key tiles
 constexpr int ROWS = 2 * TILE;
+constexpr int EXPAND_WARPS = 4;      // of a CTA of the expansion
 
 struct Segment {  // a run's part of one unit
   int c0, head, tok0;       // first token of the sequence in q; kv head; first token of the unit
@@ -124,17 +124,18 @@ __device__ __forceinline__ int64_t block_scan(int64_t mine, int64_t* scratch, in
 // One CTA: the segments of every run. Units in the order (sequence, token block, kv head);
 // segment of unit u in run c at index c + u.
 __device__ void make_plan(const Params& P) {
-  __shared__ int64_t s_scratch[8];
+  constexpr int N = 32 * EXPAND_WARPS;
+  __shared__ int64_t s_scratch[EXPAND_WARPS];
   __shared__ int64_t s_cost, s_units, s_keys;  // before the sequence (and round of units) at hand
   const int tid = threadIdx.x;
   const int h = P.p.kv_heads;
-  for (int c = tid; c < P.runs; c += 256) {
+  for (int c = tid; c < P.runs; c += N) {
     P.run[c] = make_int2(0x7fffffff, 0);
     P.joins[c].first = -1;
   }
   // totals
   int64_t cost = 0;
-  for (int b = tid; b < P.p.batch; b += 256) {
+  for (int b = tid; b < P.p.batch; b += N) {
     const Seq s = sequence(P, b);
     for (int u = 0; u < (s.n ? units_of(P, s) : 0); ++u) {
       const int kt = key_tiles(P, s, u);
@@ -142,7 +143,7 @@ __device__ void make_plan(const Params& P) {
     }
   }
   int64_t total;
-  block_scan<8>(cost, s_scratch, &total);
+  block_scan<EXPAND_WARPS>(cost, s_scratch, &total);
   const int64_t per = std::max<int64_t>((total + P.runs - 1) / P.runs, COST + 2);
   if (tid == 0) s_cost = s_units = s_keys = 0;
   __syncthreads();
@@ -153,12 +154,12 @@ __device__ void make_plan(const Params& P) {
     const int64_t key_row = s_keys;
     const bool fits = key_row + padded(s) <= P.cap && s_units + static_cast<int64_t>(nu) * h <= P.max_units;
     if (!fits && tid == 0) atomicOr(&g_status, FAQ_STATUS_BAD_BOUND);
-    for (int u0 = 0; u0 < nu; u0 += 256) {
+    for (int u0 = 0; u0 < nu; u0 += N) {
       const int u = u0 + tid;
       const int kt = u < nu && fits ? key_tiles(P, s, u) : 0;
       int64_t cost_sum, unit_sum;
-      const int64_t at0 = s_cost + block_scan<8>(kt ? static_cast<int64_t>(kt + COST) * h : 0, s_scratch, &cost_sum);
-      const int64_t id0 = s_units + block_scan<8>(kt ? h : 0, s_scratch, &unit_sum);
+      const int64_t at0 = s_cost + block_scan<EXPAND_WARPS>(kt ? static_cast<int64_t>(kt + COST) * h : 0, s_scratch, &cost_sum);
+      const int64_t id0 = s_units + block_scan<EXPAND_WARPS>(kt ? h : 0, s_scratch, &unit_sum);
       for (int hk = 0; kt && hk < h; ++hk) {
         const int64_t at = at0 + static_cast<int64_t>(hk) * (kt + COST), first = at + COST, end = first + kt;
         const int64_t id = id0 + hk;
@@ -201,74 +202,69 @@ __device__ void make_plan(const Params& P) {
 }
 
 // ---------------------------------------------------------------- expand
-// Work items: (key tile of 128 tokens, kv head), a block of 16 tokens per warp. The last CTA
-// makes the plan.
+// A warp takes a block of K or of V; it finds its sequence by a prefix over the sequences' key
+// tiles, 32 sequences at a time. The first CTA makes the plan.
 template <int NG>
-__global__ void __launch_bounds__(256) paged_expand_kernel(Params P) {
+__global__ void __launch_bounds__(32 * EXPAND_WARPS) paged_expand_kernel(Params P) {
   constexpr int D = 64 * NG;
   grid_dependency_wait();
   allow_dependent_launch();
-  if (blockIdx.x == gridDim.x - 1) {
+  if (blockIdx.x == 0) {
     make_plan(P);
     return;
   }
-  __shared__ int64_t s_scratch[8];
-  __shared__ int64_t s_tiles[257];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int h = P.p.kv_heads, ctas = gridDim.x - 1;
-  const Expand expand;
-  int64_t base = 0, next = blockIdx.x;  // tiles before these sequences; this CTA's next item
-  for (int b0 = 0; b0 < P.p.batch; b0 += 256) {
-    Seq mine = {0, 0};
-    if (b0 + tid < P.p.batch) mine = sequence(P, b0 + tid);
-    int64_t sum;
-    const int64_t before = block_scan<8>(padded(mine) / TILE, s_scratch, &sum);
-    __syncthreads();
-    s_tiles[tid] = before;
-    if (tid == 0) s_tiles[256] = sum;
-    __syncthreads();
-    for (; next < (base + sum) * h; next += ctas) {
-      const int64_t q = next / h - base;
-      const int head = static_cast<int>(next % h);
-      int lo = 0, hi = 256;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_tiles[mid] <= q) lo = mid; else hi = mid;
-      }
-      const int b = b0 + lo;
-      const Seq s = sequence(P, b);
-      const int pos = static_cast<int>(q - s_tiles[lo]) * TILE + warp * BLOCK;
-      const int64_t row = (base + q) * TILE + warp * BLOCK;
-      if (row + BLOCK > P.cap) continue;  // recorded by the plan
-      const int64_t page = pos < s.len ? page_of(P.p, b, pos) : -1;
-      const int have = page < 0 ? 0 : min(BLOCK, s.len - pos);
-      const int64_t stride = static_cast<int64_t>(h) * D;
-      __nv_bfloat16* k = P.k + row * stride + head * D;
-      __nv_bfloat16* v = P.v + row * stride + head * D;
-      if (have) {
-        const uint8_t* unit = P.p.base + page * P.p.page_stride;
-        expand_block_k<__nv_bfloat16, NG>(expand, unit + block_in_page<NG>(P.p, 0, head, pos), k, stride, 0, have, lane);
-        expand_block_v<__nv_bfloat16, NG>(expand, unit + block_in_page<NG>(P.p, 1, head, pos), v, stride, 0, have, lane);
-      }
-      for (int i = have * (D / 8) + lane; i < BLOCK * (D / 8); i += 32) {  // zeros behind the end
-        *reinterpret_cast<uint4*>(k + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(v + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
-      }
+  const int lane = threadIdx.x & 31, h = P.p.kv_heads;
+  // rows that see no key are zero
+  for (int b = blockIdx.x - 1; b < P.p.batch; b += gridDim.x - 1) {
+    const Seq s = sequence(P, b);
+    const int none = min(s.n, s.n - s.len), heads = P.group * h;
+    for (int64_t x = threadIdx.x; x < static_cast<int64_t>(none) * heads * (D / 8); x += blockDim.x) {
+      const int64_t r = x / (D / 8);
+      *reinterpret_cast<uint4*>(P.out + (P.p.cu[b] + r / heads) * P.ot + (r % heads) * P.oh + x % (D / 8) * 8) =
+          make_uint4(0, 0, 0, 0);
     }
-    base += sum;
-    // rows of these sequences that see no key are zero
-    for (int i = 0; i < 256 && b0 + i < P.p.batch; ++i) {
-      if ((b0 + i) % ctas != blockIdx.x) continue;
-      const Seq s = sequence(P, b0 + i);
-      const int none = min(s.n, s.n - s.len), heads = P.group * h;
-      for (int64_t x = tid; x < static_cast<int64_t>(none) * heads * (D / 8); x += 256) {
-        const int64_t r = x / (D / 8);
-        *reinterpret_cast<uint4*>(P.out + (P.p.cu[b0 + i] + r / heads) * P.ot + (r % heads) * P.oh + x % (D / 8) * 8) =
-            make_uint4(0, 0, 0, 0);
-      }
-    }
-    __syncthreads();
   }
+  const int64_t item = static_cast<int64_t>(blockIdx.x - 1) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int which = static_cast<int>(item & 1), head = static_cast<int>((item >> 1) % h);
+  const int64_t block = (item >> 1) / h, row = block * BLOCK;  // of the workspace
+  if (row + BLOCK > P.cap) return;
+  int64_t before = 0;  // rows of the sequences before
+  int b = -1, pos = 0, len = 0;
+  for (int b0 = 0; b0 < P.p.batch; b0 += 32) {
+    Seq s = {0, 0};
+    if (b0 + lane < P.p.batch) s = sequence(P, b0 + lane);
+    const int64_t mine = padded(s);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, row < before + upto);
+    if (past) {
+      const int who = __ffs(past) - 1;
+      b = b0 + who;
+      pos = static_cast<int>(row - before - __shfl_sync(0xffffffffu, upto - mine, who));
+      len = __shfl_sync(0xffffffffu, s.len, who);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (b < 0) return;
+  const int64_t page = pos < len ? page_of(P.p, b, pos) : -1;
+  const int have = page < 0 ? 0 : min(BLOCK, len - pos);
+  const int64_t stride = static_cast<int64_t>(h) * D;
+  __nv_bfloat16* dst = (which ? P.v : P.k) + row * stride + head * D;
+  if (have) {
+    const Expand expand;
+    const uint8_t* src = P.p.base + page * P.p.page_stride + block_in_page<NG>(P.p, which, head, pos);
+    if (which)
+      expand_block_v<__nv_bfloat16, NG>(expand, src, dst, stride, 0, have, lane);
+    else
+      expand_block_k<__nv_bfloat16, NG>(expand, src, dst, stride, 0, have, lane);
+  }
+  for (int i = have * (D / 8) + lane; i < BLOCK * (D / 8); i += 32)  // zeros behind the end
+    *reinterpret_cast<uint4*>(dst + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // ---------------------------------------------------------------- attention
@@ -277,25 +273,17 @@ struct Smem {
   static constexpr int tile = NG * CHUNK;  // bytes of a Q, K or V tile
   static constexpr int q = 0;
   static constexpr int k = q + 2 * tile;
-  static constexpr int v = k + 2 * tile;
-  static constexpr int x = v + 2 * tile;  // what the halves of a row exchange: [2][2 tiles][2 halves][128] fp32
-  static constexpr int bar = x + 4096;
+  static constexpr int v = k + 2 * tile;     // one stage
+  static constexpr int p = v + tile;         // P of both tiles; after a unit's last product, its row sums
+  static constexpr int bar = p + 4 * CHUNK;
   static constexpr int bytes = 1024 + bar + 256;
 };
 constexpr int TMEM_COLS = 512;
-__device__ __forceinline__ uint32_t s_col(int t) { return 128u * t; }        // S_t, then P_t in its first 64
+__device__ __forceinline__ uint32_t s_col(int t) { return 128u * t; }        
 __device__ __forceinline__ uint32_t o_col(int t) { return 256u + 128u * t; }
 constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, TILE, false, false);
 constexpr uint32_t idesc_pv(int d) { return idesc_bf16_f32(TILE, d, false, true); }
 
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-               : "=r"(done)
-               : "r"(bar), "r"(parity)
-               : "memory");
-  return done != 0;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -310,15 +298,6 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo,
       "elect.sync _|e, 0xffffffff;\n"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p; }" ::"r"(d),
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(SW128_DESC_HI)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p, e; .reg .b64 bd; setp.ne.b32 p, %4, 0;\n"
-      "mov.b64 bd, {%2, %5};\n"
-      "elect.sync _|e, 0xffffffff;\n"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p; }" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(SW128_DESC_HI)
       : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -340,29 +319,30 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* q_full = bars + 0;
   uint64_t* q_empty = bars + 1;
   uint64_t* k_full = bars + 2;   // [2 stages]
-  uint64_t* k_empty = bars + 4;  // both tiles' products have read the stage
+  uint64_t* k_empty = bars + 4;
   uint64_t* v_full = bars + 6;
-  uint64_t* v_empty = bars + 8;
-  uint64_t* s_full = bars + 10;  // [2 tiles] S_t computed
-  uint64_t* p_full = bars + 12;  // P_t written (and O_t rescaled) by the tile's four warps
+  uint64_t* v_empty = bars + 7;
+  uint64_t* s_full = bars + 8;   // [2 tiles] S_t computed
+  uint64_t* s_free = bars + 10;  // S_t in the registers of the tile's eight warps
+  uint64_t* p_full = bars + 12;  // P_t written (and O_t rescaled) by them
   uint64_t* pv_done = bars + 14; // O_t += P_t V completed
-  uint64_t* met = bars + 16;     // [2 tiles][4 quarters] both halves' warps have read S_t
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
-  float* s_x = reinterpret_cast<float*>(base + L::x);
+  uint64_t* sums = bars + 16;    // [2 tiles] a unit's row sums are there (even phases), read (odd)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(q_full), 1);
     mbar_init(smem_addr(q_empty), 1);
+    mbar_init(smem_addr(v_full), 1);
+    mbar_init(smem_addr(v_empty), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&k_full[i]), 1);
-      mbar_init(smem_addr(&k_empty[i]), 2);
-      mbar_init(smem_addr(&v_full[i]), 1);
-      mbar_init(smem_addr(&v_empty[i]), 2);
+      mbar_init(smem_addr(&k_empty[i]), 1);
       mbar_init(smem_addr(&s_full[i]), 1);
+      mbar_init(smem_addr(&s_free[i]), 8);
       mbar_init(smem_addr(&p_full[i]), 8);
       mbar_init(smem_addr(&pv_done[i]), 1);
+      mbar_init(smem_addr(&sums[i]), 8);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(smem_addr(&met[i]), 2);
     fence_barrier_init();
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
@@ -421,16 +401,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int i = 0; i < nseg && ok; ++i) {
           const Segment g = segments[i];
           for (int j = 0; j < g.count; ++j, ++step) {
-            const int st = step & 1;
-            if (!mbar_wait_site(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 52, step)) { ok = false; break; }
-            mbar_arrive_expect_tx(smem_addr(&v_full[st]), L::tile);
+            if (!mbar_wait_site(smem_addr(v_empty), (step & 1) ^ 1, 52, step)) { ok = false; break; }
+            mbar_arrive_expect_tx(smem_addr(v_full), L::tile);
             for (int c = 0; c < NG; ++c)
-              tma_load_3d(smem_addr(base + L::v + st * L::tile + c * CHUNK), &tmap_v, smem_addr(&v_full[st]), c * 64,
-                          g.head, g.key_row + (g.k0 + j) * TILE);
+              tma_load_3d(smem_addr(base + L::v + c * CHUNK), &tmap_v, smem_addr(v_full), c * 64, g.head,
+                          g.key_row + (g.k0 + j) * TILE);
           }
         }
-        for (int x = std::max(0, step - 2); x < step; ++x)
-          if (!mbar_wait_site(smem_addr(&v_empty[x & 1]), (x >> 1) & 1, 54, x)) break;
+        if (step > 0) mbar_wait_site(smem_addr(v_empty), (step - 1) & 1, 54, step);
       }
     } else if (warp == 18) {
       // The whole warp walks this loop and one elected lane issues each instruction, so that
@@ -439,11 +417,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
       const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
       const uint32_t v_desc = sw128_desc_lo(smem_addr(base + L::v), CHUNK);
+      const uint32_t p_desc = sw128_desc_lo(smem_addr(base + L::p), 16);
       constexpr uint32_t TILE_D = L::tile >> 4;
-      auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(smem_addr(bar), parity)); };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site, int step) {
+        return mbar_wait_warp(smem_addr(bar), parity & 1, site, step);
+      };
       // S_t = Q_t K^T with K in stage st; t and st are constants
       auto issue_qk = [&](auto tile, auto stage) {
         constexpr int t = decltype(tile)::value, st = decltype(stage)::value;
+        tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           constexpr uint32_t a0 = t * TILE_D, b0 = st * TILE_D;
@@ -451,76 +433,59 @@ __global__ void __launch_bounds__(THREADS, 1)
           mma_ss(tmem + s_col(t), q_desc + a0 + off, k_desc + b0 + off, IDESC_QK, kk != 0);
         }
         commit(smem_addr(&s_full[t]));
-        commit(smem_addr(&k_empty[st]));
       };
-      // O_t += P_t V with V in stage st
-      auto issue_pv = [&](auto tile, auto stage, bool add) {
-        constexpr int t = decltype(tile)::value, st = decltype(stage)::value;
+      // O_t += P_t V
+      auto issue_pv = [&](auto tile, bool add) {
+        constexpr int t = decltype(tile)::value;
+        tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < TILE / 16; ++kk)
-          mma_ts(tmem + o_col(t), tmem + s_col(t) + kk * 8, v_desc + st * TILE_D + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
+        for (int kk = 0; kk < TILE / 16; ++kk) {
+          const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + o_col(t), p_desc + t * ((2 * CHUNK) >> 4) + off, v_desc + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
+        }
         commit(smem_addr(&pv_done[t]));
-        commit(smem_addr(&v_empty[st]));
       };
       const std::integral_constant<int, 0> c0;
       const std::integral_constant<int, 1> c1;
-      int ring = 0;                 // key tiles before this segment
-      uint32_t done0 = 0, done1 = 0;  // steps of each tile so far
+      uint32_t ring = 0;                // key tiles so far
+      uint32_t s0 = 0, s1 = 0;          // S_t computed so far
+      uint32_t p0 = 0, p1 = 0;          // O_t products so far
       bool ok = true;
+      // both tiles' S with the key tile `step`, each when its last one has been read
+      auto scores = [&](uint32_t step, bool two) {
+        if (!wait(&k_full[step & 1], step >> 1, 67, step)) return false;
+        if (s0 > 0 && !wait(&s_free[0], s0 - 1, 68, step)) return false;
+        if (step & 1) issue_qk(c0, c1); else issue_qk(c0, c0);
+        ++s0;
+        if (two) {
+          if (s1 > 0 && !wait(&s_free[1], s1 - 1, 69, step)) return false;
+          if (step & 1) issue_qk(c1, c1); else issue_qk(c1, c0);
+          ++s1;
+        }
+        commit(smem_addr(&k_empty[step & 1]));
+        return true;
+      };
       for (int i = 0; i < nseg && ok; ++i) {
         const int n = __shfl_sync(0xffffffffu, segments[i].count, 0);
         const bool two = __all_sync(0xffffffffu, two_tiles(segments[i]));
-        if (!mbar_wait_warp(smem_addr(q_full), i & 1, 55, i)) break;
-        int qk0 = 0, pv0 = 0, qk1 = two ? 0 : n, pv1 = two ? 0 : n;  // issued
-        bool q_read = false;
-        uint64_t since = 0;
-        uint32_t misses = 0;
-        while (pv0 < n || pv1 < n) {
-          bool moved = false;
-          // tile t's next product, if its operands are there: S_t over P_t once P_t's is done, else O_t
-          auto advance = [&](auto tile, int& qk, int& pv, uint32_t& done) {
-            constexpr int t = decltype(tile)::value;
-            if (qk == pv && qk < n) {
-              const int step = ring + qk;
-              if ((done == 0 || ready(&pv_done[t], (done - 1) & 1)) && ready(&k_full[step & 1], (step >> 1) & 1)) {
-                tc_fence_after();
-                if (step & 1) issue_qk(tile, c1); else issue_qk(tile, c0);
-                if (!two) commit(smem_addr(&k_empty[step & 1]));  // for the tile that is not there
-                ++qk;
-                moved = true;
-              }
-            } else if (qk > pv) {
-              const int step = ring + pv;
-              if (ready(&p_full[t], done & 1) && ready(&v_full[step & 1], (step >> 1) & 1)) {
-                tc_fence_after();
-                if (step & 1) issue_pv(tile, c1, pv != 0); else issue_pv(tile, c0, pv != 0);
-                if (!two) commit(smem_addr(&v_empty[step & 1]));
-                ++pv;
-                ++done;
-                moved = true;
-              }
-            }
-          };
-          advance(c0, qk0, pv0, done0);
-          advance(c1, qk1, pv1, done1);
-          if (!q_read && qk0 == n && qk1 == n) {
-            commit(smem_addr(q_empty));  // the next unit's Q may come
-            q_read = true;
+        if (!wait(q_full, i, 55, i)) break;
+        ok = scores(ring, two);
+        if (n == 1) commit(smem_addr(q_empty));
+        for (int j = 0; j < n && ok; ++j, ++ring) {
+          if (j + 1 < n) {
+            if (!scores(ring + 1, two)) { ok = false; break; }
+            if (j + 2 == n) commit(smem_addr(q_empty));  // the next unit's Q may come
           }
-          if (moved) {
-            misses = 0;
-          } else if (++misses == 256) {
-            since = globaltimer();
-          } else if ((misses & 255) == 0 && __any_sync(0xffffffffu, globaltimer() - since > kWaitLimitNs)) {
-            if (lane == 0) {
-              report_timeout();
-              trace_timeout(56, ring + pv0);
-            }
-            ok = false;
-            break;
+          if (!wait(v_full, ring, 70, ring) || !wait(&p_full[0], p0, 71, ring)) { ok = false; break; }
+          issue_pv(c0, j != 0);
+          ++p0;
+          if (two) {
+            if (!wait(&p_full[1], p1, 72, ring)) { ok = false; break; }
+            issue_pv(c1, j != 0);
+            ++p1;
           }
+          commit(smem_addr(v_empty));
         }
-        ring += n;
       }
     }
     __syncwarp();
@@ -528,27 +493,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
     const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + s_col(t) + 64 * half;   // this half's 64 keys
-    const uint32_t p_addr = tmem + lanes + s_col(t) + 32 * half;   // and their P, two to a column
-    const uint32_t o_addr = tmem + lanes + o_col(t) + D / 2 * half;  // this half's channels
-    const uint32_t met_bar = smem_addr(&met[t * 4 + quarter]);
-    float* x_mine = s_x + (t * 2 + half) * TILE + row;         // + 512 floats on odd meetings
-    const float* x_other = s_x + (t * 2 + (half ^ 1)) * TILE + row;
-    uint32_t meetings = 0;
-    // this thread's value for the row's other half's
-    auto exchange = [&](float mine, float& other, int site) {
-      const int buffer = (meetings & 1) * 4 * TILE;
-      x_mine[buffer] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(met_bar);
-      const bool there = mbar_wait_warp(met_bar, meetings & 1, site, meetings);
-      other = x_other[buffer];
-      ++meetings;
-      return there;
-    };
+    const uint32_t s_addr = tmem + lanes + s_col(t) + 64 * half;         // this half's 64 keys
+    const uint32_t s_other = tmem + lanes + s_col(t) + 64 * (half ^ 1);
+    const uint32_t o_addr = tmem + lanes + o_col(t) + D / 2 * half;      // this half's channels
+    // P_t as TMA would lay out a tile: key chunk `half`, row `row`, unit u at u ^ (row % 8)
+    uint8_t* p_tile = base + L::p + t * 2 * CHUNK;
+    const uint32_t p_row = smem_addr(p_tile + half * CHUNK + row * 128);
     const float2 c2 = make_float2(P.scale_log2, P.scale_log2);
     const int row_tok = row / P.group, row_head = row - row_tok * P.group;
     uint32_t done = 0;  // steps of this tile so far
+    int units = 0;
     bool ok = true;
     for (int i = 0; i < nseg && ok; ++i) {
       const Segment g = segments[i];
@@ -561,12 +515,48 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!mbar_wait_warp(smem_addr(&s_full[t]), done & 1, 57 + t, j)) { ok = false; break; }
         tc_fence_after();
         float f[64];
-        tmem_ld32f(s_addr, f);
-        tmem_ld32f(s_addr + 32, f + 32);
-        tc_wait_ld();
-        reg_fence32f(f);
-        reg_fence32f(f + 32);
-        const int rel = lim - (g.k0 + j) * TILE - 64 * half;
+        float other;
+        const int rel = lim - (g.k0 + j) * TILE - 64 * half, rel_other = rel + 64 * (2 * half - 1);
+        {
+          float h[32];
+          tmem_ld32f(s_addr, f);
+          tmem_ld32f(s_addr + 32, f + 32);
+          tmem_ld32f(s_other, h);
+          tc_wait_ld();
+          reg_fence32f(f);
+          reg_fence32f(f + 32);
+          reg_fence32f(h);
+          const bool cut = __any_sync(0xffffffffu, rel_other < 63);
+          if (cut) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (x > rel_other) h[x] = -INFINITY;
+          }
+          float mo[2] = {h[0], h[1]};
+#pragma unroll
+          for (int x = 2; x < 32; x += 4) {
+            mo[0] = max3(mo[0], h[x], h[x + 1]);
+            if (x + 3 < 32) mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
+          }
+          tmem_ld32f(s_other + 32, h);
+          tc_wait_ld();
+          reg_fence32f(h);
+          // S_t is in registers: the tensor core may write the next one
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&s_free[t]));
+          if (cut) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (x + 32 > rel_other) h[x] = -INFINITY;
+          }
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            mo[0] = max3(mo[0], h[x], h[x + 1]);
+            mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
+          }
+          other = fmaxf(mo[0], mo[1]);
+        }
         if (__any_sync(0xffffffffu, rel < 63)) {
 #pragma unroll
           for (int x = 0; x < 64; ++x)
@@ -580,62 +570,77 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
         }
         const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
-        float other;
-        // also: both halves have read S_t, so P_t may be written over it
-        tc_fence_before();
-        if (!exchange(mine, other, 63 + t)) { ok = false; break; }
-        tc_fence_after();
         const float top = __fmul_rn(fmaxf(mine, other), P.scale_log2);
-        if (__any_sync(0xffffffffu, top > m + RAISE)) {  // the same rows in both halves' warps
+        float a = 1.0f;
+        const bool raise = __any_sync(0xffffffffu, top > m + RAISE);  // the same rows in both halves' warps
+        if (raise) {
           const float next = fmaxf(top, m);
-          const float a = ex2(m - next);
+          a = ex2(m - next);
           m = next;
           l *= a;
-          if (j > 0) {  // O_t of the steps before is complete, then rescaled
-            if (!mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 59 + t, j)) { ok = false; break; }
-            tc_fence_after();
-            const float2 a2 = make_float2(a, a);
-#pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
-              float o[32];
-              tmem_ld32f(o_addr + 32 * c, o);
-              tc_wait_ld();
-              reg_fence32f(o);
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
-                o[2 * x] = v.x;
-                o[2 * x + 1] = v.y;
-              }
-              tmem_st32f(o_addr + 32 * c, o);
-            }
-          }
         }
         const float2 mneg = make_float2(-m, -m);
         float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        float w[32];
+        uint32_t w[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
           const float2 d = __ffma2_rn(make_float2(f[2 * x], f[2 * x + 1]), c2, mneg);
           const float2 e = make_float2(ex2(d.x), ex2(d.y));
           sum[x & 3] = __fadd2_rn(sum[x & 3], e);
-          w[x] = __uint_as_float(pack_bf16(e.x, e.y));
+          w[x] = pack_bf16(e.x, e.y);
         }
-        tmem_st32f(p_addr, w);
         const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
         l += s4.x + s4.y;
-        tc_wait_st();
+        // the product of the step before has read P_t, and O_t is its
+        if (j > 0 ? !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 59 + t, j)
+                  : units > 0 && !mbar_wait_warp(smem_addr(&sums[t]), 1, 73 + t, j)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((u ^ (row & 7)) << 4)), "r"(w[4 * u]),
+                       "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
+                       : "memory");
+        fence_proxy_async_smem();  // the tensor core reads P through the async proxy
+        tc_fence_after();
+        if (raise && j > 0) {
+          const float2 a2 = make_float2(a, a);
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            float o[32];
+            tmem_ld32f(o_addr + 32 * c, o);
+            tc_wait_ld();
+            reg_fence32f(o);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
+              o[2 * x] = v.x;
+              o[2 * x + 1] = v.y;
+            }
+            tmem_st32f(o_addr + 32 * c, o);
+          }
+          tc_wait_st();
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&p_full[t]));
       }
-      float other;
-      if (!ok || !exchange(l, other, 65 + t) || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) {
+      if (!ok || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      l = half ? other + l : l + other;  // the same sum in both halves
+      // the halves' row sums meet in P_t's place
+      float* row_sums = reinterpret_cast<float*>(p_tile);
+      row_sums[half * TILE + row] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&sums[t]));
+      if (!mbar_wait_warp(smem_addr(&sums[t]), 0, 65 + t, i)) { ok = false; break; }
+      l = row_sums[row] + row_sums[TILE + row];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&sums[t]));  // read: the next unit's P may come
+      ++units;
       const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
       float* part = g.slot < 0 ? nullptr : P.parts + static_cast<int64_t>(g.slot) * (ROWS * D + 2 * ROWS);
       __nv_bfloat16* dst =
@@ -687,17 +692,41 @@ __global__ void __launch_bounds__(256) prefill_combine_kernel(Params P) {
   const int t = r / TILE, in_tile = r % TILE, tok_in = in_tile / P.group;
   const int tok = j.tok0 + t * P.tile_tokens + tok_in;
   if (tok_in >= P.tile_tokens || tok >= j.n) return;
+  // 32 partials at a time: their weights one per lane, then their rows, loads in flight
   float sum[V], den = 0.0f, top = LOWEST;
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.0f;
-  for (int c = j.first; c <= static_cast<int>(blockIdx.x); ++c) {
+  for (int c0 = j.first; c0 <= static_cast<int>(blockIdx.x); c0 += 32) {
+    const int c = c0 + lane, n = min(32, static_cast<int>(blockIdx.x) - c0 + 1);
     const float* src = P.parts + (2 * static_cast<int64_t>(c) + (c == j.first)) * SIZE;
-    const float m = src[ROWS * D + r], l = src[ROWS * D + ROWS + r];
-    const float next = fmaxf(top, m), f = ex2(top - next), e = ex2(m - next);
+    const float m = lane < n ? src[ROWS * D + r] : LOWEST, l = lane < n ? src[ROWS * D + ROWS + r] : 0.0f;
+    float next = fmaxf(top, m);
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f + src[r * D + lane * V + i] * e;
-    den = den * f + l * e;
+    for (int o = 16; o > 0; o >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, o));
+    const float f = ex2(top - next), e = lane < n ? ex2(m - next) : 0.0f;
+    float dl = lane < n ? e * l : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, o);
+    den = den * f + dl;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] *= f;
     top = next;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const float w = __shfl_sync(0xffffffffu, e, x);
+      const float* row = P.parts + (2 * static_cast<int64_t>(c0 + x) + (c0 + x == j.first)) * SIZE + r * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(row);
+        sum[0] += u.x * w;
+        sum[1] += u.y * w;
+        sum[2] += u.z * w;
+        sum[3] += u.w * w;
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(row);
+        sum[0] += u.x * w;
+        sum[1] += u.y * w;
+      }
+    }
   }
   const float inv = den > 0.0f ? __fdiv_rn(1.0f, den) : (den == 0.0f ? 0.0f : den);
   __nv_bfloat16* dst = P.out + static_cast<int64_t>(j.c0 + tok) * P.ot +
@@ -765,9 +794,9 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
   static std::atomic<uint64_t> set{0};
   rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
   if (rc) return rc;
-  const int64_t items = P.cap / TILE * P.p.kv_heads;
-  const unsigned ctas = static_cast<unsigned>(std::min<int64_t>(items, num_sms() * 6)) + 1;
-  FAQ_CUDA(launch_early(paged_expand_kernel<NG>, dim3(ctas), 256, 0, stream, P));
+  const int64_t ctas = (P.cap / BLOCK * P.p.kv_heads * 2 + EXPAND_WARPS - 1) / EXPAND_WARPS + 1;
+  FAQ_CHECK_ARG(ctas < (int64_t(1) << 31), "too many keys for one call");
+  FAQ_CUDA(launch_early(paged_expand_kernel<NG>, dim3(static_cast<unsigned>(ctas)), 32 * EXPAND_WARPS, 0, stream, P));
   FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(P.runs)), THREADS, Smem<NG>::bytes, stream, mq, mk, mv, P));
   FAQ_CUDA(launch_early(prefill_combine_kernel<D>, dim3(static_cast<unsigned>(P.runs), ROWS / 8), 256, 0, stream, P));
   return FAQ_OK;
