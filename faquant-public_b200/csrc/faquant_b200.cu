@@ -105,6 +105,7 @@ __global__ void selftest_wait_kernel(uint64_t limit_ns) {
 #include "kv_cache.cu"
 #include "paged_attention.cu"
 #include "paged_prefill.cu"
+#include "paged_chunk.cu"
 #include "verify.cu"
 
 extern "C" int faq_version(void) { return 100; }

@@ -289,94 +289,121 @@ __device__ __forceinline__ void store_pairs(float* dst, bool vec, const uint32_t
   }
 }
 
-// The tokens [from, to) of a block of one head, K or V, as rows of `stride` elements from dst
-// (the block's first token), by one warp: K sixteen channels of each group per lane and half, V
-// a sub-block of both tokens of a pair. y = (n - 8) 2^(e - 3) times twice the scale is exact
-// in bf16 (six significant bits), so a pair costs one packed product.
+// A block of one head's K or V, as a warp loads it and hands it out: for K a lane has sixteen
+// channels of each group of two tokens, for V a sub-block of both tokens of two pairs.
+// each(expand, lane, f) calls f(token, group, unit, four bf16 pairs) for every eight channels 8
+// unit .. of a group. y = (n - 8) 2^(e - 3) times twice the scale is exact in bf16 (six
+// significant bits), so a pair costs one packed product.
 __device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
   const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
   return s | (s << 16);
 }
-template <typename T, int NG>
-__device__ __forceinline__ void expand_block_k(const Expand& expand, const uint8_t* src, T* dst, int64_t stride, int from,
-                                               int to, int lane, bool vec = true) {
-  const int t = lane & 3;
+template <int NG>
+struct KBlock {
+  uint32_t w[2][2 * NG], e[2][NG], sc[2];
+  __device__ __forceinline__ void load(const uint8_t* src, int lane) {
+    const int t = lane & 3;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = (lane >> 2) + 8 * h;
-    if (r < from || r >= to) continue;
-    uint32_t w[2 * NG], e[NG], sc[NG];
-    if constexpr (NG == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * r + 16 * t);
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * r);
-      e[0] = x.x; e[1] = x.y;
-      const uint32_t c = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * r);
-      sc[0] = scale_pair(c & 255); sc[1] = scale_pair(c >> 8);
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + 32 * r + 8 * t);
-      w[0] = u.x; w[1] = u.y;
-      e[0] = *reinterpret_cast<const uint32_t*>(src + exp_offset(NG) + 4 * r);
-      sc[0] = scale_pair(src[scale_offset(NG) + r]);
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
-        uint32_t y[4];
-        expand.word(w[2 * g + i], expand.exponents(e[g], (7 - 4 * t - 2 * i) & 31), y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], sc[g]);
-        const uint32_t row[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
-                                 __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)};
-        store_pairs(dst + r * stride + 64 * g + 16 * t + 8 * i, vec, row);
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h;
+      if constexpr (NG == 2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src + 64 * r + 16 * t);
+        w[h][0] = u.x; w[h][1] = u.y; w[h][2] = u.z; w[h][3] = u.w;
+        const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * r);
+        e[h][0] = x.x; e[h][1] = x.y;
+        sc[h] = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * r);
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(src + 32 * r + 8 * t);
+        w[h][0] = u.x; w[h][1] = u.y;
+        e[h][0] = *reinterpret_cast<const uint32_t*>(src + exp_offset(NG) + 4 * r);
+        sc[h] = src[scale_offset(NG) + r];
       }
     }
   }
-}
-template <typename T, int NG>
-__device__ __forceinline__ void expand_block_v(const Expand& expand, const uint8_t* src, T* dst, int64_t stride, int from,
-                                               int to, int lane, bool vec = true) {
-  const int s = lane & 7;
+  template <typename F>
+  __device__ __forceinline__ void each(const Expand& expand, int lane, F&& f) const {
+    const int t = lane & 3;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int p = (lane >> 3) + 4 * h;  // tokens 2 p, 2 p + 1
-    if (2 * p + 1 < from || 2 * p >= to) continue;
-    uint32_t w[2 * NG], e[2 * NG], sc[NG];
-    if constexpr (NG == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + 128 * p + 16 * (s ^ (2 * (p & 3))));
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-      const uint4 x = *reinterpret_cast<const uint4*>(src + exp_offset(NG) + 16 * p);
-      e[0] = x.x; e[1] = x.y; e[2] = x.z; e[3] = x.w;
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(src + scale_offset(NG) + 4 * p);  // [token][group]
-      sc[0] = __byte_perm(scale_pair(c & 255), scale_pair((c >> 16) & 255), 0x5410);
-      sc[1] = __byte_perm(scale_pair((c >> 8) & 255), scale_pair(c >> 24), 0x5410);
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + 64 * p + 8 * (s ^ (2 * (p & 3))));
-      w[0] = u.x; w[1] = u.y;
-      const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * p);
-      e[0] = x.x; e[1] = x.y;
-      const uint32_t c = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * p);
-      sc[0] = __byte_perm(scale_pair(c & 255), scale_pair(c >> 8), 0x5410);
-    }
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t s = scale_pair((sc[h] >> (8 * g)) & 255);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        expand.word(w[2 * g + q], expand.exponents(e[2 * g + q], (7 - 2 * s) & 31), y[q]);
+        for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
+          uint32_t y[4];
+          expand.word(w[h][2 * g + i], expand.exponents(e[h][g], (7 - 4 * t - 2 * i) & 31), y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], sc[g]);
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t sel = k ? 0x7632 : 0x5410;
-        const uint32_t row[4] = {__byte_perm(y[0][0], y[0][1], sel), __byte_perm(y[0][2], y[0][3], sel),
-                                 __byte_perm(y[1][0], y[1][1], sel), __byte_perm(y[1][2], y[1][3], sel)};
-        if (2 * p + k >= from && 2 * p + k < to) store_pairs(dst + (2 * p + k) * stride + 64 * g + 8 * s, vec, row);
+          for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], s);
+          const uint32_t row[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                                   __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)};
+          f(r, g, 2 * t + i, row);
+        }
       }
     }
   }
+};
+template <int NG>
+struct VBlock {
+  uint32_t w[2][2 * NG], e[2][2 * NG], sc[2];
+  __device__ __forceinline__ void load(const uint8_t* src, int lane) {
+    const int s = lane & 7;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int p = (lane >> 3) + 4 * h;  // tokens 2 p, 2 p + 1
+      if constexpr (NG == 2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src + 128 * p + 16 * (s ^ (2 * (p & 3))));
+        w[h][0] = u.x; w[h][1] = u.y; w[h][2] = u.z; w[h][3] = u.w;
+        const uint4 x = *reinterpret_cast<const uint4*>(src + exp_offset(NG) + 16 * p);
+        e[h][0] = x.x; e[h][1] = x.y; e[h][2] = x.z; e[h][3] = x.w;
+        sc[h] = *reinterpret_cast<const uint32_t*>(src + scale_offset(NG) + 4 * p);  // [token][group]
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(src + 64 * p + 8 * (s ^ (2 * (p & 3))));
+        w[h][0] = u.x; w[h][1] = u.y;
+        const uint2 x = *reinterpret_cast<const uint2*>(src + exp_offset(NG) + 8 * p);
+        e[h][0] = x.x; e[h][1] = x.y;
+        sc[h] = *reinterpret_cast<const uint16_t*>(src + scale_offset(NG) + 2 * p);
+      }
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(const Expand& expand, int lane, F&& f) const {
+    const int s = lane & 7;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int p = (lane >> 3) + 4 * h;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t pair = __byte_perm(scale_pair((sc[h] >> (8 * g)) & 255), scale_pair((sc[h] >> (8 * (NG + g))) & 255), 0x5410);
+        uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          expand.word(w[h][2 * g + q], expand.exponents(e[h][2 * g + q], (7 - 2 * s) & 31), y[q]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], pair);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t sel = k ? 0x7632 : 0x5410;
+          const uint32_t row[4] = {__byte_perm(y[0][0], y[0][1], sel), __byte_perm(y[0][2], y[0][3], sel),
+                                   __byte_perm(y[1][0], y[1][1], sel), __byte_perm(y[1][2], y[1][3], sel)};
+          f(2 * p + k, g, s, row);
+        }
+      }
+    }
+  }
+};
+
+// The tokens [from, to) of a block as rows of `stride` elements from dst (the block's first token).
+template <typename T, template <int> class Block, int NG>
+__device__ __forceinline__ void expand_block(const uint8_t* src, T* dst, int64_t stride, int from, int to, int lane,
+                                             bool vec = true) {
+  const Expand expand;
+  Block<NG> x;
+  x.load(src, lane);
+  x.each(expand, lane, [&](int token, int g, int unit, const uint32_t (&w)[4]) {
+    if (token >= from && token < to) store_pairs(dst + token * stride + 64 * g + 8 * unit, vec, w);
+  });
 }
 
 // Zeros for `count` tokens' rows, which have no place in the cache.
@@ -404,12 +431,11 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv_read_kernel(ReadParams w, 
   T* rows = which ? static_cast<T*>(w.v) + head * w.vh : static_cast<T*>(w.k) + head * w.kh;
   const int64_t page = x.to ? page_of(p, x.b, x.pos) : -1;
   if (page >= 0) {
-    const Expand expand;
     const uint8_t* src = p.base + page * p.page_stride + block_in_page<NG>(p, which, head, x.pos);
     if (which)
-      expand_block_v<T, NG>(expand, src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
+      expand_block<T, VBlock, NG>(src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
     else
-      expand_block_k<T, NG>(expand, src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
+      expand_block<T, KBlock, NG>(src, rows + x.token * stride, stride, x.from, x.to, lane, vec);
   } else {
     zero_rows<T>(rows + (x.token + x.from) * stride, stride, x.to - x.from, 64 * NG, lane);
   }

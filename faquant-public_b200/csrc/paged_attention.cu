@@ -4,7 +4,7 @@
 //
 // for the n new tokens (i = 0 .. n - 1) of each sequence of a ragged batch, the G = heads /
 // kv_heads query heads of a kv head sharing its keys. A row of the problem is (token i, query
-// head), r = i G + g; a unit is (sequence, kv head, 8 NB rows).
+// head), r = i G + g; a unit is (sequence, kv head, 8 rows).
 //
 // The cache holds 4.6 bits per value, so per byte of HBM a lot is computed: each code becomes a
 // bf16 register value (about two instructions per value), which feeds mma.sync m16n8k16
@@ -39,6 +39,11 @@ namespace pat {
 
 using namespace kvp;
 
+constexpr int RB = 8;       // rows of a unit
+constexpr int W = 16;       // warps of a CTA, one CTA per SM: 128 registers a thread
+constexpr int THREADS = 32 * W;
+constexpr int S = 4;        // blocks in flight per warp, 2 x 1184 bytes each at d = 128
+constexpr int COST = W;     // of a unit beyond its blocks, see below
 constexpr float RAISE = 8.0f;  // log2 headroom of a row's reference maximum
 constexpr float LOWEST = -3.402823466e38f;  // where it starts: below every finite score
 
@@ -49,7 +54,6 @@ struct Params {
   __nv_bfloat16* out;
   int64_t ot, oh;
   int64_t total;   // rows of q and out
-  int max_rows;    // sequences with more rows are the prompt kernel's
   int group;       // query heads per kv head
   uint32_t group_magic;  // ceil(2^32 / group), see small_div
   float scale_log2;
@@ -65,17 +69,14 @@ __device__ __forceinline__ int small_div(const Params& P, int x) {
 struct Seq {
   int n, len, nrb;  // new tokens, length, row blocks of RB rows
 };
-template <int RB>
 __device__ __forceinline__ Seq sequence(const Params& P, int b) {
   Seq s;
   const int c0 = P.p.cu[b], c1 = P.p.cu[b + 1];
   s.n = (c0 >= 0 && c1 > c0 && c1 <= P.total) ? c1 - c0 : 0;
-  if (static_cast<int64_t>(s.n) * P.group > P.max_rows) s.n = 0;
   s.len = length_of(P.p, b);
   s.nrb = (s.n * P.group + RB - 1) / RB;
   return s;
 }
-template <int RB>
 __device__ __forceinline__ int key_blocks(const Params& P, const Seq& s, int rb) {
   // the row block's last token
   const int last = rb + 1 >= s.nrb ? s.n - 1 : ((rb + 1) * RB - 1) / P.group;
@@ -83,12 +84,11 @@ __device__ __forceinline__ int key_blocks(const Params& P, const Seq& s, int rb)
   return seen <= 0 ? 0 : (seen + BLOCK - 1) / BLOCK;
 }
 // cost of a sequence's units of one kv head; units without a key cost nothing
-template <int RB>
-__device__ __forceinline__ int64_t head_cost(const Params& P, const Seq& s, int unit_cost) {
+__device__ __forceinline__ int64_t head_cost(const Params& P, const Seq& s) {
   int64_t sum = 0;
   for (int rb = 0; rb < s.nrb; ++rb) {
-    const int blocks = key_blocks<RB>(P, s, rb);
-    sum += blocks ? blocks + unit_cost : 0;
+    const int blocks = key_blocks(P, s, rb);
+    sum += blocks ? blocks + COST : 0;
   }
   return sum;
 }
@@ -113,30 +113,24 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// Warps per CTA (one CTA per SM): with 8 rows a warp needs 128 registers, with more O and Q
-// fill up to 255.
-__host__ __device__ constexpr int warps_of(int nb) { return nb == 1 ? 16 : 8; }
-constexpr int S = 4;  // blocks in flight per warp, 2 x 1184 bytes each at d = 128
 // shared memory: the warps' rings | their O (rows padded) and (m, l) at a unit's end | Q
 // fragments | mbarriers
-template <int NG, int NB>
+template <int NG>
 struct Smem {
-  static constexpr int W = warps_of(NB), RB = 8 * NB, OLD = 64 * NG + 8;
+  static constexpr int old = 64 * NG + 8;  // floats of an O row
   static constexpr int stage = 2 * block_bytes(NG);
   static constexpr int o = W * S * stage;
-  static constexpr int m = o + W * RB * OLD * 4;
+  static constexpr int m = o + W * RB * old * 4;
   static constexpr int l = m + W * RB * 4;
   static constexpr int q = l + W * RB * 4;
-  static constexpr int bar = q + NB * NG * 2 * 32 * 16;
+  static constexpr int bar = q + NG * 2 * 32 * 16;
   static constexpr int bytes = bar + W * S * 8;
 };
 
-// What a unit costs beyond its blocks (filling the rings, joining the warps), in blocks: the
-// runs are cut in this measure. Without it a CTA whose run holds many short units works
-// four times as long as the others (32 sequences of 1 .. 16000 tokens: 129 us against TODO).
-template <int NB>
-__host__ __device__ constexpr int unit_cost() { return warps_of(NB); }
-
+// A unit costs COST blocks beyond its own (filling the rings, joining the warps), a round of
+// the warps: the runs are cut in this measure. Without it a CTA whose run holds many short
+// units works four times as long as the others (32 sequences of 1 .. 16000 tokens: 129 us,
+// 57 us with it).
 // A run's part of one unit, made by one thread for the CTA.
 struct Segment {
   int b, head, rb;       // the unit
@@ -147,16 +141,15 @@ struct Segment {
   int64_t at;            // the unit's place in the order of all costs
 };
 
-template <int NG, int NB>
-__global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(Params P) {
-  using L = Smem<NG, NB>;
-  constexpr int RB = 8 * NB, D = 64 * NG, W = L::W, THREADS = 32 * W, OLD = L::OLD;
-  constexpr int UNIT = block_bytes(NG), STAGE = L::stage, COST = unit_cost<NB>();
+template <int NG>
+__global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
+  using L = Smem<NG>;
+  constexpr int D = 64 * NG, OLD = L::old, UNIT = block_bytes(NG), STAGE = L::stage;
   extern __shared__ __align__(128) unsigned char smem[];
   float* s_o = reinterpret_cast<float*>(smem + L::o);  // [W][RB][OLD]
   float* s_m = reinterpret_cast<float*>(smem + L::m);  // [W][RB]
   float* s_l = reinterpret_cast<float*>(smem + L::l);
-  uint4* s_q = reinterpret_cast<uint4*>(smem + L::q);  // [NB][NG][2 step pairs][32 lanes]
+  uint4* s_q = reinterpret_cast<uint4*>(smem + L::q);  // [NG][2 step pairs][32 lanes]
   uint64_t* s_bar = reinterpret_cast<uint64_t*>(smem + L::bar);  // [W][S]
   __shared__ int64_t s_scan[W], s_per, s_end;
   __shared__ Segment s_seg[3];  // this one, the next, the one after
@@ -200,11 +193,11 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
           x.head = 0;
           do {
             if (++x.b >= p.batch) return;
-            s = sequence<RB>(P, x.b);
+            s = sequence(P, x.b);
           } while (s.nrb == 0);
         }
       }
-      x.blocks = key_blocks<RB>(P, s, x.rb);
+      x.blocks = key_blocks(P, s, x.rb);
     } while (x.blocks == 0);
     fill(x, s, begin, end);
   };
@@ -216,8 +209,8 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
   auto count_blocks = [&](int b) {  // warps without a sequence do nothing
     if (b - lane >= p.batch) return;
     sq = {0, 0, 0};
-    if (b < p.batch) sq = sequence<RB>(P, b);
-    mine = head_cost<RB>(P, sq, COST) * p.kv_heads;
+    if (b < p.batch) sq = sequence(P, b);
+    mine = head_cost(P, sq) * p.kv_heads;
     if (sq.n > sq.len) s_empty = 1;
     upto = mine;
 #pragma unroll
@@ -263,10 +256,10 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
                                                             : at / per_head);
         x.at = start + x.head * per_head;
         x.rb = 0;
-        x.blocks = key_blocks<RB>(P, sq, 0);
+        x.blocks = key_blocks(P, sq, 0);
         while (begin >= x.at + (x.blocks ? x.blocks + COST : 0)) {
           x.at += x.blocks ? x.blocks + COST : 0;
-          x.blocks = key_blocks<RB>(P, sq, ++x.rb);
+          x.blocks = key_blocks(P, sq, ++x.rb);
         }
         s_per = per;
         s_end = end;
@@ -288,7 +281,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
   __syncthreads();
   if (s_empty) {  // rows that see no key are zero: tokens at positions below zero
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      const Seq e = sequence<RB>(P, b);
+      const Seq e = sequence(P, b);
       const int none = min(e.n, e.n - e.len), heads = P.group * p.kv_heads;
       for (int64_t i = tid; i < static_cast<int64_t>(none) * heads * (D / 8); i += THREADS) {
         const int64_t row = i / (D / 8);
@@ -336,12 +329,12 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
     ++issued;
     ++ahead;
   };
-  // The fragments of n-block `nb` of a unit's rows, by one warp: a B fragment's column is row
+  // The fragments of a unit's rows, by one warp: a B fragment's column is row
   // g, and lane t holds channels 16 t .. 16 t + 15 of each group; step ks takes channels
   // 16 t + ks and + 4 (pair ks of word 2 t), then + 8 and + 12 (of word 2 t + 1).
-  auto make_q = [&](const Segment& x, int nb) {
-    const int r = x.rem0 + nb * 8 + g, tok = small_div(P, r);
-    const bool live = nb * 8 + g < x.rows;
+  auto make_q = [&](const Segment& x) {
+    const int r = x.rem0 + g, tok = small_div(P, r);
+    const bool live = g < x.rows;
     const __nv_bfloat16* row = P.q + static_cast<int64_t>(x.c0 + x.tok0 + (live ? tok : 0)) * P.qt +
                                (x.head * P.group + (live ? r - tok * P.group : 0)) * P.qh;
 #pragma unroll
@@ -351,7 +344,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
       const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        s_q[((nb * NG + gr) * 2 + i) * 32 + lane] =
+        s_q[(gr * 2 + i) * 32 + lane] =
             make_uint4(__byte_perm(w[i], w[2 + i], 0x5410), __byte_perm(w[4 + i], w[6 + i], 0x5410),
                        __byte_perm(w[i], w[2 + i], 0x7632), __byte_perm(w[4 + i], w[6 + i], 0x7632));
     }
@@ -374,7 +367,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
   bool ok = true;
   ahead_blocks = blocks_of(s_seg[0]);
   top_up(0, 0, false);
-  if (warp < NB) make_q(s_seg[0], warp);
+  if (warp == 0) make_q(s_seg[0]);
   __syncthreads();
 
   while (true) {
@@ -382,32 +375,22 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
     const int next = cur == 2 ? 0 : cur + 1;
     const bool more = s_seg[next].count > 0;
     const int mine_blocks = blocks_of(x);
-    const int nbs = (x.rows + 7) / 8;
     top_up(cur, next, more);
-    uint4 qr[NB == 1 ? NG * 2 : 1];  // one n-block: Q stays in registers
-    if constexpr (NB == 1) {
+    uint4 q[NG * 2];
 #pragma unroll
-      for (int i = 0; i < NG * 2; ++i) qr[i] = s_q[i * 32 + lane];
-    }
-    // last visible key of the C fragments' columns (rows 2 t, 2 t + 1 of each n-block); the
+    for (int i = 0; i < NG * 2; ++i) q[i] = s_q[i * 32 + lane];
+    // last visible key of the C fragments' columns (rows 2 t, 2 t + 1); the
     // rows past the unit's are not masked (their scores are 0) and not written
     const int lim0 = x.len - x.n + x.tok0;
-    int lim[NB][2];
+    int lim[2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) lim[nb][h] = lim0 + small_div(P, x.rem0 + nb * 8 + 2 * t + h);
+    for (int h = 0; h < 2; ++h) lim[h] = lim0 + small_div(P, x.rem0 + 2 * t + h);
 
-    float o[NB][NG * 4][4], m[NB][2], l[NB][2];
+    float o[NG * 4][4], m[2] = {LOWEST, LOWEST}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int i = 0; i < NG * 4; ++i)
 #pragma unroll
-      for (int i = 0; i < NG * 4; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[nb][i][c] = 0.0f;
-      m[nb][0] = m[nb][1] = LOWEST;
-      l[nb][0] = l[nb][1] = 0.0f;
-    }
+      for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
 
     for (int i = 0; i < mine_blocks; ++i) {
       if (!mbar_wait_warp(smem_addr(&bars[used % S]), (used / S) & 1, 42, used)) {
@@ -420,13 +403,11 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
       ++used;
 
       // ---- S^T = K Q^T
-      float acc[NB][NG][4];
+      float acc[NG][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[nb][gr][c] = 0.0f;
+        for (int c = 0; c < 4; ++c) acc[gr][c] = 0.0f;
       uint32_t kw[2][2 * NG];  // [key g / g + 8][group][word 2 t, 2 t + 1]
       uint32_t ke[2][NG];
       float ks[2][NG], vs[2][NG];
@@ -462,70 +443,61 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
         for (int i2 = 0; i2 < 2; ++i2) {
           const uint32_t f0[4] = {a[0][0][2 * i2], a[1][0][2 * i2], a[0][1][2 * i2], a[1][1][2 * i2]};
           const uint32_t f1[4] = {a[0][0][2 * i2 + 1], a[1][0][2 * i2 + 1], a[0][1][2 * i2 + 1], a[1][1][2 * i2 + 1]};
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (NB > 1 && nb >= nbs) continue;
-            const uint4 qf = NB == 1 ? qr[gr * 2 + i2] : s_q[((nb * NG + gr) * 2 + i2) * 32 + lane];
-            mma_bf16_16816(acc[nb][gr], f0, qf.x, qf.y);
-            mma_bf16_16816(acc[nb][gr], f1, qf.z, qf.w);
-          }
+          mma_bf16_16816(acc[gr], f0, q[gr * 2 + i2].x, q[gr * 2 + i2].y);
+          mma_bf16_16816(acc[gr], f1, q[gr * 2 + i2].z, q[gr * 2 + i2].w);
         }
       }
       // ---- softmax; c of the fragment: key g + 8 (c / 2), row 2 t + c % 2
       const int first_key = (x.k0 + warp + i * W) * BLOCK, key0 = first_key + g;
       const bool edge = first_key + BLOCK - 1 > lim0 || !page;  // lim0: the unit's first row's
-      uint32_t pf[NB][NG][2];
+      uint32_t pf[NG][2];
+      float s[4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (NB > 1 && nb >= nbs) continue;
-        float s[4];
+      for (int c = 0; c < 4; ++c) {
+        s[c] = __fmul_rn(acc[0][c], ks[c >> 1][0]);
+        if constexpr (NG == 2) s[c] = __fmaf_rn(acc[1][c], ks[c >> 1][1], s[c]);
+      }
+      if (edge) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          s[c] = __fmul_rn(acc[nb][0][c], ks[c >> 1][0]);
-          if constexpr (NG == 2) s[c] = __fmaf_rn(acc[nb][1][c], ks[c >> 1][1], s[c]);
+        for (int c = 0; c < 4; ++c)
+          if (key0 + 8 * (c >> 1) > lim[c & 1] || !page) s[c] = -INFINITY;
+      }
+      // log2 p against the reference maxima (finite from the start, so no case of its own)
+      float e[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[c & 1]);
+      if (__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > RAISE)) {
+        float n0 = __fmul_rn(fmaxf(s[0], s[2]), P.scale_log2), n1 = __fmul_rn(fmaxf(s[1], s[3]), P.scale_log2);
+#pragma unroll
+        for (int y = 4; y < 32; y <<= 1) {
+          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, y));
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, y));
         }
-        if (edge) {
+        n0 = fmaxf(n0, m[0]);
+        n1 = fmaxf(n1, m[1]);
+        const float a0 = ex2(m[0] - n0), a1 = ex2(m[1] - n1);
+        m[0] = n0;
+        m[1] = n1;
+        l[0] *= a0;
+        l[1] *= a1;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (key0 + 8 * (c >> 1) > lim[nb][c & 1] || !page) s[c] = -INFINITY;
-        }
-        // log2 p against the reference maxima (finite from the start, so no case of its own)
-        float e[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[nb][c & 1]);
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > RAISE)) {
-          float n0 = __fmul_rn(fmaxf(s[0], s[2]), P.scale_log2), n1 = __fmul_rn(fmaxf(s[1], s[3]), P.scale_log2);
-#pragma unroll
-          for (int y = 4; y < 32; y <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, y));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, y));
-          }
-          n0 = fmaxf(n0, m[nb][0]);
-          n1 = fmaxf(n1, m[nb][1]);
-          const float a0 = ex2(m[nb][0] - n0), a1 = ex2(m[nb][1] - n1);
-          m[nb][0] = n0;
-          m[nb][1] = n1;
-          l[nb][0] *= a0;
-          l[nb][1] *= a1;
-#pragma unroll
-          for (int j = 0; j < NG * 4; ++j) {
-            o[nb][j][0] *= a0;
-            o[nb][j][1] *= a1;
-            o[nb][j][2] *= a0;
-            o[nb][j][3] *= a1;
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[nb][c & 1]);
+        for (int j = 0; j < NG * 4; ++j) {
+          o[j][0] *= a0;
+          o[j][1] *= a1;
+          o[j][2] *= a0;
+          o[j][3] *= a1;
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) e[c] = ex2(e[c]);
-        l[nb][0] += e[0] + e[2];
-        l[nb][1] += e[1] + e[3];
+        for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[c & 1]);
+      }
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          pf[nb][gr][0] = transpose8x8(pack_bf16(e[0] * vs[0][gr], e[1] * vs[0][gr]));
-          pf[nb][gr][1] = transpose8x8(pack_bf16(e[2] * vs[1][gr], e[3] * vs[1][gr]));
-        }
+      for (int c = 0; c < 4; ++c) e[c] = ex2(e[c]);
+      l[0] += e[0] + e[2];
+      l[1] += e[1] + e[3];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        pf[gr][0] = transpose8x8(pack_bf16(e[0] * vs[0][gr], e[1] * vs[0][gr]));
+        pf[gr][1] = transpose8x8(pack_bf16(e[2] * vs[1][gr], e[3] * vs[1][gr]));
       }
       // ---- O^T += V^T P^T: pairs t and t + 4, sub-block g of each group
       uint32_t vw[2][2 * NG], ve[2][2 * NG];  // [pair][group][quad]
@@ -555,9 +527,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t fa[4] = {a[0][0][j], a[0][1][j], a[1][0][j], a[1][1][j]};
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            if (NB == 1 || nb < nbs) mma_bf16_16816(o[nb][gr * 4 + j], fa, pf[nb][gr][0], pf[nb][gr][1]);
+          mma_bf16_16816(o[gr * 4 + j], fa, pf[gr][0], pf[gr][1]);
         }
       }
       __syncwarp();  // the slot may be refilled: every lane has read it
@@ -566,29 +536,24 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
     }
 
     // ---- the warps' results meet
-    const bool worked = warp < x.count;  // warps without a block hold nothing
-    if (worked) {
+    if (warp < x.count) {  // warps without a block hold nothing
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (nb >= nbs) continue;
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int y = 4; y < 32; y <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], y);
+        const int r = 2 * t + h;
+        if (r < x.rows) {
+          float* dst = s_o + (warp * RB + r) * OLD + 8 * g;
 #pragma unroll
-          for (int y = 4; y < 32; y <<= 1) l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], y);
-          const int r = nb * 8 + 2 * t + h;
-          if (r < x.rows) {
-            float* dst = s_o + (warp * RB + r) * OLD + 8 * g;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-              *reinterpret_cast<float4*>(dst + 64 * gr) =
-                  make_float4(o[nb][4 * gr][h], o[nb][4 * gr + 1][h], o[nb][4 * gr + 2][h], o[nb][4 * gr + 3][h]);
-              *reinterpret_cast<float4*>(dst + 64 * gr + 4) =
-                  make_float4(o[nb][4 * gr][2 + h], o[nb][4 * gr + 1][2 + h], o[nb][4 * gr + 2][2 + h], o[nb][4 * gr + 3][2 + h]);
-            }
-            if (g == 0) {
-              s_m[warp * RB + r] = m[nb][h];
-              s_l[warp * RB + r] = l[nb][h];
-            }
+          for (int gr = 0; gr < NG; ++gr) {
+            *reinterpret_cast<float4*>(dst + 64 * gr) =
+                make_float4(o[4 * gr][h], o[4 * gr + 1][h], o[4 * gr + 2][h], o[4 * gr + 3][h]);
+            *reinterpret_cast<float4*>(dst + 64 * gr + 4) =
+                make_float4(o[4 * gr][2 + h], o[4 * gr + 1][2 + h], o[4 * gr + 2][2 + h], o[4 * gr + 3][2 + h]);
+          }
+          if (g == 0) {
+            s_m[warp * RB + r] = m[h];
+            s_l[warp * RB + r] = l[h];
           }
         }
       }
@@ -646,7 +611,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
     }
     if (!more) break;
     cur = next;
-    if (warp < NB) make_q(s_seg[cur], warp);
+    if (warp == 0) make_q(s_seg[cur]);
     __syncthreads();  // s_o has been read, Q is there
   }
   // a timeout leaves copies in flight: wait for them (bounded) before the CTA's memory goes
@@ -658,7 +623,7 @@ __global__ void __launch_bounds__(32 * warps_of(NB), 1) paged_attention_kernel(P
 // Joins the partials of the unit that ended in run blockIdx.x: its first run's (slot 2 c + 1),
 // then those of the runs up to this one (slot 2 c). One CTA per row: eight warps take the
 // partials in turn, four channels (two at d = 64) per lane, and meet in shared memory.
-template <int D, int RB>
+template <int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(Params P) {
   constexpr int V = D / 32;
   constexpr int64_t SIZE = RB * D + 2 * RB;
@@ -718,24 +683,20 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(Params P) {
 
 constexpr int JOIN_BYTES_PER_CTA = 32;
 inline int ctas() { return num_sms(); }
-inline int n_blocks(int64_t max_rows) { return max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4; }
-inline size_t workspace(int nb, int d) {
-  const int64_t rows = 8 * nb;
-  return static_cast<size_t>(ctas()) * (JOIN_BYTES_PER_CTA + 2 * (rows * d + 2 * rows) * 4);
-}
+inline size_t workspace(int d) { return static_cast<size_t>(ctas()) * (JOIN_BYTES_PER_CTA + 2 * (RB * d + 2 * RB) * 4); }
 
-template <int NG, int NB>
+template <int NG>
 static int launch(Params& P, void* ws, void* stream) {
   const int grid = ctas();
   P.joins = static_cast<int32_t*>(ws);
   P.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + static_cast<size_t>(grid) * JOIN_BYTES_PER_CTA);
-  constexpr int bytes = Smem<NG, NB>::bytes;
-  auto kern = paged_attention_kernel<NG, NB>;
+  constexpr int bytes = Smem<NG>::bytes;
+  auto kern = paged_attention_kernel<NG>;
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
   int rc = allow_smem(reinterpret_cast<const void*>(kern), bytes, set);
   if (rc) return rc;
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(grid)), 32 * warps_of(NB), bytes, stream, P));
-  FAQ_CUDA(launch_early(paged_combine_kernel<64 * NG, 8 * NB>, dim3(static_cast<unsigned>(grid), 8 * NB), 256, 0, stream, P));
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(grid)), THREADS, bytes, stream, P));
+  FAQ_CUDA(launch_early(paged_combine_kernel<64 * NG>, dim3(static_cast<unsigned>(grid), RB), 256, 0, stream, P));
   return FAQ_OK;
 }
 

@@ -256,12 +256,11 @@ __global__ void __launch_bounds__(32 * EXPAND_WARPS) paged_expand_kernel(Params 
   const int64_t stride = static_cast<int64_t>(h) * D;
   __nv_bfloat16* dst = (which ? P.v : P.k) + row * stride + head * D;
   if (have) {
-    const Expand expand;
     const uint8_t* src = P.p.base + page * P.p.page_stride + block_in_page<NG>(P.p, which, head, pos);
     if (which)
-      expand_block_v<__nv_bfloat16, NG>(expand, src, dst, stride, 0, have, lane);
+      expand_block<__nv_bfloat16, VBlock, NG>(src, dst, stride, 0, have, lane);
     else
-      expand_block_k<__nv_bfloat16, NG>(expand, src, dst, stride, 0, have, lane);
+      expand_block<__nv_bfloat16, KBlock, NG>(src, dst, stride, 0, have, lane);
   }
   for (int i = have * (D / 8) + lane; i < BLOCK * (D / 8); i += 32)  // zeros behind the end
     *reinterpret_cast<uint4*>(dst + i / (D / 8) * stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
@@ -279,7 +278,7 @@ struct Smem {
   static constexpr int bytes = 1024 + bar + 256;
 };
 constexpr int TMEM_COLS = 512;
-__device__ __forceinline__ uint32_t s_col(int t) { return 128u * t; }        
+__device__ __forceinline__ uint32_t s_col(int t) { return 128u * t; }
 __device__ __forceinline__ uint32_t o_col(int t) { return 256u + 128u * t; }
 constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, TILE, false, false);
 constexpr uint32_t idesc_pv(int d) { return idesc_bf16_f32(TILE, d, false, true); }
@@ -306,6 +305,197 @@ __device__ __forceinline__ void commit(uint32_t bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar)
       : "memory");
 }
+
+// The softmax of a tile of 128 rows by eight warps: warps 0-3 of them (by TMEM lane quarter)
+// take keys 0..63 of every key tile and the lower half of O's channels, warps 4-7 the others.
+template <int D>
+struct Softmax {
+  int row, half, lane, site;
+  uint32_t s_addr, s_other, o_addr, p_row;
+  float* row_sums;
+  uint32_t s_full, s_free, p_full, pv_done, sums;
+  float scale_log2;
+  uint32_t done = 0;  // steps so far
+  int units = 0;
+  float m, l;         // the unit's reference maximum (log2) and, after run(), the row's sum
+
+  __device__ __forceinline__ Softmax(uint32_t tmem, int t, int warp, int lane_, uint8_t* p_tile, uint64_t* full, uint64_t* free_,
+                                     uint64_t* pfull, uint64_t* pv, uint64_t* sum, float scale)
+      : lane(lane_), site(57 + t), row_sums(reinterpret_cast<float*>(p_tile)), s_full(smem_addr(full)), s_free(smem_addr(free_)),
+        p_full(smem_addr(pfull)), pv_done(smem_addr(pv)), sums(smem_addr(sum)), scale_log2(scale) {
+    const int quarter = warp & 3;
+    half = (warp >> 2) & 1;
+    row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    s_addr = tmem + lanes + s_col(t) + 64 * half;  // this half's 64 keys
+    s_other = tmem + lanes + s_col(t) + 64 * (half ^ 1);
+    o_addr = tmem + lanes + o_col(t) + D / 2 * half;  // this half's channels
+    // P_t as TMA would lay out a tile: key chunk `half`, row `row`, unit u at u ^ (row % 8)
+    p_row = smem_addr(p_tile + half * CHUNK + row * 128);
+  }
+
+  // Key tiles k0 .. k0 + count - 1 for a row whose last visible key is lim. False: a wait ran out.
+  __device__ __forceinline__ bool run(int k0, int count, int lim) {
+    const float2 c2 = make_float2(scale_log2, scale_log2);
+    m = LOWEST;
+    l = 0.0f;
+    for (int j = 0; j < count; ++j, ++done) {
+      if (!mbar_wait_warp(s_full, done & 1, site, j)) return false;
+      tc_fence_after();
+      float f[64];
+      float other;
+      const int rel = lim - (k0 + j) * TILE - 64 * half, rel_other = rel + 64 * (2 * half - 1);
+      {
+        float h[32];
+        tmem_ld32f(s_addr, f);
+        tmem_ld32f(s_addr + 32, f + 32);
+        tmem_ld32f(s_other, h);
+        tc_wait_ld();
+        reg_fence32f(f);
+        reg_fence32f(f + 32);
+        reg_fence32f(h);
+        const bool cut = __any_sync(0xffffffffu, rel_other < 63);
+        if (cut) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (x > rel_other) h[x] = -INFINITY;
+        }
+        float mo[2] = {h[0], h[1]};
+#pragma unroll
+        for (int x = 2; x < 32; x += 4) {
+          mo[0] = max3(mo[0], h[x], h[x + 1]);
+          if (x + 3 < 32) mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
+        }
+        tmem_ld32f(s_other + 32, h);
+        tc_wait_ld();
+        reg_fence32f(h);
+        // S_t is in registers: the tensor core may write the next one
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        if (cut) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (x + 32 > rel_other) h[x] = -INFINITY;
+        }
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          mo[0] = max3(mo[0], h[x], h[x + 1]);
+          mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
+        }
+        other = fmaxf(mo[0], mo[1]);
+      }
+      if (__any_sync(0xffffffffu, rel < 63)) {
+#pragma unroll
+        for (int x = 0; x < 64; ++x)
+          if (x > rel) f[x] = -INFINITY;
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = max3(f[16 * c], f[16 * c + 1], f[16 * c + 2]);
+#pragma unroll
+        for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
+      }
+      const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
+      const float top = __fmul_rn(fmaxf(mine, other), scale_log2);
+      float a = 1.0f;
+      const bool raise = __any_sync(0xffffffffu, top > m + RAISE);  // the same rows in both halves' warps
+      if (raise) {
+        const float next = fmaxf(top, m);
+        a = ex2(m - next);
+        m = next;
+        l *= a;
+      }
+      const float2 mneg = make_float2(-m, -m);
+      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t w[32];
+#pragma unroll
+      for (int x = 0; x < 32; ++x) {
+        const float2 d = __ffma2_rn(make_float2(f[2 * x], f[2 * x + 1]), c2, mneg);
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        sum[x & 3] = __fadd2_rn(sum[x & 3], e);
+        w[x] = pack_bf16(e.x, e.y);
+      }
+      const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+      l += s4.x + s4.y;
+// the product of the step before has read P_t, and O_t is its
+      if (j > 0 ? !mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j)
+                : units > 0 && !mbar_wait_warp(sums, 1, site + 16, j))
+        return false;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((u ^ (row & 7)) << 4)), "r"(w[4 * u]),
+                     "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
+                     : "memory");
+      fence_proxy_async_smem();  // the tensor core reads P through the async proxy
+      tc_fence_after();
+      if (raise && j > 0) {
+        const float2 a2 = make_float2(a, a);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          float o[32];
+          tmem_ld32f(o_addr + 32 * c, o);
+          tc_wait_ld();
+          reg_fence32f(o);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
+            o[2 * x] = v.x;
+            o[2 * x + 1] = v.y;
+          }
+          tmem_st32f(o_addr + 32 * c, o);
+        }
+        tc_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (!mbar_wait_warp(pv_done, (done - 1) & 1, site + 4, count)) return false;
+    tc_fence_after();
+    // the halves' row sums meet in P_t's place
+    row_sums[half * TILE + row] = l;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sums);
+    if (!mbar_wait_warp(sums, 0, site + 8, count)) return false;
+    l = row_sums[row] + row_sums[TILE + row];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sums);  // read: the next unit's P may come
+    ++units;
+    return true;
+  }
+
+  // O of the row: to dst (bf16, normalized) or, unnormalized with m and l, to row `at` of a
+  // partial of `rows` rows. Every lane takes part; only live ones store.
+  __device__ __forceinline__ void store(bool live, float* part, int rows, int at, __nv_bfloat16* dst) {
+    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
+#pragma unroll 1
+    for (int c = 0; c < D / 64; ++c) {
+      float o[32];
+      tmem_ld32f(o_addr + 32 * c, o);
+      tc_wait_ld();
+      reg_fence32f(o);
+      if (live && part) {
+        float4* d4 = reinterpret_cast<float4*>(part + at * D + D / 2 * half + 32 * c);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) d4[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+      } else if (live) {
+        uint4* d4 = reinterpret_cast<uint4*>(dst + D / 2 * half + 32 * c);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          d4[x] = make_uint4(pack_bf16(o[8 * x] * inv, o[8 * x + 1] * inv), pack_bf16(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                             pack_bf16(o[8 * x + 4] * inv, o[8 * x + 5] * inv), pack_bf16(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+      }
+      __syncwarp();  // the loads above are made by whole warps
+    }
+    if (live && part && half == 0) {
+      part[rows * D + at] = m;
+      part[rows * D + rows + at] = l;
+    }
+    tc_fence_before();
+  }
+};
 
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -491,185 +681,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
-    const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + s_col(t) + 64 * half;         // this half's 64 keys
-    const uint32_t s_other = tmem + lanes + s_col(t) + 64 * (half ^ 1);
-    const uint32_t o_addr = tmem + lanes + o_col(t) + D / 2 * half;      // this half's channels
-    // P_t as TMA would lay out a tile: key chunk `half`, row `row`, unit u at u ^ (row % 8)
-    uint8_t* p_tile = base + L::p + t * 2 * CHUNK;
-    const uint32_t p_row = smem_addr(p_tile + half * CHUNK + row * 128);
-    const float2 c2 = make_float2(P.scale_log2, P.scale_log2);
-    const int row_tok = row / P.group, row_head = row - row_tok * P.group;
-    uint32_t done = 0;  // steps of this tile so far
-    int units = 0;
-    bool ok = true;
-    for (int i = 0; i < nseg && ok; ++i) {
+    const int t = warp >> 3;
+    Softmax<D> sm(tmem, t, warp, lane, base + L::p + t * 2 * CHUNK, &s_full[t], &s_free[t], &p_full[t], &pv_done[t], &sums[t],
+                  P.scale_log2);
+    const int row_tok = sm.row / P.group, row_head = sm.row - row_tok * P.group;
+    for (int i = 0; i < nseg; ++i) {
       const Segment g = segments[i];
       if (t == 1 && !two_tiles(g)) continue;
       const int tok = g.tok0 + t * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < g.n;
-      const int lim = live ? g.len - g.n + tok : 0x7fffffff;  // last visible key; rows that are not there see all
-      float m = LOWEST, l = 0.0f;
-      for (int j = 0; j < g.count; ++j, ++done) {
-        if (!mbar_wait_warp(smem_addr(&s_full[t]), done & 1, 57 + t, j)) { ok = false; break; }
-        tc_fence_after();
-        float f[64];
-        float other;
-        const int rel = lim - (g.k0 + j) * TILE - 64 * half, rel_other = rel + 64 * (2 * half - 1);
-        {
-          float h[32];
-          tmem_ld32f(s_addr, f);
-          tmem_ld32f(s_addr + 32, f + 32);
-          tmem_ld32f(s_other, h);
-          tc_wait_ld();
-          reg_fence32f(f);
-          reg_fence32f(f + 32);
-          reg_fence32f(h);
-          const bool cut = __any_sync(0xffffffffu, rel_other < 63);
-          if (cut) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (x > rel_other) h[x] = -INFINITY;
-          }
-          float mo[2] = {h[0], h[1]};
-#pragma unroll
-          for (int x = 2; x < 32; x += 4) {
-            mo[0] = max3(mo[0], h[x], h[x + 1]);
-            if (x + 3 < 32) mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
-          }
-          tmem_ld32f(s_other + 32, h);
-          tc_wait_ld();
-          reg_fence32f(h);
-          // S_t is in registers: the tensor core may write the next one
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_addr(&s_free[t]));
-          if (cut) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (x + 32 > rel_other) h[x] = -INFINITY;
-          }
-#pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            mo[0] = max3(mo[0], h[x], h[x + 1]);
-            mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
-          }
-          other = fmaxf(mo[0], mo[1]);
-        }
-        if (__any_sync(0xffffffffu, rel < 63)) {
-#pragma unroll
-          for (int x = 0; x < 64; ++x)
-            if (x > rel) f[x] = -INFINITY;
-        }
-        float mx[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = max3(f[16 * c], f[16 * c + 1], f[16 * c + 2]);
-#pragma unroll
-          for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
-        }
-        const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
-        const float top = __fmul_rn(fmaxf(mine, other), P.scale_log2);
-        float a = 1.0f;
-        const bool raise = __any_sync(0xffffffffu, top > m + RAISE);  // the same rows in both halves' warps
-        if (raise) {
-          const float next = fmaxf(top, m);
-          a = ex2(m - next);
-          m = next;
-          l *= a;
-        }
-        const float2 mneg = make_float2(-m, -m);
-        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t w[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const float2 d = __ffma2_rn(make_float2(f[2 * x], f[2 * x + 1]), c2, mneg);
-          const float2 e = make_float2(ex2(d.x), ex2(d.y));
-          sum[x & 3] = __fadd2_rn(sum[x & 3], e);
-          w[x] = pack_bf16(e.x, e.y);
-        }
-        const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
-        l += s4.x + s4.y;
-        // the product of the step before has read P_t, and O_t is its
-        if (j > 0 ? !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 59 + t, j)
-                  : units > 0 && !mbar_wait_warp(smem_addr(&sums[t]), 1, 73 + t, j)) {
-          ok = false;
-          break;
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((u ^ (row & 7)) << 4)), "r"(w[4 * u]),
-                       "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
-                       : "memory");
-        fence_proxy_async_smem();  // the tensor core reads P through the async proxy
-        tc_fence_after();
-        if (raise && j > 0) {
-          const float2 a2 = make_float2(a, a);
-#pragma unroll 1
-          for (int c = 0; c < D / 64; ++c) {
-            float o[32];
-            tmem_ld32f(o_addr + 32 * c, o);
-            tc_wait_ld();
-            reg_fence32f(o);
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
-              o[2 * x] = v.x;
-              o[2 * x + 1] = v.y;
-            }
-            tmem_st32f(o_addr + 32 * c, o);
-          }
-          tc_wait_st();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&p_full[t]));
-      }
-      if (!ok || !mbar_wait_warp(smem_addr(&pv_done[t]), (done - 1) & 1, 61 + t, i)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      // the halves' row sums meet in P_t's place
-      float* row_sums = reinterpret_cast<float*>(p_tile);
-      row_sums[half * TILE + row] = l;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sums[t]));
-      if (!mbar_wait_warp(smem_addr(&sums[t]), 0, 65 + t, i)) { ok = false; break; }
-      l = row_sums[row] + row_sums[TILE + row];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&sums[t]));  // read: the next unit's P may come
-      ++units;
-      const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
+      // last visible key; rows that are not there see all
+      if (!sm.run(g.k0, g.count, live ? g.len - g.n + tok : 0x7fffffff)) break;
       float* part = g.slot < 0 ? nullptr : P.parts + static_cast<int64_t>(g.slot) * (ROWS * D + 2 * ROWS);
-      __nv_bfloat16* dst =
-          P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh + D / 2 * half;
-#pragma unroll 1
-      for (int c = 0; c < D / 64; ++c) {
-        float o[32];
-        tmem_ld32f(o_addr + 32 * c, o);
-        tc_wait_ld();
-        reg_fence32f(o);
-        if (live && part) {
-          float4* d4 = reinterpret_cast<float4*>(part + (t * TILE + row) * D + D / 2 * half + 32 * c);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) d4[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        } else if (live) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + 32 * c);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            d4[x] = make_uint4(pack_bf16(o[8 * x] * inv, o[8 * x + 1] * inv), pack_bf16(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
-                               pack_bf16(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
-                               pack_bf16(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
-        }
-        __syncwarp();  // the loads above are made by whole warps
-      }
-      if (part && live && half == 0) {
-        part[ROWS * D + t * TILE + row] = m;
-        part[ROWS * D + ROWS + t * TILE + row] = l;
-      }
-      tc_fence_before();
+      sm.store(live, part, ROWS, t * TILE + sm.row,
+               P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh);
     }
   }
   __syncthreads();
@@ -680,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // Joins the partials of the unit that ended in run blockIdx.x, a warp per row, in run order.
-template <int D>
+template <int D, int ROWS, typename Params>
 __global__ void __launch_bounds__(256) prefill_combine_kernel(Params P) {
   constexpr int V = D / 32;
   constexpr int64_t SIZE = ROWS * D + 2 * ROWS;
@@ -798,105 +823,9 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
   FAQ_CHECK_ARG(ctas < (int64_t(1) << 31), "too many keys for one call");
   FAQ_CUDA(launch_early(paged_expand_kernel<NG>, dim3(static_cast<unsigned>(ctas)), 32 * EXPAND_WARPS, 0, stream, P));
   FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(P.runs)), THREADS, Smem<NG>::bytes, stream, mq, mk, mv, P));
-  FAQ_CUDA(launch_early(prefill_combine_kernel<D>, dim3(static_cast<unsigned>(P.runs), ROWS / 8), 256, 0, stream, P));
+  FAQ_CUDA(launch_early(prefill_combine_kernel<D, ROWS, Params>, dim3(static_cast<unsigned>(P.runs), ROWS / 8), 256, 0, stream, P));
   return FAQ_OK;
 }
 
 }  // namespace pre
 }  // namespace faq
-
-namespace faq {
-namespace pre {
-// From this many rows (new tokens x query heads of a kv head) a sequence is the prompt kernel's.
-constexpr int MIN_ROWS = 65;
-// Whether a call may have such a sequence, and whether all of its sequences are.
-inline bool any_prompt(int64_t group, int64_t max_new, int64_t total) {
-  return group <= TILE && group * std::min(max_new, total) >= MIN_ROWS;
-}
-inline bool all_prompts(int64_t group, int64_t max_new, int64_t total, int64_t batch) {
-  return any_prompt(group, max_new, total) && total == batch * max_new;
-}
-}  // namespace pre
-}  // namespace faq
-
-extern "C" size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch,
-                                                           int64_t max_new, int64_t max_len, int64_t total_len, int d) {
-  using namespace faq;
-  if (total < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || batch <= 0 || max_new < 0 || max_len < 0 ||
-      total_len < 0 || (d != 64 && d != 128))
-    return 0;
-  const int64_t group = heads / kv_heads;
-  const size_t few = pat::workspace(pat::n_blocks(std::min<int64_t>(max_new, 4096) * group), d);
-  if (!pre::any_prompt(group, max_new, total)) return few;
-  return std::max(few, pre::layout(total, heads, kv_heads, batch, max_len, total_len, pre::MIN_ROWS, d).bytes);
-}
-
-extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride,
-                                        int64_t q_head_stride, const void* pages, int64_t num_pages,
-                                        int64_t page_stride, int page_size, int64_t kv_heads, int d,
-                                        const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
-                                        const int32_t* lens, int64_t batch, int64_t max_new, int64_t max_len,
-                                        int64_t total_len, float scale, void* out, int64_t out_token_stride,
-                                        int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
-  using namespace faq;
-  kvp::Pages pages_;
-  int rc = kvp::make_pages(pages_, pages, num_pages, page_stride, page_size, kv_heads, d, table, table_ld, table_cols, cu,
-                           lens, batch);
-  if (rc) return rc;
-  FAQ_CHECK_ARG(heads > 0 && heads % kv_heads == 0, "query heads must be divisible by key/value heads");
-  const int64_t group = heads / kv_heads;
-  FAQ_CHECK_ARG(group < 4096, "more than 4095 query heads per key/value head");
-  FAQ_CHECK_ARG(total >= 0 && max_new >= 0 && max_len >= 0 && total_len >= 0 && total * heads < (int64_t(1) << 31) &&
-                    max_len < (int64_t(1) << 31) && total_len < (int64_t(1) << 40), "bad token count");
-  if (total == 0) return FAQ_OK;
-  FAQ_CHECK_ARG(q && out, "null pointer");
-  FAQ_CHECK_ARG(scale > 0.0f && scale < 3.0e38f, "scale must be positive and finite");
-  FAQ_CHECK_ARG(aligned16(q) && aligned16(out) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
-                    out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
-                "q and out must be 16-byte aligned with strides multiple of 8");
-  FAQ_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
-                "workspace must be a 256-byte aligned device buffer");
-  FAQ_CHECK_ARG(workspace_bytes >= faq_hif4_paged_attention_workspace_bytes(total, heads, kv_heads, batch, max_new, max_len,
-                                                                            total_len, d),
-                "workspace too small: faq_hif4_paged_attention_workspace_bytes() bytes needed");
-  const float scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  const bool prompts = pre::any_prompt(group, max_new, total);
-  if (!prompts || !pre::all_prompts(group, max_new, total, batch)) {
-    pat::Params P;
-    P.p = pages_;
-    P.q = static_cast<const __nv_bfloat16*>(q);
-    P.qt = q_token_stride;
-    P.qh = q_head_stride;
-    P.out = static_cast<__nv_bfloat16*>(out);
-    P.ot = out_token_stride;
-    P.oh = out_head_stride;
-    P.total = total;
-    P.max_rows = prompts ? pre::MIN_ROWS - 1 : 0x7fffffff;
-    P.group = static_cast<int>(group);
-    P.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + group - 1) / group);
-    P.scale_log2 = scale_log2;
-    const int nb = pat::n_blocks(std::min<int64_t>(max_new, 4096) * group);
-    if (d == 64)
-      rc = nb == 1 ? pat::launch<1, 1>(P, workspace, stream) : nb == 2 ? pat::launch<1, 2>(P, workspace, stream)
-                                                                       : pat::launch<1, 4>(P, workspace, stream);
-    else
-      rc = nb == 1 ? pat::launch<2, 1>(P, workspace, stream) : nb == 2 ? pat::launch<2, 2>(P, workspace, stream)
-                                                                       : pat::launch<2, 4>(P, workspace, stream);
-    if (rc || !prompts) return rc;
-  }
-  pre::Params P;
-  P.p = pages_;
-  P.total = total;
-  P.group = static_cast<int>(group);
-  P.tile_tokens = static_cast<int>(pre::TILE / group);
-  P.min_rows = pre::MIN_ROWS;
-  P.scale_log2 = scale_log2;
-  P.out = static_cast<__nv_bfloat16*>(out);
-  P.ot = out_token_stride;
-  P.oh = out_head_stride;
-  const pre::Layout a = pre::layout(total, heads, kv_heads, batch, max_len, total_len, pre::MIN_ROWS, d);
-  return d == 64 ? pre::launch<1>(P, static_cast<const __nv_bfloat16*>(q), heads, q_token_stride, q_head_stride, a,
-                                  static_cast<char*>(workspace), stream)
-                 : pre::launch<2>(P, static_cast<const __nv_bfloat16*>(q), heads, q_token_stride, q_head_stride, a,
-                                  static_cast<char*>(workspace), stream);
-}
