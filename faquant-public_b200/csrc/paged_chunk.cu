@@ -130,8 +130,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
   uint64_t* s_free = bars + 11;
   uint64_t* p_full = bars + 12;
   uint64_t* pv_done = bars + 13;
-  uint64_t* sums = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   __shared__ int64_t s_scan[WARPS], s_begin, s_end, s_per;
   __shared__ Walk s_walk;
   __shared__ int s_empty;
@@ -144,7 +143,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
     mbar_init(smem_addr(s_free), 8);
     mbar_init(smem_addr(p_full), 8);
     mbar_init(smem_addr(pv_done), 1);
-    mbar_init(smem_addr(sums), 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&k_full[i]), 8);  // the eight expanding warps
       mbar_init(smem_addr(&k_empty[i]), 1);
@@ -367,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
-    Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, sums, P.scale_log2);
+    Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
     const int row_tok = sm.row / P.group, row_head = sm.row - row_tok * P.group;
     for (Walk w = s_walk; w.count > 0; next_unit(P, w, begin, end)) {
       const int tok = w.u * P.tile_tokens + row_tok;

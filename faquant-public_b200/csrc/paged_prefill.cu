@@ -273,7 +273,7 @@ struct Smem {
   static constexpr int q = 0;
   static constexpr int k = q + 2 * tile;
   static constexpr int v = k + 2 * tile;     // one stage
-  static constexpr int p = v + tile;         // P of both tiles; after a unit's last product, its row sums
+  static constexpr int p = v + tile;         // P of both tiles
   static constexpr int bar = p + 4 * CHUNK;
   static constexpr int bytes = 1024 + bar + 256;
 };
@@ -306,85 +306,79 @@ __device__ __forceinline__ void commit(uint32_t bar) {
       : "memory");
 }
 
+// Named barriers over `count` threads that also AND or OR a predicate across them.
+__device__ __forceinline__ bool bar_and(int id, int count, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v)), "r"(id), "r"(count)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ bool bar_or(int id, int count, bool v) { return !bar_and(id, count, !v); }
+
 // The softmax of a tile of 128 rows by eight warps: warps 0-3 of them (by TMEM lane quarter)
 // take keys 0..63 of every key tile and the lower half of O's channels, warps 4-7 the others.
 template <int D>
 struct Softmax {
-  int row, half, lane, site;
-  uint32_t s_addr, s_other, o_addr, p_row;
-  float* row_sums;
-  uint32_t s_full, s_free, p_full, pv_done, sums;
+  int row, half, lane, site, barrier;
+  uint32_t s_addr, o_addr, p_row;
+  float *mine_at, *other_at;  // what the row's halves tell each other, where their P stands
+  uint32_t s_full, s_free, p_full, pv_done;
   float scale_log2;
   uint32_t done = 0;  // steps so far
-  int units = 0;
   float m, l;         // the unit's reference maximum (log2) and, after run(), the row's sum
 
-  __device__ __forceinline__ Softmax(uint32_t tmem, int t, int warp, int lane_, uint8_t* p_tile, uint64_t* full, uint64_t* free_,
-                                     uint64_t* pfull, uint64_t* pv, uint64_t* sum, float scale)
-      : lane(lane_), site(57 + t), row_sums(reinterpret_cast<float*>(p_tile)), s_full(smem_addr(full)), s_free(smem_addr(free_)),
-        p_full(smem_addr(pfull)), pv_done(smem_addr(pv)), sums(smem_addr(sum)), scale_log2(scale) {
+  __device__ __forceinline__ Softmax(uint32_t tmem, int t, int warp, int lane_, uint8_t* p_tile, uint64_t* full,
+                                     uint64_t* free_, uint64_t* pfull, uint64_t* pv, float scale)
+      : lane(lane_), site(57 + t), s_full(smem_addr(full)), s_free(smem_addr(free_)), p_full(smem_addr(pfull)),
+        pv_done(smem_addr(pv)), scale_log2(scale) {
     const int quarter = warp & 3;
     half = (warp >> 2) & 1;
+    barrier = 1 + t * 4 + quarter;
     row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     s_addr = tmem + lanes + s_col(t) + 64 * half;  // this half's 64 keys
-    s_other = tmem + lanes + s_col(t) + 64 * (half ^ 1);
     o_addr = tmem + lanes + o_col(t) + D / 2 * half;  // this half's channels
     // P_t as TMA would lay out a tile: key chunk `half`, row `row`, unit u at u ^ (row % 8)
-    p_row = smem_addr(p_tile + half * CHUNK + row * 128);
+    mine_at = reinterpret_cast<float*>(p_tile + half * CHUNK + row * 128);
+    other_at = reinterpret_cast<float*>(p_tile + (half ^ 1) * CHUNK + row * 128);
+    p_row = smem_addr(mine_at);
   }
 
-  // Key tiles k0 .. k0 + count - 1 for a row whose last visible key is lim. False: a wait ran out.
+  // The row's other half's value, between the two warps of 32 rows, through P_t's place (no
+  // product may be reading it). Both come here together, whatever happened before: `ok` tells
+  // whether both are well, so that neither is left waiting.
+  __device__ __forceinline__ bool exchange(bool ok, float mine, float& other) {
+    *mine_at = mine;
+    const bool both = bar_and(barrier, 64, ok);
+    other = *other_at;
+    return bar_and(barrier, 64, both);  // read: P_t may be written
+  }
+
+  // Key tiles k0 .. k0 + count - 1 for a row whose last visible key is lim. False: a wait ran
+  // out. (Warps whose rows are all dead work like the others: leaving their exponentials out
+  // gained nothing, the live ones are bound by their own latency.)
   __device__ __forceinline__ bool run(int k0, int count, int lim) {
     const float2 c2 = make_float2(scale_log2, scale_log2);
     m = LOWEST;
     l = 0.0f;
+    bool ok = true;
     for (int j = 0; j < count; ++j, ++done) {
-      if (!mbar_wait_warp(s_full, done & 1, site, j)) return false;
+      ok = ok && mbar_wait_warp(s_full, done & 1, site, j);
       tc_fence_after();
       float f[64];
-      float other;
-      const int rel = lim - (k0 + j) * TILE - 64 * half, rel_other = rel + 64 * (2 * half - 1);
-      {
-        float h[32];
-        tmem_ld32f(s_addr, f);
-        tmem_ld32f(s_addr + 32, f + 32);
-        tmem_ld32f(s_other, h);
-        tc_wait_ld();
-        reg_fence32f(f);
-        reg_fence32f(f + 32);
-        reg_fence32f(h);
-        const bool cut = __any_sync(0xffffffffu, rel_other < 63);
-        if (cut) {
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (x > rel_other) h[x] = -INFINITY;
-        }
-        float mo[2] = {h[0], h[1]};
-#pragma unroll
-        for (int x = 2; x < 32; x += 4) {
-          mo[0] = max3(mo[0], h[x], h[x + 1]);
-          if (x + 3 < 32) mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
-        }
-        tmem_ld32f(s_other + 32, h);
-        tc_wait_ld();
-        reg_fence32f(h);
-        // S_t is in registers: the tensor core may write the next one
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
-        if (cut) {
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (x + 32 > rel_other) h[x] = -INFINITY;
-        }
-#pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          mo[0] = max3(mo[0], h[x], h[x + 1]);
-          mo[1] = max3(mo[1], h[x + 2], h[x + 3]);
-        }
-        other = fmaxf(mo[0], mo[1]);
-      }
+      tmem_ld32f(s_addr, f);
+      tmem_ld32f(s_addr + 32, f + 32);
+      tc_wait_ld();
+      reg_fence32f(f);
+      reg_fence32f(f + 32);
+      // S_t is in registers: the tensor core may write the next one
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
+      const int rel = lim - (k0 + j) * TILE - 64 * half;
       if (__any_sync(0xffffffffu, rel < 63)) {
 #pragma unroll
         for (int x = 0; x < 64; ++x)
@@ -398,11 +392,14 @@ struct Softmax {
         for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
       }
       const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
-      const float top = __fmul_rn(fmaxf(mine, other), scale_log2);
+      // raise the maxima of the 32 rows when either half has a score far above them (or has to give up)
       float a = 1.0f;
-      const bool raise = __any_sync(0xffffffffu, top > m + RAISE);  // the same rows in both halves' warps
+      const bool raise = bar_or(barrier, 64, __fmul_rn(mine, scale_log2) > m + RAISE || !ok);
       if (raise) {
-        const float next = fmaxf(top, m);
+        if (j > 0) ok = ok && mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j);
+        float other;
+        if (!exchange(ok, mine, other)) return false;
+        const float next = fmaxf(__fmul_rn(fmaxf(mine, other), scale_log2), m);
         a = ex2(m - next);
         m = next;
         l *= a;
@@ -419,10 +416,8 @@ struct Softmax {
       }
       const float2 s4 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
       l += s4.x + s4.y;
-// the product of the step before has read P_t, and O_t is its
-      if (j > 0 ? !mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j)
-                : units > 0 && !mbar_wait_warp(sums, 1, site + 16, j))
-        return false;
+      // the product of the step before has read P_t, and O_t is its
+      if (j > 0) ok = mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j);
 #pragma unroll
       for (int u = 0; u < 8; ++u)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((u ^ (row & 7)) << 4)), "r"(w[4 * u]),
@@ -452,17 +447,11 @@ struct Softmax {
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
-    if (!mbar_wait_warp(pv_done, (done - 1) & 1, site + 4, count)) return false;
+    ok = ok && mbar_wait_warp(pv_done, (done - 1) & 1, site + 4, count);
     tc_fence_after();
-    // the halves' row sums meet in P_t's place
-    row_sums[half * TILE + row] = l;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(sums);
-    if (!mbar_wait_warp(sums, 0, site + 8, count)) return false;
-    l = row_sums[row] + row_sums[TILE + row];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(sums);  // read: the next unit's P may come
-    ++units;
+    float other;
+    if (!exchange(ok, l, other)) return false;
+    l = half ? other + l : l + other;  // the same sum in both halves
     return true;
   }
 
@@ -516,8 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_free = bars + 10;  // S_t in the registers of the tile's eight warps
   uint64_t* p_full = bars + 12;  // P_t written (and O_t rescaled) by them
   uint64_t* pv_done = bars + 14; // O_t += P_t V completed
-  uint64_t* sums = bars + 16;    // [2 tiles] a unit's row sums are there (even phases), read (odd)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(q_full), 1);
@@ -531,7 +519,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(smem_addr(&s_free[i]), 8);
       mbar_init(smem_addr(&p_full[i]), 8);
       mbar_init(smem_addr(&pv_done[i]), 1);
-      mbar_init(smem_addr(&sums[i]), 8);
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmap_q);
@@ -682,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
     const int t = warp >> 3;
-    Softmax<D> sm(tmem, t, warp, lane, base + L::p + t * 2 * CHUNK, &s_full[t], &s_free[t], &p_full[t], &pv_done[t], &sums[t],
+    Softmax<D> sm(tmem, t, warp, lane, base + L::p + t * 2 * CHUNK, &s_full[t], &s_free[t], &p_full[t], &pv_done[t],
                   P.scale_log2);
     const int row_tok = sm.row / P.group, row_head = sm.row - row_tok * P.group;
     for (int i = 0; i < nseg; ++i) {
