@@ -205,12 +205,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
   // ---- this CTA's run of key blocks: a prefix sum over the sequences, one per thread (and
   // round, past THREADS sequences); the thread that holds the run's start makes its segment
   Seq sq = {0, 0, 0};
-  int64_t mine = 0, upto = 0;
+  int64_t per_head = 0, mine = 0, upto = 0;
   auto count_blocks = [&](int b) {  // warps without a sequence do nothing
     if (b - lane >= p.batch) return;
     sq = {0, 0, 0};
     if (b < p.batch) sq = sequence(P, b);
-    mine = head_cost(P, sq) * p.kv_heads;
+    per_head = head_cost(P, sq);
+    mine = per_head * p.kv_heads;
     if (sq.n > sq.len) s_empty = 1;
     upto = mine;
 #pragma unroll
@@ -250,7 +251,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
       if (begin < end && begin >= start && begin < start + mine) {
         Segment x;
         x.b = b;
-        const int64_t per_head = mine / p.kv_heads;
         const int64_t at = begin - start;
         x.head = static_cast<int>(mine < (int64_t(1) << 31) ? static_cast<uint32_t>(at) / static_cast<uint32_t>(per_head)
                                                             : at / per_head);
@@ -266,9 +266,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
         fill(x, sq, begin, end);
         if (x.count == 0) next_unit(x, begin, end);  // the run starts behind the unit's last block
         s_seg[0] = x;
-        Segment y = x;
-        if (y.count) next_unit(y, begin, end);
-        s_seg[1] = y;
         s_any = x.count > 0;
       }
     }
@@ -366,8 +363,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
   int cur = 0;
   bool ok = true;
   ahead_blocks = blocks_of(s_seg[0]);
+  // the last warps have the fewest blocks: Q and the second segment are theirs to make
+  if (warp == W - 1) make_q(s_seg[0]);
+  if (tid == THREADS - 64) {
+    Segment y = s_seg[0];
+    next_unit(y, blockIdx.x * s_per, s_end);
+    s_seg[1] = y;
+  }
   top_up(0, 0, false);
-  if (warp == 0) make_q(s_seg[0]);
   __syncthreads();
 
   while (true) {
