@@ -43,7 +43,7 @@ constexpr int RB = 8;       // rows of a unit
 constexpr int W = 16;       // warps of a CTA, one CTA per SM: 128 registers a thread
 constexpr int THREADS = 32 * W;
 constexpr int S = 4;        // blocks in flight per warp, 2 x 1184 bytes each at d = 128
-constexpr int COST = W;     // of a unit beyond its blocks, see below
+constexpr int COST = 2 * W; // of a unit beyond its blocks, see below
 constexpr float RAISE = 8.0f;  // log2 headroom of a row's reference maximum
 constexpr float LOWEST = -3.402823466e38f;  // where it starts: below every finite score
 
