@@ -6,7 +6,9 @@ Mirrors ``qwen3._attention_forward`` (``src/faquant/qwen3.py:56-172``) with the 
 :282-346``): q/k/v projections, q_norm/k_norm, RoPE, then one fp32 excursion for
 ``k - offset``, Smooth-QK ``q * s`` / ``k / s`` and the Hadamard over head_dim with a
 single bf16 rounding -- here one K4 launch per operand -- then the HiF4 attention
-backend (``faquant_b200.attention``) and ``o_proj``.
+backend (``faquant_b200.attention``) and ``o_proj``. With ``faquant_attention_kernel =
+"paged"`` and a :class:`~faquant_b200.kv_cache.PagedKVCache` as ``past_key_values`` the keys and
+values go to 4-bit pages instead and the paged attention runs on them.
 """
 
 from __future__ import annotations
@@ -17,6 +19,7 @@ import torch
 
 from . import ops
 from .attention import simulated_flash_attention_forward
+from .kv_cache import PagedKVCache
 
 
 def qk_pretransform(module, query_states: torch.Tensor, key_states: torch.Tensor):
@@ -76,10 +79,17 @@ def attention_forward(
         query_states = ops.qk_prep(query_states, levels=ops.default_levels("act"), rotate=False)[0]
         key_states = ops.qk_prep(key_states, levels=ops.default_levels("act"), rotate=False)[0]
         value_states = ops.qk_prep(value_states, levels=ops.default_levels("act"), rotate=False)[0]
+    kernel = getattr(self, "faquant_attention_kernel", "simulated")
+    if kernel == "paged":  # write to the HiF4 pages, attend over them (P not quantized)
+        if not isinstance(past_key_values, PagedKVCache):
+            raise ValueError('faquant_attention_kernel "paged" needs a PagedKVCache as past_key_values')
+        if attention_mask is not None:
+            raise NotImplementedError("attention masks are not implemented by the paged attention of faquant_b200")
+        attn_output = past_key_values.forward(self.layer_idx, query_states, key_states, value_states, self.scaling)
+        return _project(self, attn_output, input_shape), None
     if past_key_values is not None:
         cache_kwargs = {"sin": sin, "cos": cos, "cache_position": cache_position}
         key_states, value_states = past_key_values.update(key_states, value_states, self.layer_idx, cache_kwargs)
-    kernel = getattr(self, "faquant_attention_kernel", "simulated")
     if kernel == "simulated":  # the HiF4 attention of this package
         kwargs["cache_position"] = cache_position
         interface = simulated_flash_attention_forward
@@ -94,7 +104,12 @@ def attention_forward(
     attn_output, attn_weights = interface(
         self, query_states, key_states, value_states, attention_mask, dropout=0.0, scaling=self.scaling,
         sliding_window=getattr(self, "sliding_window", None), **kwargs)
+    return _project(self, attn_output, input_shape), attn_weights
+
+
+def _project(module, attn_output: torch.Tensor, input_shape) -> torch.Tensor:
+    """The output projection, with its input quantized first where the adapter asks for it."""
     attn_output = attn_output.reshape(*input_shape, -1).contiguous()
-    if getattr(self, "faquant_attention_output_quant", False) and not getattr(self.o_proj, "faquant_quantizes_input", False):
+    if getattr(module, "faquant_attention_output_quant", False) and not getattr(module.o_proj, "faquant_quantizes_input", False):
         attn_output = ops.hif4_quantize(attn_output, levels=ops.default_levels("act"))[0]
-    return self.o_proj(attn_output), attn_weights
+    return module.o_proj(attn_output)

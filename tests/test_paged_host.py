@@ -70,3 +70,35 @@ def test_operators_refuse_cpu_tensors() -> None:
         ops.hif4_paged_attention(x, pages, table, cu, lens, page_size=16, max_new=1)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.verify_drafts(torch.zeros(1, 1, dtype=torch.int64), torch.ones(1, 2, 4), None, torch.ones(1, 1), torch.ones(1))
+
+
+def test_lookup_drafts() -> None:
+    from faquant_b200.generate import lookup_drafts
+
+    assert lookup_drafts([1, 2, 3, 9, 1, 2, 3], 3, 3) == [9, 1, 2]
+    assert lookup_drafts([1, 2, 3, 9, 7, 2, 3], 2, 3) == [9, 7]  # the last three do not recur, the last two do
+    assert lookup_drafts([5, 6, 5, 7, 5], 4, 1) == [7, 5]  # the latest occurrence
+    assert lookup_drafts([1, 2, 3], 4, 3) == [] and lookup_drafts([1], 4, 3) == [] and lookup_drafts([1, 1], 0, 2) == []
+
+
+def test_paged_attention_needs_its_cache_and_no_mask() -> None:
+    import types
+
+    from faquant_b200.generate import paged_speculative_generate
+    from faquant_b200.kv_cache import PagedKVCache
+
+    with pytest.raises(ValueError):
+        paged_speculative_generate(types.SimpleNamespace(), input_ids=torch.zeros(2, 3, dtype=torch.int64), max_length=9)
+    with pytest.raises(ValueError):
+        paged_speculative_generate(types.SimpleNamespace(), input_ids=torch.zeros(1, 3, dtype=torch.int64), max_length=9,
+                                   num_drafts=-1)
+    out, stats = paged_speculative_generate(types.SimpleNamespace(), input_ids=torch.zeros(1, 3, dtype=torch.int64), max_length=3)
+    assert out.shape == (1, 3) and stats["steps"] == 0
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 2, 96, max_length=10, device="cpu")
+    cache = PagedKVCache(2, 2, 64, max_length=100, page_size=16, device="cpu")  # host bookkeeping runs anywhere
+    cache.extend([33])
+    assert cache.get_seq_length() == 33 and cache.table[0, :4].tolist() == [0, 1, 2, -1]
+    cache.truncate([16])
+    cache.extend([1])
+    assert cache.lengths == [17] and len(cache._held[0]) == 2 and cache.get_mask_sizes(5) == (22, 0)
