@@ -492,6 +492,7 @@ extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t he
     P.oh = out_head_stride;
     P.total = total;
     P.group = static_cast<int>(group);
+    P.split = max_len > pat::WHOLE;
     P.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + group - 1) / group);
     P.scale_log2 = scale_log2;
     return d == 64 ? pat::launch<1>(P, ws, stream) : pat::launch<2>(P, ws, stream);
