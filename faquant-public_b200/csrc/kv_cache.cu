@@ -10,6 +10,11 @@
 // (V's words interleave them) and stores 8 or 16 bytes. The packed tokens of a ragged batch
 // are found without a prefix sum over its blocks: sequence b's blocks get the slots from
 // cu[b] / 16 + 2 b on, always enough of them (n tokens touch at most n / 16 + 2 blocks).
+//
+// Measured (one B200, 8 kv heads of 128): writing 8192 tokens and reading them back 25.3 us for
+// 86 MB, 3.4 TB/s, where the write is bound by the fit's instructions; reading whole contexts
+// of 8 sequences back (156 MB) 35.8 us, 4.4 TB/s, bound by HBM and the ramps of a launch. A decode step's
+// tokens take the 8 us of two launches.
 #include <algorithm>
 #include <atomic>
 

@@ -18,9 +18,17 @@
 // soon as it is in their registers, so the next S_t is computed under their exponentials, and
 // write P_t (bf16) to shared memory as the A operand of O_t += P_t V. (P_t in tensor memory,
 // over S_t, saves shared-memory traffic but chains the next S_t behind this product: 4700
-// cycles per key tile against TODO.)
+// cycles per pair of 128 x 128 tiles against 4000.)
 // Softmax: a row's reference maximum is raised only when a score passes it by more than 2^8
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
+//
+// Measured (one B200, d = 128): the last 512 of 32768 tokens with 64 query heads on 8 kv heads
+// in 554 us, 985 TFLOP/s counting the visible pairs (642 us and 850 TFLOP/s in a long series,
+// where the power limit lowers the clocks); all of a 16384-token prompt with 32 heads 1078
+// TFLOP/s. The expansion takes 36 us of the first. Bound by the exponentials: a pair of tiles has
+// 32768 of them per key tile, 2048 cycles of the SM's special function units, and with the
+// maxima, conversions and stores around them a key tile takes about 4000 cycles where the
+// products alone need 2048.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -37,7 +37,7 @@ struct Params {
 
 // CTAs per sequence: as many (up to 8) as fill the GPU's two CTAs per SM once. More than that
 // run in waves whose gathers and joins leave the memory idle: 128 sequences of 151936 fp32
-// weights took 43 us with clusters of 8 against TODO with 2.
+// weights and their draft distributions took 43 us with clusters of 8, 28.8 with 2.
 inline int cluster_of(int64_t batch) {
   int c = 8;
   while (c > 1 && batch * c > 2 * num_sms()) c /= 2;

@@ -58,14 +58,16 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     device = None
+    index = -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()  # -1 for a host tensor
+        if at < 0:
             raise RuntimeError("faquant_b200 operators run on CUDA tensors only (no CPU fallback)")
         if device is None:
-            device = t.device
-        elif t.device != device:
+            device, index = t.device, at
+        elif at != index:
             raise RuntimeError("all tensors must be on the same CUDA device")
     if device is None:
         raise RuntimeError("no CUDA tensor given")
@@ -694,32 +696,41 @@ def hif4_page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
 
 
 def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, kv_heads: int,
-            head_dim: int, page_size: int) -> int:
-    """Checks of a pool and the arrays that describe a ragged batch on it; the batch size."""
+            head_dim: int, page_size: int) -> tuple:
+    """Checks of a pool and the arrays that describe a ragged batch on it. Returns the C
+    calls' arguments for them: ``(pages, num_pages, page_stride, page_size)`` and ``(table, row
+    stride, columns, cu, lens, batch)``."""
     size = hif4_page_bytes(kv_heads, head_dim, page_size)
     shape, stride = pages.shape, pages.stride()
     if pages.dtype is not torch.uint8 or len(shape) < 2:
         raise TypeError("pages must be a uint8 tensor [num_pages, ...]")
-    if len(shape) == 4 and shape[1:3] != (2, kv_heads):
-        raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
-    inner = 1
-    for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
-        if st != inner and n != 1:
-            raise ValueError("a page must be contiguous bytes")
-        inner *= n
-    if inner != size:
-        raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) bytes")
+    if len(shape) == 4:
+        if shape[1] != 2 or shape[2] != kv_heads:
+            raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
+        inner = size // (2 * kv_heads)
+        whole = shape[3] == inner and stride[1:] == (kv_heads * inner, inner, 1)
+    else:
+        inner = 1
+        whole = True
+        for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
+            whole = whole and (st == inner or n == 1)
+            inner *= n
+        whole = whole and inner == size
+    if not whole:
+        raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
     if table.dtype is not torch.int32 or cu.dtype is not torch.int32 or lens.dtype is not torch.int32:
         raise TypeError("table, cu and lens must be int32")
-    columns = table.shape
-    if len(columns) != 2 or columns[1] < 1 or table.stride(1) != 1:
+    columns, ld = table.shape, table.stride()
+    if len(columns) != 2 or columns[1] < 1 or ld[1] != 1:
         raise ValueError("table must be [batch, columns] with unit column stride")
     batch = columns[0]
     if cu.shape != (batch + 1,) or lens.shape != (batch,):
         raise ValueError("cu must be [batch + 1] and lens [batch]")
-    if not cu.is_contiguous() or not lens.is_contiguous():
+    if (batch and cu.stride() != (1,)) or (batch > 1 and lens.stride() != (1,)):
         raise ValueError("cu and lens must be contiguous")
-    return batch
+    # a single row may have any stride
+    return ((pages.data_ptr(), shape[0], stride[0] if shape[0] > 1 else size, page_size),
+            (table.data_ptr(), ld[0] if batch > 1 else columns[1], columns[1], cu.data_ptr(), lens.data_ptr(), batch))
 
 
 def _kv_heads(pages: torch.Tensor, head_dim: int, page_size: int) -> int:
@@ -761,7 +772,7 @@ def hif4_kv_write(
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of one shape and dtype")
     total, h, d = k.shape
-    batch = _ragged(pages, table, cu, lens, h, d, page_size)
+    pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
     ks, vs = k.stride(), v.stride()
     if ks[2] != 1:
         k = k.contiguous()
@@ -770,9 +781,7 @@ def hif4_kv_write(
         v = v.contiguous()
         vs = v.stride()
     _lib.call("faq_hif4_kv_write", k.data_ptr(), v.data_ptr(), _dtype_code(k), total, h, d, ks[0], ks[1], vs[0], vs[1],
-              pages.data_ptr(), pages.shape[0], pages.stride(0), page_size, table.data_ptr(), table.stride(0),
-              table.shape[1], cu.data_ptr(), lens.data_ptr(), batch, levels_code(levels[0]), levels_code(levels[1]),
-              _stream(device))
+              *pool, *ragged, levels_code(levels[0]), levels_code(levels[1]), _stream(device))
 
 
 def hif4_kv_read(
@@ -792,7 +801,7 @@ def hif4_kv_read(
     packed in sequence order; ``out`` takes tensors of that shape with unit channel stride."""
     device = _require_cuda(pages, table, cu, lens, *(out or ()))
     h = _kv_heads(pages, head_dim, page_size)
-    batch = _ragged(pages, table, cu, lens, h, head_dim, page_size)
+    pool, ragged = _ragged(pages, table, cu, lens, h, head_dim, page_size)
     if total < 0:
         raise ValueError("total must not be negative")
     if out is None:
@@ -805,9 +814,8 @@ def hif4_kv_read(
                 or v.stride(2) != 1):
             raise ValueError("out must be two [total, kv_heads, head_dim] tensors of one dtype with unit channel stride")
         ks, vs = k.stride(), v.stride()
-    _lib.call("faq_hif4_kv_read", pages.data_ptr(), pages.shape[0], pages.stride(0), page_size, h, head_dim,
-              table.data_ptr(), table.stride(0), table.shape[1], cu.data_ptr(), lens.data_ptr(), batch,
-              k.data_ptr(), v.data_ptr(), _dtype_code(k), total, ks[0], ks[1], vs[0], vs[1], _stream(device))
+    _lib.call("faq_hif4_kv_read", *pool, h, head_dim, *ragged, k.data_ptr(), v.data_ptr(), _dtype_code(k), total, ks[0],
+              ks[1], vs[0], vs[1], _stream(device))
     return k, v
 
 
@@ -841,7 +849,7 @@ def hif4_paged_attention(
         raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
     total, heads, d = q.shape
     h = _kv_heads(pages, d, page_size)
-    batch = _ragged(pages, table, cu, lens, h, d, page_size)
+    pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
     if heads % h:
         raise ValueError("query heads must be divisible by key/value heads")
     qs = q.stride()
@@ -855,18 +863,17 @@ def hif4_paged_attention(
         if out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
             raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
         os_ = out.stride()
-    columns = table.shape[1]
+    batch = ragged[5]
     if max_len is None:
-        max_len = columns * page_size
+        max_len = ragged[2] * page_size
     if total_len is None:
         total_len = batch * max_len
     need = _attention_workspace(device.index, total, heads, h, batch, max_new, max_len, total_len, d)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = pages.new_empty(need)
-    _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, qs[0], qs[1], pages.data_ptr(), pages.shape[0],
-              pages.stride(0), page_size, h, d, table.data_ptr(), table.stride(0), columns, cu.data_ptr(),
-              lens.data_ptr(), batch, max_new, max_len, total_len, d**-0.5 if scale is None else float(scale),
-              out.data_ptr(), os_[0], os_[1], workspace.data_ptr(), need, _stream(device))
+    _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, qs[0], qs[1], *pool, h, d, *ragged, max_new, max_len,
+              total_len, d**-0.5 if scale is None else float(scale), out.data_ptr(), os_[0], os_[1],
+              workspace.data_ptr() if need else None, need, _stream(device))
     return out
 
 

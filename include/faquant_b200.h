@@ -444,11 +444,12 @@ int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t page_stride, 
  * zero. Covers one decode step, chunks of drafted tokens and prompt chunks in one batch.
  * max_new, max_len and total_len are upper bounds on the sequences' new tokens, their lengths
  * and the sum of the lengths, known on the host (nothing is copied from the device): they
- * choose the kernels and size the workspace, which for sequences of 65 or more rows (new
- * tokens x query heads of a kv head) also holds the keys and values of those in bf16. A batch
- * beyond max_len or total_len sets FAQ_STATUS_BAD_BOUND and leaves those sequences' rows as
- * they are. `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 256-byte
- * aligned, not initialized.
+ * choose the kernels and size the workspace, which for sequences of more than 128 rows
+ * (new tokens x query heads of a kv head) also holds the keys and values of those in bf16. A
+ * batch beyond them is either computed all the same or sets FAQ_STATUS_BAD_BOUND and leaves
+ * those sequences' rows as they are. cu[batch] may be less than total: the rows beyond it are
+ * neither read nor written. `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 256-byte
+ * aligned, not initialized (null where that is 0).
  */
 size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch,
                                                 int64_t max_new, int64_t max_len, int64_t total_len, int d);

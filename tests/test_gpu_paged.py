@@ -177,7 +177,7 @@ SHAPES = [  # heads, kv_heads, d, page_size, lens, new
     (12, 4, 128, 16, [130], [130]),
     (24, 2, 128, 256, [700, 20], [40, 20]),
     (3, 3, 128, 16, [0, 0, 9], [0, 0, 1]),
-    # from 65 rows (tokens x query heads of a kv head) a sequence is the prompt kernel's
+    # sequences of tens of rows (tokens x query heads of a kv head), from 129 the prompt kernel's
     (4, 1, 128, 16, [17], [17]),
     (4, 1, 128, 16, [200, 16, 17], [17, 16, 16]),
     (8, 8, 128, 64, [65, 128, 129, 300], [65, 128, 129, 256]),
@@ -367,6 +367,42 @@ def test_batches_beyond_their_bounds_are_reported() -> None:
     assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
     ref, size = attention(q, quantized(k), quantized(v), lens, new)  # the first one fits
     assert bool(((out.double().cpu() - ref).abs() <= BOUND * size)[:50].all()) and not out[50:].any()
+
+
+def test_a_sequence_beyond_max_new_is_reported() -> None:
+    from faquant_b200 import _lib, ops
+
+    lens, new = [300, 300], [5, 60]
+    pool = Pool(lens, 2, 128, 16, DEV)
+    k, v = _randn(600, 2, 128, seed=69), _randn(600, 2, 128, seed=70)
+    pool.write(k, v)
+    q = _randn(65, 8, 128, seed=71)
+    out = torch.zeros_like(q)
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=30, max_len=300,
+                             out=out)
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
+    ref, size = attention(q, quantized(k), quantized(v), lens, new)
+    assert bool(((out.double().cpu() - ref).abs() <= BOUND * size)[:5].all()) and not out[5:].any()
+
+
+@pytest.mark.parametrize("new", [[60, 7, 1, 0], [60, 60, 60, 60], [1, 1, 0, 1]])
+def test_rows_beyond_the_batch_stay_as_they_are(new) -> None:
+    """A q of a fixed size (batch x max_new rows), of which the batch uses the first."""
+    from faquant_b200 import ops
+
+    lens = [400, 90, 33, 200]
+    pool = Pool(lens, 2, 128, 16, DEV)
+    k, v = _randn(sum(lens), 2, 128, seed=72), _randn(sum(lens), 2, 128, seed=73)
+    pool.write(k, v)
+    used, most = sum(new), max(new)
+    q = _randn(4 * most, 8, 128, seed=74)
+    q[used:] = float("nan")
+    out = torch.full_like(q, 7.0)
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=most, max_len=400,
+                             out=out)
+    _close(out[:used], lens, new, q[:used], quantized(k), quantized(v))
+    assert bool((out[used:] == 7.0).all())
+    _no_status()
 
 
 # ------------------------------------------------------------------ refusals

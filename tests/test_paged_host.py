@@ -38,9 +38,9 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
     assert write(levels=1) == 1 and "levels" in _lib.last_error()
     assert write(dtype=7) == 1 and "dtype" in _lib.last_error()
 
-    def attend(heads=4, scale=1.0, ws=1 << 30, qs=512, max_new=1):
-        return lib.faq_hif4_paged_attention(p, 4, heads, qs, 128, p, 4, 1 << 20, 16, 2, 128, p, 3, 3, p, p, 1, max_new, 48,
-                                            48, ctypes.c_float(scale), p, 512, 128, p, ws, None)
+    def attend(heads=4, scale=1.0, ws=1 << 30, qs=512, max_new=4):
+        return lib.faq_hif4_paged_attention(p, 4, heads, qs, 128, p, 4, 1 << 20, 16, 2, 128, p, 3, 3, p, p, 1, max_new, 2000,
+                                            2000, ctypes.c_float(scale), p, 512, 128, p, ws, None)
 
     assert attend(heads=3) == 1 and "divisible" in _lib.last_error()
     assert attend(scale=0.0) == 1 and "scale" in _lib.last_error()
@@ -48,6 +48,9 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
     assert attend(qs=12) == 1 and "strides" in _lib.last_error()
     assert attend(ws=16) == 1 and "workspace" in _lib.last_error()
     assert attend(max_new=-1) == 1
+    # one kernel without joins needs no workspace: eight rows, short sequences
+    assert lib.faq_hif4_paged_attention_workspace_bytes(4, 4, 2, 1, 4, 1024, 1024, 128) == 0
+    assert lib.faq_hif4_paged_attention_workspace_bytes(4, 4, 2, 1, 4, 1025, 1025, 128) > 0
     assert lib.faq_hif4_paged_attention_workspace_bytes(4, 6, 4, 1, 1, 48, 48, 128) == 0
 
     def verify(batch=1, k=2, vocab=10, dtype=1, target=p):
