@@ -303,6 +303,7 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
   const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
   return s | (s << 16);
 }
+// each<UNROLL>: 1 keeps the loop over the lane's two tokens (of V: token pairs), half the code.
 template <int NG>
 struct KBlock {
   uint32_t w[2][2 * NG], e[2][NG], sc[2];
@@ -325,19 +326,19 @@ struct KBlock {
       }
     }
   }
-  template <typename F>
+  template <int UNROLL = 2, typename F>
   __device__ __forceinline__ void each(const Expand& expand, int lane, F&& f) const {
     const int t = lane & 3;
-#pragma unroll
+#pragma unroll UNROLL
     for (int h = 0; h < 2; ++h) {
       const int r = (lane >> 2) + 8 * h;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t s = scale_pair((sc[h] >> (8 * g)) & 255);
+        const uint32_t s = scale_pair(((h ? sc[1] : sc[0]) >> (8 * g)) & 255), eg = h ? e[1][g] : e[0][g];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
           uint32_t y[4];
-          expand.word(w[h][2 * g + i], expand.exponents(e[h][g], (7 - 4 * t - 2 * i) & 31), y);
+          expand.word(h ? w[1][2 * g + i] : w[0][2 * g + i], expand.exponents(eg, (7 - 4 * t - 2 * i) & 31), y);
 #pragma unroll
           for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], s);
           const uint32_t row[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
@@ -371,19 +372,21 @@ struct VBlock {
       }
     }
   }
-  template <typename F>
+  template <int UNROLL = 2, typename F>
   __device__ __forceinline__ void each(const Expand& expand, int lane, F&& f) const {
     const int s = lane & 7;
-#pragma unroll
+#pragma unroll UNROLL
     for (int h = 0; h < 2; ++h) {
       const int p = (lane >> 3) + 4 * h;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t pair = __byte_perm(scale_pair((sc[h] >> (8 * g)) & 255), scale_pair((sc[h] >> (8 * (NG + g))) & 255), 0x5410);
+        const uint32_t c = h ? sc[1] : sc[0];
+        const uint32_t pair = __byte_perm(scale_pair((c >> (8 * g)) & 255), scale_pair((c >> (8 * (NG + g))) & 255), 0x5410);
         uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          expand.word(w[h][2 * g + q], expand.exponents(e[h][2 * g + q], (7 - 2 * s) & 31), y[q]);
+          expand.word(h ? w[1][2 * g + q] : w[0][2 * g + q], expand.exponents(h ? e[1][2 * g + q] : e[0][2 * g + q], (7 - 2 * s) & 31),
+                      y[q]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], pair);
         }

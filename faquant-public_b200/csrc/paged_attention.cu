@@ -19,7 +19,7 @@
 //                 keys. P^T comes from S^T's registers by movmatrix; V's scale (per key and
 //                 group) multiplies P before its bf16 rounding, once per group.
 // Softmax: one reference maximum per row and warp, raised only when a score passes it by
-// more than 2^8 (p stays below 2^8, the sum and the accumulator are fp32, so the result does
+// more than 2^8 (the sum and the accumulator are fp32, with room for that, so the result does
 // not depend on when it is raised beyond fp32 rounding); raising it takes a warp reduction
 // and rescales O. The denominator sums the fp32 p before its rounding to bf16.
 //
@@ -56,7 +56,13 @@ constexpr int COST = 2 * W; // of a unit beyond its blocks, see below
 // them and joining the parts in a second kernel, whose launch is saved (a sequence of 1000
 // tokens with 8 kv heads: 10.7 us against 11.3, 16 such sequences: 11.7 against 15.7).
 constexpr int64_t WHOLE = 4 * W * BLOCK;
-constexpr float RAISE = 8.0f;  // log2 headroom of a row's reference maximum
+// A row's exponentials are p = 2^(score - m): m is put LIFT below the greatest score when it is
+// raised, and raised when a score lies RAISE above it. The lift costs nothing (fp32 and bf16 hold
+// 2^72 as they hold 2^8) and keeps keys that far below the others: p is flushed to zero at
+// 2^-126, 190 binary places below the greatest, where its value times the largest of the
+// cache (2^18.4) is below the output's own least. So that the factors 2^(m - m') of rescaling
+// and joining lose nothing above that either, their half powers are multiplied in twice.
+constexpr float LIFT = 64.0f, RAISE = LIFT + 8.0f;
 constexpr float LOWEST = -3.402823466e38f;  // where it starts: below every finite score
 
 struct Params {
@@ -490,19 +496,19 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
           n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, y));
           n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, y));
         }
-        n0 = fmaxf(n0, m[0]);
-        n1 = fmaxf(n1, m[1]);
-        const float a0 = ex2(m[0] - n0), a1 = ex2(m[1] - n1);
+        n0 = fmaxf(n0 - LIFT, m[0]);
+        n1 = fmaxf(n1 - LIFT, m[1]);
+        const float a0 = ex2(0.5f * (m[0] - n0)), a1 = ex2(0.5f * (m[1] - n1));
         m[0] = n0;
         m[1] = n1;
-        l[0] *= a0;
-        l[1] *= a1;
+        l[0] = l[0] * a0 * a0;
+        l[1] = l[1] * a1 * a1;
 #pragma unroll
         for (int j = 0; j < NG * 4; ++j) {
-          o[j][0] *= a0;
-          o[j][1] *= a1;
-          o[j][2] *= a0;
-          o[j][3] *= a1;
+          o[j][0] = o[j][0] * a0 * a0;
+          o[j][1] = o[j][1] * a1 * a1;
+          o[j][2] = o[j][2] * a0 * a0;
+          o[j][3] = o[j][3] * a1 * a1;
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) e[c] = __fmaf_rn(s[c], P.scale_log2, -m[c & 1]);
@@ -602,13 +608,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
       float den = 0.0f;
 #pragma unroll 4
       for (int w = 0; w < parts; ++w) {
-        const float f = ex2(s_m[w * RB + r] - top);
+        const float f = ex2(0.5f * (s_m[w * RB + r] - top));
         const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * OLD + c);
-        sum.x += f * v.x;
-        sum.y += f * v.y;
-        sum.z += f * v.z;
-        sum.w += f * v.w;
-        den += f * s_l[w * RB + r];
+        sum.x += f * v.x * f;
+        sum.y += f * v.y * f;
+        sum.z += f * v.z * f;
+        sum.w += f * v.w * f;
+        den += f * s_l[w * RB + r] * f;
       }
       if (whole) {
         const int tok = small_div(P, x.rem0 + r);
@@ -667,10 +673,10 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(Params P) {
     }
     const float m = src[RB * D + r], l = src[RB * D + RB + r];
     const float next = fmaxf(top, m);
-    const float f = ex2(top - next), e = ex2(m - next);
+    const float f = ex2(0.5f * (top - next)), e = ex2(0.5f * (m - next));
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f + v[i] * e;
-    den = den * f + l * e;
+    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f * f + v[i] * e * e;
+    den = den * f * f + l * e * e;
     top = next;
   }
 #pragma unroll
@@ -687,10 +693,10 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(Params P) {
   for (int w = 0; w < 8; ++w) all = fmaxf(all, s_top[w]);
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
-    const float f = ex2(s_top[w] - all);
-    o0 += f * s_sum[w][c];
-    o1 += f * s_sum[w][c + 1];
-    d += f * s_den[w];
+    const float f = ex2(0.5f * (s_top[w] - all));
+    o0 += f * s_sum[w][c] * f;
+    o1 += f * s_sum[w][c + 1] * f;
+    d += f * s_den[w] * f;
   }
   const float inv = d > 0.0f ? __fdiv_rn(1.0f, d) : (d == 0.0f ? 0.0f : d);
   const int row = join[3] + r, tok = small_div(P, row);

@@ -4,16 +4,20 @@
 //
 // With so few rows the bf16 keys would be read once or twice, so they are not written to memory
 // first: eight warps load a key tile's blocks from the pages (the next tile's while this one
-// is expanded), and write K and V to shared memory as TMA would have laid them out. Per key
-// tile and SM that is some 3500 instructions of expansion beside 2800 of softmax, which
-// bounds the kernel by instruction issue; the products (a quarter of their rate) hide
-// under it. Work is cut into equal runs of key tiles, one per CTA, as in paged_attention.cu,
-// and paged_prefill.cu's join adds up the units of several runs.
+// is expanded), and write K and V to shared memory as TMA would have laid them out. The
+// products take the whole tile whatever its rows (a quarter of the tensor cores' time), so
+// units of at most 64 or 32 rows stand in it two or four times: each copy's scores give it a
+// half or a quarter of the keys, and the softmax has no work on rows that mean nothing.
+// Work is cut into equal runs of key tiles, one per CTA, as in paged_attention.cu, and
+// paged_prefill.cu's join adds up the units of several runs.
 //
 // Measured (one B200): 8 new tokens for each of 16 sequences of 1 .. 8192 tokens, 32 query heads
-// on 8 kv heads of 128, in 36.6 us. A key tile takes an SM about 3400 cycles, the chain from the scores
-// to the P of their tile, beside which the expansion of the next tile runs; 16 expander warps
-// instead of eight were slower.
+// on 8 kv heads of 128, in 32.8 us (36.6 without the copies). A key tile takes an SM about 3000
+// cycles, of which a warp's expansion of its block of K and of V is 1900, at one instruction in
+// more than four cycles: it runs straight through some 400 instructions, and the warps' different
+// places in them are more than the instruction caches hold. Hence the rolled loops; 16 expanding
+// warps, K and V apart, were slower (92 us against 58 for 16 sequences of 4096 tokens, 77 with
+// rolled loops), their stalls "no instruction" 5.7 times the issued ones against 1.0.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -73,6 +77,14 @@ __device__ __forceinline__ void enter(const Params& P, Walk& w, int b) {
   w.len = length_of(P.p, b);
   w.units = (w.n + P.tile_tokens - 1) / P.tile_tokens;
 }
+// Copies of the unit's rows in the tile, see Softmax.
+__device__ __forceinline__ int copies_of(const Params& P, const Walk& w) {
+  const int rows = min(P.tile_tokens, w.n - w.u * P.tile_tokens) * P.group;
+  return rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+}
+struct QMaps {
+  CUtensorMap q[3];  // boxes of whole tokens, at most 128, 64, 32 rows
+};
 __device__ __forceinline__ int key_tiles(const Params& P, const Walk& w, int u) {
   const int seen = w.len - w.n + min(w.n, (u + 1) * P.tile_tokens);
   return seen <= 0 ? 0 : (seen + TILE - 1) / TILE;
@@ -123,7 +135,7 @@ struct Smem {
 };
 
 template <int NG>
-__global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, Params P) {
+__global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_constant__ QMaps maps, Params P) {
   using L = Smem<NG>;
   constexpr int D = 64 * NG, WARPS = THREADS / 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -159,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
       mbar_init(smem_addr(&v_empty[i]), 1);
     }
     fence_barrier_init();
-    tma_prefetch_desc(&tmap_q);
+    for (int i = 0; i < 3; ++i) tma_prefetch_desc(&maps.q[i]);
     s_walk.count = 0;
     s_empty = 0;
   }
@@ -252,10 +264,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
             P.joins[blockIdx.x] = j;
           }
           if (i > 0 && !mbar_wait_site(smem_addr(q_empty), (i - 1) & 1, 80, i)) break;
-          mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(P.group * P.tile_tokens) * 128 * NG);
-          for (int c = 0; c < NG; ++c)
-            tma_load_3d(smem_addr(base + L::q + c * CHUNK), &tmap_q, smem_addr(q_full), c * 64, w.head * P.group,
-                        w.c0 + w.u * P.tile_tokens);
+          const int copies = copies_of(P, w), rows = TILE / copies;
+          const int map = copies >> 1;  // the box of 128, 64 or 32 rows
+          mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(copies * (rows / P.group) * P.group) * 128 * NG);
+          for (int c = 0; c < NG * copies; ++c)
+            tma_load_3d(smem_addr(base + L::q + (c / copies) * CHUNK + c % copies * rows * 128), &maps.q[map],
+                        smem_addr(q_full), c / copies * 64, w.head * P.group, w.c0 + w.u * P.tile_tokens);
         }
         // drain (bounded): the last Q was read before the CTA exits
         if (i > 0) mbar_wait_site(smem_addr(q_empty), (i - 1) & 1, 81, i);
@@ -360,13 +374,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
         };
       };
       if (!mbar_wait_warp(smem_addr(&k_empty[st]), ((step >> 1) & 1) ^ 1, 87, step)) break;
-      kb.each(expand, lane, write(base + L::k + st * L::tile));
+      kb.template each<1>(expand, lane, write(base + L::k + st * L::tile));
       fence_proxy_async_smem();  // the tensor core reads it through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
       if (src) kb.load(src, lane);
       if (!mbar_wait_warp(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 88, step)) break;
-      vb.each(expand, lane, write(base + L::v + st * L::tile));
+      vb.template each<1>(expand, lane, write(base + L::v + st * L::tile));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
@@ -375,15 +389,25 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
     Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
-    const int row_tok = sm.row / P.group, row_head = sm.row - row_tok * P.group;
-    for (Walk w = s_walk; w.count > 0; next_unit(P, w, begin, end)) {
+    auto unit = [&](const Walk& w, auto parts) {
+      constexpr int PARTS = decltype(parts)::value;
+      const int row = sm.template row<PARTS>(), row_tok = row / P.group, row_head = row - row_tok * P.group;
       const int tok = w.u * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < w.n;
-      if (!sm.run(w.k0, w.count, live ? w.len - w.n + tok : 0x7fffffff)) break;
+      if (!sm.template run<PARTS>(w.k0, w.count, live ? w.len - w.n + tok : 0x7fffffff)) return false;
+      if (!sm.template first_copy<PARTS>()) return true;
       float* part = w.count == w.tiles ? nullptr
                                        : P.parts + (2 * static_cast<int64_t>(blockIdx.x) + (w.k0 == 0)) * (TILE * D + 2 * TILE);
-      sm.store(live, part, TILE, sm.row,
+      sm.store(live, part, TILE, row,
                P.out + static_cast<int64_t>(w.c0 + (live ? tok : 0)) * P.ot + (w.head * P.group + row_head) * P.oh);
+      return true;
+    };
+    for (Walk w = s_walk; w.count > 0; next_unit(P, w, begin, end)) {
+      const int copies = copies_of(P, w);
+      const bool ok = copies == 4   ? unit(w, std::integral_constant<int, 8>())
+                      : copies == 2 ? unit(w, std::integral_constant<int, 4>())
+                                    : unit(w, std::integral_constant<int, 2>());
+      if (!ok) break;
     }
   }
   __syncthreads();
@@ -403,17 +427,20 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
   const int runs = num_sms();
   P.joins = reinterpret_cast<Join*>(ws);
   P.parts = reinterpret_cast<float*>(ws + runs * sizeof(Join));
-  CUtensorMap mq;
+  QMaps maps;
   const uint64_t dims[3] = {D, static_cast<uint64_t>(heads), static_cast<uint64_t>(P.total)};
   const uint64_t str[2] = {static_cast<uint64_t>(qh) * 2, static_cast<uint64_t>(qt) * 2};
-  const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(P.tile_tokens)};
-  int rc = make_tmap(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc) return rc;
+  int rc = FAQ_OK;
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(std::max((TILE >> i) / P.group, 1))};
+    rc = make_tmap(&maps.q[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
   auto kern = paged_chunk_kernel<NG>;
   static std::atomic<uint64_t> set{0};
   rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
   if (rc) return rc;
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(runs)), THREADS, Smem<NG>::bytes, stream, mq, P));
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(runs)), THREADS, Smem<NG>::bytes, stream, maps, P));
   FAQ_CUDA(launch_early(pre::prefill_combine_kernel<D, TILE, Params>, dim3(static_cast<unsigned>(runs), TILE / 8), 256, 0,
                         stream, P));
   return FAQ_OK;
@@ -422,20 +449,28 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
 }  // namespace chk
 }  // namespace faq
 
-// Which kernel takes a sequence, by its rows (new tokens x query heads of a kv head): up to
-// FEW_ROWS in every sequence of the call, paged_attention.cu's; else up to CHUNK_ROWS
-// paged_chunk.cu's, beyond them the prompt kernel's. More than 128 query heads to a kv head
-// do not fit a tile of whole tokens: paged_attention.cu takes those in units of eight rows.
+// Which kernel takes a sequence, by its rows (new tokens x query heads of a kv head):
+// - up to FEW_ROWS in every sequence of the call, paged_attention.cu's, in units of eight: 16
+//   sequences of 4096 tokens (32 query heads on 8 kv heads of 128) take 54.5 us with 12 or 16
+//   rows against 57.8 in paged_chunk.cu, with 24 rows 77 against 58. Also when no unit is split
+//   and each can have an SM: 32 rows of 4 sequences of 1000 tokens 12.5 against 15.8, but of 32
+//   such sequences 64 against 37.5;
+// - else up to CHUNK_ROWS, paged_chunk.cu's: 128 rows of those 16 sequences take 74 us against
+//   164 in the prompt kernel, whose expansion writes the keys to memory;
+// - beyond them the prompt kernel's.
+// More than 128 query heads to a kv head do not fit a tile of whole tokens: paged_attention.cu
+// takes those.
 namespace faq {
 namespace pag {
-constexpr int FEW_ROWS = 8, CHUNK_ROWS = 128;
+constexpr int FEW_ROWS = 16, CHUNK_ROWS = 128;
 struct Kinds {
   bool few, chunks, prompts;
   int min_rows() const { return chunks ? CHUNK_ROWS + 1 : 1; }  // of a sequence of the prompt kernel
 };
-inline Kinds kinds(int64_t group, int64_t max_new, int64_t total, int64_t batch) {
+inline Kinds kinds(int64_t group, int64_t kv_heads, int64_t max_new, int64_t max_len, int64_t total, int64_t batch) {
   const int64_t rows = group * std::min(max_new, total);
   if (rows <= FEW_ROWS || group > pre::TILE) return {true, false, false};
+  if (max_len <= pat::WHOLE && (rows + pat::RB - 1) / pat::RB * kv_heads * batch <= num_sms()) return {true, false, false};
   const bool prompts = rows > CHUNK_ROWS;
   // all sequences have max_new tokens when they add up to that; should rows of q lie beyond
   // cu's end, the prompt kernel takes the shorter sequences too
@@ -451,7 +486,7 @@ extern "C" size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_
       total_len < 0 || (d != 64 && d != 128))
     return 0;
   const int64_t group = heads / kv_heads;
-  const pag::Kinds kinds = pag::kinds(group, max_new, total, batch);
+  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total, batch);
   size_t bytes = kinds.few && max_len > pat::WHOLE ? pat::workspace(d) : 0;  // units that are not split need none
   if (kinds.chunks) bytes = std::max(bytes, chk::workspace(d));
   if (kinds.prompts)
@@ -492,7 +527,7 @@ extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t he
   const __nv_bfloat16* query = static_cast<const __nv_bfloat16*>(q);
   __nv_bfloat16* output = static_cast<__nv_bfloat16*>(out);
   char* ws = static_cast<char*>(workspace);
-  const pag::Kinds kinds = pag::kinds(group, max_new, total, batch);
+  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total, batch);
   if (kinds.few) {
     pat::Params P;
     P.p = pages_;

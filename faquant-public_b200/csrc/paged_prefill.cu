@@ -41,6 +41,7 @@ namespace pre {
 
 using namespace kvp;
 using pat::ex2;
+using pat::LIFT;
 using pat::LOWEST;
 using pat::pack_bf16;
 using pat::RAISE;
@@ -326,49 +327,94 @@ __device__ __forceinline__ bool bar_and(int id, int count, bool v) {
 }
 __device__ __forceinline__ bool bar_or(int id, int count, bool v) { return !bar_and(id, count, !v); }
 
-// The softmax of a tile of 128 rows by eight warps: warps 0-3 of them (by TMEM lane quarter)
-// take keys 0..63 of every key tile and the lower half of O's channels, warps 4-7 the others.
+// `n` columns of this thread's lane of tensor memory
+template <int N>
+__device__ __forceinline__ void tmem_ldf(uint32_t taddr, float* f) {
+  if constexpr (N >= 32) {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) tmem_ld32f(taddr + c, f + c);
+  } else {
+    static_assert(N == 16, "16 or whole 32s");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]),
+          "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15])
+        : "r"(taddr));
+  }
+}
+template <int N>
+__device__ __forceinline__ void reg_fencef(float* f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(f[i]));
+}
+
+// The softmax of a tile of 128 rows by eight warps. TMEM lets a warp read the lanes of its own
+// quarter (warp % 4) only, so a row's keys are shared by the two warps of its quarter: warps
+// 0-3 of them take keys 0..63 of every key tile and the lower half of O's channels, warps 4-7
+// the others. Units of at most 64 (32) rows stand two (four) times in the tile, one copy of the
+// rows per half (quarter) of the lanes: PARTS = 4 (8) warps then share a row's keys, all
+// write their P to its first copy's row, and the other copies' rows of O mean nothing.
 template <int D>
 struct Softmax {
-  int row, half, lane, site, barrier;
-  uint32_t s_addr, o_addr, p_row;
-  float *mine_at, *other_at;  // what the row's halves tell each other, where their P stands
+  int quarter, half, lane, site, tile_barrier;
+  uint32_t s_addr, o_addr;
+  uint8_t* p_tile;
   uint32_t s_full, s_free, p_full, pv_done;
   float scale_log2;
   uint32_t done = 0;  // steps so far
   float m, l;         // the unit's reference maximum (log2) and, after run(), the row's sum
 
-  __device__ __forceinline__ Softmax(uint32_t tmem, int t, int warp, int lane_, uint8_t* p_tile, uint64_t* full,
+  __device__ __forceinline__ Softmax(uint32_t tmem, int t, int warp, int lane_, uint8_t* p, uint64_t* full,
                                      uint64_t* free_, uint64_t* pfull, uint64_t* pv, float scale)
-      : lane(lane_), site(57 + t), s_full(smem_addr(full)), s_free(smem_addr(free_)), p_full(smem_addr(pfull)),
+      : lane(lane_), site(57 + t), p_tile(p), s_full(smem_addr(full)), s_free(smem_addr(free_)), p_full(smem_addr(pfull)),
         pv_done(smem_addr(pv)), scale_log2(scale) {
-    const int quarter = warp & 3;
+    quarter = warp & 3;
     half = (warp >> 2) & 1;
-    barrier = 1 + t * 4 + quarter;
-    row = quarter * 32 + lane;
+    tile_barrier = 1 + t * 4;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    s_addr = tmem + lanes + s_col(t) + 64 * half;  // this half's 64 keys
+    s_addr = tmem + lanes + s_col(t);
     o_addr = tmem + lanes + o_col(t) + D / 2 * half;  // this half's channels
-    // P_t as TMA would lay out a tile: key chunk `half`, row `row`, unit u at u ^ (row % 8)
-    mine_at = reinterpret_cast<float*>(p_tile + half * CHUNK + row * 128);
-    other_at = reinterpret_cast<float*>(p_tile + (half ^ 1) * CHUNK + row * 128);
-    p_row = smem_addr(mine_at);
   }
 
-  // The row's other half's value, between the two warps of 32 rows, through P_t's place (no
-  // product may be reading it). Both come here together, whatever happened before: `ok` tells
-  // whether both are well, so that neither is left waiting.
-  __device__ __forceinline__ bool exchange(bool ok, float mine, float& other) {
-    *mine_at = mine;
-    const bool both = bar_and(barrier, 64, ok);
-    other = *other_at;
-    return bar_and(barrier, 64, both);  // read: P_t may be written
+  // quarters of the lanes that a copy of the rows takes
+  template <int PARTS>
+  static constexpr int QUARTERS = 8 / PARTS;
+  // the thread's row, and whether it is its first copy, whose O counts
+  template <int PARTS>
+  __device__ __forceinline__ int row() const { return (quarter % QUARTERS<PARTS>)*32 + lane; }
+  template <int PARTS>
+  __device__ __forceinline__ bool first_copy() const { return quarter < QUARTERS<PARTS>; }
+
+  // Part i's place in P_t's row, as TMA would lay out a tile: key chunk, row, unit u at u ^ (row % 8)
+  template <int PARTS>
+  __device__ __forceinline__ uint8_t* place(int row, int i) const {
+    const int key = i * (TILE / PARTS);
+    return p_tile + (key >> 6) * CHUNK + row * 128 + ((((key & 63) >> 3) ^ (row & 7)) << 4);
+  }
+
+  // The values of the row's parts, among their warps, through P_t's place (no product may be
+  // reading it). They come here together, whatever happened before: `ok` tells whether all
+  // are well, so that none is left waiting.
+  template <int PARTS>
+  __device__ __forceinline__ bool exchange(bool ok, int barrier, int row, int part, float mine, float (&all)[PARTS]) {
+    *reinterpret_cast<float*>(place<PARTS>(row, part)) = mine;
+    const bool well = bar_and(barrier, 32 * PARTS, ok);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) all[i] = *reinterpret_cast<const float*>(place<PARTS>(row, i));
+    return bar_and(barrier, 32 * PARTS, well);  // read: P_t may be written
   }
 
   // Key tiles k0 .. k0 + count - 1 for a row whose last visible key is lim. False: a wait ran
   // out. (Warps whose rows are all dead work like the others: leaving their exponentials out
   // gained nothing, the live ones are bound by their own latency.)
+  template <int PARTS>
   __device__ __forceinline__ bool run(int k0, int count, int lim) {
+    constexpr int KEYS = TILE / PARTS;
+    const int row = this->row<PARTS>(), part = quarter / QUARTERS<PARTS> * 2 + half;
+    const int barrier = tile_barrier + quarter % QUARTERS<PARTS>;
+    const uint32_t p_row = smem_addr(p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
+    const int unit0 = (part * KEYS & 63) >> 3;
     const float2 c2 = make_float2(scale_log2, scale_log2);
     m = LOWEST;
     l = 0.0f;
@@ -376,47 +422,50 @@ struct Softmax {
     for (int j = 0; j < count; ++j, ++done) {
       ok = ok && mbar_wait_warp(s_full, done & 1, site, j);
       tc_fence_after();
-      float f[64];
-      tmem_ld32f(s_addr, f);
-      tmem_ld32f(s_addr + 32, f + 32);
+      float f[KEYS];
+      tmem_ldf<KEYS>(s_addr + part * KEYS, f);
       tc_wait_ld();
-      reg_fence32f(f);
-      reg_fence32f(f + 32);
+      reg_fencef<KEYS>(f);
       // S_t is in registers: the tensor core may write the next one
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
-      const int rel = lim - (k0 + j) * TILE - 64 * half;
-      if (__any_sync(0xffffffffu, rel < 63)) {
+      const int rel = lim - (k0 + j) * TILE - part * KEYS;
+      if (__any_sync(0xffffffffu, rel < KEYS - 1)) {
 #pragma unroll
-        for (int x = 0; x < 64; ++x)
+        for (int x = 0; x < KEYS; ++x)
           if (x > rel) f[x] = -INFINITY;
       }
-      float mx[4];
+      float mx[KEYS / 16];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < KEYS / 16; ++c) {
         mx[c] = max3(f[16 * c], f[16 * c + 1], f[16 * c + 2]);
 #pragma unroll
         for (int x = 3; x < 15; x += 2) mx[c] = max3(mx[c], f[16 * c + x], f[16 * c + x + 1]);
       }
-      const float mine = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(f[15], f[31], f[47])), f[63]);
-      // raise the maxima of the 32 rows when either half has a score far above them (or has to give up)
+      float mine = fmaxf(mx[0], f[15]);
+#pragma unroll
+      for (int c = 1; c < KEYS / 16; ++c) mine = max3(mine, mx[c], f[16 * c + 15]);
+      // raise the rows' maxima when a part has a score far above them (or has to give up)
       float a = 1.0f;
-      const bool raise = bar_or(barrier, 64, __fmul_rn(mine, scale_log2) > m + RAISE || !ok);
+      const bool raise = bar_or(barrier, 32 * PARTS, __fmul_rn(mine, scale_log2) > m + RAISE || !ok);
       if (raise) {
         if (j > 0) ok = ok && mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j);
-        float other;
-        if (!exchange(ok, mine, other)) return false;
-        const float next = fmaxf(__fmul_rn(fmaxf(mine, other), scale_log2), m);
-        a = ex2(m - next);
+        float all[PARTS];
+        if (!exchange<PARTS>(ok, barrier, row, part, mine, all)) return false;
+        float top = all[0];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) top = fmaxf(top, all[i]);
+        const float next = fmaxf(__fmul_rn(top, scale_log2) - LIFT, m);
+        a = ex2(0.5f * (m - next));
         m = next;
-        l *= a;
+        l = l * a * a;
       }
       const float2 mneg = make_float2(-m, -m);
       float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      uint32_t w[32];
+      uint32_t w[KEYS / 2];
 #pragma unroll
-      for (int x = 0; x < 32; ++x) {
+      for (int x = 0; x < KEYS / 2; ++x) {
         const float2 d = __ffma2_rn(make_float2(f[2 * x], f[2 * x + 1]), c2, mneg);
         const float2 e = make_float2(ex2(d.x), ex2(d.y));
         sum[x & 3] = __fadd2_rn(sum[x & 3], e);
@@ -427,13 +476,13 @@ struct Softmax {
       // the product of the step before has read P_t, and O_t is its
       if (j > 0) ok = mbar_wait_warp(pv_done, (done - 1) & 1, site + 2, j);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((u ^ (row & 7)) << 4)), "r"(w[4 * u]),
-                     "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
+      for (int u = 0; u < KEYS / 8; ++u)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (((unit0 + u) ^ (row & 7)) << 4)),
+                     "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
                      : "memory");
       fence_proxy_async_smem();  // the tensor core reads P through the async proxy
       tc_fence_after();
-      if (raise && j > 0) {
+      if (raise && j > 0 && first_copy<PARTS>()) {
         const float2 a2 = make_float2(a, a);
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
@@ -443,7 +492,7 @@ struct Softmax {
           reg_fence32f(o);
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            const float2 v = __fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2);
+            const float2 v = __fmul2_rn(__fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2), a2);
             o[2 * x] = v.x;
             o[2 * x + 1] = v.y;
           }
@@ -457,14 +506,16 @@ struct Softmax {
     }
     ok = ok && mbar_wait_warp(pv_done, (done - 1) & 1, site + 4, count);
     tc_fence_after();
-    float other;
-    if (!exchange(ok, l, other)) return false;
-    l = half ? other + l : l + other;  // the same sum in both halves
+    float all[PARTS];
+    if (!exchange<PARTS>(ok, barrier, row, part, l, all)) return false;
+    l = all[0];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) l += all[i];  // the same sum in all parts
     return true;
   }
 
   // O of the row: to dst (bf16, normalized) or, unnormalized with m and l, to row `at` of a
-  // partial of `rows` rows. Every lane takes part; only live ones store.
+  // partial of `rows` rows. Whole warps take part; only live ones store.
   __device__ __forceinline__ void store(bool live, float* part, int rows, int at, __nv_bfloat16* dst) {
     const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
 #pragma unroll 1
@@ -679,16 +730,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int t = warp >> 3;
     Softmax<D> sm(tmem, t, warp, lane, base + L::p + t * 2 * CHUNK, &s_full[t], &s_free[t], &p_full[t], &pv_done[t],
                   P.scale_log2);
-    const int row_tok = sm.row / P.group, row_head = sm.row - row_tok * P.group;
+    const int row = sm.template row<2>(), row_tok = row / P.group, row_head = row - row_tok * P.group;
     for (int i = 0; i < nseg; ++i) {
       const Segment g = segments[i];
       if (t == 1 && !two_tiles(g)) continue;
       const int tok = g.tok0 + t * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < g.n;
       // last visible key; rows that are not there see all
-      if (!sm.run(g.k0, g.count, live ? g.len - g.n + tok : 0x7fffffff)) break;
+      if (!sm.template run<2>(g.k0, g.count, live ? g.len - g.n + tok : 0x7fffffff)) break;
       float* part = g.slot < 0 ? nullptr : P.parts + static_cast<int64_t>(g.slot) * (ROWS * D + 2 * ROWS);
-      sm.store(live, part, ROWS, t * TILE + sm.row,
+      sm.store(live, part, ROWS, t * TILE + row,
                P.out + static_cast<int64_t>(g.c0 + (live ? tok : 0)) * P.ot + (g.head * P.group + row_head) * P.oh);
     }
   }
@@ -723,13 +774,13 @@ __global__ void __launch_bounds__(256) prefill_combine_kernel(Params P) {
     float next = fmaxf(top, m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, o));
-    const float f = ex2(top - next), e = lane < n ? ex2(m - next) : 0.0f;
-    float dl = lane < n ? e * l : 0.0f;
+    const float f = ex2(0.5f * (top - next)), e = lane < n ? ex2(0.5f * (m - next)) : 0.0f;
+    float dl = lane < n ? e * l * e : 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, o);
-    den = den * f + dl;
+    den = den * f * f + dl;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] *= f;
+    for (int i = 0; i < V; ++i) sum[i] = sum[i] * f * f;
     top = next;
 #pragma unroll 4
     for (int x = 0; x < n; ++x) {
@@ -737,14 +788,14 @@ __global__ void __launch_bounds__(256) prefill_combine_kernel(Params P) {
       const float* row = P.parts + (2 * static_cast<int64_t>(c0 + x) + (c0 + x == j.first)) * SIZE + r * D + lane * V;
       if constexpr (V == 4) {
         const float4 u = *reinterpret_cast<const float4*>(row);
-        sum[0] += u.x * w;
-        sum[1] += u.y * w;
-        sum[2] += u.z * w;
-        sum[3] += u.w * w;
+        sum[0] += u.x * w * w;
+        sum[1] += u.y * w * w;
+        sum[2] += u.z * w * w;
+        sum[3] += u.w * w * w;
       } else {
         const float2 u = *reinterpret_cast<const float2*>(row);
-        sum[0] += u.x * w;
-        sum[1] += u.y * w;
+        sum[0] += u.x * w * w;
+        sum[1] += u.y * w * w;
       }
     }
   }

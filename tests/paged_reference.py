@@ -47,11 +47,11 @@ class Pool:
         return ops.hif4_kv_read(self.pages, self.table, self.cu(new), self.lens, page_size=self.page_size,
                                 head_dim=self.d, total=int(sum(new)), **kw)
 
-    def attend(self, q, new, **kw):
+    def attend(self, q, new, max_len=0, **kw):
         from faquant_b200 import ops
 
         return ops.hif4_paged_attention(q, self.pages, self.table, self.cu(new), self.lens, page_size=self.page_size,
-                                        max_new=max(new), max_len=max(self.lens_host), **kw)
+                                        max_new=max(new), max_len=max(max_len, *self.lens_host), **kw)
 
 
 def quantized(x: torch.Tensor, levels="123") -> torch.Tensor:

@@ -165,6 +165,9 @@ def test_tokens_without_a_place() -> None:
 
 
 # ------------------------------------------------------------------ attention
+# Short sequences of any number of rows may be one kernel's; a higher bound on their lengths
+# gives the same batches to the kernels of long ones.
+MAX_LEN = [0, 5000]
 SHAPES = [  # heads, kv_heads, d, page_size, lens, new
     (4, 1, 128, 16, [1], [1]),
     (8, 2, 128, 16, [1, 2, 15, 16, 17, 127, 129, 500], [1] * 8),
@@ -177,7 +180,7 @@ SHAPES = [  # heads, kv_heads, d, page_size, lens, new
     (12, 4, 128, 16, [130], [130]),
     (24, 2, 128, 256, [700, 20], [40, 20]),
     (3, 3, 128, 16, [0, 0, 9], [0, 0, 1]),
-    # sequences of tens of rows (tokens x query heads of a kv head), from 129 the prompt kernel's
+    # more rows (tokens x query heads of a kv head): up to 128, beyond
     (4, 1, 128, 16, [17], [17]),
     (4, 1, 128, 16, [200, 16, 17], [17, 16, 16]),
     (8, 8, 128, 64, [65, 128, 129, 300], [65, 128, 129, 256]),
@@ -189,21 +192,23 @@ SHAPES = [  # heads, kv_heads, d, page_size, lens, new
 ]
 
 
+@pytest.mark.parametrize("max_len", MAX_LEN)
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"h{s[0]}_{s[1]}_d{s[2]}_p{s[3]}_b{len(s[4])}_n{max(s[5])}")
-def test_attention_matches_fp64(shape) -> None:
+def test_attention_matches_fp64(shape, max_len) -> None:
     heads, h, d, page, lens, new = shape
     pool = Pool(lens, h, d, page, DEV, fill=0xFF)  # unwritten slots hold the largest scales and codes
     k, v = _randn(sum(lens), h, d, seed=20), _randn(sum(lens), h, d, seed=21, scale=0.5)
     pool.write(k, v)
     q = _randn(sum(new), heads, d, seed=22, scale=2.0)
-    out = pool.attend(q, new)
+    out = pool.attend(q, new, max_len)
     assert out.shape == q.shape and out.dtype == torch.bfloat16
     _close(out, lens, new, q, quantized(k), quantized(v))
     _no_status()
 
 
-@pytest.mark.parametrize("n", [1, 2, 4, 9, 40, 150])
-def test_rows_without_a_key_are_zero(n) -> None:
+@pytest.mark.parametrize("max_len", MAX_LEN)
+@pytest.mark.parametrize("n", [1, 2, 4, 7, 9, 14, 30, 40, 150])
+def test_rows_without_a_key_are_zero(n, max_len) -> None:
     """More new tokens than the sequence holds: the first have no position."""
     lens, new = [max(1, n // 2), 0, 300], [n, n, n]
     pool = Pool(lens, 2, 128, 16, DEV)
@@ -211,7 +216,7 @@ def test_rows_without_a_key_are_zero(n) -> None:
     pool.write(k, v)
     q = _randn(3 * n, 8, 128, seed=25)
     out = torch.full_like(q, float("nan"))
-    pool.attend(q, new, out=out)
+    pool.attend(q, new, max_len, out=out)
     none = n - lens[0]
     assert not out[:none].any() and not out[n : 2 * n].any()
     _close(out, lens, new, q, quantized(k), quantized(v))
@@ -232,29 +237,32 @@ def test_a_step_of_queries_equals_each_alone() -> None:
         assert bool(((one[0] - out[i]).double().abs().cpu() <= 2 * BOUND * size[i]).all())
 
 
-def test_peaked_and_flat_scores_scale_and_ranges() -> None:
-    lens, new = [900], [4]
+@pytest.mark.parametrize("n", [4, 7, 14, 30, 40])
+def test_peaked_and_flat_scores_scale_and_ranges(n) -> None:
+    lens, new = [900], [n]
     pool = Pool(lens, 1, 128, 16, DEV)
     k, v = _randn(900, 1, 128, seed=29), _randn(900, 1, 128, seed=30)
     k[700] *= 30.0  # one key far above the others, found late
     v[3] *= 1e6     # and a value row of another magnitude
     v[600:] *= 1e-20
     pool.write(k, v)
-    q = _randn(4, 4, 128, seed=31)
+    q = _randn(n, 4, 128, seed=31)
     q[1] = 0
     for scale in (None, 0.002, 0.5):
-        _close(pool.attend(q, new, scale=scale), lens, new, q, quantized(k), quantized(v), scale)
+        _close(pool.attend(q, new, 5000, scale=scale), lens, new, q, quantized(k), quantized(v), scale)
 
 
-def test_not_a_number_stays_in_its_row() -> None:
+@pytest.mark.parametrize("max_len", MAX_LEN)
+@pytest.mark.parametrize("n", [6, 12, 30])
+def test_not_a_number_stays_in_its_row(n, max_len) -> None:
     pool = Pool([300], 2, 128, 16, DEV)
     k, v = _randn(300, 2, 128, seed=32), _randn(300, 2, 128, seed=33)
     pool.write(k, v)
-    q = _randn(6, 8, 128, seed=34)
-    good = pool.attend(q, [6])
+    q = _randn(n, 8, 128, seed=34)
+    good = pool.attend(q, [n], max_len)
     q[2, 5, 17] = float("nan")
     q[4, 0, 0] = float("inf")
-    out = pool.attend(q, [6])
+    out = pool.attend(q, [n], max_len)
     assert out[2, 5].isnan().all() and out[4, 0].isnan().any()
     out[2, 5], out[4, 0] = good[2, 5], good[4, 0]
     assert torch.equal(out, good)
@@ -344,10 +352,10 @@ def test_prompt_kernel_keeps_not_a_number_in_its_row() -> None:
     k, v = _randn(300, 2, 128, seed=63), _randn(300, 2, 128, seed=64)
     pool.write(k, v)
     q = _randn(90, 4, 128, seed=65)
-    good = pool.attend(q, [90])
+    good = pool.attend(q, [90], 5000)
     q[12, 3, 17] = float("nan")
     q[40, 0, 0] = float("inf")
-    out = pool.attend(q, [90])
+    out = pool.attend(q, [90], 5000)
     assert out[12, 3].isnan().all() and out[40, 0].isnan().any()
     out[12, 3], out[40, 0] = good[12, 3], good[40, 0]
     assert torch.equal(out, good)
@@ -362,7 +370,7 @@ def test_batches_beyond_their_bounds_are_reported() -> None:
     pool.write(k, v)
     q = _randn(100, 8, 128, seed=68)
     out = torch.zeros_like(q)
-    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=50, max_len=400,
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=50, max_len=2000,
                              total_len=300, out=out)
     assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
     ref, size = attention(q, quantized(k), quantized(v), lens, new)  # the first one fits
@@ -378,15 +386,16 @@ def test_a_sequence_beyond_max_new_is_reported() -> None:
     pool.write(k, v)
     q = _randn(65, 8, 128, seed=71)
     out = torch.zeros_like(q)
-    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=30, max_len=300,
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=30, max_len=2000,
                              out=out)
     assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
     ref, size = attention(q, quantized(k), quantized(v), lens, new)
     assert bool(((out.double().cpu() - ref).abs() <= BOUND * size)[:5].all()) and not out[5:].any()
 
 
-@pytest.mark.parametrize("new", [[60, 7, 1, 0], [60, 60, 60, 60], [1, 1, 0, 1]])
-def test_rows_beyond_the_batch_stay_as_they_are(new) -> None:
+@pytest.mark.parametrize("max_len", [400, 2000])
+@pytest.mark.parametrize("new", [[60, 7, 1, 0], [60, 60, 60, 60], [1, 1, 0, 1], [8, 2, 0, 0], [12, 9, 3, 1]])
+def test_rows_beyond_the_batch_stay_as_they_are(new, max_len) -> None:
     """A q of a fixed size (batch x max_new rows), of which the batch uses the first."""
     from faquant_b200 import ops
 
@@ -398,7 +407,7 @@ def test_rows_beyond_the_batch_stay_as_they_are(new) -> None:
     q = _randn(4 * most, 8, 128, seed=74)
     q[used:] = float("nan")
     out = torch.full_like(q, 7.0)
-    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=most, max_len=400,
+    ops.hif4_paged_attention(q, pool.pages, pool.table, pool.cu(new), pool.lens, page_size=16, max_new=most, max_len=max_len,
                              out=out)
     _close(out[:used], lens, new, q[:used], quantized(k), quantized(v))
     assert bool((out[used:] == 7.0).all())
