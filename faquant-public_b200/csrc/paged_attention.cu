@@ -32,11 +32,12 @@
 // no sequence is longer than WHOLE tokens, units are not split and nothing is joined.
 //
 // Measured (one B200, 32 query heads on 8 kv heads of 128, one new token): a context of 32768
-// tokens in 19.9 us, 32 sequences of 1 .. 16000 tokens (74 MB of cache) in 35.1 us, 2.1 TB/s
+// tokens in 20.1 us, 32 sequences of 1 .. 16000 tokens (76 MB of cache) in 35.6 us, 2.1 TB/s
 // of the pages. Bound by instruction issue, not by HBM (a third of its rate): a block of 16
-// tokens takes a warp about 470 instructions, 223 of them in the integer pipe, whose half
-// rate makes 102 cycles per block and SM; 131 are measured. Some 4.5 us of each call are its
-// start (the runs, Q, the first copies) and the last join.
+// tokens takes a warp about 470 instructions (118 cycles per block and SM), 223 of them in the
+// integer pipe at half rate (111 cycles); 150 to 170 are measured. Each call also has some 5 us
+// of dependent loads before its first block (cu and lens, the table, the pages) and 4 of its end
+// (the warps' join, the runs' join).
 #include <algorithm>
 #include <atomic>
 

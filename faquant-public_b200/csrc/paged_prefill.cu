@@ -23,12 +23,13 @@
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
 //
 // Measured (one B200, d = 128): the last 512 of 32768 tokens with 64 query heads on 8 kv heads
-// in 554 us, 985 TFLOP/s counting the visible pairs (642 us and 850 TFLOP/s in a long series,
+// in 547 us, 997 TFLOP/s counting the visible pairs (645 us and 846 TFLOP/s in a long series,
 // where the power limit lowers the clocks); all of a 16384-token prompt with 32 heads 1078
-// TFLOP/s. The expansion takes 36 us of the first. Bound by the exponentials: a pair of tiles has
-// 32768 of them per key tile, 2048 cycles of the SM's special function units, and with the
-// maxima, conversions and stores around them a key tile takes about 4000 cycles where the
-// products alone need 2048.
+// TFLOP/s. The expansion takes 32 us of the first. A key tile takes about 3900 cycles where the
+// products alone need 2048. What bounds it is shared memory: the operands of the four products
+// (2048 cycles at 128 bytes each), P's writes and the arriving K and V (512 each) fill 3072;
+// leaving all exponentials out gains only 30 us, taking them in turns (one tile's under the other's
+// waits) 4. At d = 64 it is the softmax's own chain.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
