@@ -462,19 +462,29 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
 // takes those.
 namespace faq {
 namespace pag {
-constexpr int FEW_ROWS = 16, CHUNK_ROWS = 128;
+constexpr int FEW_ROWS = 16, CHUNK_ROWS = 128, ALL_PROMPT_TILES = 600;
 struct Kinds {
   bool few, chunks, prompts;
   int min_rows() const { return chunks ? CHUNK_ROWS + 1 : 1; }  // of a sequence of the prompt kernel
 };
-inline Kinds kinds(int64_t group, int64_t kv_heads, int64_t max_new, int64_t max_len, int64_t total, int64_t batch) {
+inline Kinds kinds(int64_t group, int64_t kv_heads, int64_t max_new, int64_t max_len, int64_t total_len, int64_t total,
+                   int64_t batch) {
   const int64_t rows = group * std::min(max_new, total);
   if (rows <= FEW_ROWS || group > pre::TILE) return {true, false, false};
   if (max_len <= pat::WHOLE && (rows + pat::RB - 1) / pat::RB * kv_heads * batch <= num_sms()) return {true, false, false};
   const bool prompts = rows > CHUNK_ROWS;
-  // all sequences have max_new tokens when they add up to that; should rows of q lie beyond
-  // cu's end, the prompt kernel takes the shorter sequences too
-  return {false, !(prompts && total == batch * max_new), prompts};
+  // The prompt kernel takes the shorter sequences too when there are none (all have max_new
+  // tokens as they add up to that; rows of q may lie beyond cu's end) and when their keys are
+  // few: a key tile costs it more, the other kernel and its join cost 10 us at the least. 256 tokens
+  // on 2048 (32 query heads on 8 kv heads of 128) beside one token on 500: 55.0 us with both
+  // kernels, 44.3 with one; beside two on 4096 (512 key tiles of all heads): 58.0 and 59.9; four:
+  // 64.4 and 81.2. What is known of those keys is a bound: of all sequences' lengths, and of
+  // the sequences there can be beside one of max_new tokens. Mostly they are fewer, so it may lie
+  // a little above the lengths at which the two ways take the same time.
+  const int64_t beside = std::max<int64_t>(std::min(batch - 1, total - max_new), 0);
+  const int64_t keys = std::min(total_len - max_new, beside * max_len);
+  const bool alone = total == batch * max_new || kv_heads * keys <= ALL_PROMPT_TILES * pre::TILE;
+  return {false, !(prompts && alone), prompts};
 }
 }  // namespace pag
 }  // namespace faq
@@ -486,7 +496,7 @@ extern "C" size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_
       total_len < 0 || (d != 64 && d != 128))
     return 0;
   const int64_t group = heads / kv_heads;
-  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total, batch);
+  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total_len, total, batch);
   size_t bytes = kinds.few && max_len > pat::WHOLE ? pat::workspace(d) : 0;  // units that are not split need none
   if (kinds.chunks) bytes = std::max(bytes, chk::workspace(d));
   if (kinds.prompts)
@@ -527,7 +537,7 @@ extern "C" int faq_hif4_paged_attention(const void* q, int64_t total, int64_t he
   const __nv_bfloat16* query = static_cast<const __nv_bfloat16*>(q);
   __nv_bfloat16* output = static_cast<__nv_bfloat16*>(out);
   char* ws = static_cast<char*>(workspace);
-  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total, batch);
+  const pag::Kinds kinds = pag::kinds(group, kv_heads, max_new, max_len, total_len, total, batch);
   if (kinds.few) {
     pat::Params P;
     P.p = pages_;

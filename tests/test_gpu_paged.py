@@ -393,6 +393,22 @@ def test_a_sequence_beyond_max_new_is_reported() -> None:
     assert bool(((out.double().cpu() - ref).abs() <= BOUND * size)[:5].all()) and not out[5:].any()
 
 
+@pytest.mark.parametrize("max_len", [0, 20000])
+@pytest.mark.parametrize("new", [[200, 1, 1, 30, 0, 2], [130, 64, 64, 64, 0, 300], [0, 1, 0, 0, 1, 129]])
+def test_prompts_and_steps_in_one_batch(new, max_len) -> None:
+    """One kernel for all, or one for the long chunks and one for the others, as the bound on
+    the lengths has it."""
+    lens = [700, 64, 1, 300, 0, 350]
+    pool = Pool(lens, 8, 64, 32, DEV, fill=0xFF)
+    k, v = _randn(sum(lens), 8, 64, seed=75), _randn(sum(lens), 8, 64, seed=76)
+    pool.write(k, v)
+    q = _randn(sum(new), 16, 64, seed=77)
+    out = torch.full_like(q, float("nan"))
+    pool.attend(q, new, max_len, out=out)
+    _close(out, lens, new, q, quantized(k), quantized(v))
+    _no_status()
+
+
 @pytest.mark.parametrize("max_len", [400, 2000])
 @pytest.mark.parametrize("new", [[60, 7, 1, 0], [60, 60, 60, 60], [1, 1, 0, 1], [8, 2, 0, 0], [12, 9, 3, 1]])
 def test_rows_beyond_the_batch_stay_as_they_are(new, max_len) -> None:
