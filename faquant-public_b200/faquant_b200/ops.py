@@ -687,6 +687,7 @@ def hif4_decode_attention(
     return out
 
 
+@functools.lru_cache(maxsize=64)
 def hif4_page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
     """Bytes of one page of the HiF4 K/V cache: K and V of ``page_size`` tokens, 4.625 bits
     per value (the page format is in ``include/faquant_b200.h``)."""
@@ -701,36 +702,43 @@ def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: to
     calls' arguments for them: ``(pages, num_pages, page_stride, page_size)`` and ``(table, row
     stride, columns, cu, lens, batch)``."""
     size = hif4_page_bytes(kv_heads, head_dim, page_size)
-    shape, stride = pages.shape, pages.stride()
+    shape = pages.shape
     if pages.dtype is not torch.uint8 or len(shape) < 2:
         raise TypeError("pages must be a uint8 tensor [num_pages, ...]")
-    if len(shape) == 4:
-        if shape[1] != 2 or shape[2] != kv_heads:
-            raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
-        inner = size // (2 * kv_heads)
-        whole = shape[3] == inner and stride[1:] == (kv_heads * inner, inner, 1)
+    if len(shape) == 4 and (shape[1] != 2 or shape[2] != kv_heads):
+        raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
+    page_stride = inner = 1
+    for n in shape[1:]:
+        inner *= n
+    whole = inner == size
+    if pages.is_contiguous():
+        page_stride = size
     else:
+        stride = pages.stride()
+        page_stride = stride[0] if shape[0] > 1 else size
         inner = 1
-        whole = True
         for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
             whole = whole and (st == inner or n == 1)
             inner *= n
-        whole = whole and inner == size
     if not whole:
         raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
-    if table.dtype is not torch.int32 or cu.dtype is not torch.int32 or lens.dtype is not torch.int32:
+    int32 = torch.int32
+    if table.dtype is not int32 or cu.dtype is not int32 or lens.dtype is not int32:
         raise TypeError("table, cu and lens must be int32")
-    columns, ld = table.shape, table.stride()
-    if len(columns) != 2 or columns[1] < 1 or ld[1] != 1:
-        raise ValueError("table must be [batch, columns] with unit column stride")
-    batch = columns[0]
-    if cu.shape != (batch + 1,) or lens.shape != (batch,):
-        raise ValueError("cu must be [batch + 1] and lens [batch]")
-    if (batch and cu.stride() != (1,)) or (batch > 1 and lens.stride() != (1,)):
+    batch = lens.shape[0] if lens.dim() == 1 else -1
+    if table.dim() != 2 or table.shape[0] != batch or cu.shape != (batch + 1,):
+        raise ValueError("table must be [batch, columns], cu [batch + 1] and lens [batch]")
+    columns = ld = table.shape[1]
+    if not table.is_contiguous():
+        ld, unit = table.stride()
+        if unit != 1 and columns > 1:
+            raise ValueError("table must have unit column stride")
+        if batch == 1:
+            ld = columns  # a single row may have any stride
+    if not (cu.is_contiguous() and lens.is_contiguous()):
         raise ValueError("cu and lens must be contiguous")
-    # a single row may have any stride
-    return ((pages.data_ptr(), shape[0], stride[0] if shape[0] > 1 else size, page_size),
-            (table.data_ptr(), ld[0] if batch > 1 else columns[1], columns[1], cu.data_ptr(), lens.data_ptr(), batch))
+    return ((pages.data_ptr(), shape[0], page_stride, page_size),
+            (table.data_ptr(), ld, columns, cu.data_ptr(), lens.data_ptr(), batch))
 
 
 def _kv_heads(pages: torch.Tensor, head_dim: int, page_size: int) -> int:
@@ -805,7 +813,7 @@ def hif4_kv_read(
     if total < 0:
         raise ValueError("total must not be negative")
     if out is None:
-        k = torch.empty((total, h, head_dim), dtype=dtype, device=device)
+        k = pages.new_empty((total, h, head_dim), dtype=dtype)
         v = torch.empty_like(k)
         ks = vs = (h * head_dim, head_dim)
     else:
@@ -857,7 +865,7 @@ def hif4_paged_attention(
         q = q.contiguous()
         qs = (heads * d, d)
     if out is None:
-        out = q.new_empty((total, heads, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os_ = (heads * d, d)
     else:
         if out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
@@ -921,7 +929,7 @@ def verify_drafts(
         num_drafts = num_drafts.contiguous()
     draft_tokens, accept_u, sample_u = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
     tokens = draft_tokens.new_empty((b, k1))
-    accepted = torch.empty((b,), dtype=torch.int32, device=device)
+    accepted = draft_tokens.new_empty((b,), dtype=torch.int32)
     _lib.call("faq_verify_drafts", draft_tokens.data_ptr(), target_probs.data_ptr(), _ptr(draft_probs),
               _dtype_code(target_probs), b, k, vocab, ts[0], ts[1], ds[0], ds[1], accept_u.data_ptr(),
               sample_u.data_ptr(), _ptr(num_drafts), tokens.data_ptr(), accepted.data_ptr(), _stream(device))
