@@ -23,7 +23,7 @@
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
 //
 // Measured (one B200, d = 128): the last 512 of 32768 tokens with 64 query heads on 8 kv heads
-// in 547 us, 997 TFLOP/s counting the visible pairs (645 us and 846 TFLOP/s in a long series,
+// in 540 us, 1010 TFLOP/s counting the visible pairs (588 us and 928 TFLOP/s in a long series,
 // where the power limit lowers the clocks); all of a 16384-token prompt with 32 heads 1078
 // TFLOP/s. The expansion takes 32 us of the first. A key tile takes about 3900 cycles where the
 // products alone need 2048. What bounds it is shared memory: the operands of the four products
@@ -596,7 +596,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   grid_dependency_wait();
   allow_dependent_launch();
   const int2 run = P.run[blockIdx.x];
-  const Segment* segments = P.segments + run.x;
+  // A run's segments are taken last first. Units are mostly about as long as runs, so a run is the
+  // end of one unit and the start of the next: with the start first, all CTAs are at about the
+  // same key tile at the same time, and the tiles' readers meet in L2. (512 tokens on 32768 with
+  // 64/8 heads in a long series, where DRAM's power comes out of the clocks: 588 us against 625.)
+  const Segment* last = P.segments + run.x + run.y - 1;
   const int nseg = run.y;
   // whether tile B has rows
   auto two_tiles = [&](const Segment& g) { return g.tok0 + P.tile_tokens < g.n; };
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         int step = 0;
         const uint32_t q_bytes = static_cast<uint32_t>(P.group * P.tile_tokens) * 128;
         for (int i = 0; i < nseg && ok; ++i) {
-          const Segment g = segments[i];
+          const Segment g = last[-i];
           const int tiles = two_tiles(g) ? 2 : 1;
           if (i > 0 && !mbar_wait_site(smem_addr(q_empty), (i - 1) & 1, 50, i)) break;
           mbar_arrive_expect_tx(smem_addr(q_full), tiles * NG * q_bytes);
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true;
         int step = 0;
         for (int i = 0; i < nseg && ok; ++i) {
-          const Segment g = segments[i];
+          const Segment g = last[-i];
           for (int j = 0; j < g.count; ++j, ++step) {
             if (!mbar_wait_site(smem_addr(v_empty), (step & 1) ^ 1, 52, step)) { ok = false; break; }
             mbar_arrive_expect_tx(smem_addr(v_full), L::tile);
@@ -703,8 +707,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         return true;
       };
       for (int i = 0; i < nseg && ok; ++i) {
-        const int n = __shfl_sync(0xffffffffu, segments[i].count, 0);
-        const bool two = __all_sync(0xffffffffu, two_tiles(segments[i]));
+        const int n = __shfl_sync(0xffffffffu, last[-i].count, 0);
+        const bool two = __all_sync(0xffffffffu, two_tiles(last[-i]));
         if (!wait(q_full, i, 55, i)) break;
         ok = scores(ring, two);
         if (n == 1) commit(smem_addr(q_empty));
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                   P.scale_log2);
     const int row = sm.template row<2>(), row_tok = row / P.group, row_head = row - row_tok * P.group;
     for (int i = 0; i < nseg; ++i) {
-      const Segment g = segments[i];
+      const Segment g = last[-i];
       if (t == 1 && !two_tiles(g)) continue;
       const int tok = g.tok0 + t * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < g.n;
