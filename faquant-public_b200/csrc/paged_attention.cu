@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
     fence_barrier_init();
   }
   if (tid == 0) s_any = s_empty = 0;
+  __syncthreads();  // the count below sets s_empty from any warp
   grid_dependency_wait();
   allow_dependent_launch();
 

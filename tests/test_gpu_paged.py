@@ -430,6 +430,42 @@ def test_rows_beyond_the_batch_stay_as_they_are(new, max_len) -> None:
     _no_status()
 
 
+# ------------------------------------------------------------------ many sequences
+@pytest.mark.parametrize("most", [2, 20, 70], ids=["few", "chunk", "prompt"])
+@pytest.mark.parametrize("batch", [40, 600, 1300])
+def test_many_sequences(batch, most) -> None:
+    """More sequences than a warp's lanes (40), than the threads of the few rows' kernel (600) and
+    of the chunks' kernel (1300): ragged, with idle ones, short and long ones, and tokens
+    without a key in all of them. The prefix sums over the batch say whose keys a CTA reads."""
+    g = torch.Generator().manual_seed(batch + most)
+    lens = torch.randint(0, 40, (batch,), generator=g)
+    lens[torch.randint(0, batch, (3,), generator=g)] = 1100
+    new = torch.where(torch.rand(batch, generator=g) < 0.4, 0, torch.randint(1, most + 1, (batch,), generator=g))
+    if most == 70:  # prompts and steps in one batch
+        new = torch.where(torch.rand(batch, generator=g) < 0.9, new.clamp(max=2), new)
+    new[batch - 3], lens[batch - 3] = most, max(0, most - 1)  # the first of them has no key
+    new[5] = most
+    lens, new = lens.tolist(), new.tolist()
+    pool = Pool(lens, 1, 64, 16, DEV, fill=0xFF)
+    k, v = _randn(sum(lens), 1, 64, seed=80), _randn(sum(lens), 1, 64, seed=81)
+    pool.write(k, v)
+    rk, rv = pool.read()
+    kq, vq = quantized(k), quantized(v)
+    assert torch.equal(rk.float().cpu(), kq) and torch.equal(rv.float().cpu(), vq)
+    q = _randn(sum(new), 2, 64, seed=82)
+    ref, size = attention(q, kq, vq, lens, new)
+    for max_len in (0, 5000):
+        for _ in range(3):
+            out = torch.full_like(q, float("nan"))
+            pool.attend(q, new, max_len, out=out)
+            assert bool(((out.double().cpu() - ref).abs() <= BOUND * size + 2.0**-126).all())
+    tail, _ = pool.read(new=[min(n, length) for n, length in zip(new, lens)])
+    ends = torch.tensor(lens).cumsum(0).tolist()
+    want = torch.cat([kq[e - min(n, length) : e] for e, n, length in zip(ends, new, lens)])
+    assert torch.equal(tail.float().cpu(), want)
+    _no_status()
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals() -> None:
     from faquant_b200 import ops
