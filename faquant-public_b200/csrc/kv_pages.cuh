@@ -49,6 +49,13 @@ __device__ __forceinline__ int64_t page_of(const Pages& p, int b, int pos) {
   return page;
 }
 
+// Whether column `col` of sequence b's table row holds no page.
+__device__ __forceinline__ bool no_page(const Pages& p, int b, int col) {
+  if (col >= p.table_cols) return true;
+  const int page = p.table[b * p.table_ld + col];
+  return page < 0 || page >= p.num_pages;
+}
+
 // Length of sequence b, at most what its table row can hold (a longer one is recorded).
 __device__ __forceinline__ int length_of(const Pages& p, int b) {
   const int len = p.lens[b], most = p.table_cols << p.page_shift;

@@ -398,8 +398,9 @@ int faq_gptq_hif4_block(const float* w, int64_t ldw, int64_t rows, int cols, int
  * nothing). `table` int32 [batch, table_cols] (row stride table_ld) holds the page of tokens
  * c * page_size .. of each sequence in column c; entries past a sequence's length are not
  * read. An entry outside 0 .. num_pages - 1, or a length beyond the table's columns, sets
- * FAQ_STATUS_BAD_PAGE in the device status word: those tokens are not written and read as
- * zeros, and the attention of that sequence is not defined.
+ * FAQ_STATUS_BAD_PAGE in the device status word: those tokens are not written, read as zeros,
+ * and the attention leaves their keys out. (Where the length is beyond the table's columns the
+ * attention takes it for the most that these hold, which moves the sequence's new tokens.)
  *
  * Page format (d = 64 NG channels, NG 1 or 2): `pages` uint8, page p at p * page_stride
  * bytes (a multiple of 16; layers may interleave): [2: K, V][kv_heads][page_size / 16]

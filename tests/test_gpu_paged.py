@@ -430,6 +430,43 @@ def test_rows_beyond_the_batch_stay_as_they_are(new, max_len) -> None:
     _no_status()
 
 
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("n", [1, 4, 8, 16, 30, 60, 150])
+def test_keys_without_a_page_are_left_out(n, page) -> None:
+    """Table entries outside the pool: their tokens are read as zeros and leave the softmax, in every
+    kernel, whatever stood in the keys' place before; a sequence without pages gives zeros."""
+    from faquant_b200 import _lib
+
+    lens, new = [3000, 700, 200, 900], [n, n, n, n]
+    pool = Pool(lens, 2, 64, page, DEV, seed=n)
+    k, v = _randn(sum(lens), 2, 64, seed=83), _randn(sum(lens), 2, 64, seed=84)
+    v[:3000] += 100.0  # the first sequence's values would show in another's output
+    pool.write(k, v)
+    holes = [[2, 700 // page], [0, 699 // page], list(range(-(-200 // page))), []]
+    for b, cols in enumerate(holes):
+        for i, col in enumerate(cols):
+            pool.table[b, col] = (-1, 10**6, -(2**31), 2**31 - 1)[i % 4]
+    q = _randn(4 * n, 8, 64, seed=85)
+    out = torch.full_like(q, float("nan"))
+    pool.attend(q, new, 5000, out=out)
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_PAGE
+    rk, rv = pool.read()
+    assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_PAGE
+    kq, vq, begin = quantized(k).double(), quantized(v).double(), 0
+    for b, length in enumerate(lens):
+        here = torch.tensor([i // page not in holes[b] for i in range(length)])
+        key, value = kq[begin : begin + length], vq[begin : begin + length]
+        for got, want in ((rk, key), (rv, value)):
+            assert torch.equal(got[begin : begin + length].double().cpu(), want * here[:, None, None])
+        seen = here & (torch.arange(length) <= torch.arange(length - n, length)[:, None])
+        s = torch.einsum("nhd,khd->hnk", q[b * n : b * n + n].double().cpu(), key.repeat_interleave(4, 1)) / 8.0
+        p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1).nan_to_num(0.0)  # no key: 0 / 0
+        ref, size = (torch.einsum("hnk,khd->nhd", p, x.repeat_interleave(4, 1)) for x in (value, value.abs()))
+        assert bool(((out[b * n : b * n + n].double().cpu() - ref).abs() <= BOUND * size + 2.0**-126).all()), b
+        begin += length
+    assert not out[2 * n : 3 * n].any()
+
+
 # ------------------------------------------------------------------ many sequences
 @pytest.mark.parametrize("most", [2, 20, 70], ids=["few", "chunk", "prompt"])
 @pytest.mark.parametrize("batch", [40, 600, 1300])
