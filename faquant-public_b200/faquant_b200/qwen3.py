@@ -83,8 +83,7 @@ def attention_forward(
     if kernel == "paged":  # write to the HiF4 pages, attend over them (P not quantized)
         if not isinstance(past_key_values, PagedKVCache):
             raise ValueError('faquant_attention_kernel "paged" needs a PagedKVCache as past_key_values')
-        if attention_mask is not None:
-            raise NotImplementedError("attention masks are not implemented by the paged attention of faquant_b200")
+        _refuse_unpaged(self, attention_mask, kwargs)
         attn_output = past_key_values.forward(self.layer_idx, query_states, key_states, value_states, self.scaling)
         return _project(self, attn_output, input_shape), None
     if past_key_values is not None:
@@ -105,6 +104,26 @@ def attention_forward(
         self, query_states, key_states, value_states, attention_mask, dropout=0.0, scaling=self.scaling,
         sliding_window=getattr(self, "sliding_window", None), **kwargs)
     return _project(self, attn_output, input_shape), attn_weights
+
+
+def _refuse_unpaged(module, attention_mask, kwargs) -> None:
+    """What the paged attention does not do -- it is causal over each sequence's whole cache -- is
+    refused, as ``simulated_flash_attention_forward`` refuses what it does not do."""
+    if attention_mask is not None:
+        raise NotImplementedError("attention masks are not implemented by the paged attention of faquant_b200")
+    if getattr(module, "sliding_window", None) is not None or kwargs.get("sliding_window") is not None:
+        raise NotImplementedError("sliding windows are not implemented by the paged attention of faquant_b200")
+    if any(kwargs.get(n) is not None for n in ("cu_seq_lens_q", "cu_seq_lens_k", "max_length_q", "max_length_k")):
+        raise NotImplementedError("packed cu_seqlens are not supported: give each sequence its place in the PagedKVCache")
+    if kwargs.get("softcap") is not None:
+        raise NotImplementedError("softcap is not implemented by faquant_b200")
+    requested = kwargs.get("is_causal")
+    if not (getattr(module, "is_causal", True) if requested is None else requested):
+        raise NotImplementedError("the paged attention of faquant_b200 is causal")
+    if kwargs.get("dropout"):
+        raise ValueError("the paged attention only supports dropout=0 inference")
+    if kwargs.get("output_attentions", False):
+        raise ValueError("the paged attention does not materialize attention weights")
 
 
 def _project(module, attn_output: torch.Tensor, input_shape) -> torch.Tensor:

@@ -105,3 +105,49 @@ def test_paged_attention_needs_its_cache_and_no_mask() -> None:
     cache.truncate([16])
     cache.extend([1])
     assert cache.lengths == [17] and len(cache._held[0]) == 2 and cache.get_mask_sizes(5) == (22, 0)
+
+
+def _paged_layer(**attributes):
+    """A Qwen3 attention layer on the host that runs the adapter, and its cache."""
+    from transformers import Qwen3Config
+    from transformers.models.qwen3.modeling_qwen3 import Qwen3Attention
+
+    from faquant_b200.kv_cache import PagedKVCache
+
+    cfg = Qwen3Config(hidden_size=32, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=1, head_dim=64,
+                      use_sliding_window=True, sliding_window=8, max_window_layers=1,
+                      layer_types=["full_attention", "sliding_attention"])
+    layer = Qwen3Attention(cfg, attributes.pop("layer_idx", 0)).to(torch.bfloat16)
+    layer.faquant_attention_kernel = "paged"
+    for name, value in attributes.items():
+        setattr(layer, name, value)
+    return layer, PagedKVCache(2, 1, 64, max_length=64, page_size=16, device="cpu")
+
+
+def _forward(layer, cache, mask=None, **kwargs):
+    from faquant_b200.qwen3 import attention_forward
+
+    x = torch.zeros(1, 3, 32, dtype=torch.bfloat16)
+    cos = torch.ones(1, 3, 64, dtype=torch.bfloat16)
+    return attention_forward(layer, x, (cos, torch.zeros_like(cos)), mask, past_key_values=cache, **kwargs)
+
+
+def test_paged_layer_refuses_what_it_does_not_do() -> None:
+    layer, cache = _paged_layer()
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):  # nothing to refuse: it goes on to the kernels
+        _forward(layer, cache)
+    window = torch.tensor([0, 3], dtype=torch.int32)
+    for kwargs, error in (({"cu_seq_lens_q": window}, NotImplementedError), ({"cu_seq_lens_k": window}, NotImplementedError),
+                          ({"max_length_q": 3}, NotImplementedError), ({"is_causal": False}, NotImplementedError),
+                          ({"softcap": 30.0}, NotImplementedError), ({"sliding_window": 4}, NotImplementedError),
+                          ({"mask": torch.ones(1, 3)}, NotImplementedError), ({"dropout": 0.1}, ValueError),
+                          ({"output_attentions": True}, ValueError)):
+        layer, cache = _paged_layer()
+        with pytest.raises(error):
+            _forward(layer, cache, **kwargs)
+        assert cache.lengths == [0]  # no step was opened
+    for attributes in ({"layer_idx": 1}, {"sliding_window": 8}, {"is_causal": False}):
+        layer, cache = _paged_layer(**attributes)
+        with pytest.raises(NotImplementedError):
+            _forward(layer, cache)
+        assert cache.lengths == [0]
