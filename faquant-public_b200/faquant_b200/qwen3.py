@@ -8,7 +8,9 @@ Mirrors ``qwen3._attention_forward`` (``src/faquant/qwen3.py:56-172``) with the 
 single bf16 rounding -- here one K4 launch per operand -- then the HiF4 attention
 backend (``faquant_b200.attention``) and ``o_proj``. With ``faquant_attention_kernel =
 "paged"`` and a :class:`~faquant_b200.kv_cache.PagedKVCache` as ``past_key_values`` the keys and
-values go to 4-bit pages instead and the paged attention runs on them.
+values go to HiF4 pages instead and the paged attention runs on them: K and V are quantized, Q and
+P are not, whatever ``faquant_qk_matmul_quant`` and ``faquant_pv_matmul_quant`` say of
+those; a recipe that asks for other keys or values raises.
 """
 
 from __future__ import annotations
@@ -18,7 +20,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .attention import simulated_flash_attention_forward
+from .attention import _hif4_kwargs, simulated_flash_attention_forward
 from .kv_cache import PagedKVCache
 
 
@@ -80,7 +82,7 @@ def attention_forward(
         key_states = ops.qk_prep(key_states, levels=ops.default_levels("act"), rotate=False)[0]
         value_states = ops.qk_prep(value_states, levels=ops.default_levels("act"), rotate=False)[0]
     kernel = getattr(self, "faquant_attention_kernel", "simulated")
-    if kernel == "paged":  # write to the HiF4 pages, attend over them (P not quantized)
+    if kernel == "paged":  # write to the HiF4 pages, attend over them (Q and P not quantized)
         if not isinstance(past_key_values, PagedKVCache):
             raise ValueError('faquant_attention_kernel "paged" needs a PagedKVCache as past_key_values')
         _refuse_unpaged(self, attention_mask, kwargs)
@@ -120,6 +122,11 @@ def _refuse_unpaged(module, attention_mask, kwargs) -> None:
     requested = kwargs.get("is_causal")
     if not (getattr(module, "is_causal", True) if requested is None else requested):
         raise NotImplementedError("the paged attention of faquant_b200 is causal")
+    shared = getattr(module, "faquant_matmul_quant_kwargs", None)
+    for operand, what in (("qk", "QK operands"), ("pv", "PV operands")):
+        if not getattr(module, f"faquant_{operand}_matmul_quant", True):
+            raise NotImplementedError(f"{what}: the paged cache holds HiF4 keys and values only")
+        _hif4_kwargs(getattr(module, f"faquant_{operand}_matmul_quant_kwargs", shared), what)
     if kwargs.get("dropout"):
         raise ValueError("the paged attention only supports dropout=0 inference")
     if kwargs.get("output_attentions", False):

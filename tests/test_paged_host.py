@@ -151,3 +151,25 @@ def test_paged_layer_refuses_what_it_does_not_do() -> None:
         with pytest.raises(NotImplementedError):
             _forward(layer, cache)
         assert cache.lengths == [0]
+
+
+def test_paged_layer_reads_the_operand_recipe() -> None:
+    hif4 = {"quant_format": "hif4", "bits": 4, "group_size": 64}
+    integer = {"quant_format": "int", "bits": 4, "group_size": 64}
+    for attributes in ({"faquant_qk_matmul_quant": False}, {"faquant_pv_matmul_quant": False},
+                       {"faquant_qk_matmul_quant": True, "faquant_matmul_quant_kwargs": integer},
+                       {"faquant_pv_matmul_quant": True, "faquant_matmul_quant_kwargs": hif4,
+                        "faquant_pv_matmul_quant_kwargs": integer},
+                       {"faquant_qk_matmul_quant_kwargs": hif4 | {"group_size": 32}},
+                       {"faquant_qk_matmul_quant_kwargs": hif4 | {"bits": 8}}):
+        layer, cache = _paged_layer(**attributes)
+        with pytest.raises(NotImplementedError):
+            _forward(layer, cache)
+        assert cache.lengths == [0]
+    for attributes in ({"faquant_qk_matmul_quant": True, "faquant_pv_matmul_quant": True,
+                        "faquant_matmul_quant_kwargs": hif4},
+                       {"faquant_matmul_quant_kwargs": integer, "faquant_qk_matmul_quant_kwargs": hif4,
+                        "faquant_pv_matmul_quant_kwargs": hif4 | {"group_size": -1}}):
+        layer, cache = _paged_layer(**attributes)
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            _forward(layer, cache)
