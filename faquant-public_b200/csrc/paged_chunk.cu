@@ -390,24 +390,15 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
     Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
-    auto look = [&](const Walk& x) {
-      return x.count > 0 && pre::any_without_page(p, x.b, x.len, x.k0, x.count, lane);
-    };
-    Walk w = s_walk, next;
-    bool holes = look(w), next_holes = false;
-    auto unit = [&](auto parts) {
+    auto unit = [&](const Walk& w, auto parts) {
       constexpr int PARTS = decltype(parts)::value;
       const int row = sm.template row<PARTS>(), row_tok = row / P.group, row_head = row - row_tok * P.group;
       const int tok = w.u * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < w.n;
-      auto look_ahead = [&]() {
-        next = w;
-        next_unit(P, next, begin, end);
-        next_holes = look(next);
-      };
-      const int lim = live ? w.len - w.n + tok : 0x7fffffff;
-      if (!(holes ? sm.template run<PARTS, true>(p, w.b, w.len, w.k0, w.count, lim, look_ahead)
-                  : sm.template run<PARTS, false>(p, w.b, w.len, w.k0, w.count, lim, look_ahead)))
+      const int lim = live ? w.len - w.n + tok : pre::NO_ROW;
+      if (!(pre::any_without_page(p, w.b, w.len, w.k0, w.count, lane)
+                ? sm.template run<PARTS, true>(p, w.b, w.len, w.k0, w.count, lim, [] {})
+                : sm.template run<PARTS, false>(p, w.b, w.len, w.k0, w.count, lim, [] {})))
         return false;
       if (!sm.template first_copy<PARTS>()) return true;
       float* part = w.count == w.tiles ? nullptr
@@ -416,11 +407,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
                P.out + static_cast<int64_t>(w.c0 + (live ? tok : 0)) * P.ot + (w.head * P.group + row_head) * P.oh);
       return true;
     };
-    for (; w.count > 0; w = next, holes = next_holes) {
+    for (Walk w = s_walk; w.count > 0; next_unit(P, w, begin, end)) {
       const int copies = copies_of(P, w);
-      const bool ok = copies == 4   ? unit(std::integral_constant<int, 8>())
-                      : copies == 2 ? unit(std::integral_constant<int, 4>())
-                                    : unit(std::integral_constant<int, 2>());
+      const bool ok = copies == 4   ? unit(w, std::integral_constant<int, 8>())
+                      : copies == 2 ? unit(w, std::integral_constant<int, 4>())
+                                    : unit(w, std::integral_constant<int, 2>());
       if (!ok) break;
     }
   }

@@ -52,6 +52,7 @@ constexpr int CHUNK = TILE * 128;    // 128 rows of 64 channels
 constexpr int THREADS = 640;
 constexpr int COST = 3;              // of a unit beyond its key tiles (filling, joining), in key tiles
 constexpr int ROWS = 2 * TILE;
+constexpr int NO_ROW = 0x7fffffff;   // the last visible key of a row that is not there: it sees all
 constexpr int EXPAND_WARPS = 4;      // of a CTA of the expansion
 
 struct Segment {  // a run's part of one unit
@@ -419,11 +420,13 @@ struct Softmax {
   }
 
   // Key tiles k0 .. k0 + count - 1 of sequence b of `len` tokens for a row whose last visible key
-  // is lim. False: a wait ran out. HOLES: some of these keys have no page and are left out, tile by
-  // tile as the table has it. That is code of its own: a test of it in the loop of all units took the
-  // drafted tokens of 16 sequences from 33.0 us to 34.1, this to 33.4. meanwhile() is called while the last product runs. (Warps whose rows are
-  // all dead work like the others: leaving their exponentials out gained nothing, the live ones
-  // are bound by their own latency.)
+  // is lim (NO_ROW: there is none in its place). False: a wait ran out. HOLES: some of these keys
+  // have no page and are left out, tile by tile as the table has it. That is code of its own: a
+  // test of it in the loop of all units took the drafted tokens of 16 sequences from 33.0 us to 34.1, this
+  // to 33.4. meanwhile() is called while the last product runs: the prompt kernel sees there whether the
+  // next unit has holes (at that unit's start: 560 us instead of 535 for 512 tokens on 32768). (Warps
+  // whose rows are all dead work like the others: leaving their exponentials out gained nothing,
+  // the live ones are bound by their own latency.)
   template <int PARTS, bool HOLES, typename F>
   __device__ __forceinline__ bool run(const Pages& pages, int b, int len, int k0, int count, int lim, F&& meanwhile) {
     constexpr int KEYS = TILE / PARTS;
@@ -432,7 +435,10 @@ struct Softmax {
     const uint32_t p_row = smem_addr(p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
     const int unit0 = (part * KEYS & 63) >> 3;
     const float2 c2 = make_float2(scale_log2, scale_log2);
-    m = LOWEST;
+    // Rows that are not there hold another sequence's queries, or what shared memory held: no score
+    // of theirs is above +inf, so they never raise the live rows' maxima, whose roundings would
+    // else depend on them.
+    m = lim == NO_ROW ? INFINITY : LOWEST;
     l = 0.0f;
     bool ok = true;
     for (int j = 0; j < count; ++j, ++done) {
@@ -775,8 +781,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const int tok = g.tok0 + t * P.tile_tokens + row_tok;
       const bool live = row_tok < P.tile_tokens && tok < g.n;
-      // last visible key; rows that are not there see all
-      const int lim = live ? g.len - g.n + tok : 0x7fffffff;
+      const int lim = live ? g.len - g.n + tok : NO_ROW;
       if (!(holes ? sm.template run<2, true>(P.p, g.b, g.len, g.k0, g.count, lim, look_ahead)
                   : sm.template run<2, false>(P.p, g.b, g.len, g.k0, g.count, lim, look_ahead)))
         break;

@@ -467,6 +467,29 @@ def test_keys_without_a_page_are_left_out(n, page) -> None:
     assert not out[2 * n : 3 * n].any()
 
 
+@pytest.mark.parametrize("group,new", [(4, 5), (3, 21), (12, 10), (5, 25), (4, 9), (3, 200), (7, 90), (14, 30)])
+def test_the_bits_depend_on_a_sequences_own_queries_only(group, new) -> None:
+    """Neither the next sequence's queries, nor rows of q beyond the batch, nor what a call before left in
+    shared memory (rows of a tile that no box of whole tokens fills) may move a rounding."""
+    lens, counts = [3000, 2500], [new, new]
+    pool = Pool(lens, 2, 128, 32, DEV)
+    k, v = _randn(sum(lens), 2, 128, seed=86), _randn(sum(lens), 2, 128, seed=87)
+    pool.write(k, v)
+    q = _randn(2 * new + 40, 2 * group, 128, seed=88)
+    other = _randn(2 * new, 2 * 4 if 4 * new > 16 else 64, 128, seed=89, scale=200.0)
+    used = slice(0, 2 * new)
+    want = pool.attend(q, counts, 5000)
+    _close(want[used], lens, counts, q[used], quantized(k), quantized(v))
+    for scale in (0.0, 60.0, 200.0, float("nan")):
+        pool.attend(other, counts, 5000)
+        x = q.clone()
+        x[2 * new :] *= scale
+        assert torch.equal(pool.attend(x, counts, 5000)[used], want[used]), scale
+        x[new:] *= scale
+        assert torch.equal(pool.attend(x, counts, 5000)[:new], want[:new]), scale
+    _no_status()
+
+
 # ------------------------------------------------------------------ many sequences
 @pytest.mark.parametrize("most", [2, 20, 70], ids=["few", "chunk", "prompt"])
 @pytest.mark.parametrize("batch", [40, 600, 1300])
