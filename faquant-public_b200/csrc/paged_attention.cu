@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
     }
     valid = __ballot_sync(0xffffffffu, has);
   };
-  const uint32_t v_off = static_cast<uint32_t>(p.kv_heads << (p.page_shift - 4)) * UNIT;
+  // from a page's K to its V, in units of 16 bytes: bytes pass 32 bits in pages of 8 GiB
+  const uint32_t v_dist = static_cast<uint32_t>(p.kv_heads << (p.page_shift - 4)) * (UNIT / 16);
   auto copy_next = [&]() {  // into a free slot of the ring
     if ((ahead & 31) == 0) look_up(s_seg[ahead_seg]);
     const uint32_t slot = issued % S;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
       const uint32_t dst = smem_addr(ring + slot * STAGE);
       mbar_arrive_expect_tx(bar, STAGE);
       bulk_copy(dst, address, UNIT, bar);
-      bulk_copy(dst + UNIT, address + v_off, UNIT, bar);
+      bulk_copy(dst + UNIT, address + static_cast<uint64_t>(v_dist) * 16, UNIT, bar);
     }
     has_page = (has_page & ~(1u << slot)) | (((valid >> (ahead & 31)) & 1u) << slot);
     ++issued;

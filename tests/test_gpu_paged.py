@@ -133,6 +133,30 @@ def test_offsets_past_32_bits() -> None:
     _no_status()
 
 
+def test_a_page_of_more_than_8_gib() -> None:
+    """V stands more than 2^32 bytes behind K in a page of very many heads: for the kernels of few
+    rows, of up to 128 and of more."""
+    from faquant_b200 import ops
+
+    h, d, ps = 14400, 128, 4096
+    pages = torch.zeros(1, ops.hif4_page_bytes(h, d, ps), dtype=torch.uint8, device=DEV)
+    assert pages.shape[1] // 2 > 1 << 32
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    length = 140
+    g = torch.Generator(DEV).manual_seed(15)
+    k, v = (torch.randn(length, h, d, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    some = torch.tensor([0, 1, 7000, 14168, 14169, 14170, 14171, h - 1], device=DEV)
+    kq, vq = quantized(k[:, some]), quantized(v[:, some])
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, length], [length]))
+    ops.hif4_kv_write(k, v, pages, table, cu, lens, page_size=ps)
+    for n, most in ((1, 1), (20, 20), (140, 140), (135, 140)):  # the last: q has rows beyond the batch
+        cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+        q = torch.randn(most, h, d, generator=g, device=DEV).to(torch.bfloat16)
+        out = ops.hif4_paged_attention(q, pages, table, cu, lens, page_size=ps, max_new=n, max_len=4096, total_len=length)
+        _close(out[:n, some], [length], [n], q[:n, some], kq, vq)
+    _no_status()
+
+
 def test_tokens_without_a_place() -> None:
     """Positions below zero are skipped; bad table entries and lengths are reported."""
     from faquant_b200 import _lib, ops
