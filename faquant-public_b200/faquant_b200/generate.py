@@ -169,7 +169,10 @@ def paged_speculative_generate(
         tokens, accepted = ops.verify_drafts(torch.tensor([drafts], dtype=torch.int64, device=device).reshape(1, -1),
                                              _target_probs(logits, temperature), None, u[:, :-1], u[:, -1].contiguous())
         n = int(accepted.item())
-        return tokens[0, : n + 1].tolist(), n
+        new = tokens[0, : n + 1].tolist()
+        if new[-1] < 0:  # no token to go on with: the embedding must not see it
+            raise RuntimeError("the model's probabilities of the next token have no mass (NaN logits?)")
+        return new, n
 
     for begin in range(0, length, chunk):
         logits = forward(input_ids[:, begin : min(begin + chunk, length)], 1)

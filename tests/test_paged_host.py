@@ -173,3 +173,36 @@ def test_paged_layer_reads_the_operand_recipe() -> None:
         layer, cache = _paged_layer(**attributes)
         with pytest.raises(RuntimeError, match="CUDA tensors only"):
             _forward(layer, cache)
+
+
+@pytest.mark.parametrize("bad_call", [0, 1])
+def test_generation_stops_when_there_is_no_token_to_sample(monkeypatch, bad_call) -> None:
+    """NaN logits at a temperature leave no mass, which verification reports as token -1: it is raised and
+    never fed to the model. (Verification itself runs on a GPU only; its reference stands in.)"""
+    import types
+
+    from faquant_b200 import ops
+    from faquant_b200.generate import paged_speculative_generate
+    from faquant_b200.kv_cache import PagedKVCache
+    from paged_reference import verify
+
+    def on_host(draft, target, drafter, accept_u, sample_u):
+        tokens, accepted = verify(draft.numpy(), target.nan_to_num(0.0), drafter, accept_u.numpy(), sample_u.numpy(),
+                                  [draft.shape[1]])
+        return torch.from_numpy(tokens), torch.from_numpy(accepted)
+
+    monkeypatch.setattr(ops, "verify_drafts", on_host)
+    cache, calls = PagedKVCache(1, 1, 64, max_length=64, page_size=16, device="cpu"), []
+
+    def model(input_ids, past_key_values, logits_to_keep, **_):
+        assert int(input_ids.min()) >= 0
+        past_key_values.extend([input_ids.shape[1]])
+        logits = torch.zeros(1, logits_to_keep, 11)
+        if len(calls) == bad_call:
+            logits[:] = float("nan")
+        calls.append(input_ids)
+        return types.SimpleNamespace(logits=logits)
+
+    with pytest.raises(RuntimeError, match="no mass"):
+        paged_speculative_generate(model, input_ids=torch.tensor([[3, 4, 5]]), max_length=20, cache=cache, temperature=1.0)
+    assert len(calls) == bad_call + 1
