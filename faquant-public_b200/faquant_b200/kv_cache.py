@@ -112,9 +112,10 @@ class PagedKVCache:
         self._open()
         if q.shape[0] != sum(self._new):
             raise ValueError(f"the step has {sum(self._new)} new tokens, got {q.shape[0]}")
+        lengths = [n for n, new in zip(self.lengths, self._new) if new]  # of those that take part
         return ops.hif4_paged_attention(q, self.pages[layer], self.table, self._cu, self._lens,
-                                        page_size=self.page_size, max_new=max(self._new), max_len=max(self.lengths),
-                                        total_len=sum(self.lengths), scale=scale)
+                                        page_size=self.page_size, max_new=max(self._new), max_len=max(lengths, default=0),
+                                        total_len=sum(lengths), scale=scale)
 
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """The layer's whole cache dequantized, ``(k, v)`` each ``[sum(lengths), kv_heads, head_dim]``,

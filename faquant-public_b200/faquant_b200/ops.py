@@ -849,7 +849,7 @@ def hif4_paged_attention(
 
     ``max_new``, ``max_len`` (the table's capacity by default) and ``total_len`` (batch x
     ``max_len`` by default) bound the sequences' new tokens, their lengths and the sum of
-    the lengths from above; they are host numbers, so nothing is copied from the device, and
+    the lengths from above (sequences without a new token do not count); they are host numbers, so nothing is copied from the device, and
     with prompt chunks in the batch they size the workspace. ``workspace``: a 256-byte
     aligned device buffer to use instead of a new one."""
     device = _require_cuda(q, pages, table, cu, lens, out, workspace)

@@ -444,8 +444,8 @@ int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t page_stride, 
  * and faq_hif4_decode_attention keep the reference's HiF4 P). A row without a key is
  * zero. Covers one decode step, chunks of drafted tokens and prompt chunks in one batch.
  * max_new, max_len and total_len are upper bounds on the sequences' new tokens, their lengths
- * and the sum of the lengths, known on the host (nothing is copied from the device): they
- * choose the kernels and size the workspace, which for sequences of more than 128 rows
+ * and the sum of the lengths (of the sequences that have new tokens; the others' do not count),
+ * known on the host (nothing is copied from the device): they choose the kernels and size the workspace, which for sequences of more than 128 rows
  * (new tokens x query heads of a kv head) also holds the keys and values of those in bf16. A
  * batch beyond them is either computed all the same or sets FAQ_STATUS_BAD_BOUND and leaves
  * those sequences' rows as they are. cu[batch] may be less than total: the rows of out beyond it

@@ -145,3 +145,31 @@ def test_ragged_sequences_pages_and_refusals() -> None:
     step([8, 64, 0])  # all nine pages
     cache.truncate([0, 0, 0])
     assert sorted(cache._free) == list(range(9))
+
+
+@pytest.mark.parametrize("new", [[0, 1, 0], [0, 40, 2], [0, 200, 1], [1, 0, 70]])
+def test_a_step_beside_a_long_idle_sequence(new) -> None:
+    """Bounds of the sequences that take part only, on every kernel, against a 64-bit softmax."""
+    from faquant_b200.kv_cache import PagedKVCache
+    from paged_reference import attention, quantized
+
+    held = [6000, 90, 300]
+    cache = PagedKVCache(1, 2, 64, max_sequences=3, max_length=8192, page_size=32, device=DEV)
+    g = torch.Generator().manual_seed(4)
+    rows = [[torch.empty(0, 2, 64)] * 3 for _ in range(2)]
+
+    def step(counts):
+        cache.extend(counts)
+        kv = [torch.randn(sum(counts), 2, 64, generator=g).to(torch.bfloat16) for _ in range(2)]
+        for packed, t in zip(rows, kv):
+            for b, part in enumerate(t.split(counts)):
+                packed[b] = torch.cat((packed[b], part.float()))
+        cache.write(0, *(t.to(DEV) for t in kv))
+        q = torch.randn(sum(counts), 8, 64, generator=g).to(torch.bfloat16)
+        return q, cache.attend(0, q.to(DEV))
+
+    step(held)
+    q, out = step(new)
+    ref, size = attention(q, *(quantized(torch.cat(packed)) for packed in rows), cache.lengths, new)
+    bound = 2.0**-7 + 2.0**-12  # P and O rounded to bf16, the scores' fp32 sums
+    assert bool(((out.double().cpu() - ref).abs() <= bound * size + 2.0**-126).all())

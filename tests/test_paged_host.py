@@ -206,3 +206,18 @@ def test_generation_stops_when_there_is_no_token_to_sample(monkeypatch, bad_call
     with pytest.raises(RuntimeError, match="no mass"):
         paged_speculative_generate(model, input_ids=torch.tensor([[3, 4, 5]]), max_length=20, cache=cache, temperature=1.0)
     assert len(calls) == bad_call + 1
+
+
+def test_idle_sequences_do_not_count_in_the_bounds(monkeypatch) -> None:
+    """The bounds choose kernels and workspace: one long idle sequence must not make a short step dear."""
+    from faquant_b200 import ops
+    from faquant_b200.kv_cache import PagedKVCache
+
+    given = []
+    monkeypatch.setattr(ops, "hif4_paged_attention", lambda q, *_, **kw: given.append(kw) or q)
+    cache = PagedKVCache(1, 1, 64, max_sequences=3, max_length=4096, page_size=64, device="cpu")
+    for counts, bounds in (([4000, 0, 0], (4000, 4000, 4000)), ([0, 30, 7], (30, 30, 37)), ([0, 1, 0], (1, 31, 31)),
+                           ([1, 0, 1], (1, 4001, 4009)), ([0, 0, 0], (0, 0, 0))):
+        cache.extend(counts)
+        cache.attend(0, torch.zeros(sum(counts), 2, 64, dtype=torch.bfloat16))
+        assert tuple(given[-1][n] for n in ("max_new", "max_len", "total_len")) == bounds
