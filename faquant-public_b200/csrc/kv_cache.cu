@@ -137,7 +137,10 @@ __device__ __forceinline__ bool find_slot(const Pages& p, int64_t slot, int64_t 
   }
   s.b = lo;
   const int c0 = p.cu[lo], c1 = p.cu[lo + 1];
-  if (c0 < 0 || c1 <= c0 || c1 > total || slot < first_slot(p, lo)) return false;
+  if (c0 < 0 || c1 <= c0 || c1 > total || slot < first_slot(p, lo)) {
+    check_rows(p, lo, total);
+    return false;
+  }
   const int64_t first = static_cast<int64_t>(p.lens[lo]) - (c1 - c0);  // position of the first new token
   // positions below zero have no block; the first block is that of position max(first, 0)
   const int64_t block = (first > 0 ? first >> 4 : 0) + (slot - first_slot(p, lo));

@@ -56,6 +56,12 @@ __device__ __forceinline__ bool no_page(const Pages& p, int b, int col) {
   return page < 0 || page >= p.num_pages;
 }
 
+// Records a sequence whose new tokens do not lie in the `total` given rows (it is left out).
+__device__ __forceinline__ void check_rows(const Pages& p, int b, int64_t total) {
+  const int c0 = p.cu[b], c1 = p.cu[b + 1];
+  if (c0 < 0 || c1 < c0 || c1 > total) atomicOr(&g_status, FAQ_STATUS_BAD_BOUND);
+}
+
 // Length of sequence b, at most what its table row can hold (a longer one is recorded).
 __device__ __forceinline__ int length_of(const Pages& p, int b) {
   const int len = p.lens[b], most = p.table_cols << p.page_shift;

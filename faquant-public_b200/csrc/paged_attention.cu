@@ -231,7 +231,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attention_kernel(Params P) {
   auto count_blocks = [&](int b) {  // warps without a sequence do nothing
     if (b - lane >= p.batch) return;
     sq = {0, 0, 0};
-    if (b < p.batch) sq = sequence(P, b);
+    if (b < p.batch) {
+      sq = sequence(P, b);
+      if (sq.n == 0) check_rows(p, b, P.total);
+    }
     per_head = head_cost(P, sq);
     mine = per_head * p.kv_heads;
     if (sq.n > sq.len) s_empty = 1;

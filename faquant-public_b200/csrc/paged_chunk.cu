@@ -194,7 +194,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_chunk_kernel(const __grid_co
     auto count = [&](int r) {
       const int b = r * THREADS + tid;
       w.n = w.units = 0;
-      if (b < p.batch) enter(P, w, b);
+      if (b < p.batch) {
+        enter(P, w, b);
+        if (w.n == 0) check_rows(p, b, P.total);
+      }
       if (w.n > 0 && w.n > w.len) s_empty = 1;
       mine = head_cost(P, w) * p.kv_heads;
       before = pre::block_scan<WARPS>(mine, s_scan, &sum);

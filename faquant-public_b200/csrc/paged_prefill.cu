@@ -159,6 +159,7 @@ __device__ void make_plan(const Params& P) {
   int64_t cost = 0;
   for (int b = tid; b < P.p.batch; b += N) {
     const Seq s = sequence(P, b);
+    if (s.n == 0) check_rows(P.p, b, P.total);
     for (int u = 0; u < (s.n ? units_of(P, s) : 0); ++u) {
       const int kt = key_tiles(P, s, u);
       cost += kt ? static_cast<int64_t>(kt + COST) * h : 0;

@@ -47,7 +47,7 @@ extern "C" {
 /* device status word bits */
 #define FAQ_STATUS_TIMEOUT 1u
 #define FAQ_STATUS_BAD_PAGE 2u  /* a page table entry or a length outside the pool or the table */
-#define FAQ_STATUS_BAD_BOUND 4u /* a ragged batch beyond the bounds the host gave (max_len, total_len) */
+#define FAQ_STATUS_BAD_BOUND 4u /* a ragged batch beyond the bounds the host gave (total, max_new, max_len, total_len) */
 
 /* element types */
 #define FAQ_BF16 0
@@ -400,7 +400,10 @@ int faq_gptq_hif4_block(const float* w, int64_t ldw, int64_t rows, int cols, int
  * read. An entry outside 0 .. num_pages - 1, or a length beyond the table's columns, sets
  * FAQ_STATUS_BAD_PAGE in the device status word: those tokens are not written, read as zeros,
  * and the attention leaves their keys out. (Where the length is beyond the table's columns the
- * attention takes it for the most that these hold, which moves the sequence's new tokens.)
+ * attention takes it for the most that these hold, which moves the sequence's new tokens.) A
+ * sequence whose part of `cu` does not lie in 0 .. total sets FAQ_STATUS_BAD_BOUND and is left
+ * out: not written, its rows of an output as they were (where cu falls, the write and the read
+ * may leave out others too).
  *
  * Page format (d = 64 NG channels, NG 1 or 2): `pages` uint8, page p at p * page_stride
  * bytes (a multiple of 16; layers may interleave): [2: K, V][kv_heads][page_size / 16]

@@ -261,6 +261,39 @@ def test_a_step_of_queries_equals_each_alone() -> None:
         assert bool(((one[0] - out[i]).double().abs().cpu() <= 2 * BOUND * size[i]).all())
 
 
+@pytest.mark.parametrize("n", [1, 7, 20, 70, 200])
+def test_sequences_beyond_the_rows_given_are_reported(n) -> None:
+    """cu says more tokens than k, v, q or `total` have rows, or falls: such a sequence is left out and
+    recorded, the others are served."""
+    from faquant_b200 import _lib, ops
+
+    lens = [300, 300]
+    pool = Pool(lens, 1, 64, 16, DEV)
+    k, v = _randn(600, 1, 64, seed=45), _randn(600, 1, 64, seed=46)
+    pool.write(k, v)
+    _no_status()
+    before = pool.store.clone()
+    q = _randn(2 * n, 2, 64, seed=47)
+    kw = dict(page_size=16)
+    for bounds in ([0, n, 2 * n + 1], [0, n, n - 1]):
+        cu = torch.tensor(bounds, dtype=torch.int32, device=DEV)
+        args = (pool.pages, pool.table, cu, pool.lens)
+        for max_len in (300, 5000):
+            out = torch.full_like(q, 7.0)
+            ops.hif4_paged_attention(q, *args, max_new=n, max_len=max_len, out=out, **kw)
+            assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
+            _close(out[:n], [300], [n], q[:n], quantized(k[:300]), quantized(v[:300]))
+            assert bool((out[n:] == 7.0).all())
+        back = [torch.full((2 * n, 1, 64), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+        ops.hif4_kv_read(*args, head_dim=64, total=2 * n, out=tuple(back), **kw)
+        assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
+        assert torch.equal(back[0][:n].float().cpu(), quantized(k[300 - n : 300])) and bool((back[0][n:] == 7.0).all())
+        new = torch.cat((k[300 - n : 300], k[:n]))  # the first sequence's tokens once more
+        ops.hif4_kv_write(new, torch.cat((v[300 - n : 300], v[:n])), *args, **kw)
+        assert _lib.device_status(reset=True) == _lib.FAQ_STATUS_BAD_BOUND
+        assert torch.equal(pool.store, before)
+
+
 @pytest.mark.parametrize("n", [4, 7, 14, 30, 40])
 def test_peaked_and_flat_scores_scale_and_ranges(n) -> None:
     lens, new = [900], [n]
