@@ -11,10 +11,12 @@
 // are found without a prefix sum over its blocks: sequence b's blocks get the slots from
 // cu[b] / 16 + 2 b on, always enough of them (n tokens touch at most n / 16 + 2 blocks).
 //
-// Measured (one B200, 8 kv heads of 128): writing 8192 tokens and reading them back 25.3 us for
-// 86 MB, 3.4 TB/s, where the write is bound by the fit's instructions; reading whole contexts
-// of 8 sequences back (156 MB) 35.8 us, 4.4 TB/s, bound by HBM and the ramps of a launch. A decode step's
-// tokens take the 8 us of two launches.
+// Measured (one B200, 8 kv heads of 128): writing 8192 tokens and reading them back 26.0 us for
+// 86 MB, 3.3 TB/s: the write takes 18.8 us of it (cold), three times its bytes' time, with 63 % of the
+// issue slots and 64 % of the integer pipe taken by the fit and the rest lost to its loads'
+// latency; reading whole contexts of 8 sequences back (156 MB) 36.4 us, 4.3 TB/s, waiting for loads (7.7
+// cycles per issue): a warp has one block, behind a chain of dependent ones (cu, lens, the
+// table, the block). A decode step's tokens take the 8 us of two launches.
 #include <algorithm>
 #include <atomic>
 

@@ -32,12 +32,13 @@
 // no sequence is longer than WHOLE tokens, units are not split and nothing is joined.
 //
 // Measured (one B200, 32 query heads on 8 kv heads of 128, one new token): a context of 32768
-// tokens in 20.1 us, 32 sequences of 1 .. 16000 tokens (76 MB of cache) in 35.6 us, 2.1 TB/s
-// of the pages. Bound by instruction issue, not by HBM (a third of its rate): a block of 16
-// tokens takes a warp about 470 instructions (118 cycles per block and SM), 223 of them in the
-// integer pipe at half rate (111 cycles); 150 to 170 are measured. Each call also has some 5 us
-// of dependent loads before its first block (cu and lens, the table, the pages) and 4 of its end
-// (the warps' join, the runs' join).
+// tokens in 20.4 us, 32 sequences of 1 .. 16000 tokens (76 MB of cache) in 35.8 us, 2.1 TB/s
+// of the pages. No one resource is full: HBM runs at a third of its rate, 54 % of the issue slots
+// and 49 % of the integer pipe are taken over a call. A block of 16 tokens takes a warp about
+// 470 instructions (118 cycles per block and SM), 223 of them in the integer pipe at half rate (111
+// cycles), where 150 to 170 cycles are measured; and each call has some 5 us of dependent loads
+// before its first block (cu and lens, the table, the pages) and 4 of its end (the warps' join,
+// the runs' join), which is where the issue slots stay empty ("barrier" is the first stall).
 #include <algorithm>
 #include <atomic>
 

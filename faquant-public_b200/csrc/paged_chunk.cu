@@ -12,12 +12,13 @@
 // paged_prefill.cu's join adds up the units of several runs.
 //
 // Measured (one B200): 8 new tokens for each of 16 sequences of 1 .. 8192 tokens, 32 query heads
-// on 8 kv heads of 128, in 32.8 us (36.6 without the copies). A key tile takes an SM about 3000
+// on 8 kv heads of 128, in 33.5 us (without the copies 3.8 more). A key tile takes an SM about 3000
 // cycles, of which a warp's expansion of its block of K and of V is 1900, at one instruction in
-// more than four cycles: it runs straight through some 400 instructions, and the warps' different
-// places in them are more than the instruction caches hold. Hence the rolled loops; 16 expanding
-// warps, K and V apart, were slower (92 us against 58 for 16 sequences of 4096 tokens, 77 with
-// rolled loops), their stalls "no instruction" 5.7 times the issued ones against 1.0.
+// more than four cycles. The warps wait for loads first (2.7 cycles per issue: the table's entry,
+// then the block, both one tile ahead only), then at barriers (2.5), then for instructions (1.6):
+// the roles' code together is more than the instruction caches hold. Hence the rolled loops; 16
+// expanding warps, K and V apart, were slower (92 us against 58 for 16 sequences of 4096 tokens, 77
+// with rolled loops), "no instruction" standing at 5.7 per issue there.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -464,9 +465,13 @@ static int launch(Params& P, const __nv_bfloat16* q, int64_t heads, int64_t qt, 
 //   rows against 57.8 in paged_chunk.cu, with 24 rows 77 against 58. Also when no unit is split
 //   and each can have an SM: 32 rows of 4 sequences of 1000 tokens 12.5 against 15.8, but of 32
 //   such sequences 64 against 37.5;
-// - else up to CHUNK_ROWS, paged_chunk.cu's: 128 rows of those 16 sequences take 74 us against
-//   164 in the prompt kernel, whose expansion writes the keys to memory;
-// - beyond them the prompt kernel's.
+// - else up to CHUNK_ROWS, one tile of paged_chunk.cu: 128 rows of those 16 sequences take 78 us
+//   against 164 in the prompt kernel, whose expansion writes the keys to memory;
+// - beyond them the prompt kernel's. That is not where the two cross: with a limit of 512 rows
+//   units of several tiles in paged_chunk.cu took 130 us against 175 here for 144 rows, 135 against
+//   200 for 256, 194 against 261 for 384 (with heads of 64: 100 / 160, 114 / 166, 163 / 224; 4 sequences
+//   of 16384 tokens, heads of 128: 132 / 139, 128 / 153, 183 / 209). The limit is still
+//   one tile: raising it is a change to measure and test by itself.
 // More than 128 query heads to a kv head do not fit a tile of whole tokens: paged_attention.cu
 // takes those.
 namespace faq {

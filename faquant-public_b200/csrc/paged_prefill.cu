@@ -23,8 +23,8 @@
 // (then O is rescaled in tensor memory), so a step mostly has no rescaling.
 //
 // Measured (one B200, d = 128): the last 512 of 32768 tokens with 64 query heads on 8 kv heads
-// in 540 us, 1010 TFLOP/s counting the visible pairs (588 us and 928 TFLOP/s in a long series,
-// where the power limit lowers the clocks); all of a 16384-token prompt with 32 heads 1078
+// in 531 us, 1027 TFLOP/s counting the visible pairs (592 to 604 us and some 915 TFLOP/s in a long
+// series, where the power limit lowers the clocks); all of a 16384-token prompt with 32 heads 1078
 // TFLOP/s. The expansion takes 32 us of the first. A key tile takes about 3900 cycles where the
 // products alone need 2048. What bounds it is shared memory: the operands of the four products
 // (2048 cycles at 128 bytes each), P's writes and the arriving K and V (512 each) fill 3072;

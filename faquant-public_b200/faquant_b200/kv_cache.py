@@ -11,6 +11,11 @@ A step is: :meth:`PagedKVCache.extend` (host: pages for the new tokens), then pe
 ``past_key_values=cache`` with ``faquant_attention_kernel = "paged"`` on the attention modules
 runs a Hugging Face Qwen3 on it (``qwen3.attention_forward``); the first layer of a forward
 call opens the step.
+
+A step is not to be captured in a CUDA graph: :meth:`extend` makes the step's device arrays anew, and
+:meth:`attend` gives the step's own lengths as bounds. What a graph needs -- arrays that stay in
+their place, bounds of its last replay, one workspace -- the operators take (``ops.hif4_kv_write``,
+``ops.hif4_paged_attention``), from a caller that keeps them.
 """
 
 from __future__ import annotations
