@@ -453,8 +453,9 @@ int faq_hif4_kv_read(const void* pages, int64_t num_pages, int64_t page_stride, 
  * batch beyond them is either computed all the same or sets FAQ_STATUS_BAD_BOUND and leaves
  * those sequences' rows as they are. cu[batch] may be less than total: the rows of out beyond it
  * are not written, those of q may be read and change nothing. A sequence's result depends on its own
- * queries and keys and on the batch's cu and lens (which cut the work), to the last bit. `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes, 256-byte
- * aligned, not initialized (null where that is 0).
+ * queries and keys, scale, and the batch's cu, lens and bounds (which choose the kernel and cut the
+ * work), to the last bit. `workspace`: at least faq_hif4_paged_attention_workspace_bytes(...) bytes,
+ * 256-byte aligned, not initialized (null where that is 0).
  */
 size_t faq_hif4_paged_attention_workspace_bytes(int64_t total, int64_t heads, int64_t kv_heads, int64_t batch,
                                                 int64_t max_new, int64_t max_len, int64_t total_len, int d);
