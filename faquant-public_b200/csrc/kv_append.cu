@@ -1,0 +1,314 @@
+// K11 -- appending to the HiF4 K/V cache with everything that stands between the projections and
+// the cache: per new token at position p of its sequence
+//
+//   q' = bf16( had( rope_p( norm(q) ) * s ) ),   K = HiF4( had( (rope_p(norm(k)) - offset) / s ) ),   V = HiF4(v)
+//
+//   norm(x) = x / sqrt(mean x^2 + eps) * w over a head's d channels,
+//   rope_p(x) = (a c - b t, b c + a t) for the halves (a, b) of x and row p of the tables (c, t),
+//   had = the Hadamard transform over d (Sylvester's order) / sqrt(d),
+//
+// each step optional. The composition of faq_qk_norm_rope_prep and faq_hif4_kv_write rounds
+// to bf16 after every step, as the modules it replaces do because they store there; here nothing is stored in
+// between, so nothing is rounded: q is computed in fp32 and rounded once, and a key in fp64,
+// rounded once to the fp32 that the fit of HiF4 takes. Codes jump where a value passes a border
+// of the fit, so with fp32 sums a key's bits would depend on the order of their terms; from fp64
+// they are those of the formula, whichever kernel writes them (drafts written again, a prompt in chunks).
+//
+// Mapping: eight lanes per row of a head, lane s with channels 8 s .. of each group of 64, as the
+// fit wants them. The strides 1, 2, 4 of the transform are in a lane, 8, 16, 32 across lanes, 64 is
+// between a lane's groups, and a half's partner is the other group's channel (d = 128) or four lanes
+// away (d = 64). The first blocks of the grid take half a block of keys and values per warp as
+// kv_write_kernel does, the others one token's rows of q, four at a time.
+#include "kv_pages.cuh"
+
+namespace faq {
+namespace kvp {
+
+struct TurnParams {
+  const void *q_norm, *k_norm;  // [d] or null
+  bool norm_f32;                // fp32, else bf16
+  double eps;
+  const void *cos, *sin;        // [rope_rows, >= d / 2] or null
+  bool rope_f32;
+  int64_t rope_ld, rope_rows;
+  const float* offset;          // [kv_heads, d] or null
+  const float* smooth;          // [d] or [kv_heads, d] or null
+  int64_t smooth_head_stride;
+  bool rotate;
+};
+
+struct AppendParams {
+  WriteParams w;
+  TurnParams t;
+  const void* q;
+  int64_t qt, qh;  // token, head strides
+  __nv_bfloat16* out;
+  int64_t ot, oh;
+  int heads, group;  // query heads, per kv head
+  int hpw;           // query heads of a warp's item
+  int64_t kv_blocks; // blocks of the grid that write K and V
+};
+
+// Eight consecutive entries of a table, fp32 or bf16 (any alignment of its type).
+__device__ __forceinline__ void load8(const void* base, bool f32, int64_t at, float (&v)[8]) {
+  if (f32) {
+    const float* p = static_cast<const float*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[i];
+  } else {
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+  }
+}
+
+__device__ __forceinline__ float rsqrt_of(float x) { return rsqrtf(x); }
+__device__ __forceinline__ double rsqrt_of(double x) { return rsqrt(x); }
+
+// A row's position-dependent entries of one lane.
+struct Angles {
+  float c[8], s[8];
+  __device__ __forceinline__ void load(const TurnParams& t, int64_t pos, int lane_of_row, int ng) {
+    const int64_t at = pos * t.rope_ld + 8 * (ng == 2 ? lane_of_row : lane_of_row & 3);
+    load8(t.cos, t.rope_f32, at, c);
+    load8(t.sin, t.rope_f32, at, s);
+  }
+};
+
+// norm, rotation, offset, smoothing and transform of the lane's part of a row; all lanes take part.
+// `divide`: a key's smoothing; `head` is the kv head.
+template <typename R, int NG, bool KEY>
+__device__ __forceinline__ void turn_row(R (&x)[NG][8], const TurnParams& t, const void* norm, const Angles& a, int head,
+                                         int s) {
+  constexpr int D = 64 * NG;
+  if (norm != nullptr) {
+    R sum = 0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[g][i] * x[g][i];
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const R r = rsqrt_of(sum * (R(1) / D) + static_cast<R>(t.eps));
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float w[8];
+      load8(norm, t.norm_f32, 64 * g + 8 * s, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] = x[g][i] * r * static_cast<R>(w[i]);
+    }
+  }
+  if (t.cos != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const R c = a.c[i], n = a.s[i];
+      if constexpr (NG == 2) {
+        const R u = x[0][i], v = x[1][i];
+        x[0][i] = u * c - v * n;
+        x[1][i] = v * c + u * n;
+      } else {
+        const R other = __shfl_xor_sync(0xffffffffu, x[0][i], 4);
+        x[0][i] = x[0][i] * c + (s & 4 ? other : -other) * n;
+      }
+    }
+  }
+  if (KEY && t.offset != nullptr) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] -= t.offset[head * D + 64 * g + 8 * s + i];
+  }
+  if (t.smooth != nullptr) {
+    const float* m = t.smooth + head * t.smooth_head_stride + 8 * s;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] = KEY ? x[g][i] / static_cast<R>(m[64 * g + i]) : x[g][i] * m[64 * g + i];
+  }
+  if (t.rotate) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((i & d) == 0) {
+            const R u = x[g][i], v = x[g][i + d];
+            x[g][i] = u + v;
+            x[g][i + d] = u - v;
+          }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const R other = __shfl_xor_sync(0xffffffffu, x[g][i], o);
+          x[g][i] = (s & o) ? other - x[g][i] : x[g][i] + other;
+        }
+    }
+    const R unit = NG == 2 ? static_cast<R>(0.08838834764831843) : static_cast<R>(0.125);  // 1 / sqrt(d)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (NG == 2) {
+        const R u = x[0][i], v = x[1][i];
+        x[0][i] = (u + v) * unit;
+        x[1][i] = (u - v) * unit;
+      } else {
+        x[0][i] *= unit;
+      }
+    }
+  }
+}
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(32 * WRITE_WARPS) kv_append_kernel(AppendParams a, bool vec, bool out_vec) {
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const WriteParams& w = a.w;
+  const Pages& p = w.p;
+  const TurnParams& t = a.t;
+  const int lane = threadIdx.x & 31, s = lane & 7;
+  if (blockIdx.x < a.kv_blocks) {
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * WRITE_WARPS + (threadIdx.x >> 5);
+    const int h = static_cast<int>(item & 1);
+    const int64_t slot = (item >> 1) / p.kv_heads;
+    const int head = static_cast<int>((item >> 1) - slot * p.kv_heads);
+    Slot x;
+    if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;  // warp-uniform
+    if (t.cos != nullptr && x.pos + x.to > t.rope_rows) {  // tokens beyond the tables are not written
+      atomicOr(&g_status, FAQ_STATUS_BAD_BOUND);
+      x.to = static_cast<int>(t.rope_rows > x.pos ? t.rope_rows - x.pos : 0);
+    }
+    if (x.from >= 8 * (h + 1) || x.to <= 8 * h || x.from >= x.to) return;
+    const int64_t page = page_of(p, x.b, x.pos);
+    if (page < 0) return;
+    write_half_block<T, NG>(w, x, h, lane, static_cast<const T*>(w.k) + x.token * w.kt + head * w.kh + 8 * s,
+                            static_cast<const T*>(w.v) + x.token * w.vt + head * w.vh + 8 * s,
+                            p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, x.pos),
+                            p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, x.pos), vec,
+                            [&](float (&v)[NG][8], int r) {
+                              if (t.k_norm == nullptr && t.cos == nullptr && t.offset == nullptr && t.smooth == nullptr && !t.rotate)
+                                return;
+                              double y[NG][8];
+                              Angles ang;
+                              if (t.cos != nullptr) ang.load(t, x.pos + min(max(r, x.from), x.to - 1), s, NG);
+#pragma unroll
+                              for (int g = 0; g < NG; ++g)
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) y[g][i] = v[g][i];
+                              turn_row<double, NG, true>(y, t, t.k_norm, ang, head, s);
+#pragma unroll
+                              for (int g = 0; g < NG; ++g)
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) v[g][i] = __double2float_rn(y[g][i]);
+                            });
+    return;
+  }
+  // ---- q: heads h0 .. of one token, four at a time
+  const int64_t items = (a.heads + a.hpw - 1) / a.hpw;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) - a.kv_blocks) * WRITE_WARPS + (threadIdx.x >> 5);
+  const int64_t token = item / items;
+  if (token >= w.total) return;
+  int b;
+  int64_t pos;
+  if (!find_token(p, token, w.total, b, pos)) return;  // reported where its keys would be written
+  const int h_begin = static_cast<int>(item - token * items) * a.hpw, h_end = min(h_begin + a.hpw, a.heads);
+  const bool placed = pos >= 0 && (t.cos == nullptr || pos < t.rope_rows);
+  Angles ang;
+  if (t.cos != nullptr && placed) ang.load(t, pos, s, NG);
+  for (int h0 = h_begin; h0 < h_end; h0 += 4) {
+    const bool live = h0 + (lane >> 3) < h_end;
+    const int h = live ? h0 + (lane >> 3) : h_begin;  // idle rows redo a live one, unstored
+    const T* src = static_cast<const T*>(a.q) + token * a.qt + h * a.qh + 8 * s;
+    Raw<T> raw[NG];
+    float x[NG][8];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) raw[g].load(src + 64 * g, vec);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) raw[g].values(x[g]);
+    turn_row<float, NG, false>(x, t, t.q_norm, ang, h / a.group, s);
+    if (!live) continue;
+    __nv_bfloat16* dst = a.out + token * a.ot + h * a.oh + 8 * s;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[g][2 * i], x[g][2 * i + 1]);
+        o[i] = placed ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+      }
+      store_pairs(dst + 64 * g, out_vec, o);
+    }
+  }
+}
+
+}  // namespace kvp
+}  // namespace faq
+
+extern "C" int faq_hif4_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t total, int64_t heads,
+                                  int64_t kv_heads, int d, int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                                  int64_t v_head_stride, const void* q_norm, const void* k_norm, int norm_dtype,
+                                  double eps, const void* cos, const void* sin, int rope_dtype, int64_t rope_ld,
+                                  int64_t rope_rows, const float* key_offset, const float* smooth,
+                                  int64_t smooth_head_stride, int rotate, void* out, int64_t out_token_stride,
+                                  int64_t out_head_stride, void* pages, int64_t num_pages, int64_t page_stride,
+                                  int page_size, const int32_t* table, int64_t table_ld, int64_t table_cols,
+                                  const int32_t* cu, const int32_t* lens, int64_t batch, int k_levels, int v_levels,
+                                  void* stream) {
+  using namespace faq;
+  using namespace faq::kvp;
+  AppendParams a;
+  WriteParams& w = a.w;
+  const int rc = make_pages(w.p, pages, num_pages, page_stride, page_size, kv_heads, d, table, table_ld, table_cols, cu,
+                            lens, batch);
+  if (rc) return rc;
+  FAQ_CHECK_ARG(total >= 0 && total < (int64_t(1) << 31), "bad token count");
+  FAQ_CHECK_ARG(heads > 0 && heads < (int64_t(1) << 24) && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
+  if (total == 0) return FAQ_OK;
+  FAQ_CHECK_ARG(q && k && v && out, "null pointer");
+  FAQ_CHECK_ARG(dtype == FAQ_BF16 || dtype == FAQ_F32, "dtype must be FAQ_BF16 or FAQ_F32");
+  FAQ_CHECK_ARG((norm_dtype == FAQ_BF16 || norm_dtype == FAQ_F32) && (rope_dtype == FAQ_BF16 || rope_dtype == FAQ_F32),
+                "dtype of a table must be FAQ_BF16 or FAQ_F32");
+  FAQ_CHECK_ARG((cos == nullptr) == (sin == nullptr), "cos and sin go together");
+  FAQ_CHECK_ARG(cos == nullptr || (rope_ld >= d / 2 && rope_rows > 0), "cos and sin must be [positions, >= d / 2]");
+  FAQ_CHECK_ARG((q_norm == nullptr && k_norm == nullptr) || (eps >= 0.0 && eps < 1e30), "eps must not be negative");
+  FAQ_CHECK_ARG(smooth_head_stride == 0 || smooth_head_stride == d, "smooth is [d] or [kv_heads, d]");
+  for (const int lv : {k_levels, v_levels})
+    FAQ_CHECK_ARG(lv == 123 || lv == 12 || lv == 13, "levels must be 123/12/13");
+  w.k = k;
+  w.v = v;
+  w.total = total;
+  w.kt = k_token_stride;
+  w.kh = k_head_stride;
+  w.vt = v_token_stride;
+  w.vh = v_head_stride;
+  w.k_levels = k_levels;
+  w.v_levels = v_levels;
+  a.t = {q_norm, k_norm, norm_dtype == FAQ_F32, eps, cos, sin, rope_dtype == FAQ_F32, rope_ld, rope_rows,
+         key_offset, smooth, smooth_head_stride, rotate != 0};
+  a.q = q;
+  a.qt = q_token_stride;
+  a.qh = q_head_stride;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ot = out_token_stride;
+  a.oh = out_head_stride;
+  a.heads = static_cast<int>(heads);
+  a.group = static_cast<int>(heads / kv_heads);
+  const int unit = dtype == FAQ_BF16 ? 8 : 4;  // elements of 16 bytes
+  bool vec = aligned16(q) && aligned16(k) && aligned16(v);
+  for (const int64_t st : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride})
+    vec = vec && st % unit == 0;
+  const bool out_vec = aligned16(out) && out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
+  const int ng = d / 64;
+  a.kv_blocks = (2 * slots_of(total, batch) * kv_heads + WRITE_WARPS - 1) / WRITE_WARPS;
+  // a warp takes more of a token's heads where there are more items than the SMs hold at once
+  const int64_t iters = (heads + 3) / 4, resident = static_cast<int64_t>(num_sms()) * 32;
+  a.hpw = 4 * static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(iters, total * iters / resident)));
+  const int64_t q_blocks = (total * ((heads + a.hpw - 1) / a.hpw) + WRITE_WARPS - 1) / WRITE_WARPS;
+  FAQ_CHECK_ARG(a.kv_blocks + q_blocks < (int64_t(1) << 31), "too many tokens for one call");
+  auto kern = dtype == FAQ_BF16 ? (ng == 1 ? kv_append_kernel<__nv_bfloat16, 1> : kv_append_kernel<__nv_bfloat16, 2>)
+                                : (ng == 1 ? kv_append_kernel<float, 1> : kv_append_kernel<float, 2>);
+  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(a.kv_blocks + q_blocks)), 32 * WRITE_WARPS, 0, stream, a, vec,
+                        out_vec));
+  return launch_status("kv_append_kernel");
+}

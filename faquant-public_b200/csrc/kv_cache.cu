@@ -156,27 +156,14 @@ __device__ __forceinline__ bool find_slot(const Pages& p, int64_t slot, int64_t 
   return true;
 }
 
-// A warp takes half a block (8 tokens): its loads are then all in flight at once.
-constexpr int WRITE_WARPS = 4;
-template <typename T, int NG>
-__global__ void __launch_bounds__(32 * WRITE_WARPS, sizeof(T) == 2 ? 8 : 4) kv_write_kernel(WriteParams w, bool vec) {
-  grid_dependency_wait();
-  allow_dependent_launch();
-  const Pages& p = w.p;
-  const int lane = threadIdx.x & 31, s = lane & 7;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * WRITE_WARPS + (threadIdx.x >> 5);
-  const int h = static_cast<int>(item & 1);
-  const int64_t slot = (item >> 1) / p.kv_heads;
-  const int head = static_cast<int>((item >> 1) - slot * p.kv_heads);
-  Slot x;
-  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;  // warp-uniform
-  if (x.from >= 8 * (h + 1) || x.to <= 8 * h) return;
-  const int64_t page = page_of(p, x.b, x.pos);
-  if (page < 0) return;
-  uint8_t* kdst = p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, x.pos);
-  uint8_t* vdst = p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, x.pos);
-  const T* ksrc = static_cast<const T*>(w.k) + x.token * w.kt + head * w.kh + 8 * s;
-  const T* vsrc = static_cast<const T*>(w.v) + x.token * w.vt + head * w.vh + 8 * s;
+// Quantizes the live tokens of half a block, h, to their places: kdst and vdst are the block of one
+// head's K and V, ksrc and vsrc the lane's first channels of the block's first token. turn(v,
+// r), called by the whole warp, may change the lane's 8 NG values of K of the block's token r
+// before they are quantized.
+template <typename T, int NG, typename Turn>
+__device__ __forceinline__ void write_half_block(const WriteParams& w, const Slot& x, int h, int lane, const T* ksrc,
+                                                 const T* vsrc, uint8_t* kdst, uint8_t* vdst, bool vec, Turn&& turn) {
+  const int s = lane & 7;
   const int pr = (lane >> 3) + 4 * h;  // tokens 2 pr, 2 pr + 1 of the block
   const bool live[2] = {2 * pr >= x.from && 2 * pr < x.to, 2 * pr + 1 >= x.from && 2 * pr + 1 < x.to};
   Raw<T> rk[2][NG], rv[2][NG];
@@ -198,12 +185,15 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS, sizeof(T) == 2 ? 8 : 4) kv_w
     const int r = 2 * pr + k;
     if (!__any_sync(0xffffffffu, live[k])) continue;  // a step of one token per sequence
     uint32_t kw[NG], kx[NG], kscale = 0, vscale = 0;
+    float kv[NG][8];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) rk[k][g].values(kv[g]);
+    turn(kv, r);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float v[8];
       uint32_t ea, eb, sc;
-      rk[k][g].values(v);
-      kw[g] = quantize8(v, w.k_levels, ea, eb, sc);
+      kw[g] = quantize8(kv[g], w.k_levels, ea, eb, sc);
       kx[g] = (ea | (eb << 16)) << (2 * s);
       kscale |= sc << (8 * g);
       rv[k][g].values(v);
@@ -269,6 +259,30 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS, sizeof(T) == 2 ? 8 : 4) kv_w
       }
     }
   }
+}
+
+// A warp takes half a block (8 tokens): its loads are then all in flight at once.
+constexpr int WRITE_WARPS = 4;
+template <typename T, int NG>
+__global__ void __launch_bounds__(32 * WRITE_WARPS, sizeof(T) == 2 ? 8 : 4) kv_write_kernel(WriteParams w, bool vec) {
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const Pages& p = w.p;
+  const int lane = threadIdx.x & 31, s = lane & 7;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * WRITE_WARPS + (threadIdx.x >> 5);
+  const int h = static_cast<int>(item & 1);
+  const int64_t slot = (item >> 1) / p.kv_heads;
+  const int head = static_cast<int>((item >> 1) - slot * p.kv_heads);
+  Slot x;
+  if (slot >= slots_of(w.total, p.batch) || !find_slot(p, slot, w.total, x)) return;  // warp-uniform
+  if (x.from >= 8 * (h + 1) || x.to <= 8 * h) return;
+  const int64_t page = page_of(p, x.b, x.pos);
+  if (page < 0) return;
+  write_half_block<T, NG>(w, x, h, lane, static_cast<const T*>(w.k) + x.token * w.kt + head * w.kh + 8 * s,
+                          static_cast<const T*>(w.v) + x.token * w.vt + head * w.vh + 8 * s,
+                          p.base + page * p.page_stride + block_in_page<NG>(p, 0, head, x.pos),
+                          p.base + page * p.page_stride + block_in_page<NG>(p, 1, head, x.pos), vec,
+                          [](float (&)[NG][8], int) {});
 }
 
 struct ReadParams {

@@ -62,6 +62,25 @@ __device__ __forceinline__ void check_rows(const Pages& p, int b, int64_t total)
   if (c0 < 0 || c1 < c0 || c1 > total) atomicOr(&g_status, FAQ_STATUS_BAD_BOUND);
 }
 
+// check_rows of every sequence, by one CTA of a grid over tokens (which sees no token of some of them).
+__device__ __forceinline__ void check_batch(const Pages& p, int64_t total, int tid, int threads) {
+  for (int b = tid; b < p.batch; b += threads) check_rows(p, b, total);
+}
+
+// The sequence and position of packed token `token` (< total); false where it belongs to no
+// sequence whose new tokens lie in the `total` given rows.
+__device__ __forceinline__ bool find_token(const Pages& p, int64_t token, int64_t total, int& b, int64_t& pos) {
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu[mid] <= token) lo = mid; else hi = mid;
+  }
+  b = lo;
+  const int c0 = p.cu[lo], c1 = p.cu[lo + 1];
+  pos = static_cast<int64_t>(p.lens[lo]) - c1 + token;
+  return c0 >= 0 && c0 <= token && token < c1 && c1 <= total;
+}
+
 // Length of sequence b, at most what its table row can hold (a longer one is recorded).
 __device__ __forceinline__ int length_of(const Pages& p, int b) {
   const int len = p.lens[b], most = p.table_cols << p.page_shift;

@@ -82,6 +82,17 @@ SIGNATURES: dict[str, list] = {
                                  _i64, _c_void_p, ctypes.c_size_t, _c_void_p],
     "faq_verify_drafts": [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p,
                           _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "faq_hif4_kv_append": [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64,
+                           _c_void_p, _c_void_p, _int, ctypes.c_double, _c_void_p, _c_void_p, _int, _i64, _i64, _c_void_p,
+                           _c_void_p, _i64, _int, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _int, _c_void_p, _i64,
+                           _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p],
+    "faq_hif4_key_bounds": [_c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
+                            _i64, _c_void_p, _c_void_p],
+    "faq_hif4_select_pages": [_c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _int, _i64, _int, _c_void_p, _i64, _i64,
+                              _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "faq_hif4_sparse_attention": [_c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64, _int, _i64, _int, _c_void_p,
+                                  _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, ctypes.c_float, _c_void_p,
+                                  _i64, _i64, _c_void_p],
     "faq_selftest_wait_timeout": [_i64, _c_void_p],
     "faq_selftest_ex2_monotone": [ctypes.POINTER(ctypes.c_uint64), _c_void_p],
     "faq_device_trace": [ctypes.POINTER(ctypes.c_uint), _int, _int],

@@ -722,6 +722,12 @@ def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: to
             inner *= n
     if not whole:
         raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
+    return ((pages.data_ptr(), shape[0], page_stride, page_size), _batch(table, cu, lens))
+
+
+def _batch(table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor) -> tuple:
+    """Checks of the arrays that describe a ragged batch. Returns the C calls' ``(table, row
+    stride, columns, cu, lens, batch)``."""
     int32 = torch.int32
     if table.dtype is not int32 or cu.dtype is not int32 or lens.dtype is not int32:
         raise TypeError("table, cu and lens must be int32")
@@ -737,8 +743,7 @@ def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: to
             ld = columns  # a single row may have any stride
     if not (cu.is_contiguous() and lens.is_contiguous()):
         raise ValueError("cu and lens must be contiguous")
-    return ((pages.data_ptr(), shape[0], page_stride, page_size),
-            (table.data_ptr(), ld, columns, cu.data_ptr(), lens.data_ptr(), batch))
+    return table.data_ptr(), ld, columns, cu.data_ptr(), lens.data_ptr(), batch
 
 
 def _kv_heads(pages: torch.Tensor, head_dim: int, page_size: int) -> int:
@@ -882,6 +887,237 @@ def hif4_paged_attention(
     _lib.call("faq_hif4_paged_attention", q.data_ptr(), total, heads, qs[0], qs[1], *pool, h, d, *ragged, max_new, max_len,
               total_len, d**-0.5 if scale is None else float(scale), out.data_ptr(), os_[0], os_[1],
               workspace.data_ptr() if need else None, need, _stream(device))
+    return out
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """A C call for ``device``'s tensors, whichever device is the current one."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with unit stride in its last dimension."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def hif4_kv_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    rotate: bool = False,
+    smooth_scale: torch.Tensor | None = None,
+    key_offset: torch.Tensor | None = None,
+    levels: tuple[str | int, str | int] = ("123", "123"),
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """From the projections' ``q [T, H, D]`` and ``k``/``v [T, Hkv, D]`` (bf16 or fp32, D 64 or 128, any token
+    and head strides) to the cache and the attention's queries in one pass
+    (``faq_hif4_kv_append``): per-head RMSNorm (``q_norm``/``k_norm [D]``), the rotation of each token's
+    position, Smooth-QK (``q * smooth_scale``, ``(k - key_offset) / smooth_scale``; ``[D]`` or ``[Hkv, D]``, ``key_offset
+    [Hkv, D]``), the Hadamard transform over D (``rotate``), each where given. K and V are quantized and written to
+    their ``pages`` as :func:`hif4_kv_write` does (``table``, ``cu``, ``lens``, ``levels`` as there); the queries
+    are returned in bf16 ``[T, H, D]`` (in ``out`` where given; it may be ``q`` itself).
+
+    ``cos``/``sin [positions, D / 2]`` (or ``[positions, D]``, of which the first half is read; bf16 or fp32) hold
+    a row per position: the first channel half a and the second b become ``a cos - b sin`` and ``b cos + a sin``.
+    Nothing is rounded between the steps: q is computed in fp32, k in fp64 and rounded to fp32 for the fit, so
+    a key's bits do not depend on the step in which it was written. A token without a place (a position below
+    zero, or beyond the tables, which sets ``FAQ_STATUS_BAD_BOUND``) is not written, its row of q is zero;
+    rows beyond ``cu[B]`` stay as they are."""
+    device = _require_cuda(q, k, v, pages, table, cu, lens, cos, sin, q_norm, k_norm, smooth_scale, key_offset, out)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must have one dtype")
+    total, heads, d = q.shape
+    h = k.shape[1]
+    pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
+    if h == 0 or heads % h or heads == 0:
+        raise ValueError("query heads must be divisible by key/value heads")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    norms = [n for n in (q_norm, k_norm) if n is not None]
+    for n in norms:
+        if n.shape != (d,) or n.dtype != norms[0].dtype:
+            raise ValueError("q_norm and k_norm must be [head_dim] tensors of one dtype")
+    norm_dtype = _dtype_code(norms[0]) if norms else _lib.FAQ_F32
+    q_norm, k_norm = (None if n is None else n.contiguous() for n in (q_norm, k_norm))
+    rope_dtype, rope_ld, rope_rows = _lib.FAQ_F32, 0, 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] not in (d // 2, d) or cos.dtype != sin.dtype:
+            raise ValueError("cos and sin must be [positions, head_dim / 2] or [positions, head_dim], of one dtype")
+        if cos.stride(1) != 1 or cos.stride() != sin.stride() or cos.stride(0) < d // 2:
+            cos, sin = cos.contiguous(), sin.contiguous()
+        rope_dtype, rope_ld, rope_rows = _dtype_code(cos), max(cos.stride(0), d // 2), cos.shape[0]
+    smooth_stride = 0
+    if smooth_scale is not None:
+        if smooth_scale.shape not in ((d,), (h, d)):
+            raise ValueError("smooth_scale must be [head_dim] or [kv_heads, head_dim]")
+        smooth_stride = d if smooth_scale.dim() == 2 else 0
+        smooth_scale = smooth_scale.to(torch.float32).contiguous()
+    if key_offset is not None:
+        if key_offset.shape != (h, d):
+            raise ValueError("key_offset must be [kv_heads, head_dim]")
+        key_offset = key_offset.to(torch.float32).contiguous()
+    if out is None:
+        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    _call_on(device, "faq_hif4_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), total, heads, h, d, qs[0],
+             qs[1], ks[0], ks[1], vs[0], vs[1], _ptr(q_norm), _ptr(k_norm), norm_dtype, float(eps), _ptr(cos), _ptr(sin),
+             rope_dtype, rope_ld, rope_rows, _ptr(key_offset), _ptr(smooth_scale), smooth_stride, int(rotate),
+             out.data_ptr(), os_[0], os_[1], *pool, *ragged, levels_code(levels[0]), levels_code(levels[1]), _stream(device))
+    return out
+
+
+def hif4_bounds_bytes(head_dim: int) -> int:
+    """Bytes of the bounds of one page's keys of one kv head (:func:`hif4_key_bounds`)."""
+    if head_dim not in (64, 128):
+        raise ValueError("head_dim must be 64 or 128")
+    return 2 * head_dim + 16
+
+
+def hif4_key_bounds(
+    pages: torch.Tensor,
+    bounds: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    total: int,
+) -> None:
+    """The bounds of the keys of every page that the batch's new tokens lie in, anew from the page's tokens
+    below ``lens`` (``faq_hif4_key_bounds``): ``bounds`` uint8 ``[num_pages, Hkv, hif4_bounds_bytes(D)]``, per
+    page and kv head the least and the greatest value of each channel, in 8 bits with one exponent,
+    rounded outward. Call it after the tokens are written (:func:`hif4_kv_append`, :func:`hif4_kv_write`) and before
+    :func:`hif4_select_pages`. ``total`` is a host number, at least ``cu[B]``."""
+    device = _require_cuda(pages, bounds, table, cu, lens)
+    h, d = _bounds_shape(bounds)
+    pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
+    if bounds.shape[0] != pool[1]:
+        raise ValueError("pages and bounds must have one number of pages")
+    _call_on(device, "faq_hif4_key_bounds", *pool, h, d, *ragged, total, bounds.data_ptr(), _stream(device))
+
+
+def _bounds_shape(bounds: torch.Tensor) -> tuple[int, int]:
+    """``(kv_heads, head_dim)`` of a bounds tensor."""
+    if bounds.dtype is not torch.uint8 or bounds.dim() != 3 or not bounds.is_contiguous():
+        raise TypeError("bounds must be a contiguous uint8 tensor [num_pages, kv_heads, hif4_bounds_bytes(head_dim)]")
+    d = (bounds.shape[2] - 16) // 2
+    if d not in (64, 128) or bounds.shape[2] != hif4_bounds_bytes(d):
+        raise ValueError("bounds must be [num_pages, kv_heads, hif4_bounds_bytes(head_dim)]")
+    return bounds.shape[1], d
+
+
+def hif4_select_pages(
+    q: torch.Tensor,
+    bounds: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    *,
+    page_size: int,
+    count: int,
+    first: int = 1,
+    last: int = 2,
+    want_scores: bool = False,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """The pages that each new token attends to: int32 ``[T, Hkv, count]``, columns of the sequence's row of
+    ``table`` in ascending order, -1 behind them (``faq_hif4_select_pages``). ``q [T, H, D]`` bf16 are the queries
+    of the attention, ``bounds`` those of :func:`hif4_key_bounds`.
+
+    A page's score is the greatest ``q . K`` that its bounds allow, ``sum_d max(q_d lo_d, q_d hi_d)``, the greatest over
+    the query heads of the kv head, with q in 8 bits (one exponent for the kv head's queries): whole numbers, so the
+    choice is exact. Taken are the sequence's ``first`` pages, the ``last`` ones up to the token's own (at
+    least one), then those of the greatest scores, ties to the lowest column. Pages that the table does not hold
+    are not taken and set ``FAQ_STATUS_BAD_PAGE``; entries of q that are not finite count as zero. With
+    ``want_scores`` returns ``(selected, scores)``, scores fp32 of the same shape, -inf behind the pages. Rows
+    beyond ``cu[B]`` stay as they are. At most 32768 columns and 128 query heads per kv head."""
+    device = _require_cuda(q, bounds, table, cu, lens, out)
+    if q.dtype is not torch.bfloat16 or q.dim() != 3:
+        raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
+    total, heads, d = q.shape
+    h, bd = _bounds_shape(bounds)
+    if bd != d or h == 0 or heads % h or heads == 0:
+        raise ValueError("q's heads must be divisible by the kv heads of the bounds, of one head_dim")
+    hif4_page_bytes(h, d, page_size)
+    ragged = _batch(table, cu, lens)
+    q = _unit(q)
+    shape = (total, h, count)
+    if out is None:
+        if count < 1:
+            raise ValueError("count must be positive")
+        out = torch.empty(shape, dtype=torch.int32, device=device)
+    elif out.shape != shape or out.dtype is not torch.int32 or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int32 tensor [tokens, kv_heads, count]")
+    scores = torch.empty(shape, dtype=torch.float32, device=device) if want_scores else None
+    _call_on(device, "faq_hif4_select_pages", q.data_ptr(), total, heads, q.stride(0), q.stride(1), bounds.data_ptr(),
+             bounds.shape[0], page_size, h, d, *ragged, count, first, last, out.data_ptr(), _ptr(scores), _stream(device))
+    return (out, scores) if want_scores else out
+
+
+def hif4_sparse_attention(
+    q: torch.Tensor,
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cu: torch.Tensor,
+    lens: torch.Tensor,
+    selected: torch.Tensor,
+    *,
+    page_size: int,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each new token over the tokens of the pages listed for it: ``q [T, H, D]`` bf16, returns
+    ``[T, H, D]`` bf16 (``faq_hif4_sparse_attention``). ``selected`` int32 ``[T, Hkv, count]``
+    (:func:`hif4_select_pages`) holds columns of the sequence's row of ``table``, in any order; entries below zero and
+    pages behind the token are passed over, a column listed twice counts twice, and no token sees keys behind
+    itself. With every visible page listed this is :func:`hif4_paged_attention`, up to the rounding of its sums.
+    A row without a key is zero; rows beyond ``cu[B]`` stay as they are; pages that the table does not hold are
+    left out and set ``FAQ_STATUS_BAD_PAGE``."""
+    device = _require_cuda(q, pages, table, cu, lens, selected, out)
+    if q.dtype is not torch.bfloat16 or q.dim() != 3:
+        raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
+    total, heads, d = q.shape
+    h = _kv_heads(pages, d, page_size)
+    pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
+    if heads % h or heads == 0:
+        raise ValueError("query heads must be divisible by key/value heads")
+    if selected.dtype is not torch.int32 or selected.dim() != 3 or selected.shape[:2] != (total, h):
+        raise ValueError("selected must be int32 [tokens, kv_heads, count]")
+    selected = selected.contiguous()
+    qs = q.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        qs = (heads * d, d)
+    if out is None:
+        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+    _call_on(device, "faq_hif4_sparse_attention", q.data_ptr(), total, heads, qs[0], qs[1], *pool, h, d, *ragged,
+             selected.data_ptr(), selected.shape[2], d**-0.5 if scale is None else float(scale), out.data_ptr(),
+             out.stride(0), out.stride(1), _stream(device))
     return out
 
 

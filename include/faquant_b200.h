@@ -485,6 +485,77 @@ int faq_verify_drafts(const int64_t* draft_tokens, const void* target_probs, con
                       const float* accept_u, const float* sample_u, const int32_t* num_drafts, int64_t* tokens,
                       int32_t* accepted, void* stream);
 
+/*
+ * K11 -- from the projections to the paged cache (no counterpart in the reference): per new token
+ * at position p of its sequence, with every step optional,
+ *   out = bf16(had(rope_p(norm(q)) * s)),  K = HiF4(had((rope_p(norm(k)) - offset) / s)),  V = HiF4(v)
+ *   norm(x) = x / sqrt(mean x^2 + eps) * w per head; rope_p(a, b) = (a c - b t, b c + a t) on the
+ *   channel halves with row p of the tables cos and sin; had: the Hadamard transform over d / sqrt(d).
+ * q [total, heads, d], k and v [total, kv_heads, d] of one dtype (bf16 or fp32; token and head
+ * strides in elements, d contiguous); q_norm, k_norm [d] (norm_dtype; null: no norm); cos, sin
+ * [rope_rows, >= d / 2] with row stride rope_ld (rope_dtype; null: no rotation), row p of
+ * position p; key_offset fp32 [kv_heads, d] or null; smooth fp32 [d] (smooth_head_stride 0) or
+ * [kv_heads, d] (smooth_head_stride d) or null: q heads times it, keys divided by it; rotate:
+ * the Hadamard transform. out bf16 [total, heads, d]; it may be q. q is computed in fp32 and rounded
+ * once; K in fp64 and rounded to fp32, which faq_hif4_kv_write's fit takes: a key's bits are those of
+ * the formula, whatever the batch. The batch, the pages and their errors are as in
+ * faq_hif4_kv_write; further, a token at a position of rope_rows or more is not written and sets
+ * FAQ_STATUS_BAD_BOUND. The rows of out of tokens without a place (there, or below zero) are zero; those of
+ * sequences that are left out and those beyond cu[batch] are not written.
+ */
+int faq_hif4_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t total, int64_t heads,
+                       int64_t kv_heads, int d, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void* q_norm,
+                       const void* k_norm, int norm_dtype, double eps, const void* cos, const void* sin, int rope_dtype,
+                       int64_t rope_ld, int64_t rope_rows, const float* key_offset, const float* smooth,
+                       int64_t smooth_head_stride, int rotate, void* out, int64_t out_token_stride,
+                       int64_t out_head_stride, void* pages, int64_t num_pages, int64_t page_stride, int page_size,
+                       const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
+                       const int32_t* lens, int64_t batch, int k_levels, int v_levels, void* stream);
+
+/*
+ * K12 -- the pages a token attends to. `bounds` [num_pages][kv_heads][2 d + 16] bytes, 16-byte aligned:
+ * the least and the greatest key of each channel over a page's tokens, floor(lo / 2^e) and ceil(hi /
+ * 2^e) as int8 [d] each, then e as int8 (the least that holds them in -127 .. 127; 0 for a page of
+ * zeros) and 15 zero bytes. faq_hif4_key_bounds makes them anew, from the tokens below lens, for every page that
+ * the batch's new tokens (at most `total`) lie in; call it after they are written.
+ *
+ * faq_hif4_select_pages takes, per token and kv head, the sequence's `first` pages, the `last` ones
+ * up to the token's own (at least one; first + last <= count) and those of the greatest scores, ties to the lowest
+ * column, `count` in all where there are as many: selected int32 [total, kv_heads, count], columns of the table
+ * in ascending order, then -1; scores fp32 of the same shape (or null), then -infinity. The score of a
+ * page is max over the kv head's query heads of sum_d (q_d >= 0 ? q_d hi_d : q_d lo_d), where q (bf16, as
+ * in K9; any strides) stands for the whole numbers round(q / 2^f) (ties to even), f the least that holds the
+ * kv head's in -127 .. 127, times 2^f; what is not finite in q counts as zero. The sums are whole numbers
+ * times powers of two, exact in fp32. Columns without a page are not taken and set FAQ_STATUS_BAD_PAGE.
+ * Rows beyond cu[batch] are not written; a token below position zero has -1 only. table_cols is at
+ * most 32768, heads / kv_heads at most 128 (FAQ_ERR_UNSUPPORTED).
+ */
+int faq_hif4_key_bounds(const void* pages, int64_t num_pages, int64_t page_stride, int page_size, int64_t kv_heads, int d,
+                        const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
+                        const int32_t* lens, int64_t batch, int64_t total, void* bounds, void* stream);
+int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
+                          const void* bounds, int64_t num_pages, int page_size, int64_t kv_heads, int d,
+                          const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* cu,
+                          const int32_t* lens, int64_t batch, int64_t count, int64_t first, int64_t last,
+                          int32_t* selected, float* scores, void* stream);
+
+/*
+ * K13 -- K9's attention over listed pages only: selected int32 [total, kv_heads, count] holds columns
+ * of the token's sequence's row of the table, one list per kv head, in any order. Entries below zero and
+ * pages behind the token are passed over, a column listed twice counts twice, keys behind the token are not
+ * seen; an entry whose page is missing is left out and sets FAQ_STATUS_BAD_PAGE. q, out and scale as in
+ * faq_hif4_paged_attention (which a list of every page equals, up to the rounding of the sums). A row without a key is
+ * zero; rows beyond cu[batch] are not written. No workspace. A row's bits depend on its own queries,
+ * keys and list, scale, count, and through the split of the work on total, heads and kv_heads.
+ */
+int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride,
+                              int64_t q_head_stride, const void* pages, int64_t num_pages, int64_t page_stride,
+                              int page_size, int64_t kv_heads, int d, const int32_t* table, int64_t table_ld,
+                              int64_t table_cols, const int32_t* cu, const int32_t* lens, int64_t batch,
+                              const int32_t* selected, int64_t count, float scale, void* out, int64_t out_token_stride,
+                              int64_t out_head_stride, void* stream);
+
 /* Diagnostics: copy up to max_records records of the waits that gave up (3 words
  * each: site | tile << 8, blockIdx.x | blockIdx.y << 16, blockIdx.z) into `records`
  * (host memory); returns the number of timeouts recorded (>= 0) or -FAQ_ERR_*.
