@@ -526,6 +526,26 @@ static cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads,
   return cudaLaunchKernelEx(&cfg, kernel, given...);
 }
 
+// The same in clusters of `cluster` CTAs.
+template <typename... Args, typename... Given>
+static cudaError_t launch_clusters(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int cluster, void* stream,
+                                   Given... given) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, given...);
+}
+
 }  // namespace kvp
 }  // namespace faq
 

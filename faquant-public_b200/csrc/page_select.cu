@@ -12,8 +12,10 @@
 // q in 8 bits too (one exponent for the group, so that its heads can be compared) the sums are
 // whole numbers below 2^21 times 2^e: exact in fp32 in any order, so that the same pages
 // are taken by every kernel, batch and split.
+// The products of 16 pages with 8 query heads are mma.sync m16n8k32 of 8-bit numbers, [lo | hi] times
+// [negative | positive entries of q], whose lanes load 16 bytes of a page's row each.
 // Selection. The first pages and the token's last ones, then the greatest scores, ties to the
-// lowest column: a search for the count-th greatest key byte by byte, then one pass in order.
+// lowest column: a search for the count-th greatest key, then one pass in order.
 #include "kv_pages.cuh"
 
 namespace faq {
@@ -163,11 +165,17 @@ struct SelectParams {
   int count, first, last;
   int32_t* out;   // [total, kv_heads, count]
   float* scores;  // the same, or null
+  int slots;      // log2 of the columns of a product that a token's heads take: 3 to 0
+  int key_ld;     // keys of a token in shared memory
+  bool vec;       // q can be read 16 bytes at a time
 };
 
-constexpr int SELECT_THREADS = 256;
+constexpr int SELECT_WARPS = 8, SELECT_THREADS = 32 * SELECT_WARPS;
 constexpr int MAX_COLUMNS = 32768;  // pages of a sequence whose keys fit in shared memory
 constexpr int MAX_GROUP = 128;
+constexpr int WARP_COLUMNS = 1024;  // keys that one warp searches
+constexpr int SELECT_KEY_BYTES = 96 << 10;  // of a CTA whose warps have a token each: two to an SM
+constexpr int HELD = 16;            // keys of a lane that it holds in registers while it searches
 
 // The greatest-first order of fp32 as an order of whole numbers; 0 and 2^32 - 1 are no number's.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -178,106 +186,231 @@ __device__ __forceinline__ float number_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// One CTA per token and kv head.
+__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight query heads in 8 bits, as the B operand of the products with the pages' bounds: column
+// lane / 4, and per 64 bytes of the bounds [lo | hi] the lane's 16 from 16 (lane % 4) on; lo meets
+// the negative entries, hi the others. (The order of the channels in a product is free.)
 template <int NG>
-__global__ void __launch_bounds__(SELECT_THREADS) select_pages_kernel(SelectParams w) {
-  constexpr int D = 64 * NG, LANES = D / 16;  // lanes of a page: 16 channels each
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ int s_hist[256], s_part[2][SELECT_THREADS / 32], s_found[2];
-  __shared__ float s_top[SELECT_THREADS / 32];
-  const Pages& p = w.p;
-  int8_t* s_q = reinterpret_cast<int8_t*>(smem);  // [group][positive, negative][D]
-  uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + 2 * w.group * D);
-  grid_dependency_wait();
-  allow_dependent_launch();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t token = blockIdx.x / p.kv_heads;
-  const int head = static_cast<int>(blockIdx.x - token * p.kv_heads);
-  int b;
-  int64_t pos;
-  if (blockIdx.x == 0) check_batch(p, w.total, tid, SELECT_THREADS);
-  if (!find_token(p, token, w.total, b, pos)) return;
-  const int64_t list = (token * p.kv_heads + head) * w.count;
-  int32_t* out = w.out + list;
-  float* scores = w.scores == nullptr ? nullptr : w.scores + list;
-  int columns = 0;
-  if (pos >= 0) {
-    columns = static_cast<int>(std::min<int64_t>((pos >> p.page_shift) + 1, p.table_cols));
-    if (tid == 0 && (pos >> p.page_shift) >= p.table_cols) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
-  }
-
-  // ---- q of the group in 8 bits
-  const __nv_bfloat16* q = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
-  float top = 0.0f;
-  for (int i = tid; i < w.group * D; i += SELECT_THREADS) {
-    const float a = fabsf(__bfloat162float(q[(i / D) * w.qh + i % D]));
-    if (a < INFINITY) top = fmaxf(top, a);
-  }
+struct Query {
+  uint4 b[2 * NG];
+  int e;  // the exponent of the lane's column
+  // rows: the lane's column's query, heads stride `step` apart to further passes; `slots` as above
+  __device__ __forceinline__ float top_of(const __nv_bfloat16* row, int lane, bool vec) const {
+    float top = 0.0f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) s_top[warp] = top;
-  if (tid < 2) s_found[tid] = 0;
-  __syncthreads();
+    for (int j = 0; j < 2 * NG; ++j) {
+      Raw<__nv_bfloat16> r;
+      float v[8];
+      r.load(row + 64 * (j >> 1) + 16 * (lane & 3) + 8 * (j & 1), vec);
+      r.values(v);
 #pragma unroll
-  for (int k = 0; k < SELECT_THREADS / 32; ++k) top = fmaxf(top, s_top[k]);
-  const int eq = shared_exponent(top);
-  for (int i = tid; i < w.group * D; i += SELECT_THREADS) {
-    float a = __bfloat162float(q[(i / D) * w.qh + i % D]);
-    if (!(fabsf(a) < INFINITY)) a = 0.0f;  // what is not finite does not count
-    const int n = __float2int_rn(ldexpf(a, -eq));
-    s_q[(i / D) * 2 * D + i % D] = static_cast<int8_t>(max(n, 0));
-    s_q[(i / D) * 2 * D + D + i % D] = static_cast<int8_t>(min(n, 0));
-  }
-  __syncthreads();
-
-  // ---- the pages' keys
-  const int32_t* row = p.table + b * p.table_ld;
-  int have = 0;  // pages that can be taken, of this thread's lane groups
-  const int sub = lane % LANES;
-  for (int c0 = warp * (32 / LANES); c0 < columns; c0 += SELECT_THREADS / LANES) {  // warp-uniform
-    const int c = c0 + lane / LANES;
-    const int page = c < columns ? row[c] : -1;
-    const bool ok = page >= 0 && page < p.num_pages;
-    if (c < columns && !ok) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
-    const uint8_t* src = w.bounds + (static_cast<int64_t>(ok ? page : 0) * p.kv_heads + head) * bounds_bytes(D);
-    const int4 lo = *reinterpret_cast<const int4*>(src + 16 * sub), hi = *reinterpret_cast<const int4*>(src + D + 16 * sub);
-    const int e = static_cast<int8_t>(src[2 * D]);
-    int best = INT32_MIN;
-    for (int g = 0; g < w.group; ++g) {
-      const int4 a = *reinterpret_cast<const int4*>(s_q + g * 2 * D + 16 * sub);
-      const int4 n = *reinterpret_cast<const int4*>(s_q + g * 2 * D + D + 16 * sub);
-      int sum = __dp4a(a.x, hi.x, __dp4a(n.x, lo.x, 0));
-      sum = __dp4a(a.y, hi.y, __dp4a(n.y, lo.y, sum));
-      sum = __dp4a(a.z, hi.z, __dp4a(n.z, lo.z, sum));
-      sum = __dp4a(a.w, hi.w, __dp4a(n.w, lo.w, sum));
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      best = max(best, sum);
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
     }
-    if (sub == 0 && c < columns) {
-      s_key[c] = ok ? order_key(static_cast<float>(best) * pow2f(min(max(e, -100), 100))) : 0;
-      have += ok;
+    return top;
+  }
+  __device__ __forceinline__ void round(const __nv_bfloat16* row, int lane, bool vec) {
+    const float u0 = pow2f(-(e / 2)), u1 = pow2f(e / 2 - e);  // 2^-e passes fp32's range
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      uint32_t pos[4], neg[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        Raw<__nv_bfloat16> r;
+        float v[8];
+        r.load(row + 64 * j + 16 * (lane & 3) + 8 * h, vec);
+        r.values(v);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t x = 0, y = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = v[4 * w + i];
+            const int n = fabsf(a) < INFINITY ? __float2int_rn(a * u0 * u1) : 0;  // what is not finite does not count
+            x |= static_cast<uint32_t>(max(n, 0) & 255) << (8 * i);
+            y |= static_cast<uint32_t>(min(n, 0) & 255) << (8 * i);
+          }
+          pos[2 * h + w] = x;
+          neg[2 * h + w] = y;
+        }
+      }
+      b[j] = make_uint4(neg[0], neg[1], neg[2], neg[3]);
+      b[NG + j] = make_uint4(pos[0], pos[1], pos[2], pos[3]);
     }
   }
-  atomicAdd(&s_found[0], have);
-  __syncthreads();
+};
 
-  auto rank = [&](int c) -> uint32_t {
-    const uint32_t key = s_key[c];
-    return key != 0 && (c < w.first || c >= columns - w.last) ? 0xFFFFFFFFu : key;
+// The keys of 16 pages from column c0 on (of `columns`) for the eight columns of `q`: key(slot, c,
+// value) is called for column c and the tokens' slots (0 .. 7 >> slots) with each its greatest score, or 0
+// for a page that is not there.
+template <int NG, typename F>
+__device__ __forceinline__ void score_pages(const SelectParams& w, const int32_t* row, int head, const Query<NG>& q, int c0,
+                                            int columns, int lane, F&& key) {
+  constexpr int D = 64 * NG;
+  const int g = lane >> 2, t = lane & 3;
+  uint4 a[2][2 * NG];
+  bool ok[2];
+  int e[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = c0 + g + 8 * h, page = c < columns ? row[c] : -1;
+    ok[h] = page >= 0 && page < w.p.num_pages;
+    if (c < columns && !ok[h]) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
+    const uint8_t* src = w.bounds + (static_cast<int64_t>(ok[h] ? page : 0) * w.p.kv_heads + head) * bounds_bytes(D);
+#pragma unroll
+    for (int j = 0; j < 2 * NG; ++j) a[h][j] = *reinterpret_cast<const uint4*>(src + 64 * j + 16 * t);
+    e[h] = static_cast<int8_t>(src[2 * D]);
+  }
+  int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 2 * NG; ++j) {
+    mma_s8_16832(acc, a[0][j].x, a[1][j].x, a[0][j].y, a[1][j].y, q.b[j].x, q.b[j].y);
+    mma_s8_16832(acc, a[0][j].z, a[1][j].z, a[0][j].w, a[1][j].w, q.b[j].z, q.b[j].w);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = c0 + g + 8 * h;
+    const float unit = pow2f(min(max(e[h], -100), 100));
+    int v0 = acc[2 * h], v1 = acc[2 * h + 1];
+    if (w.slots > 0) v0 = max(v0, v1);
+    if (w.slots > 1) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
+    if (w.slots > 2) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
+    if (c >= columns) continue;
+    if (w.slots == 0) {
+      key(2 * t, c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+      key(2 * t + 1, c, ok[h] ? order_key(static_cast<float>(v1) * unit) : 0u);
+    } else if ((t & ((1 << (w.slots - 1)) - 1)) == 0) {
+      key(t >> (w.slots - 1), c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+    }
+  }
+}
+
+// What a token's search knows.
+struct Wanted {
+  int columns;  // visible pages
+  int count, first, last;
+  __device__ __forceinline__ bool forced(int c) const { return c < first || c >= columns - last; }
+};
+
+// One warp: the count-th greatest of the keys bit by bit, then one pass in order. The keys of
+// pages that are always taken do not take part in the search.
+__device__ __forceinline__ void take_by_warp(const uint32_t* keys, const Wanted& w, int eq, int32_t* out, float* scores,
+                                             int lane) {
+  uint32_t held[HELD];
+  const bool few = w.columns <= 32 * HELD;
+  uint32_t top = 0, low = 0xFFFFFFFFu;
+  int always = 0, others = 0;
+  auto look = [&](int c) -> uint32_t {  // 0: not a choice
+    const uint32_t key = c < w.columns ? keys[c] : 0;
+    const bool f = w.forced(c);
+    always += key != 0 && f;
+    others += key != 0 && !f;
+    return f ? 0 : key;
   };
-  // ---- the count-th greatest key, and how many of its equals are taken
-  uint32_t limit = 1;  // every page that is there
-  int ties = s_found[0];
-  if (s_found[0] > w.count) {
+  if (few) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      held[i] = look(32 * i + lane);
+      top = max(top, held[i]);
+      if (held[i]) low = min(low, held[i]);
+    }
+  } else {
+    for (int c = lane; c < w.columns; c += 32) {
+      const uint32_t key = look(c);
+      top = max(top, key);
+      if (key) low = min(low, key);
+    }
+  }
+  always = __reduce_add_sync(0xffffffffu, always);
+  others = __reduce_add_sync(0xffffffffu, others);
+  const int need = max(w.count - always, 0);
+  // taken are the keys above the limit and the first `ties` of those equal to it
+  uint32_t limit = 0;
+  int ties = 0;
+  if (need == 0) {
+    limit = 0xFFFFFFFFu;
+  } else if (others > need) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    int bit = 31 - __clz(top ^ low);  // the keys agree above it; -1: they are one
+    uint32_t found = bit < 0 ? top : top & ~((2u << bit) - 1);
+    int above = 0;
+    bool exact = false;
+    for (; bit >= 0; --bit) {
+      const uint32_t at = found | (1u << bit);
+      int n = 0;
+      if (few) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) n += held[i] >= at;
+      } else {
+        for (int c = lane; c < w.columns; c += 32) n += !w.forced(c) && keys[c] >= at;
+      }
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n >= need) found = at; else above = n;
+      if (n == need) {
+        exact = true;
+        break;
+      }
+    }
+    limit = exact ? found - 1 : found;
+    ties = exact ? 0 : need - above;
+  }
+  int at = 0, equal = 0;
+  const uint32_t below = (1u << lane) - 1;
+  for (int c0 = 0; c0 < w.columns; c0 += 32) {
+    const int c = c0 + lane;
+    const uint32_t key = c < w.columns ? keys[c] : 0;
+    const bool f = w.forced(c), same = key != 0 && !f && key == limit;
+    const uint32_t vs = __ballot_sync(0xffffffffu, same);
+    const bool take = key != 0 && (f || key > limit || (same && equal + __popc(vs & below) < ties));
+    const uint32_t vt = __ballot_sync(0xffffffffu, take);
+    const int mine = at + __popc(vt & below);
+    if (take && mine < w.count) {
+      out[mine] = c;
+      if (scores != nullptr) scores[mine] = ldexpf(number_of(key), eq);
+    }
+    at += __popc(vt);
+    equal += __popc(vs);
+  }
+  for (int i = min(at, w.count) + lane; i < w.count; i += 32) {
+    out[i] = -1;
+    if (scores != nullptr) scores[i] = -INFINITY;
+  }
+}
+
+// The same by a CTA, byte by byte.
+__device__ void take_by_cta(const uint32_t* keys, const Wanted& w, int eq, int32_t* out, float* scores) {
+  __shared__ int s_hist[256], s_part[2][SELECT_WARPS], s_found[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto rank = [&](int c) -> uint32_t {
+    const uint32_t key = keys[c];
+    return key != 0 && w.forced(c) ? 0xFFFFFFFFu : key;
+  };
+  if (tid == 0) s_found[0] = 0;
+  __syncthreads();
+  int have = 0;
+  for (int c = tid; c < w.columns; c += SELECT_THREADS) have += keys[c] != 0;
+  have = __reduce_add_sync(0xffffffffu, have);
+  if (lane == 0) atomicAdd(&s_found[0], have);
+  __syncthreads();
+  uint32_t limit = 0;  // taken are the keys above it and the first `ties` of its equals
+  int ties = 0;
+  const bool search = s_found[0] > w.count;
+  if (search) {
     int need = w.count;
-    uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
       s_hist[tid] = 0;
       __syncthreads();
-      for (int c = tid; c < columns; c += SELECT_THREADS) {
+      for (int c = tid; c < w.columns; c += SELECT_THREADS) {
         const uint32_t key = rank(c);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255], 1);
+        if (shift == 24 || (key >> (shift + 8)) == (limit >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255], 1);
       }
       __syncthreads();
       if (warp == 0) {  // lane l: the bins 255 - 8 l .. 248 - 8 l, from the greatest down
@@ -287,35 +420,36 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_kernel(SelectPara
           n[i] = s_hist[255 - 8 * lane - i];
           sum += n[i];
         }
-        int upto = sum;
+        int before = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += y;
+          const int y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
         }
-        int before = upto - sum;
-        if (before < need && need <= upto) {  // one lane's
-          int i = 0;
-          while (before + n[i] < need) before += n[i++];
-          s_found[0] = 255 - 8 * lane - i;
+        before -= sum;
+        if (before < need && need <= before + sum) {  // one lane's
+          int bin = -1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (bin < 0 && before + n[i] >= need) bin = i;
+            if (bin < 0) before += n[i];
+          }
+          s_found[0] = 255 - 8 * lane - bin;
           s_found[1] = need - before;
         }
       }
       __syncthreads();
-      prefix |= static_cast<uint32_t>(s_found[0]) << shift;
+      limit |= static_cast<uint32_t>(s_found[0]) << shift;
       need = s_found[1];
       __syncthreads();
     }
-    limit = prefix;
     ties = need;
   }
-
-  // ---- one pass in order: those above the limit, and the first of its equals
   int done = 0, equal = 0;
-  for (int c0 = 0; c0 < columns; c0 += SELECT_THREADS) {
+  for (int c0 = 0; c0 < w.columns; c0 += SELECT_THREADS) {
     const int c = c0 + tid;
-    const uint32_t key = c < columns ? rank(c) : 0;
-    const bool above = limit == 1 ? key != 0 : key > limit, same = limit != 1 && key == limit;
+    const uint32_t key = c < w.columns ? rank(c) : 0;
+    const bool above = key > limit, same = search && key == limit;
     const uint32_t va = __ballot_sync(0xffffffffu, above), vs = __ballot_sync(0xffffffffu, same);
     if (lane == 0) {
       s_part[0][warp] = __popc(va);
@@ -323,29 +457,145 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_kernel(SelectPara
     }
     __syncthreads();
     int a = done, s = equal;
-    for (int k = 0; k < warp; ++k) {
-      a += s_part[0][k];
-      s += s_part[1][k];
+    for (int k = 0; k < SELECT_WARPS; ++k) {
+      if (k < warp) {
+        a += s_part[0][k];
+        s += s_part[1][k];
+      }
+      done += s_part[0][k];
+      equal += s_part[1][k];
     }
     const uint32_t below = (1u << lane) - 1;
     a += __popc(va & below);
     s += __popc(vs & below);
-    if (above || (same && s < ties)) {
-      const int at = a + min(s, ties);
-      if (at < w.count) {
-        out[at] = c;
-        if (scores != nullptr) scores[at] = ldexpf(number_of(s_key[c]), eq);
-      }
-    }
-    for (int k = 0; k < SELECT_THREADS / 32; ++k) {
-      done += s_part[0][k];
-      equal += s_part[1][k];
+    const int at = a + min(s, ties);
+    if ((above || (same && s < ties)) && at < w.count) {
+      out[at] = c;
+      if (scores != nullptr) scores[at] = ldexpf(number_of(keys[c]), eq);
     }
     __syncthreads();
   }
   for (int i = min(done + min(equal, ties), w.count) + tid; i < w.count; i += SELECT_THREADS) {
     out[i] = -1;
     if (scores != nullptr) scores[i] = -INFINITY;
+  }
+}
+
+// The exponent of column lane / 4's token, from its heads' greatest magnitudes: `passes` times 8 of them.
+template <int NG>
+__device__ __forceinline__ int query_exponent(const Query<NG>& q, const SelectParams& w, const __nv_bfloat16* heads, int first,
+                                              int lane) {
+  float top = 0.0f;
+  for (int h = first; h < w.group; h += 8) top = fmaxf(top, q.top_of(heads + h * w.qh, lane, w.vec));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  for (int o = 0; o < w.slots; ++o) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4 << o));
+  return shared_exponent(top);
+}
+
+// Few rows: a cluster of `split` CTAs per token and kv head. Their warps score the pages in turn; the keys
+// meet in the first CTA, which searches them.
+template <int NG>
+__global__ void __launch_bounds__(SELECT_THREADS) select_pages_cta_kernel(SelectParams w, int split) {
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  const Pages& p = w.p;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (split > 1) cluster_sync();  // the first CTA is there to be written to
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const int rank = static_cast<int>(blockIdx.x % split);
+  const int64_t unit = blockIdx.x / split, token = unit / p.kv_heads;
+  const int head = static_cast<int>(unit - token * p.kv_heads);
+  if (blockIdx.x == 0) check_batch(p, w.total, tid, SELECT_THREADS);
+  int b;
+  int64_t pos;
+  if (!find_token(p, token, w.total, b, pos)) return;  // the whole cluster
+  Wanted want = {0, w.count, w.first, w.last};
+  if (pos >= 0) {
+    want.columns = static_cast<int>(std::min<int64_t>((pos >> p.page_shift) + 1, p.table_cols));
+    if (tid == 0 && (pos >> p.page_shift) >= p.table_cols) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
+  }
+  const __nv_bfloat16* heads = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
+  const int32_t* row = p.table + b * p.table_ld;
+  const uint32_t dst = split > 1 ? mapa_shared(smem_addr(s_keys), 0) : smem_addr(s_keys);
+  Query<NG> q;
+  q.e = query_exponent(q, w, heads, min(lane >> 2, w.group - 1), lane);
+  for (int h = 0; h < w.group; h += 8) {
+    q.round(heads + min(h + (lane >> 2), w.group - 1) * w.qh, lane, w.vec);
+    for (int c0 = 16 * (warp + SELECT_WARPS * rank); c0 < want.columns; c0 += 16 * SELECT_WARPS * split)
+      score_pages(w, row, head, q, c0, want.columns, lane, [&](int, int c, uint32_t key) {
+        const uint32_t at = dst + 4 * c;  // a column's passes are one warp's
+        if (h > 0) {
+          uint32_t old;
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(old) : "r"(at) : "memory");
+          key = max(key, old);
+        }
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(key) : "memory");
+      });
+  }
+  if (split > 1) cluster_sync(); else __syncthreads();
+  if (rank > 0) return;
+  const int64_t list = unit * w.count;
+  int32_t* out = w.out + list;
+  float* scores = w.scores == nullptr ? nullptr : w.scores + list;
+  if (want.columns > WARP_COLUMNS)
+    take_by_cta(s_keys, want, q.e, out, scores);
+  else if (warp == 0)
+    take_by_warp(s_keys, want, q.e, out, scores, lane);
+}
+
+// Many rows: a warp per kv head and (8 >> slots) tokens, whose heads share the products with a page.
+template <int NG>
+__global__ void __launch_bounds__(SELECT_THREADS) select_pages_warp_kernel(SelectParams w) {
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  const Pages& p = w.p;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_wait();
+  allow_dependent_launch();
+  if (blockIdx.x == 0) check_batch(p, w.total, tid, SELECT_THREADS);
+  const int tokens = 8 >> w.slots;
+  const int64_t block = blockIdx.x / p.kv_heads, token0 = (block * SELECT_WARPS + warp) * tokens;
+  const int head = static_cast<int>(blockIdx.x - block * p.kv_heads);
+  uint32_t* keys = s_keys + static_cast<int64_t>(warp) * tokens * w.key_ld;
+  const int mine = lane >> 2 >> w.slots;  // the token of the lane's column
+  int done = 0;  // tokens of the group that have been looked at
+  while (done < tokens && token0 + done < w.total) {
+    // a run of tokens of one sequence
+    int b;
+    int64_t pos;
+    const bool placed = find_token(p, token0 + done, w.total, b, pos);
+    if (!placed) {
+      ++done;
+      continue;
+    }
+    const int run = static_cast<int>(std::min<int64_t>(p.cu[b + 1] - (token0 + done), tokens - done));
+    const int64_t last = pos + run - 1;
+    const int columns = last < 0 ? 0 : static_cast<int>(std::min<int64_t>((last >> p.page_shift) + 1, p.table_cols));
+    if (lane == 0 && last >= 0 && (last >> p.page_shift) >= p.table_cols) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
+    const int64_t token = token0 + min(max(mine, done), done + run - 1);  // columns of other tokens repeat one of the run
+    const __nv_bfloat16* heads = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
+    const int32_t* row = p.table + b * p.table_ld;
+    Query<NG> q;
+    const int column = (lane >> 2) & ((1 << w.slots) - 1);
+    q.e = query_exponent(q, w, heads, min(column, w.group - 1), lane);
+    for (int h = 0; h < w.group; h += 8) {
+      q.round(heads + min(h + column, w.group - 1) * w.qh, lane, w.vec);
+      for (int c0 = 0; c0 < columns; c0 += 16)
+        score_pages(w, row, head, q, c0, columns, lane, [&](int slot, int c, uint32_t key) {
+          uint32_t* at = keys + static_cast<int64_t>(slot) * w.key_ld + c;
+          *at = h > 0 ? max(key, *at) : key;
+        });
+    }
+    __syncwarp();
+    for (int i = done; i < done + run; ++i) {
+      const int64_t at = pos + i - done, list = ((token0 + i) * p.kv_heads + head) * w.count;
+      const Wanted want = {at < 0 ? 0 : static_cast<int>(std::min<int64_t>((at >> p.page_shift) + 1, p.table_cols)), w.count,
+                           w.first, w.last};
+      take_by_warp(keys + static_cast<int64_t>(i) * w.key_ld, want, __shfl_sync(0xffffffffu, q.e, i << w.slots << 2),
+                   w.out + list, w.scores == nullptr ? nullptr : w.scores + list, lane);
+    }
+    __syncwarp();
+    done += run;
   }
 }
 
@@ -395,7 +645,7 @@ extern "C" int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads
                 "count must hold the first pages and the last ones, of which there is at least one");
   if (total == 0) return FAQ_OK;
   FAQ_CHECK_ARG(q && selected, "null pointer");
-  FAQ_CHECK_ARG(total * kv_heads < (int64_t(1) << 31), "too many tokens for one call");
+  FAQ_CHECK_ARG(total * kv_heads < (int64_t(1) << 28), "too many tokens for one call");
   w.bounds = static_cast<const uint8_t*>(bounds);
   w.q = static_cast<const __nv_bfloat16*>(q);
   w.qt = q_token_stride;
@@ -407,12 +657,33 @@ extern "C" int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads
   w.last = static_cast<int>(last);
   w.out = selected;
   w.scores = scores;
-  const int bytes = 2 * w.group * d + 4 * static_cast<int>(table_cols);
-  auto kern = d == 64 ? select_pages_kernel<1> : select_pages_kernel<2>;
-  static std::atomic<uint64_t> set[2];
-  const int most = 2 * MAX_GROUP * d + 4 * MAX_COLUMNS;
-  const int rs = allow_smem(reinterpret_cast<const void*>(kern), most, set[d == 64 ? 0 : 1]);
+  w.vec = aligned16(q) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
+  const int64_t units = total * kv_heads;
+  static std::atomic<uint64_t> set[4];  // devices on which the kernels' shared memory is set
+  // Many rows, and room for the keys of a CTA's warps: a warp each, whose heads of several tokens share a
+  // product.
+  int slots = 0;
+  while (slots < 3 && (1 << slots) < w.group) ++slots;
+  const int64_t keys = (SELECT_WARPS * 8 >> slots) * table_cols;
+  if (units << slots >= 64 * static_cast<int64_t>(num_sms()) && 4 * keys <= SELECT_KEY_BYTES) {
+    w.slots = slots;
+    w.key_ld = static_cast<int>(table_cols);
+    const int64_t tokens = SELECT_WARPS * 8 >> slots;
+    auto kern = d == 64 ? select_pages_warp_kernel<1> : select_pages_warp_kernel<2>;
+    const int rs = allow_smem(reinterpret_cast<const void*>(kern), SELECT_KEY_BYTES, set[d == 64 ? 0 : 1]);
+    if (rs) return rs;
+    FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>((total + tokens - 1) / tokens * kv_heads)), SELECT_THREADS,
+                          4 * static_cast<size_t>(keys), stream, w));
+    return launch_status("select_pages_warp_kernel");
+  }
+  // a CTA for every 128 columns (16 to a warp) as far as there are SMs
+  int split = 1;
+  while (split < 8 && 2 * split * units <= num_sms() && table_cols > 16 * SELECT_WARPS * split) split *= 2;
+  w.slots = 3;
+  w.key_ld = static_cast<int>(table_cols);
+  auto kern = d == 64 ? select_pages_cta_kernel<1> : select_pages_cta_kernel<2>;
+  const int rs = allow_smem(reinterpret_cast<const void*>(kern), 4 * MAX_COLUMNS, set[d == 64 ? 2 : 3]);
   if (rs) return rs;
-  FAQ_CUDA(launch_early(kern, dim3(static_cast<unsigned>(total * kv_heads)), SELECT_THREADS, bytes, stream, w));
-  return launch_status("select_pages_kernel");
+  FAQ_CUDA(launch_clusters(kern, units * split, SELECT_THREADS, 4 * static_cast<size_t>(table_cols), split, stream, w, split));
+  return launch_status("select_pages_cta_kernel");
 }

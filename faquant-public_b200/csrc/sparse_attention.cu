@@ -422,20 +422,7 @@ static int launch(const Params& P, int split, void* stream) {
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), bytes, set);
   if (rc) return rc;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(split);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(P.total * P.p.kv_heads * P.passes * split));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 2 : 1;
-  FAQ_CUDA(cudaLaunchKernelEx(&cfg, kern, P, split));
+  FAQ_CUDA(launch_clusters(kern, P.total * P.p.kv_heads * P.passes * split, THREADS, bytes, split, stream, P, split));
   return launch_status("sparse_attention_kernel");
 }
 

@@ -76,23 +76,23 @@ def select(q, keys, lens, new, page, count, first, last, missing=()):
             continue
         columns = pos // page + 1
         for j in range(h):
+            if (b, j) not in known:
+                parts = [page_bounds(part) for part in keys[starts[b] : starts[b] + lens[b], j].split(page)]
+                lo, hi = (torch.stack([x[i] for x in parts]) for i in (0, 1))
+                known[b, j] = lo, hi, torch.tensor([2.0 ** x[2] for x in parts], dtype=torch.float64)
+            lo, hi, unit = (x[:columns] for x in known[b, j])
             row = q[t, j * group : (j + 1) * group].double().cpu()
             row = torch.where(row.isfinite(), row, torch.zeros_like(row))
             f = exponent(float(row.abs().max()))
             row = torch.round(row * 2.0**-f)
-            ranked = []
-            for c in range(columns):
-                if (b, c) in missing:
-                    continue
-                if (b, j, c) not in known:
-                    known[b, j, c] = page_bounds(keys[starts[b] + c * page : starts[b] + min(lens[b], c * page + page), j])
-                lo, hi, e = known[b, j, c]
-                score = float((row.clamp(min=0) @ hi + row.clamp(max=0) @ lo).max()) * 2.0**e
-                forced = c < first or c >= columns - last
-                ranked.append((not forced, -score, c))
-            taken = sorted((c, -s) for _, s, c in sorted(ranked)[:count])
-            for i, (c, s) in enumerate(taken):
-                out[t, j, i], scores[t, j, i] = c, s * 2.0**f
+            score = (row.clamp(min=0) @ hi.T + row.clamp(max=0) @ lo.T).amax(0) * unit
+            rank = score.clone()
+            rank[:first] = rank[max(0, columns - last) :] = math.inf
+            there = [c for c in range(columns) if (b, c) not in missing]
+            best = torch.sort(rank[there], dim=0, descending=True, stable=True).indices[:count].tolist()
+            taken = sorted(there[i] for i in best)
+            out[t, j, : len(taken)] = torch.tensor(taken, dtype=torch.int32)
+            scores[t, j, : len(taken)] = score[taken] * 2.0**f
     return out, scores
 
 
