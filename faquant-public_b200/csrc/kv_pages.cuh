@@ -67,13 +67,16 @@ __device__ __forceinline__ void check_batch(const Pages& p, int64_t total, int t
   for (int b = tid; b < p.batch; b += threads) check_rows(p, b, total);
 }
 
-// The sequence and position of packed token `token` (< total); false where it belongs to no
-// sequence whose new tokens lie in the `total` given rows.
+// The sequence and position of packed token `token` (< total), by a whole warp; false where it
+// belongs to no sequence whose new tokens lie in the `total` given rows.
 __device__ __forceinline__ bool find_token(const Pages& p, int64_t token, int64_t total, int& b, int64_t& pos) {
-  int lo = 0, hi = p.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid] <= token) lo = mid; else hi = mid;
+  int lo = 0, n = p.batch;  // the last of n sequences from lo on that begins at the token or before
+  while (n > 1) {
+    const int step = (n + 31) >> 5, i = static_cast<int>(threadIdx.x & 31) * step;
+    const uint32_t before = __ballot_sync(0xffffffffu, i < n && p.cu[lo + i] <= token);
+    const int k = before ? 31 - __clz(before) : 0;
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   b = lo;
   const int c0 = p.cu[lo], c1 = p.cu[lo + 1];

@@ -173,7 +173,7 @@ struct SelectParams {
 constexpr int SELECT_WARPS = 8, SELECT_THREADS = 32 * SELECT_WARPS;
 constexpr int MAX_COLUMNS = 32768;  // pages of a sequence whose keys fit in shared memory
 constexpr int MAX_GROUP = 128;
-constexpr int WARP_COLUMNS = 1024;  // keys that one warp searches
+constexpr int WARP_COLUMNS = 256;   // keys that one warp searches
 constexpr int SELECT_KEY_BYTES = 96 << 10;  // of a CTA whose warps have a token each: two to an SM
 constexpr int HELD = 16;            // keys of a lane that it holds in registers while it searches
 
@@ -247,50 +247,64 @@ struct Query {
   }
 };
 
-// The keys of 16 pages from column c0 on (of `columns`) for the eight columns of `q`: key(slot, c,
-// value) is called for column c and the tokens' slots (0 .. 7 >> slots) with each its greatest score, or 0
-// for a page that is not there.
-template <int NG, typename F>
-__device__ __forceinline__ void score_pages(const SelectParams& w, const int32_t* row, int head, const Query<NG>& q, int c0,
-                                            int columns, int lane, F&& key) {
-  constexpr int D = 64 * NG;
-  const int g = lane >> 2, t = lane & 3;
+// The bounds of 16 pages from column c0 on as the A operand: rows lane / 4 and 8 further.
+template <int NG>
+struct PageRows {
   uint4 a[2][2 * NG];
-  bool ok[2];
   int e[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = c0 + g + 8 * h, page = c < columns ? row[c] : -1;
-    ok[h] = page >= 0 && page < w.p.num_pages;
-    if (c < columns && !ok[h]) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
-    const uint8_t* src = w.bounds + (static_cast<int64_t>(ok[h] ? page : 0) * w.p.kv_heads + head) * bounds_bytes(D);
-#pragma unroll
-    for (int j = 0; j < 2 * NG; ++j) a[h][j] = *reinterpret_cast<const uint4*>(src + 64 * j + 16 * t);
-    e[h] = static_cast<int8_t>(src[2 * D]);
+  bool ok[2];
+  // entry: the table's entry of column c0 + lane % 16 (-1 from `columns` on), loaded ahead
+  static __device__ __forceinline__ int entry(const int32_t* row, int c0, int columns, int lane) {
+    const int c = c0 + (lane & 15);
+    return c < columns ? row[c] : -1;
   }
-  int acc[4] = {0, 0, 0, 0};
+  __device__ __forceinline__ void load(const SelectParams& w, int head, int entry, int lane) {
+    constexpr int D = 64 * NG;
 #pragma unroll
-  for (int j = 0; j < 2 * NG; ++j) {
-    mma_s8_16832(acc, a[0][j].x, a[1][j].x, a[0][j].y, a[1][j].y, q.b[j].x, q.b[j].y);
-    mma_s8_16832(acc, a[0][j].z, a[1][j].z, a[0][j].w, a[1][j].w, q.b[j].z, q.b[j].w);
-  }
+    for (int h = 0; h < 2; ++h) {
+      const int page = __shfl_sync(0xffffffffu, entry, (lane >> 2) + 8 * h);
+      ok[h] = page >= 0 && page < w.p.num_pages;
+      const uint8_t* src = w.bounds + (static_cast<int64_t>(ok[h] ? page : 0) * w.p.kv_heads + head) * bounds_bytes(D);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = c0 + g + 8 * h;
-    const float unit = pow2f(min(max(e[h], -100), 100));
-    int v0 = acc[2 * h], v1 = acc[2 * h + 1];
-    if (w.slots > 0) v0 = max(v0, v1);
-    if (w.slots > 1) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
-    if (w.slots > 2) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
-    if (c >= columns) continue;
-    if (w.slots == 0) {
-      key(2 * t, c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
-      key(2 * t + 1, c, ok[h] ? order_key(static_cast<float>(v1) * unit) : 0u);
-    } else if ((t & ((1 << (w.slots - 1)) - 1)) == 0) {
-      key(t >> (w.slots - 1), c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+      for (int j = 0; j < 2 * NG; ++j) a[h][j] = *reinterpret_cast<const uint4*>(src + 64 * j + 16 * (lane & 3));
+      e[h] = static_cast<int8_t>(src[2 * D]);
     }
   }
-}
+  // key(slot, c, value) is called, by one lane each, for the columns below `columns` and the tokens' slots
+  // (0 .. 7 >> slots) of `q` with the greatest score of the token's heads, 0 for a page that is not there.
+  template <typename F>
+  __device__ __forceinline__ void score(const SelectParams& w, const Query<NG>& q, int c0, int columns, int lane,
+                                        F&& key) const {
+    const int g = lane >> 2, t = lane & 3;
+    int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 2 * NG; ++j) {
+      mma_s8_16832(acc, a[0][j].x, a[1][j].x, a[0][j].y, a[1][j].y, q.b[j].x, q.b[j].y);
+      mma_s8_16832(acc, a[0][j].z, a[1][j].z, a[0][j].w, a[1][j].w, q.b[j].z, q.b[j].w);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + g + 8 * h;
+      const float unit = pow2f(min(max(e[h], -100), 100));
+      int v0 = acc[2 * h], v1 = acc[2 * h + 1];
+      if (w.slots > 0) v0 = max(v0, v1);
+      if (w.slots > 1) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
+      if (w.slots > 2) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
+      if (c >= columns) continue;
+      if (w.slots == 0) {
+        key(2 * t, c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+        key(2 * t + 1, c, ok[h] ? order_key(static_cast<float>(v1) * unit) : 0u);
+      } else if ((t & ((1 << (w.slots - 1)) - 1)) == 0) {
+        key(t >> (w.slots - 1), c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+      }
+    }
+  }
+  // A page that the table does not hold is reported, once per row of it.
+  __device__ __forceinline__ void report(int c0, int columns, int lane) const {
+    if ((!ok[0] && c0 + (lane >> 2) < columns) || (!ok[1] && c0 + (lane >> 2) + 8 < columns))
+      atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
+  }
+};
 
 // What a token's search knows.
 struct Wanted {
@@ -299,37 +313,68 @@ struct Wanted {
   __device__ __forceinline__ bool forced(int c) const { return c < first || c >= columns - last; }
 };
 
-// One warp: the count-th greatest of the keys bit by bit, then one pass in order. The keys of
-// pages that are always taken do not take part in the search.
-__device__ __forceinline__ void take_by_warp(const uint32_t* keys, const Wanted& w, int eq, int32_t* out, float* scores,
-                                             int lane) {
-  uint32_t held[HELD];
-  const bool few = w.columns <= 32 * HELD;
-  uint32_t top = 0, low = 0xFFFFFFFFu;
+// The `count` greatest keys, bit by bit, by one warp or by all of a CTA (WARPS): warp k has the k-th
+// equal part of the columns, in rounds of 32. The pages that are always taken have no part in the search.
+struct SearchScratch {
+  int sum[2][SELECT_WARPS], part[2][SELECT_WARPS];
+};
+template <int WARPS>
+__device__ __forceinline__ void take(const uint32_t* keys, const Wanted& w, int eq, int32_t* out, float* scores,
+                                     SearchScratch* scratch) {
+  const int lane = threadIdx.x & 31, warp = WARPS > 1 ? threadIdx.x >> 5 : 0;
+  const int rounds = (w.columns + 32 * WARPS - 1) / (32 * WARPS), c0 = warp * rounds * 32 + lane;
+  const bool few = rounds <= HELD;
+  int turn = 0;
+  auto all = [&](int n) {  // the sum over the lanes of all warps
+    n = __reduce_add_sync(0xffffffffu, n);
+    if constexpr (WARPS > 1) {
+      turn ^= 1;
+      if (lane == 0) scratch->sum[turn][warp] = n;
+      __syncthreads();
+      n = 0;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) n += scratch->sum[turn][k];
+    }
+    return n;
+  };
+  uint32_t held[HELD], top = 0, low = 0xFFFFFFFFu;  // of the choices
   int always = 0, others = 0;
-  auto look = [&](int c) -> uint32_t {  // 0: not a choice
-    const uint32_t key = c < w.columns ? keys[c] : 0;
-    const bool f = w.forced(c);
-    always += key != 0 && f;
-    others += key != 0 && !f;
-    return f ? 0 : key;
+  auto choice = [&](int c) -> uint32_t {  // 0: none
+    return c < w.columns && !w.forced(c) ? keys[c] : 0;
   };
   if (few) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      held[i] = look(32 * i + lane);
-      top = max(top, held[i]);
-      if (held[i]) low = min(low, held[i]);
-    }
-  } else {
-    for (int c = lane; c < w.columns; c += 32) {
-      const uint32_t key = look(c);
+    for (int i = 0; i < HELD; ++i) held[i] = i < rounds ? choice(c0 + 32 * i) : 0;
+  }
+  for (int i = 0; i < rounds; ++i) {
+    const int c = c0 + 32 * i;
+    const uint32_t key = c < w.columns ? keys[c] : 0;
+    if (key && w.forced(c)) {
+      ++always;
+    } else if (key) {
+      ++others;
       top = max(top, key);
-      if (key) low = min(low, key);
+      low = min(low, key);
     }
   }
-  always = __reduce_add_sync(0xffffffffu, always);
-  others = __reduce_add_sync(0xffffffffu, others);
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  if constexpr (WARPS > 1) {
+    if (lane == 0) {
+      scratch->part[0][warp] = static_cast<int>(top);
+      scratch->part[1][warp] = static_cast<int>(low);
+    }
+  }
+  const int found_both = all(always | others << 16);  // at most 32768 of the others: their sum passes no bit of 32
+  always = found_both & 0xFFFF;
+  others = static_cast<int>(static_cast<uint32_t>(found_both) >> 16);
+  if constexpr (WARPS > 1) {
+    for (int k = 0; k < WARPS; ++k) {
+      top = max(top, static_cast<uint32_t>(scratch->part[0][k]));
+      low = min(low, static_cast<uint32_t>(scratch->part[1][k]));
+    }
+    __syncthreads();  // the parts are written again
+  }
   const int need = max(w.count - always, 0);
   // taken are the keys above the limit and the first `ties` of those equal to it
   uint32_t limit = 0;
@@ -337,145 +382,68 @@ __device__ __forceinline__ void take_by_warp(const uint32_t* keys, const Wanted&
   if (need == 0) {
     limit = 0xFFFFFFFFu;
   } else if (others > need) {
-    top = __reduce_max_sync(0xffffffffu, top);
-    low = __reduce_min_sync(0xffffffffu, low);
-    int bit = 31 - __clz(top ^ low);  // the keys agree above it; -1: they are one
-    uint32_t found = bit < 0 ? top : top & ~((2u << bit) - 1);
+    const int first_bit = 31 - __clz(top ^ low);  // the keys agree above it; -1: they are one
+    uint32_t found = first_bit < 0 ? top : top & ~((2u << first_bit) - 1);
     int above = 0;
     bool exact = false;
-    for (; bit >= 0; --bit) {
+    for (int bit = first_bit; bit >= 0 && !exact; --bit) {
       const uint32_t at = found | (1u << bit);
       int n = 0;
       if (few) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i) n += held[i] >= at;
       } else {
-        for (int c = lane; c < w.columns; c += 32) n += !w.forced(c) && keys[c] >= at;
+        for (int i = 0; i < rounds; ++i) n += choice(c0 + 32 * i) >= at;
       }
-      n = __reduce_add_sync(0xffffffffu, n);
+      n = all(n);
       if (n >= need) found = at; else above = n;
-      if (n == need) {
-        exact = true;
-        break;
-      }
+      exact = n == need;
     }
     limit = exact ? found - 1 : found;
     ties = exact ? 0 : need - above;
   }
+  // where this warp's part of the list begins
   int at = 0, equal = 0;
+  if constexpr (WARPS > 1) {
+    int sure = 0, same = 0;
+    for (int i = 0; i < rounds; ++i) {
+      const int c = c0 + 32 * i;
+      const uint32_t key = c < w.columns ? keys[c] : 0;
+      const bool f = w.forced(c);
+      sure += key != 0 && (f || key > limit);
+      same += key != 0 && !f && key == limit;
+    }
+    sure = __reduce_add_sync(0xffffffffu, sure);
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (lane == 0) {
+      scratch->part[0][warp] = sure;
+      scratch->part[1][warp] = same;
+    }
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) {
+      at += scratch->part[0][k];
+      equal += scratch->part[1][k];
+    }
+    at += min(equal, ties);
+  }
   const uint32_t below = (1u << lane) - 1;
-  for (int c0 = 0; c0 < w.columns; c0 += 32) {
-    const int c = c0 + lane;
+  for (int i = 0; i < rounds; ++i) {
+    const int c = c0 + 32 * i;
     const uint32_t key = c < w.columns ? keys[c] : 0;
     const bool f = w.forced(c), same = key != 0 && !f && key == limit;
     const uint32_t vs = __ballot_sync(0xffffffffu, same);
-    const bool take = key != 0 && (f || key > limit || (same && equal + __popc(vs & below) < ties));
-    const uint32_t vt = __ballot_sync(0xffffffffu, take);
+    const bool taken = key != 0 && (f || key > limit || (same && equal + __popc(vs & below) < ties));
+    const uint32_t vt = __ballot_sync(0xffffffffu, taken);
     const int mine = at + __popc(vt & below);
-    if (take && mine < w.count) {
+    if (taken && mine < w.count) {
       out[mine] = c;
       if (scores != nullptr) scores[mine] = ldexpf(number_of(key), eq);
     }
     at += __popc(vt);
     equal += __popc(vs);
   }
-  for (int i = min(at, w.count) + lane; i < w.count; i += 32) {
-    out[i] = -1;
-    if (scores != nullptr) scores[i] = -INFINITY;
-  }
-}
-
-// The same by a CTA, byte by byte.
-__device__ void take_by_cta(const uint32_t* keys, const Wanted& w, int eq, int32_t* out, float* scores) {
-  __shared__ int s_hist[256], s_part[2][SELECT_WARPS], s_found[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto rank = [&](int c) -> uint32_t {
-    const uint32_t key = keys[c];
-    return key != 0 && w.forced(c) ? 0xFFFFFFFFu : key;
-  };
-  if (tid == 0) s_found[0] = 0;
-  __syncthreads();
-  int have = 0;
-  for (int c = tid; c < w.columns; c += SELECT_THREADS) have += keys[c] != 0;
-  have = __reduce_add_sync(0xffffffffu, have);
-  if (lane == 0) atomicAdd(&s_found[0], have);
-  __syncthreads();
-  uint32_t limit = 0;  // taken are the keys above it and the first `ties` of its equals
-  int ties = 0;
-  const bool search = s_found[0] > w.count;
-  if (search) {
-    int need = w.count;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      s_hist[tid] = 0;
-      __syncthreads();
-      for (int c = tid; c < w.columns; c += SELECT_THREADS) {
-        const uint32_t key = rank(c);
-        if (shift == 24 || (key >> (shift + 8)) == (limit >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (warp == 0) {  // lane l: the bins 255 - 8 l .. 248 - 8 l, from the greatest down
-        int n[8], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          n[i] = s_hist[255 - 8 * lane - i];
-          sum += n[i];
-        }
-        int before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += y;
-        }
-        before -= sum;
-        if (before < need && need <= before + sum) {  // one lane's
-          int bin = -1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (bin < 0 && before + n[i] >= need) bin = i;
-            if (bin < 0) before += n[i];
-          }
-          s_found[0] = 255 - 8 * lane - bin;
-          s_found[1] = need - before;
-        }
-      }
-      __syncthreads();
-      limit |= static_cast<uint32_t>(s_found[0]) << shift;
-      need = s_found[1];
-      __syncthreads();
-    }
-    ties = need;
-  }
-  int done = 0, equal = 0;
-  for (int c0 = 0; c0 < w.columns; c0 += SELECT_THREADS) {
-    const int c = c0 + tid;
-    const uint32_t key = c < w.columns ? rank(c) : 0;
-    const bool above = key > limit, same = search && key == limit;
-    const uint32_t va = __ballot_sync(0xffffffffu, above), vs = __ballot_sync(0xffffffffu, same);
-    if (lane == 0) {
-      s_part[0][warp] = __popc(va);
-      s_part[1][warp] = __popc(vs);
-    }
-    __syncthreads();
-    int a = done, s = equal;
-    for (int k = 0; k < SELECT_WARPS; ++k) {
-      if (k < warp) {
-        a += s_part[0][k];
-        s += s_part[1][k];
-      }
-      done += s_part[0][k];
-      equal += s_part[1][k];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    a += __popc(va & below);
-    s += __popc(vs & below);
-    const int at = a + min(s, ties);
-    if ((above || (same && s < ties)) && at < w.count) {
-      out[at] = c;
-      if (scores != nullptr) scores[at] = ldexpf(number_of(keys[c]), eq);
-    }
-    __syncthreads();
-  }
-  for (int i = min(done + min(equal, ties), w.count) + tid; i < w.count; i += SELECT_THREADS) {
+  const int listed = min(always + min(others, need), w.count);
+  for (int i = listed + (WARPS > 1 ? static_cast<int>(threadIdx.x) : lane); i < w.count; i += 32 * WARPS) {
     out[i] = -1;
     if (scores != nullptr) scores[i] = -INFINITY;
   }
@@ -496,8 +464,9 @@ __device__ __forceinline__ int query_exponent(const Query<NG>& q, const SelectPa
 // Few rows: a cluster of `split` CTAs per token and kv head. Their warps score the pages in turn; the keys
 // meet in the first CTA, which searches them.
 template <int NG>
-__global__ void __launch_bounds__(SELECT_THREADS) select_pages_cta_kernel(SelectParams w, int split) {
+__global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_cta_kernel(SelectParams w, int split) {
   extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ SearchScratch s_search;
   const Pages& p = w.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (split > 1) cluster_sync();  // the first CTA is there to be written to
@@ -518,13 +487,25 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_cta_kernel(Select
   const __nv_bfloat16* heads = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
   const int32_t* row = p.table + b * p.table_ld;
   const uint32_t dst = split > 1 ? mapa_shared(smem_addr(s_keys), 0) : smem_addr(s_keys);
+  const int begin = 16 * (warp + SELECT_WARPS * rank), step = 16 * SELECT_WARPS * split;
+  PageRows<NG> rows;  // the first pages' loads fly while q is rounded
+  rows.load(w, head, PageRows<NG>::entry(row, begin, want.columns, lane), lane);
+  int entry = PageRows<NG>::entry(row, begin + step, want.columns, lane);
   Query<NG> q;
   q.e = query_exponent(q, w, heads, min(lane >> 2, w.group - 1), lane);
   for (int h = 0; h < w.group; h += 8) {
     q.round(heads + min(h + (lane >> 2), w.group - 1) * w.qh, lane, w.vec);
-    for (int c0 = 16 * (warp + SELECT_WARPS * rank); c0 < want.columns; c0 += 16 * SELECT_WARPS * split)
-      score_pages(w, row, head, q, c0, want.columns, lane, [&](int, int c, uint32_t key) {
-        const uint32_t at = dst + 4 * c;  // a column's passes are one warp's
+    if (h > 0) {
+      rows.load(w, head, PageRows<NG>::entry(row, begin, want.columns, lane), lane);
+      entry = PageRows<NG>::entry(row, begin + step, want.columns, lane);
+    }
+    for (int c0 = begin; c0 < want.columns; c0 += step) {
+      const PageRows<NG> now = rows;
+      if (c0 + step < want.columns) rows.load(w, head, entry, lane);
+      entry = PageRows<NG>::entry(row, c0 + 2 * step, want.columns, lane);
+      now.report(c0, want.columns, lane);
+      now.score(w, q, c0, want.columns, lane, [&](int, int c, uint32_t key) {
+        const uint32_t at = dst + 4 * c;  // a column's passes are one lane's
         if (h > 0) {
           uint32_t old;
           asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(old) : "r"(at) : "memory");
@@ -532,6 +513,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_cta_kernel(Select
         }
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(key) : "memory");
       });
+    }
   }
   if (split > 1) cluster_sync(); else __syncthreads();
   if (rank > 0) return;
@@ -539,32 +521,33 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_cta_kernel(Select
   int32_t* out = w.out + list;
   float* scores = w.scores == nullptr ? nullptr : w.scores + list;
   if (want.columns > WARP_COLUMNS)
-    take_by_cta(s_keys, want, q.e, out, scores);
+    take<SELECT_WARPS>(s_keys, want, q.e, out, scores, &s_search);
   else if (warp == 0)
-    take_by_warp(s_keys, want, q.e, out, scores, lane);
+    take<1>(s_keys, want, q.e, out, scores, nullptr);
 }
 
-// Many rows: a warp per kv head and (8 >> slots) tokens, whose heads share the products with a page.
+// Many rows: a warp per kv head and two products' columns, 16 >> slots tokens: the heads of several tokens
+// share a product, and two products a page's bounds.
+constexpr int PRODUCTS = 2;
 template <int NG>
-__global__ void __launch_bounds__(SELECT_THREADS) select_pages_warp_kernel(SelectParams w) {
+__global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_warp_kernel(SelectParams w) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   const Pages& p = w.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dependency_wait();
   allow_dependent_launch();
   if (blockIdx.x == 0) check_batch(p, w.total, tid, SELECT_THREADS);
-  const int tokens = 8 >> w.slots;
+  const int each = 8 >> w.slots, tokens = PRODUCTS * each;
   const int64_t block = blockIdx.x / p.kv_heads, token0 = (block * SELECT_WARPS + warp) * tokens;
   const int head = static_cast<int>(blockIdx.x - block * p.kv_heads);
   uint32_t* keys = s_keys + static_cast<int64_t>(warp) * tokens * w.key_ld;
-  const int mine = lane >> 2 >> w.slots;  // the token of the lane's column
+  const int column = (lane >> 2) & ((1 << w.slots) - 1);  // the lane's head of a pass
   int done = 0;  // tokens of the group that have been looked at
   while (done < tokens && token0 + done < w.total) {
     // a run of tokens of one sequence
     int b;
     int64_t pos;
-    const bool placed = find_token(p, token0 + done, w.total, b, pos);
-    if (!placed) {
+    if (!find_token(p, token0 + done, w.total, b, pos)) {
       ++done;
       continue;
     }
@@ -572,27 +555,42 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_pages_warp_kernel(Selec
     const int64_t last = pos + run - 1;
     const int columns = last < 0 ? 0 : static_cast<int>(std::min<int64_t>((last >> p.page_shift) + 1, p.table_cols));
     if (lane == 0 && last >= 0 && (last >> p.page_shift) >= p.table_cols) atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
-    const int64_t token = token0 + min(max(mine, done), done + run - 1);  // columns of other tokens repeat one of the run
-    const __nv_bfloat16* heads = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
     const int32_t* row = p.table + b * p.table_ld;
-    Query<NG> q;
-    const int column = (lane >> 2) & ((1 << w.slots) - 1);
-    q.e = query_exponent(q, w, heads, min(column, w.group - 1), lane);
+    const __nv_bfloat16* heads[PRODUCTS];
+    Query<NG> q[PRODUCTS];
+#pragma unroll
+    for (int k = 0; k < PRODUCTS; ++k) {  // columns of other tokens repeat one of the run
+      const int64_t token = token0 + min(max(k * each + (lane >> 2 >> w.slots), done), done + run - 1);
+      heads[k] = w.q + token * w.qt + static_cast<int64_t>(head) * w.group * w.qh;
+      q[k].e = query_exponent(q[k], w, heads[k], min(column, w.group - 1), lane);
+    }
     for (int h = 0; h < w.group; h += 8) {
-      q.round(heads + min(h + column, w.group - 1) * w.qh, lane, w.vec);
-      for (int c0 = 0; c0 < columns; c0 += 16)
-        score_pages(w, row, head, q, c0, columns, lane, [&](int slot, int c, uint32_t key) {
-          uint32_t* at = keys + static_cast<int64_t>(slot) * w.key_ld + c;
-          *at = h > 0 ? max(key, *at) : key;
-        });
+#pragma unroll
+      for (int k = 0; k < PRODUCTS; ++k) q[k].round(heads[k] + min(h + column, w.group - 1) * w.qh, lane, w.vec);
+      PageRows<NG> rows;
+      rows.load(w, head, PageRows<NG>::entry(row, 0, columns, lane), lane);
+      int entry = PageRows<NG>::entry(row, 16, columns, lane);
+      for (int c0 = 0; c0 < columns; c0 += 16) {
+        const PageRows<NG> now = rows;
+        if (c0 + 16 < columns) rows.load(w, head, entry, lane);
+        entry = PageRows<NG>::entry(row, c0 + 32, columns, lane);
+        now.report(c0, columns, lane);
+#pragma unroll
+        for (int k = 0; k < PRODUCTS; ++k)
+          now.score(w, q[k], c0, columns, lane, [&](int slot, int c, uint32_t key) {
+            uint32_t* at = keys + static_cast<int64_t>(k * each + slot) * w.key_ld + c;
+            *at = h > 0 ? max(key, *at) : key;
+          });
+      }
     }
     __syncwarp();
     for (int i = done; i < done + run; ++i) {
       const int64_t at = pos + i - done, list = ((token0 + i) * p.kv_heads + head) * w.count;
       const Wanted want = {at < 0 ? 0 : static_cast<int>(std::min<int64_t>((at >> p.page_shift) + 1, p.table_cols)), w.count,
                            w.first, w.last};
-      take_by_warp(keys + static_cast<int64_t>(i) * w.key_ld, want, __shfl_sync(0xffffffffu, q.e, i << w.slots << 2),
-                   w.out + list, w.scores == nullptr ? nullptr : w.scores + list, lane);
+      const int k = i / each, e = __shfl_sync(0xffffffffu, k == 0 ? q[0].e : q[1].e, (i - k * each) << w.slots << 2);
+      take<1>(keys + static_cast<int64_t>(i) * w.key_ld, want, e, w.out + list, w.scores == nullptr ? nullptr : w.scores + list,
+              nullptr);
     }
     __syncwarp();
     done += run;
@@ -664,11 +662,10 @@ extern "C" int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads
   // product.
   int slots = 0;
   while (slots < 3 && (1 << slots) < w.group) ++slots;
-  const int64_t keys = (SELECT_WARPS * 8 >> slots) * table_cols;
-  if (units << slots >= 64 * static_cast<int64_t>(num_sms()) && 4 * keys <= SELECT_KEY_BYTES) {
+  const int64_t tokens = SELECT_WARPS * PRODUCTS * 8 >> slots, keys = tokens * table_cols;  // of a CTA
+  if (units << slots >= 8 * SELECT_WARPS * static_cast<int64_t>(num_sms()) && 4 * keys <= SELECT_KEY_BYTES) {
     w.slots = slots;
     w.key_ld = static_cast<int>(table_cols);
-    const int64_t tokens = SELECT_WARPS * 8 >> slots;
     auto kern = d == 64 ? select_pages_warp_kernel<1> : select_pages_warp_kernel<2>;
     const int rs = allow_smem(reinterpret_cast<const void*>(kern), SELECT_KEY_BYTES, set[d == 64 ? 0 : 1]);
     if (rs) return rs;
