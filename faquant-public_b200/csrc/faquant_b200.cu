@@ -109,6 +109,7 @@ __global__ void selftest_wait_kernel(uint64_t limit_ns) {
 #include "verify.cu"
 #include "kv_append.cu"
 #include "page_select.cu"
+#include "sparse_tile.cu"
 #include "sparse_attention.cu"
 
 extern "C" int faq_version(void) { return 100; }

@@ -67,20 +67,26 @@ __device__ __forceinline__ void check_batch(const Pages& p, int64_t total, int t
   for (int b = tid; b < p.batch; b += threads) check_rows(p, b, total);
 }
 
-// The sequence and position of packed token `token` (< total), by a whole warp; false where it
-// belongs to no sequence whose new tokens lie in the `total` given rows.
-__device__ __forceinline__ bool find_token(const Pages& p, int64_t token, int64_t total, int& b, int64_t& pos) {
-  int lo = 0, n = p.batch;  // the last of n sequences from lo on that begins at the token or before
+// The last i < n with at(i) (0 if there is none), for at() true up to it, by a whole warp.
+template <typename F>
+__device__ __forceinline__ int last_of(int n, F&& at) {
+  int lo = 0;
   while (n > 1) {
     const int step = (n + 31) >> 5, i = static_cast<int>(threadIdx.x & 31) * step;
-    const uint32_t before = __ballot_sync(0xffffffffu, i < n && p.cu[lo + i] <= token);
-    const int k = before ? 31 - __clz(before) : 0;
+    const uint32_t yes = __ballot_sync(0xffffffffu, i < n && at(lo + i));
+    const int k = yes ? 31 - __clz(yes) : 0;
     lo += k * step;
     n = min(step, n - k * step);
   }
-  b = lo;
-  const int c0 = p.cu[lo], c1 = p.cu[lo + 1];
-  pos = static_cast<int64_t>(p.lens[lo]) - c1 + token;
+  return lo;
+}
+
+// The sequence and position of packed token `token` (< total), by a whole warp; false where it
+// belongs to no sequence whose new tokens lie in the `total` given rows.
+__device__ __forceinline__ bool find_token(const Pages& p, int64_t token, int64_t total, int& b, int64_t& pos) {
+  b = last_of(p.batch, [&](int i) { return p.cu[i] <= token; });
+  const int c0 = p.cu[b], c1 = p.cu[b + 1];
+  pos = static_cast<int64_t>(p.lens[b]) - c1 + token;
   return c0 >= 0 && c0 <= token && token < c1 && c1 <= total;
 }
 

@@ -71,11 +71,7 @@ __global__ void __launch_bounds__(32 * BOUNDS_WARPS) key_bounds_kernel(BoundsPar
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t slot = blockIdx.x / p.kv_heads;
   const int head = static_cast<int>(blockIdx.x - slot * p.kv_heads);
-  int lo = 0, hi = p.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first_page_slot(p, mid) <= slot) lo = mid; else hi = mid;
-  }
+  const int lo = last_of(p.batch, [&](int i) { return first_page_slot(p, i) <= slot; });
   const int c0 = p.cu[lo], c1 = p.cu[lo + 1];
   if (c0 < 0 || c1 <= c0 || c1 > w.total || slot < first_page_slot(p, lo)) {
     if (tid == 0) check_rows(p, lo, w.total);

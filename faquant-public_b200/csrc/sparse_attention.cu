@@ -26,23 +26,9 @@ using pat::pack_bf16;
 using pat::RAISE;
 using pat::transpose8x8;
 
-constexpr int RB = 8;  // rows (query heads) of a unit
 constexpr int W = 8;   // warps of a CTA, two CTAs per SM: 128 registers a thread
 constexpr int THREADS = 32 * W;
 constexpr int S = 4;   // blocks in flight per warp
-
-struct Params {
-  Pages p;
-  const __nv_bfloat16* q;
-  int64_t qt, qh;  // token, head strides
-  __nv_bfloat16* out;
-  int64_t ot, oh;
-  int64_t total;   // rows of q and out
-  int group, passes;  // query heads per kv head, units of a token and kv head
-  const int32_t* list;  // [total, kv_heads, count]
-  int count;
-  float scale_log2;
-};
 
 // shared memory: the warps' rings, then in their place the warps' O (rows padded) | the CTA's O | (m, l) of
 // warps and CTA | the ring slots' first keys | mbarriers
@@ -59,17 +45,6 @@ struct Smem {
   static constexpr int bar = key + W * S * 4;
   static constexpr int bytes = bar + W * S * 8;
 };
-
-__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float cluster_load(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
 
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, int split) {
@@ -101,12 +76,19 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, 
   unit /= P.passes;
   const int head = static_cast<int>(unit % p.kv_heads);
   const int64_t token = unit / p.kv_heads;
+  const int32_t* list = P.list + (token * p.kv_heads + head) * P.count;
+  // whether the columns of the list are in ascending order, hence none is there twice
+  bool ascending = true;
+  for (int j = lane; j < P.count; j += 32) {
+    const int before = j > 0 ? list[j - 1] : 0, col = list[j];
+    ascending = ascending && (col < 0 || j == 0 || (before >= 0 && before < col));
+  }
+  ascending = __all_sync(0xffffffffu, ascending);
   int b;
   int64_t pos;
   if (blockIdx.x == 0) check_batch(p, P.total, tid, THREADS);
   if (!find_token(p, token, P.total, b, pos)) return;  // the whole cluster
   const int rows = min(RB, P.group - pass * RB);
-  const int32_t* list = P.list + (token * p.kv_heads + head) * P.count;
 
   // ---- the warp's blocks: numbers warp + W rank + W split i of the count << block_shift listed ones
   const int block_shift = p.page_shift - 4;
@@ -129,7 +111,10 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, 
       const int64_t block = begin + i * stride;
       const int col = list[block >> block_shift];
       const int64_t key = (static_cast<int64_t>(col) << p.page_shift) + ((block & ((1 << block_shift) - 1)) << 4);
-      if (col >= 0 && key <= pos) {
+      bool again = false;  // a column counts once
+      if (!ascending)
+        for (int64_t j = 0; j < block >> block_shift; ++j) again = again || list[j] == col;
+      if (col >= 0 && key <= pos && !again) {
         const int64_t page = page_of(p, b, static_cast<int>(key));
         has = page >= 0;
         first_of = static_cast<int>(key);
@@ -391,9 +376,7 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, 
   cluster_sync();
   bool all = true;
   for (int k = 0; k < split; ++k) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_addr(&s_ok), k)));
-    all = all && v != 0;
+    all = all && cluster_load_int(mapa_shared(smem_addr(&s_ok), k)) != 0;
   }
   for (int i = tid + THREADS * rank; i < rows * (D / 4); i += THREADS * split) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
@@ -463,6 +446,12 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   P.list = selected;
   P.count = static_cast<int>(count);
   P.scale_log2 = scale * 1.4426950408889634f;
+  // Tokens of a sequence mostly want the same pages: from eight of them to a sequence on (or fewer, with more than eight
+  // query heads to a kv head) a tile of them is taken together.
+  const int tokens = P.group <= pre::TILE ? spt::tile_tokens(P.group) : 0;
+  if (tokens && total * P.passes >= 8 * batch && std::min(tokens * count, table_cols) <= spt::MAX_UNION &&
+      table_cols <= spt::columns(d) && q_token_stride >= 8 && q_head_stride >= 8)
+    return d == 64 ? spt::launch<1>(P, heads, stream) : spt::launch<2>(P, heads, stream);
   const int64_t units = total * kv_heads * P.passes, blocks = count << (P.p.page_shift - 4);
   int split = 1;
   while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > W * split) split *= 2;

@@ -1,0 +1,444 @@
+// K13 for chunks of tokens: a tile of up to 128 rows (tokens x query heads of a kv head) over the
+// union of its tokens' lists.
+//
+// Neighbouring tokens mostly list the same pages. Expanding a page's codes for each token apart is
+// what the kernel of single tokens (sparse_attention.cu) spends its time on; here a page is expanded
+// once for all rows of a tile, on the tensor cores of paged_chunk.cu (the same roles, operands and
+// softmax), and a row's scores with pages that its token does not list are masked. At the start
+// the CTA marks, per column, which of its tokens list it (one bit each, up to 32 tokens), and writes the
+// marked columns in order: page, column, tokens. A column counts once, however often it is listed.
+// Key tiles are 8 blocks of 16 tokens, as they come in that order.
+//
+// One CTA per (sequence, kv head, tile of tokens), or a cluster of 2, 4 or 8 that share the union's key tiles
+// and add up their rows through distributed shared memory.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "kv_pages.cuh"
+#include "tma.h"
+
+namespace faq {
+namespace spa {
+
+using namespace kvp;
+
+constexpr int RB = 8;  // rows (query heads) of a unit of single tokens
+
+struct Params {
+  Pages p;
+  const __nv_bfloat16* q;
+  int64_t qt, qh;  // token, head strides
+  __nv_bfloat16* out;
+  int64_t ot, oh;
+  int64_t total;   // rows of q and out
+  int group, passes;  // query heads per kv head, units of a token and kv head
+  const int32_t* list;  // [total, kv_heads, count]
+  int count;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float cluster_load(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int cluster_load_int(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+}  // namespace spa
+
+namespace spt {
+
+using namespace kvp;
+using chk::QMaps;
+using pat::ex2;
+using pat::LOWEST;
+using pat::pack_bf16;
+using pre::block_scan;
+using pre::CHUNK;
+using pre::commit;
+using pre::IDESC_QK;
+using pre::idesc_pv;
+using pre::mma_ss;
+using pre::o_col;
+using pre::s_col;
+using pre::Softmax;
+using pre::THREADS;
+using pre::TILE;
+using pre::TMEM_COLS;
+using spa::cluster_load;
+using spa::cluster_load4;
+using spa::cluster_load_int;
+using spa::Params;
+
+constexpr int MAX_UNION = 2048;  // columns of a tile's union
+// the table's columns whose marks fit where K and V will be
+__host__ __device__ constexpr int columns(int d) { return d / 64 * 4 * CHUNK / 4; }
+__host__ __device__ constexpr int tile_tokens(int group) { return TILE / group < 32 ? TILE / group : 32; }
+
+template <int NG>
+struct Smem {
+  static constexpr int tile = NG * CHUNK;
+  static constexpr int q = 0;
+  static constexpr int k = q + tile;
+  static constexpr int v = k + 2 * tile;
+  static constexpr int p = v + 2 * tile;
+  static constexpr int page = p + 2 * CHUNK;  // [MAX_UNION]
+  static constexpr int col = page + 4 * MAX_UNION;
+  static constexpr int mark = col + 4 * MAX_UNION;
+  static constexpr int bar = mark + 4 * MAX_UNION;
+  static constexpr int bytes = 1024 + bar + 256;
+  // at the end, where K and V were: O [TILE][D], m and l [TILE]
+  static constexpr int o = k;
+};
+static_assert(Smem<2>::bytes <= 227 * 1024, "shared memory");
+
+// As the slots of blocks (kv_cache.cu): n tokens are at most n / T + 1 tiles of T, so sequence b's
+// tiles get the slots from cu[b] / T + b on.
+__host__ __device__ inline int64_t slots_of(int64_t total, int64_t batch, int tokens) { return total / tokens + batch; }
+
+template <int NG>
+__global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_constant__ QMaps maps, Params P, int split) {
+  using L = Smem<NG>;
+  constexpr int D = 64 * NG, WARPS = THREADS / 32;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::bar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* k_full = bars + 2;  // [2 stages]
+  uint64_t* k_empty = bars + 4;
+  uint64_t* v_full = bars + 6;
+  uint64_t* v_empty = bars + 8;
+  uint64_t* s_full = bars + 10;
+  uint64_t* s_free = bars + 11;
+  uint64_t* p_full = bars + 12;
+  uint64_t* pv_done = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  int* s_page = reinterpret_cast<int*>(base + L::page);
+  int* s_column = reinterpret_cast<int*>(base + L::col);
+  uint32_t* s_mark = reinterpret_cast<uint32_t*>(base + L::mark);
+  __shared__ int64_t s_scan[WARPS];
+  __shared__ int s_well;  // softmax warps that came to their end
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Pages& p = P.p;
+  grid_dependency_wait();
+  allow_dependent_launch();
+
+  // ---- the unit
+  const int T = tile_tokens(P.group);
+  const int rank = static_cast<int>(blockIdx.x % split);
+  const int64_t unit = blockIdx.x / split, slot = unit / p.kv_heads;
+  const int head = static_cast<int>(unit - slot * p.kv_heads);
+  if (blockIdx.x == 0) check_batch(p, P.total, tid, THREADS);
+  const int b = last_of(p.batch, [&](int i) { return p.cu[i] / T + static_cast<int64_t>(i) <= slot; });
+  const int64_t c0 = p.cu[b], n = p.cu[b + 1] - c0;
+  const int64_t u = slot - (c0 / T + b);
+  if (c0 < 0 || n <= 0 || c0 + n > P.total || u < 0 || u * T >= n) return;  // the whole cluster
+  const int64_t tok0 = u * T;
+  const int tokens = static_cast<int>(std::min<int64_t>(T, n - tok0));
+  const int64_t pos0 = p.lens[b] - n + tok0;  // of the tile's first token
+  const int64_t last_pos = pos0 + tokens - 1;
+
+  // ---- which of the tokens list a column
+  uint32_t* marks = reinterpret_cast<uint32_t*>(base + L::k);
+  const int seen = last_pos < 0 ? 0 : static_cast<int>(std::min<int64_t>((last_pos >> p.page_shift) + 1, p.table_cols));
+  for (int c = tid; c < seen; c += THREADS) marks[c] = 0;
+  if (tid == 0) {
+    s_well = 0;
+    mbar_init(smem_addr(q_full), 1);
+    mbar_init(smem_addr(s_full), 1);
+    mbar_init(smem_addr(s_free), 8);
+    mbar_init(smem_addr(p_full), 8);
+    mbar_init(smem_addr(pv_done), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&k_full[i]), 8);  // the eight expanding warps
+      mbar_init(smem_addr(&k_empty[i]), 1);
+      mbar_init(smem_addr(&v_full[i]), 8);
+      mbar_init(smem_addr(&v_empty[i]), 1);
+    }
+    fence_barrier_init();
+    for (int i = 0; i < 3; ++i) tma_prefetch_desc(&maps.q[i]);
+  }
+  if (warp == 18) {
+    tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  for (int i = tid; i < tokens * P.count; i += THREADS) {
+    const int tok = i / P.count;
+    const int col = P.list[((c0 + tok0 + tok) * p.kv_heads + head) * P.count + (i - tok * P.count)];
+    if (col >= 0 && static_cast<int64_t>(col) << p.page_shift <= pos0 + tok) {
+      if (col < seen)
+        atomicOr(&marks[col], 1u << tok);
+      else
+        atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);  // beyond the table
+    }
+  }
+  __syncthreads();
+  int found;
+  {
+    const int per = (seen + THREADS - 1) / THREADS, begin = tid * per, end = min(begin + per, seen);
+    int64_t mine = 0, all;
+    for (int c = begin; c < end; ++c)
+      if (marks[c]) {
+        const int page = p.table[b * p.table_ld + c];
+        if (page < 0 || page >= p.num_pages) {
+          atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);
+          marks[c] = 0;
+        } else {
+          ++mine;
+        }
+      }
+    int i = static_cast<int>(block_scan<WARPS>(mine, s_scan, &all));
+    found = static_cast<int>(all);
+    for (int c = begin; c < end; ++c)
+      if (marks[c]) {
+        s_page[i] = p.table[b * p.table_ld + c];
+        s_column[i] = c;
+        s_mark[i++] = marks[c];
+      }
+  }
+  __syncthreads();
+  const int block_shift = p.page_shift - 4, in_page = (1 << block_shift) - 1;
+  // blocks of the union; of the last token's own page those up to it
+  const bool own = found > 0 && s_column[found - 1] == last_pos >> p.page_shift;
+  const int blocks = own ? ((found - 1) << block_shift) + (static_cast<int>(last_pos & ((1 << p.page_shift) - 1)) >> 4) + 1
+                         : found << block_shift;
+  const int tiles = (blocks + 7) >> 3;
+  const int k0 = static_cast<int>(static_cast<int64_t>(tiles) * rank / split);
+  const int count = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / split) - k0;
+  const int copies = tokens * P.group <= 32 ? 4 : tokens * P.group <= 64 ? 2 : 1;  // of the rows, see Softmax
+
+  // Registers: 640 x 96 at launch = 512 x 104 + 128 x 64.
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::: "memory");
+    if (warp == 16) {
+      if (lane == 0 && count > 0) {
+        const int rows = TILE / copies, map = copies >> 1;  // the box of 128, 64 or 32 rows
+        mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(copies * (rows / P.group) * P.group) * 128 * NG);
+        for (int c = 0; c < NG * copies; ++c)
+          tma_load_3d(smem_addr(base + L::q + (c / copies) * CHUNK + c % copies * rows * 128), &maps.q[map],
+                      smem_addr(q_full), c / copies * 64, head * P.group, static_cast<int>(c0 + tok0));
+        mbar_wait_site(smem_addr(q_full), 0, 90, 0);  // (bounded) it is there before the CTA's end
+      }
+    } else if (warp == 18) {
+      // the whole warp walks the steps, one elected lane issues (paged_prefill.cu)
+      const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
+      const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
+      const uint32_t v_desc = sw128_desc_lo(smem_addr(base + L::v), CHUNK);
+      const uint32_t p_desc = sw128_desc_lo(smem_addr(base + L::p), 16);
+      constexpr uint32_t TILE_D = L::tile >> 4;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site, int step) {
+        return mbar_wait_warp(smem_addr(bar), parity & 1, site, step);
+      };
+      auto issue_qk = [&](auto stage) {
+        constexpr int st = decltype(stage)::value;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + s_col(0), q_desc + off, k_desc + st * TILE_D + off, IDESC_QK, kk != 0);
+        }
+        commit(smem_addr(s_full));
+        commit(smem_addr(&k_empty[st]));
+      };
+      auto issue_pv = [&](auto stage, bool add) {
+        constexpr int st = decltype(stage)::value;
+#pragma unroll
+        for (int kk = 0; kk < TILE / 16; ++kk) {
+          const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + o_col(0), p_desc + off, v_desc + st * TILE_D + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
+        }
+        commit(smem_addr(pv_done));
+        commit(smem_addr(&v_empty[st]));
+      };
+      const std::integral_constant<int, 0> st0;
+      const std::integral_constant<int, 1> st1;
+      auto scores = [&](uint32_t step) {
+        if (!wait(&k_full[step & 1], step >> 1, 91, step)) return false;
+        if (step > 0 && !wait(s_free, step - 1, 92, step)) return false;
+        tc_fence_after();
+        if (step & 1) issue_qk(st1); else issue_qk(st0);
+        return true;
+      };
+      const bool ok = count > 0 && wait(q_full, 0, 93, 0) && scores(0);
+      for (int j = 0; j < count && ok; ++j) {
+        if (j + 1 < count && !scores(j + 1)) break;
+        if (!wait(&v_full[j & 1], j >> 1, 94, j) || !wait(p_full, j, 95, j)) break;
+        tc_fence_after();
+        if (j & 1) issue_pv(st1, j != 0); else issue_pv(st0, j != 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
+    // ------------------------------------------------------------ expansion: block ew of each key tile
+    const int ew = warp - 8;
+    const int64_t v_off = (static_cast<int64_t>(p.kv_heads) << block_shift) * block_bytes(NG);  // from a page's K to its V
+    // where block ew of tile j is (null: past the end; the softmax leaves such keys out, and the
+    // registers' last block stands in for them, whose values are finite)
+    auto block_of = [&](int j) -> const uint8_t* {
+      const int i = (k0 + j) * 8 + ew;
+      if (i >= blocks) return nullptr;
+      return p.base + s_page[i >> block_shift] * p.page_stride + block_in_page<NG>(p, 0, head, (i & in_page) << 4);
+    };
+    const Expand expand;
+    KBlock<NG> kb = {};
+    VBlock<NG> vb = {};
+    const uint8_t* src = count > 0 ? block_of(0) : nullptr;
+    if (src) {
+      kb.load(src, lane);
+      vb.load(src + v_off, lane);
+    }
+    for (int step = 0; step < count; ++step) {
+      src = step + 1 < count ? block_of(step + 1) : nullptr;  // of the next step
+      const int st = step & 1;
+      // rows of 128 bytes per group, token ew * 16 + i, unit at unit ^ (token % 8)
+      auto write = [&](uint8_t* tile) {
+        return [=](int token, int g, int at, const uint32_t (&x)[4]) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_addr(tile) + g * CHUNK +
+                                                                         (ew * BLOCK + token) * 128 + ((at ^ (token & 7)) << 4)),
+                       "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                       : "memory");
+        };
+      };
+      if (!mbar_wait_warp(smem_addr(&k_empty[st]), ((step >> 1) & 1) ^ 1, 96, step)) break;
+      kb.template each<1>(expand, lane, write(base + L::k + st * L::tile));
+      fence_proxy_async_smem();  // the tensor core reads it through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
+      if (src) kb.load(src, lane);
+      if (!mbar_wait_warp(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 97, step)) break;
+      vb.template each<1>(expand, lane, write(base + L::v + st * L::tile));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
+      if (src) vb.load(src + v_off, lane);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
+    Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
+    auto work = [&](auto parts) {
+      constexpr int PARTS = decltype(parts)::value, KEYS = TILE / PARTS;
+      const int row = sm.template row<PARTS>(), tok = row / P.group;
+      const bool live = tok < tokens;
+      const int64_t pos = pos0 + tok;
+      auto mask = [&](int j, int part, float (&f)[KEYS]) {
+#pragma unroll
+        for (int x = 0; x < KEYS; x += BLOCK) {
+          const int i = (k0 + j) * 8 + (part * KEYS + x) / BLOCK, e = i >> block_shift;
+          // keys of the block that the row sees: those up to its own place, if its token lists the page
+          int keys = 0;
+          if (live && i < blocks && (s_mark[e] >> tok & 1)) {
+            const int64_t left = pos - ((static_cast<int64_t>(s_column[e]) << p.page_shift) + ((i & in_page) << 4)) + 1;
+            keys = static_cast<int>(std::min<int64_t>(std::max<int64_t>(left, 0), BLOCK));
+          }
+          if (__all_sync(0xffffffffu, keys == BLOCK)) continue;
+#pragma unroll
+          for (int k = 0; k < BLOCK; ++k)
+            if (k >= keys) f[x + k] = -INFINITY;
+        }
+      };
+      if (count > 0 && !sm.template run_masked<PARTS>(count, live, mask, [] {})) return;
+      if (lane == 0) atomicAdd(&s_well, 1);
+      if (count == 0 || !sm.template first_copy<PARTS>()) return;
+      const int row_head = row - tok * P.group;
+      sm.store(live, split == 1 ? nullptr : reinterpret_cast<float*>(base + L::o), TILE, row,
+               P.out + (c0 + tok0 + (live ? tok : 0)) * P.ot + (static_cast<int64_t>(head) * P.group + row_head) * P.oh);
+    };
+    if (copies == 4) work(std::integral_constant<int, 8>());
+    else if (copies == 2) work(std::integral_constant<int, 4>());
+    else work(std::integral_constant<int, 2>());
+  }
+  __syncthreads();
+  if (warp == 18) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+  const int rows = tokens * P.group;
+  auto place = [&](int row) {
+    const int tok = row / P.group;
+    return P.out + (c0 + tok0 + tok) * P.ot + (static_cast<int64_t>(head) * P.group + row - tok * P.group) * P.oh;
+  };
+  if (split == 1) {
+    if (tiles == 0)  // rows without a key are zero
+      for (int i = tid; i < rows * (D / 8); i += THREADS)
+        *reinterpret_cast<uint4*>(place(i / (D / 8)) + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  // ---- the CTAs' rows meet, each takes a part of them
+  cluster_sync();
+  const uint32_t o_addr = smem_addr(base + L::o), m_addr = o_addr + TILE * D * 4, l_addr = m_addr + TILE * 4;
+  bool all = true;
+  int parts = 0;  // bit k: CTA k had key tiles
+  for (int k = 0; k < split; ++k) {
+    all = all && cluster_load_int(mapa_shared(smem_addr(&s_well), k)) == 8;
+    if (static_cast<int64_t>(tiles) * (k + 1) / split > static_cast<int64_t>(tiles) * k / split) parts |= 1 << k;
+  }
+  for (int i = tid + THREADS * rank; i < rows * (D / 4); i += THREADS * split) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float top = LOWEST;
+    for (int k = 0; k < split; ++k)
+      if (parts >> k & 1) top = fmaxf(top, cluster_load(mapa_shared(m_addr + 4 * r, k)));
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = 0.0f;
+    for (int k = 0; k < split; ++k) {
+      if (!(parts >> k & 1)) continue;
+      const float f = ex2(0.5f * (cluster_load(mapa_shared(m_addr + 4 * r, k)) - top));
+      const float4 v = cluster_load4(mapa_shared(o_addr + (r * D + c) * 4, k));
+      sum.x += f * v.x * f;
+      sum.y += f * v.y * f;
+      sum.z += f * v.z * f;
+      sum.w += f * v.w * f;
+      den += f * cluster_load(mapa_shared(l_addr + 4 * r, k)) * f;
+    }
+    const float inv = den > 0.0f ? __fdiv_rn(1.0f, den) : (den == 0.0f ? 0.0f : den);  // NaN stays
+    if (all)
+      *reinterpret_cast<uint2*>(place(r) + c) =
+          make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+  }
+  cluster_sync();  // the others have read this CTA's rows
+}
+
+template <int NG>
+static int launch(const Params& P, int64_t heads, void* stream) {
+  constexpr int D = 64 * NG;
+  QMaps maps;
+  const uint64_t dims[3] = {D, static_cast<uint64_t>(heads), static_cast<uint64_t>(P.total)};
+  const uint64_t str[2] = {static_cast<uint64_t>(P.qh) * 2, static_cast<uint64_t>(P.qt) * 2};
+  int rc = FAQ_OK;
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(std::max((TILE >> i) / P.group, 1))};
+    rc = make_tmap(&maps.q[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  auto kern = sparse_tile_kernel<NG>;
+  static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
+  rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
+  if (rc) return rc;
+  const int64_t units = slots_of(P.total, P.p.batch, tile_tokens(P.group)) * P.p.kv_heads;
+  // as many CTAs as fill the SMs once, of some key tiles each
+  const int64_t tiles = (static_cast<int64_t>(P.count) << (P.p.page_shift - 4)) / 8;
+  int split = 1;
+  while (split < 8 && units * split * 2 <= num_sms() && tiles >= 4 * split) split *= 2;
+  FAQ_CHECK_ARG(units * split < (int64_t(1) << 31), "too many tokens for one call");
+  FAQ_CUDA(launch_clusters(kern, units * split, THREADS, Smem<NG>::bytes, split, stream, maps, P, split));
+  return launch_status("sparse_tile_kernel");
+}
+
+}  // namespace spt
+}  // namespace faq

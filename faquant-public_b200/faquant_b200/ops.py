@@ -1090,7 +1090,7 @@ def hif4_sparse_attention(
     """Attention of each new token over the tokens of the pages listed for it: ``q [T, H, D]`` bf16, returns
     ``[T, H, D]`` bf16 (``faq_hif4_sparse_attention``). ``selected`` int32 ``[T, Hkv, count]``
     (:func:`hif4_select_pages`) holds columns of the sequence's row of ``table``, in any order; entries below zero and
-    pages behind the token are passed over, a column listed twice counts twice, and no token sees keys behind
+    pages behind the token are passed over, a column listed twice counts once, and no token sees keys behind
     itself. With every visible page listed this is :func:`hif4_paged_attention`, up to the rounding of its sums.
     A row without a key is zero; rows beyond ``cu[B]`` stay as they are; pages that the table does not hold are
     left out and set ``FAQ_STATUS_BAD_PAGE``."""
@@ -1106,7 +1106,7 @@ def hif4_sparse_attention(
         raise ValueError("selected must be int32 [tokens, kv_heads, count]")
     selected = selected.contiguous()
     qs = q.stride()
-    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] < 8 or qs[1] < 8 or q.data_ptr() % 16:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()

@@ -543,11 +543,12 @@ int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads, int64_t q
 /*
  * K13 -- K9's attention over listed pages only: selected int32 [total, kv_heads, count] holds columns
  * of the token's sequence's row of the table, one list per kv head, in any order. Entries below zero and
- * pages behind the token are passed over, a column listed twice counts twice, keys behind the token are not
+ * pages behind the token are passed over, a column listed twice counts once, keys behind the token are not
  * seen; an entry whose page is missing is left out and sets FAQ_STATUS_BAD_PAGE. q, out and scale as in
  * faq_hif4_paged_attention (which a list of every page equals, up to the rounding of the sums). A row without a key is
  * zero; rows beyond cu[batch] are not written. No workspace. A row's bits depend on its own queries,
- * keys and list, scale, count, and through the split of the work on total, heads and kv_heads.
+ * keys and list, scale, and through the choice of the kernel and the split of the work on the call's sizes; where
+ * tokens are taken together, on cu and the lists of its neighbours.
  */
 int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t heads, int64_t q_token_stride,
                               int64_t q_head_stride, const void* pages, int64_t num_pages, int64_t page_stride,

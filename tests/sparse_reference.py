@@ -97,7 +97,8 @@ def select(q, keys, lens, new, page, count, first, last, missing=()):
 
 
 def attention(q, k, v, lens, new, page, selected, scale=None, missing=()):
-    """``(O, A)`` in fp64 over the listed pages, A = sum_k p_k |v_k|, from quantized packed keys and values."""
+    """``(O, A)`` in fp64 over the listed pages (each once), A = sum_k p_k |v_k|, from quantized packed keys
+    and values."""
     q, k, v = (t.double().cpu() for t in (q, k, v))
     h, d = k.shape[1:]
     group = q.shape[1] // h
@@ -107,7 +108,7 @@ def attention(q, k, v, lens, new, page, selected, scale=None, missing=()):
     for t, (b, pos) in enumerate(positions(lens, new)):
         for j in range(h):
             rows = []
-            for c in selected[t, j].tolist():
+            for c in sorted(set(selected[t, j].tolist())):
                 if c >= 0 and (b, c) not in missing:
                     rows += range(starts[b] + c * page, starts[b] + min(pos + 1, c * page + page))
             if not rows:

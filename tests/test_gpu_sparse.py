@@ -460,6 +460,17 @@ SHAPES = [  # heads, kv_heads, d, page, lens, new, count
     (16, 8, 128, 16, [600], [300], 6),
     (7, 7, 64, 4096, [5000], [1], 2),
     (1, 1, 128, 16, [4000], [1], 250),
+    # tokens taken together: one to 32 of them, all ratios of heads, one CTA or a cluster
+    (1, 1, 128, 16, [700], [200], 9),
+    (3, 1, 64, 16, [300, 5, 90], [100, 5, 33], 4),
+    (5, 1, 128, 64, [2000, 100], [64, 30], 6),
+    (33, 1, 64, 32, [200], [20], 3),
+    (100, 1, 128, 16, [150], [9], 5),
+    (64, 8, 128, 64, [1500], [130], 10),
+    (8, 1, 64, 4096, [9000], [16], 3),
+    (16, 2, 128, 16, [40] * 10, [20] * 10, 3),
+    (8, 1, 128, 16, [3500], [16], 100),
+    (4, 4, 64, 32, [3000, 2, 700], [90, 2, 1], 60),
 ]
 
 
@@ -483,27 +494,28 @@ def test_attention_over_listed_pages_matches_fp64(shape) -> None:
     assert _status() in (0, 2)
 
 
-@pytest.mark.parametrize("n", [1, 5, 90])
+@pytest.mark.parametrize("n", [1, 5, 8, 90])
 def test_every_page_listed_is_the_dense_attention(n) -> None:
     lens, page = [1000, 300], 32
     pool = Pool(lens, 2, 128, page, DEV)
     k, v = _randn(1300, 2, 128, seed=54), _randn(1300, 2, 128, seed=55)
     pool.write(k, v)
     q = _randn(2 * n, 8, 128, seed=56, scale=2.0)
-    lists = torch.arange(32, dtype=torch.int32).expand(2 * n, 2, 32)
+    lists = torch.arange(33, dtype=torch.int32).expand(2 * n, 2, 33)  # up to one behind the table
     dense, sparse = pool.attend(q, [n, n]), _attend(pool, q, [n, n], lists)
     _, size = ref.attention(q, quantized(k), quantized(v), lens, [n, n], page, lists)
     assert bool(((dense - sparse).double().abs().cpu() <= 2 * BOUND * size).all())
     _no_status()
 
 
-def test_rows_without_a_key_and_rows_left_alone() -> None:
+@pytest.mark.parametrize("heads", [3, 17])  # the kernel of single tokens, that of tiles
+def test_rows_without_a_key_and_rows_left_alone(heads) -> None:
     from faquant_b200 import _lib
 
     pool = Pool([4, 30], 1, 64, 16, DEV)
     k = _randn(34, 1, 64, seed=57)
     pool.write(k, k)
-    q = _randn(12, 3, 64, seed=58)
+    q = _randn(12, heads, 64, seed=58)
     lists = torch.zeros(12, 1, 2, dtype=torch.int32)
     lists[:, :, 1] = -5
     lists[8] = -1      # a token without a list
@@ -529,17 +541,18 @@ def test_rows_without_a_key_and_rows_left_alone() -> None:
     assert _status() == _lib.FAQ_STATUS_BAD_PAGE and bool(((out.double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
 
 
-def test_peaked_scores_ranges_and_not_a_number() -> None:
-    lens, new, page = [900], [6], 16
+@pytest.mark.parametrize("n", [6, 20])
+def test_peaked_scores_ranges_and_not_a_number(n) -> None:
+    lens, new, page = [900], [n], 16
     pool = Pool(lens, 1, 128, page, DEV)
     k, v = _randn(900, 1, 128, seed=59), _randn(900, 1, 128, seed=60)
     k[700] *= 30.0  # one key far above the others, found late
     v[3] *= 1e6     # and a value row of another magnitude
     v[600:] *= 1e-20
     pool.write(k, v)
-    q = _randn(6, 4, 128, seed=61)
+    q = _randn(n, 4, 128, seed=61)
     q[1] = 0
-    lists = torch.arange(57, dtype=torch.int32).expand(6, 1, 57)
+    lists = torch.arange(57, dtype=torch.int32).expand(n, 1, 57)
     for scale in (None, 0.002, 0.5):
         out = _attend(pool, q, new, lists, scale=scale)
         want, size = ref.attention(q, quantized(k), quantized(v), lens, new, page, lists, scale)
