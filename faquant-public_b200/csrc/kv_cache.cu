@@ -316,8 +316,9 @@ __device__ __forceinline__ void store_pairs(float* dst, bool vec, const uint32_t
 // A block of one head's K or V, as a warp loads it and hands it out: for K a lane has sixteen
 // channels of each group of two tokens, for V a sub-block of both tokens of two pairs.
 // each(expand, lane, f) calls f(token, group, unit, four bf16 pairs) for every eight channels 8
-// unit .. of a group. y = (n - 8) 2^(e - 3) times twice the scale is exact in bf16 (six
-// significant bits), so a pair costs one packed product.
+// unit .. of a group. The scale is multiplied into the exponent's power before the word is expanded:
+// with E = 2^(e - 3) times twice the scale (three significant bits) 136 E and (n - 8) E are exact in
+// bf16 (seven and six), so it costs one packed product a word.
 __device__ __forceinline__ uint32_t scale_pair(uint32_t code) {
   const uint32_t s = (code << 5) + (80u << 7);  // bf16 bits of twice the scale
   return s | (s << 16);
@@ -357,9 +358,7 @@ struct KBlock {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // pair j: channels j and 4 + j of sub-block 2 t + i
           uint32_t y[4];
-          expand.word(h ? w[1][2 * g + i] : w[0][2 * g + i], expand.exponents(eg, (7 - 4 * t - 2 * i) & 31), y);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = hmul2_bf16(y[j], s);
+          expand.word(h ? w[1][2 * g + i] : w[0][2 * g + i], hmul2_bf16(expand.exponents(eg, (7 - 4 * t - 2 * i) & 31), s), y);
           const uint32_t row[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
                                    __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)};
           f(r, g, 2 * t + i, row);
@@ -404,10 +403,8 @@ struct VBlock {
         uint32_t y[2][4];  // [quad]: pair j is channel j of both tokens
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          expand.word(h ? w[1][2 * g + q] : w[0][2 * g + q], expand.exponents(h ? e[1][2 * g + q] : e[0][2 * g + q], (7 - 2 * s) & 31),
-                      y[q]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[q][j] = hmul2_bf16(y[q][j], pair);
+          expand.word(h ? w[1][2 * g + q] : w[0][2 * g + q],
+                      hmul2_bf16(expand.exponents(h ? e[1][2 * g + q] : e[0][2 * g + q], (7 - 2 * s) & 31), pair), y[q]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {

@@ -431,7 +431,28 @@ struct Softmax {
   template <int PARTS, bool HOLES, typename F>
   __device__ __forceinline__ bool run(const Pages& pages, int b, int len, int k0, int count, int lim, F&& meanwhile) {
     constexpr int KEYS = TILE / PARTS;
-    auto mask = [&](int j, int part, float (&f)[KEYS]) {
+    const int row = this->row<PARTS>(), part = quarter / QUARTERS<PARTS> * 2 + half;
+    const int barrier = tile_barrier + quarter % QUARTERS<PARTS>;
+    const uint32_t p_row = smem_addr(p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
+    const int unit0 = (part * KEYS & 63) >> 3;
+    const float2 c2 = make_float2(scale_log2, scale_log2);
+    // Rows that are not there hold another sequence's queries, or what shared memory held: no score
+    // of theirs is above +inf, so they never raise the live rows' maxima, whose roundings would
+    // else depend on them.
+    m = lim == NO_ROW ? INFINITY : LOWEST;
+    l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < count; ++j, ++done) {
+      ok = ok && mbar_wait_warp(s_full, done & 1, site, j);
+      tc_fence_after();
+      float f[KEYS];
+      tmem_ldf<KEYS>(s_addr + part * KEYS, f);
+      tc_wait_ld();
+      reg_fencef<KEYS>(f);
+      // S_t is in registers: the tensor core may write the next one
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
       const int rel = lim - (k0 + j) * TILE - part * KEYS;
       if (__any_sync(0xffffffffu, rel < KEYS - 1)) {
 #pragma unroll
@@ -448,38 +469,6 @@ struct Softmax {
             if (none) f[x + i] = -INFINITY;
         }
       }
-    };
-    return run_masked<PARTS>(count, lim != NO_ROW, mask, meanwhile);
-  }
-
-  // The same with mask(j, part, f), which sets the scores of a row's keys of part `part` of key tile j that
-  // it does not see to -infinity; `there`: the row is one of the unit's.
-  template <int PARTS, typename Mask, typename F>
-  __device__ __forceinline__ bool run_masked(int count, bool there, Mask&& mask, F&& meanwhile) {
-    constexpr int KEYS = TILE / PARTS;
-    const int row = this->row<PARTS>(), part = quarter / QUARTERS<PARTS> * 2 + half;
-    const int barrier = tile_barrier + quarter % QUARTERS<PARTS>;
-    const uint32_t p_row = smem_addr(p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
-    const int unit0 = (part * KEYS & 63) >> 3;
-    const float2 c2 = make_float2(scale_log2, scale_log2);
-    // Rows that are not there hold another sequence's queries, or what shared memory held: no score
-    // of theirs is above +inf, so they never raise the live rows' maxima, whose roundings would
-    // else depend on them.
-    m = there ? LOWEST : INFINITY;
-    l = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < count; ++j, ++done) {
-      ok = ok && mbar_wait_warp(s_full, done & 1, site, j);
-      tc_fence_after();
-      float f[KEYS];
-      tmem_ldf<KEYS>(s_addr + part * KEYS, f);
-      tc_wait_ld();
-      reg_fencef<KEYS>(f);
-      // S_t is in registers: the tensor core may write the next one
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
-      mask(j, part, f);
       float mx[KEYS / 16];
 #pragma unroll
       for (int c = 0; c < KEYS / 16; ++c) {

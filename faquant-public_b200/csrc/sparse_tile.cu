@@ -109,6 +109,132 @@ static_assert(Smem<2>::bytes <= 227 * 1024, "shared memory");
 // tiles get the slots from cu[b] / T + b on.
 __host__ __device__ inline int64_t slots_of(int64_t total, int64_t batch, int tokens) { return total / tokens + batch; }
 
+// The softmax of a tile's rows (paged_prefill.cu) where a row sees some of a key tile's blocks only.
+template <int D>
+struct ListSoftmax : Softmax<D> {
+  using Base = Softmax<D>;
+  using Base::Base;
+
+  // `count` key tiles; keys(j, block) is how many keys of block `block` (0 .. 7) of key tile j the row sees.
+  // A block that none of the warp's rows sees costs nothing but its zeros. False: a wait ran out.
+  template <int PARTS, typename F>
+  __device__ __forceinline__ bool run(int count, bool there, F&& keys) {
+    constexpr int KEYS = TILE / PARTS, BLOCKS = KEYS / BLOCK;
+    const int row = this->template row<PARTS>(), part = this->quarter / Base::template QUARTERS<PARTS> * 2 + this->half;
+    const int barrier = this->tile_barrier + this->quarter % Base::template QUARTERS<PARTS>;
+    const uint32_t p_row = smem_addr(this->p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
+    const int unit0 = (part * KEYS & 63) >> 3;
+    const float2 c2 = make_float2(this->scale_log2, this->scale_log2);
+    this->m = there ? LOWEST : INFINITY;  // rows that are not there never raise the others' maxima
+    this->l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < count; ++j, ++this->done) {
+      int seen[BLOCKS];
+#pragma unroll
+      for (int c = 0; c < BLOCKS; ++c) seen[c] = keys(j, part * BLOCKS + c);
+      ok = ok && mbar_wait_warp(this->s_full, this->done & 1, this->site, j);
+      tc_fence_after();
+      float f[KEYS];
+      pre::tmem_ldf<KEYS>(this->s_addr + part * KEYS, f);
+      tc_wait_ld();
+      pre::reg_fencef<KEYS>(f);
+      // S is in registers: the tensor core may write the next one
+      tc_fence_before();
+      __syncwarp();
+      if (this->lane == 0) mbar_arrive(this->s_free);
+      float mine = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < BLOCKS; ++c) {
+        float* x = f + BLOCK * c;
+        if (__any_sync(0xffffffffu, seen[c] > 0 && seen[c] < BLOCK)) {  // the token's own place
+#pragma unroll
+          for (int k = 0; k < BLOCK; ++k)
+            if (k >= seen[c]) x[k] = -INFINITY;
+        }
+        float top = pre::max3(x[0], x[1], x[2]);
+#pragma unroll
+        for (int k = 3; k < 15; k += 2) top = pre::max3(top, x[k], x[k + 1]);
+        top = fmaxf(top, x[15]);
+        mine = fmaxf(mine, seen[c] > 0 ? top : -INFINITY);
+      }
+      // raise the rows' maxima when a part has a score far above them (or has to give up)
+      float a = 1.0f;
+      const bool raise = pre::bar_or(barrier, 32 * PARTS, __fmul_rn(mine, this->scale_log2) > this->m + pat::RAISE || !ok);
+      if (raise) {
+        if (j > 0) ok = ok && mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 2, j);
+        float all[PARTS];
+        if (!this->template exchange<PARTS>(ok, barrier, row, part, mine, all)) return false;
+        float top = all[0];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) top = fmaxf(top, all[i]);
+        const float next = fmaxf(__fmul_rn(top, this->scale_log2) - pat::LIFT, this->m);
+        a = ex2(0.5f * (this->m - next));
+        this->m = next;
+        this->l = this->l * a * a;
+      }
+      const float2 mneg = make_float2(-this->m, -this->m);
+      uint32_t w[KEYS / 2];
+#pragma unroll
+      for (int c = 0; c < BLOCKS; ++c) {
+        if (__any_sync(0xffffffffu, seen[c] > 0)) {
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int x = 0; x < BLOCK / 2; ++x) {
+            const float2 d = __ffma2_rn(make_float2(f[BLOCK * c + 2 * x], f[BLOCK * c + 2 * x + 1]), c2, mneg);
+            const float2 e = make_float2(ex2(d.x), ex2(d.y));
+            sum[x & 1] = __fadd2_rn(sum[x & 1], e);
+            const uint32_t pair = pack_bf16(e.x, e.y);
+            w[BLOCK / 2 * c + x] = seen[c] > 0 ? pair : 0u;  // whatever the score was
+          }
+          const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+          if (seen[c] > 0) this->l += s2.x + s2.y;
+        } else {
+#pragma unroll
+          for (int x = 0; x < BLOCK / 2; ++x) w[BLOCK / 2 * c + x] = 0u;
+        }
+      }
+      // the product of the step before has read P, and O is its
+      if (j > 0) ok = mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 2, j);
+#pragma unroll
+      for (int u = 0; u < KEYS / 8; ++u)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (((unit0 + u) ^ (row & 7)) << 4)),
+                     "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
+                     : "memory");
+      fence_proxy_async_smem();  // the tensor core reads P through the async proxy
+      tc_fence_after();
+      if (raise && j > 0 && this->template first_copy<PARTS>()) {
+        const float2 a2 = make_float2(a, a);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          float o[32];
+          tmem_ld32f(this->o_addr + 32 * c, o);
+          tc_wait_ld();
+          reg_fence32f(o);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float2 v = __fmul2_rn(__fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2), a2);
+            o[2 * x] = v.x;
+            o[2 * x + 1] = v.y;
+          }
+          tmem_st32f(this->o_addr + 32 * c, o);
+        }
+        tc_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (this->lane == 0) mbar_arrive(this->p_full);
+    }
+    ok = ok && mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 4, count);
+    tc_fence_after();
+    float all[PARTS];
+    if (!this->template exchange<PARTS>(ok, barrier, row, part, this->l, all)) return false;
+    this->l = all[0];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) this->l += all[i];  // the same sum in all parts
+    return true;
+  }
+};
+
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_constant__ QMaps maps, Params P, int split) {
   using L = Smem<NG>;
@@ -331,29 +457,20 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
-    Softmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
+    ListSoftmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
     auto work = [&](auto parts) {
-      constexpr int PARTS = decltype(parts)::value, KEYS = TILE / PARTS;
+      constexpr int PARTS = decltype(parts)::value;
       const int row = sm.template row<PARTS>(), tok = row / P.group;
       const bool live = tok < tokens;
       const int64_t pos = pos0 + tok;
-      auto mask = [&](int j, int part, float (&f)[KEYS]) {
-#pragma unroll
-        for (int x = 0; x < KEYS; x += BLOCK) {
-          const int i = (k0 + j) * 8 + (part * KEYS + x) / BLOCK, e = i >> block_shift;
-          // keys of the block that the row sees: those up to its own place, if its token lists the page
-          int keys = 0;
-          if (live && i < blocks && (s_mark[e] >> tok & 1)) {
-            const int64_t left = pos - ((static_cast<int64_t>(s_column[e]) << p.page_shift) + ((i & in_page) << 4)) + 1;
-            keys = static_cast<int>(std::min<int64_t>(std::max<int64_t>(left, 0), BLOCK));
-          }
-          if (__all_sync(0xffffffffu, keys == BLOCK)) continue;
-#pragma unroll
-          for (int k = 0; k < BLOCK; ++k)
-            if (k >= keys) f[x + k] = -INFINITY;
-        }
+      const int own_column = pos < 0 ? 0x7fffffff : static_cast<int>(std::min<int64_t>(pos >> p.page_shift, 0x7fffffff));
+      const int own_keys = static_cast<int>(pos & ((1 << p.page_shift) - 1)) + 1;  // it sees of its own page
+      auto keys = [&](int j, int block) {
+        const int i = (k0 + j) * 8 + block, e = i >> block_shift;
+        if (!live || i >= blocks || !(s_mark[e] >> tok & 1)) return 0;
+        return s_column[e] == own_column ? min(max(own_keys - ((i & in_page) << 4), 0), BLOCK) : BLOCK;
       };
-      if (count > 0 && !sm.template run_masked<PARTS>(count, live, mask, [] {})) return;
+      if (count > 0 && !sm.template run<PARTS>(count, live, keys)) return;
       if (lane == 0) atomicAdd(&s_well, 1);
       if (count == 0 || !sm.template first_copy<PARTS>()) return;
       const int row_head = row - tok * P.group;
