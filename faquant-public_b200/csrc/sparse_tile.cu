@@ -3,8 +3,7 @@
 //
 // Neighbouring tokens mostly list the same pages. Expanding a page's codes for each token apart is
 // what the kernel of single tokens (sparse_attention.cu) spends its time on; here a page is expanded
-// once for all rows of a tile, on the tensor cores of paged_chunk.cu (the same roles, operands and
-// softmax), and a row's scores with pages that its token does not list are masked. At the start
+// once for all rows of a tile, on the tensor cores as in paged_chunk.cu (the same operands), and a row's scores with pages that its token does not list are masked. At the start
 // the CTA marks, per column, which of its tokens list it (one bit each, up to 32 tokens), and writes the
 // marked columns in order: page, column, tokens. A column counts once, however often it is listed.
 // Key tiles are 8 blocks of 16 tokens, as they come in that order.
@@ -62,7 +61,6 @@ __device__ __forceinline__ int cluster_load_int(uint32_t addr) {
 namespace spt {
 
 using namespace kvp;
-using chk::QMaps;
 using pat::ex2;
 using pat::LOWEST;
 using pat::pack_bf16;
@@ -74,8 +72,6 @@ using pre::idesc_pv;
 using pre::mma_ss;
 using pre::o_col;
 using pre::s_col;
-using pre::Softmax;
-using pre::THREADS;
 using pre::TILE;
 using pre::TMEM_COLS;
 using spa::cluster_load;
@@ -83,6 +79,9 @@ using spa::cluster_load4;
 using spa::cluster_load_int;
 using spa::Params;
 
+constexpr int SOFTMAX_WARPS = 16, EXPAND_WARPS = 8;
+constexpr int THREADS = 32 * (SOFTMAX_WARPS + EXPAND_WARPS + 4);  // and a warpgroup for Q and the products
+constexpr int PRODUCTS = SOFTMAX_WARPS + EXPAND_WARPS;  // the warp that issues them
 constexpr int MAX_UNION = 2048;  // columns of a tile's union
 // the table's columns whose marks fit where K and V will be
 __host__ __device__ constexpr int columns(int d) { return d / 64 * 4 * CHUNK / 4; }
@@ -95,10 +94,10 @@ struct Smem {
   static constexpr int k = q + tile;
   static constexpr int v = k + 2 * tile;
   static constexpr int p = v + 2 * tile;
-  static constexpr int page = p + 2 * CHUNK;  // [MAX_UNION]
-  static constexpr int col = page + 4 * MAX_UNION;
-  static constexpr int mark = col + 4 * MAX_UNION;
-  static constexpr int bar = mark + 4 * MAX_UNION;
+  static constexpr int page = p + 2 * CHUNK;        // [MAX_UNION]
+  static constexpr int entry = page + 4 * MAX_UNION;  // [MAX_UNION + 8], the last ones' tokens none
+  static constexpr int scratch = entry + 8 * (MAX_UNION + 8);  // [4][TILE]
+  static constexpr int bar = scratch + 16 * TILE;
   static constexpr int bytes = 1024 + bar + 256;
   // at the end, where K and V were: O [TILE][D], m and l [TILE]
   static constexpr int o = k;
@@ -109,39 +108,76 @@ static_assert(Smem<2>::bytes <= 227 * 1024, "shared memory");
 // tiles get the slots from cu[b] / T + b on.
 __host__ __device__ inline int64_t slots_of(int64_t total, int64_t batch, int tokens) { return total / tokens + batch; }
 
-// The softmax of a tile's rows (paged_prefill.cu) where a row sees some of a key tile's blocks only.
-template <int D>
-struct ListSoftmax : Softmax<D> {
-  using Base = Softmax<D>;
-  using Base::Base;
+template <int N>
+__device__ __forceinline__ void tmem_stf(uint32_t taddr, const float* v) {
+  if constexpr (N == 32) {
+    tmem_st32f(taddr, v);
+  } else {
+    static_assert(N == 16, "16 or 32 columns");
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+            taddr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+  }
+}
 
-  // `count` key tiles; keys(j, block) is how many keys of block `block` (0 .. 7) of key tile j the row sees.
-  // A block that none of the warp's rows sees costs nothing but its zeros. False: a wait ran out.
-  template <int PARTS, typename F>
+// The softmax of a tile's rows, of which each sees some of a key tile's blocks only, by sixteen warps.
+// TMEM lets a warp read the lanes of its own quarter (warp % 4), so the four warps of a quarter share
+// its 32 rows: part warp / 4 has the keys 32 part .. of every key tile and that quarter of O's channels.
+// (Eight warps with 64 keys a thread spilled their registers and took XXX us instead of YYY.)
+template <int D>
+struct Softmax {
+  static constexpr int KEYS = TILE / 4, BLOCKS = KEYS / BLOCK, CHANNELS = D / 4;
+  int lane, quarter, part, row;
+  uint32_t s_addr, o_addr, p_row;
+  float* scratch;  // [4][TILE]
+  uint32_t s_full, s_free, p_full, pv_done;
+  float scale_log2, m, l;  // the reference maximum (log2) and, after run(), the row's sum
+
+  __device__ __forceinline__ Softmax(uint32_t tmem, int warp, int lane_, uint8_t* p, float* x, uint64_t* full, uint64_t* free_,
+                                     uint64_t* pfull, uint64_t* pv, float scale)
+      : lane(lane_), quarter(warp & 3), part(warp >> 2), scratch(x), s_full(smem_addr(full)), s_free(smem_addr(free_)),
+        p_full(smem_addr(pfull)), pv_done(smem_addr(pv)), scale_log2(scale) {
+    row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    s_addr = tmem + lanes + s_col(0) + part * KEYS;
+    o_addr = tmem + lanes + o_col(0) + part * CHANNELS;
+    p_row = smem_addr(p) + (part >> 1) * CHUNK + row * 128;
+  }
+
+  // The values of a row's parts, among its four warps. They come here together, whatever happened
+  // before: `ok` tells whether all are well.
+  __device__ __forceinline__ bool exchange(bool ok, float mine, float (&all)[4]) {
+    scratch[part * TILE + row] = mine;
+    const bool well = pre::bar_and(1 + quarter, 128, ok);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all[i] = scratch[i * TILE + row];
+    return pre::bar_and(1 + quarter, 128, well);  // read: it may be written again
+  }
+
+  // `count` key tiles; keys(j, block) is how many keys of block `block` (0 .. 7) of key tile j the row
+  // sees. A block that none of the warp's rows sees costs nothing but its zeros. False: a wait ran out.
+  template <typename F>
   __device__ __forceinline__ bool run(int count, bool there, F&& keys) {
-    constexpr int KEYS = TILE / PARTS, BLOCKS = KEYS / BLOCK;
-    const int row = this->template row<PARTS>(), part = this->quarter / Base::template QUARTERS<PARTS> * 2 + this->half;
-    const int barrier = this->tile_barrier + this->quarter % Base::template QUARTERS<PARTS>;
-    const uint32_t p_row = smem_addr(this->p_tile + (part * KEYS >> 6) * CHUNK + row * 128);
-    const int unit0 = (part * KEYS & 63) >> 3;
-    const float2 c2 = make_float2(this->scale_log2, this->scale_log2);
-    this->m = there ? LOWEST : INFINITY;  // rows that are not there never raise the others' maxima
-    this->l = 0.0f;
+    m = there ? LOWEST : INFINITY;  // rows that are not there never raise the others' maxima
+    l = 0.0f;
     bool ok = true;
-    for (int j = 0; j < count; ++j, ++this->done) {
+    for (int j = 0; j < count; ++j) {
       int seen[BLOCKS];
 #pragma unroll
       for (int c = 0; c < BLOCKS; ++c) seen[c] = keys(j, part * BLOCKS + c);
-      ok = ok && mbar_wait_warp(this->s_full, this->done & 1, this->site, j);
+      ok = ok && mbar_wait_warp(s_full, j & 1, 98, j);
       tc_fence_after();
       float f[KEYS];
-      pre::tmem_ldf<KEYS>(this->s_addr + part * KEYS, f);
+      tmem_ld32f(s_addr, f);
       tc_wait_ld();
-      pre::reg_fencef<KEYS>(f);
+      reg_fence32f(f);
       // S is in registers: the tensor core may write the next one
       tc_fence_before();
       __syncwarp();
-      if (this->lane == 0) mbar_arrive(this->s_free);
+      if (lane == 0) mbar_arrive(s_free);
       float mine = -INFINITY;
 #pragma unroll
       for (int c = 0; c < BLOCKS; ++c) {
@@ -159,20 +195,18 @@ struct ListSoftmax : Softmax<D> {
       }
       // raise the rows' maxima when a part has a score far above them (or has to give up)
       float a = 1.0f;
-      const bool raise = pre::bar_or(barrier, 32 * PARTS, __fmul_rn(mine, this->scale_log2) > this->m + pat::RAISE || !ok);
+      const bool raise = pre::bar_or(1 + quarter, 128, __fmul_rn(mine, scale_log2) > m + pat::RAISE || !ok);
       if (raise) {
-        if (j > 0) ok = ok && mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 2, j);
-        float all[PARTS];
-        if (!this->template exchange<PARTS>(ok, barrier, row, part, mine, all)) return false;
-        float top = all[0];
-#pragma unroll
-        for (int i = 1; i < PARTS; ++i) top = fmaxf(top, all[i]);
-        const float next = fmaxf(__fmul_rn(top, this->scale_log2) - pat::LIFT, this->m);
-        a = ex2(0.5f * (this->m - next));
-        this->m = next;
-        this->l = this->l * a * a;
+        if (j > 0) ok = ok && mbar_wait_warp(pv_done, (j - 1) & 1, 99, j);
+        float all[4];
+        if (!exchange(ok, mine, all)) return false;
+        const float top = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3]));
+        const float next = fmaxf(__fmul_rn(top, scale_log2) - pat::LIFT, m);
+        a = ex2(0.5f * (m - next));
+        m = next;
+        l = l * a * a;
       }
-      const float2 mneg = make_float2(-this->m, -this->m);
+      const float2 c2 = make_float2(scale_log2, scale_log2), mneg = make_float2(-m, -m);
       uint32_t w[KEYS / 2];
 #pragma unroll
       for (int c = 0; c < BLOCKS; ++c) {
@@ -187,56 +221,72 @@ struct ListSoftmax : Softmax<D> {
             w[BLOCK / 2 * c + x] = seen[c] > 0 ? pair : 0u;  // whatever the score was
           }
           const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-          if (seen[c] > 0) this->l += s2.x + s2.y;
+          if (seen[c] > 0) l += s2.x + s2.y;
         } else {
 #pragma unroll
           for (int x = 0; x < BLOCK / 2; ++x) w[BLOCK / 2 * c + x] = 0u;
         }
       }
       // the product of the step before has read P, and O is its
-      if (j > 0) ok = mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 2, j);
+      if (j > 0) ok = mbar_wait_warp(pv_done, (j - 1) & 1, 99, j);
 #pragma unroll
-      for (int u = 0; u < KEYS / 8; ++u)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (((unit0 + u) ^ (row & 7)) << 4)),
+      for (int u = 0; u < KEYS / 8; ++u)  // key chunk, row, unit at unit ^ (row % 8), as TMA would lay it out
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((((part & 1) * 4 + u) ^ (row & 7)) << 4)),
                      "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3])
                      : "memory");
       fence_proxy_async_smem();  // the tensor core reads P through the async proxy
       tc_fence_after();
-      if (raise && j > 0 && this->template first_copy<PARTS>()) {
-        const float2 a2 = make_float2(a, a);
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          float o[32];
-          tmem_ld32f(this->o_addr + 32 * c, o);
-          tc_wait_ld();
-          reg_fence32f(o);
+      if (raise && j > 0) {
+        float o[CHANNELS];
+        pre::tmem_ldf<CHANNELS>(o_addr, o);
+        tc_wait_ld();
+        pre::reg_fencef<CHANNELS>(o);
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float2 v = __fmul2_rn(__fmul2_rn(make_float2(o[2 * x], o[2 * x + 1]), a2), a2);
-            o[2 * x] = v.x;
-            o[2 * x + 1] = v.y;
-          }
-          tmem_st32f(this->o_addr + 32 * c, o);
-        }
+        for (int x = 0; x < CHANNELS; ++x) o[x] = o[x] * a * a;
+        tmem_stf<CHANNELS>(o_addr, o);
         tc_wait_st();
       }
       tc_fence_before();
       __syncwarp();
-      if (this->lane == 0) mbar_arrive(this->p_full);
+      if (lane == 0) mbar_arrive(p_full);
     }
-    ok = ok && mbar_wait_warp(this->pv_done, (this->done - 1) & 1, this->site + 4, count);
+    ok = ok && mbar_wait_warp(pv_done, (count - 1) & 1, 99, count);
     tc_fence_after();
-    float all[PARTS];
-    if (!this->template exchange<PARTS>(ok, barrier, row, part, this->l, all)) return false;
-    this->l = all[0];
-#pragma unroll
-    for (int i = 1; i < PARTS; ++i) this->l += all[i];  // the same sum in all parts
+    float all[4];
+    if (!exchange(ok, l, all)) return false;
+    l = (all[0] + all[1]) + (all[2] + all[3]);
     return true;
+  }
+
+  // O of the row: to dst (bf16, normalized) or, unnormalized with m and l, to the rows `o` of a
+  // partial. Whole warps take part; only live ones store.
+  __device__ __forceinline__ void store(bool live, float* o, __nv_bfloat16* dst) {
+    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
+    float v[CHANNELS];
+    pre::tmem_ldf<CHANNELS>(o_addr, v);
+    tc_wait_ld();
+    pre::reg_fencef<CHANNELS>(v);
+    if (live && o) {
+      float4* d4 = reinterpret_cast<float4*>(o + row * D + part * CHANNELS);
+#pragma unroll
+      for (int x = 0; x < CHANNELS / 4; ++x) d4[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+      if (part == 0) {
+        o[TILE * D + row] = m;
+        o[TILE * D + TILE + row] = l;
+      }
+    } else if (live) {
+      uint4* d4 = reinterpret_cast<uint4*>(dst + part * CHANNELS);
+#pragma unroll
+      for (int x = 0; x < CHANNELS / 8; ++x)
+        d4[x] = make_uint4(pack_bf16(v[8 * x] * inv, v[8 * x + 1] * inv), pack_bf16(v[8 * x + 2] * inv, v[8 * x + 3] * inv),
+                           pack_bf16(v[8 * x + 4] * inv, v[8 * x + 5] * inv), pack_bf16(v[8 * x + 6] * inv, v[8 * x + 7] * inv));
+    }
+    tc_fence_before();
   }
 };
 
 template <int NG>
-__global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_constant__ QMaps maps, Params P, int split) {
+__global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_constant__ CUtensorMap map_q, Params P, int split) {
   using L = Smem<NG>;
   constexpr int D = 64 * NG, WARPS = THREADS / 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -253,8 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   uint64_t* pv_done = bars + 13;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   int* s_page = reinterpret_cast<int*>(base + L::page);
-  int* s_column = reinterpret_cast<int*>(base + L::col);
-  uint32_t* s_mark = reinterpret_cast<uint32_t*>(base + L::mark);
+  int2* s_entry = reinterpret_cast<int2*>(base + L::entry);  // a page's first block in the sequence, its tokens
   __shared__ int64_t s_scan[WARPS];
   __shared__ int s_well;  // softmax warps that came to their end
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -285,19 +334,19 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     s_well = 0;
     mbar_init(smem_addr(q_full), 1);
     mbar_init(smem_addr(s_full), 1);
-    mbar_init(smem_addr(s_free), 8);
-    mbar_init(smem_addr(p_full), 8);
+    mbar_init(smem_addr(s_free), SOFTMAX_WARPS);
+    mbar_init(smem_addr(p_full), SOFTMAX_WARPS);
     mbar_init(smem_addr(pv_done), 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&k_full[i]), 8);  // the eight expanding warps
+      mbar_init(smem_addr(&k_full[i]), EXPAND_WARPS);
       mbar_init(smem_addr(&k_empty[i]), 1);
-      mbar_init(smem_addr(&v_full[i]), 8);
+      mbar_init(smem_addr(&v_full[i]), EXPAND_WARPS);
       mbar_init(smem_addr(&v_empty[i]), 1);
     }
     fence_barrier_init();
-    for (int i = 0; i < 3; ++i) tma_prefetch_desc(&maps.q[i]);
+    tma_prefetch_desc(&map_q);
   }
-  if (warp == 18) {
+  if (warp == PRODUCTS) {
     tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
@@ -335,34 +384,32 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     for (int c = begin; c < end; ++c)
       if (marks[c]) {
         s_page[i] = p.table[b * p.table_ld + c];
-        s_column[i] = c;
-        s_mark[i++] = marks[c];
+        s_entry[i++] = make_int2(c << (p.page_shift - 4), static_cast<int>(marks[c]));
       }
+    if (tid < 8) s_entry[found + tid] = make_int2(0, 0);
   }
   __syncthreads();
   const int block_shift = p.page_shift - 4, in_page = (1 << block_shift) - 1;
   // blocks of the union; of the last token's own page those up to it
-  const bool own = found > 0 && s_column[found - 1] == last_pos >> p.page_shift;
+  const bool own = found > 0 && s_entry[found - 1].x >> block_shift == last_pos >> p.page_shift;
   const int blocks = own ? ((found - 1) << block_shift) + (static_cast<int>(last_pos & ((1 << p.page_shift) - 1)) >> 4) + 1
                          : found << block_shift;
   const int tiles = (blocks + 7) >> 3;
   const int k0 = static_cast<int>(static_cast<int64_t>(tiles) * rank / split);
   const int count = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / split) - k0;
-  const int copies = tokens * P.group <= 32 ? 4 : tokens * P.group <= 64 ? 2 : 1;  // of the rows, see Softmax
 
-  // Registers: 640 x 96 at launch = 512 x 104 + 128 x 64.
-  if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::: "memory");
-    if (warp == 16) {
+  // Registers: 896 x 72 at launch = 512 x 72 + 256 x 80 + 128 x 56.
+  if (warp >= SOFTMAX_WARPS + EXPAND_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n" ::: "memory");
+    if (warp == PRODUCTS + 1) {
       if (lane == 0 && count > 0) {
-        const int rows = TILE / copies, map = copies >> 1;  // the box of 128, 64 or 32 rows
-        mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(copies * (rows / P.group) * P.group) * 128 * NG);
-        for (int c = 0; c < NG * copies; ++c)
-          tma_load_3d(smem_addr(base + L::q + (c / copies) * CHUNK + c % copies * rows * 128), &maps.q[map],
-                      smem_addr(q_full), c / copies * 64, head * P.group, static_cast<int>(c0 + tok0));
+        mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(T * P.group) * 128 * NG);
+        for (int c = 0; c < NG; ++c)
+          tma_load_3d(smem_addr(base + L::q + c * CHUNK), &map_q, smem_addr(q_full), c * 64, head * P.group,
+                      static_cast<int>(c0 + tok0));
         mbar_wait_site(smem_addr(q_full), 0, 90, 0);  // (bounded) it is there before the CTA's end
       }
-    } else if (warp == 18) {
+    } else if (warp == PRODUCTS) {
       // the whole warp walks the steps, one elected lane issues (paged_prefill.cu)
       const uint32_t q_desc = sw128_desc_lo(smem_addr(base + L::q), 16);
       const uint32_t k_desc = sw128_desc_lo(smem_addr(base + L::k), 16);
@@ -410,10 +457,10 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp >= 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
+  } else if (warp >= SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 80;\n" ::: "memory");
     // ------------------------------------------------------------ expansion: block ew of each key tile
-    const int ew = warp - 8;
+    const int ew = warp - SOFTMAX_WARPS;
     const int64_t v_off = (static_cast<int64_t>(p.kv_heads) << block_shift) * block_bytes(NG);  // from a page's K to its V
     // where block ew of tile j is (null: past the end; the softmax leaves such keys out, and the
     // registers' last block stands in for them, whose values are finite)
@@ -456,33 +503,29 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
       if (src) vb.load(src + v_off, lane);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
-    ListSoftmax<D> sm(tmem, 0, warp, lane, base + L::p, s_full, s_free, p_full, pv_done, P.scale_log2);
-    auto work = [&](auto parts) {
-      constexpr int PARTS = decltype(parts)::value;
-      const int row = sm.template row<PARTS>(), tok = row / P.group;
-      const bool live = tok < tokens;
-      const int64_t pos = pos0 + tok;
-      const int own_column = pos < 0 ? 0x7fffffff : static_cast<int>(std::min<int64_t>(pos >> p.page_shift, 0x7fffffff));
-      const int own_keys = static_cast<int>(pos & ((1 << p.page_shift) - 1)) + 1;  // it sees of its own page
-      auto keys = [&](int j, int block) {
-        const int i = (k0 + j) * 8 + block, e = i >> block_shift;
-        if (!live || i >= blocks || !(s_mark[e] >> tok & 1)) return 0;
-        return s_column[e] == own_column ? min(max(own_keys - ((i & in_page) << 4), 0), BLOCK) : BLOCK;
-      };
-      if (count > 0 && !sm.template run<PARTS>(count, live, keys)) return;
-      if (lane == 0) atomicAdd(&s_well, 1);
-      if (count == 0 || !sm.template first_copy<PARTS>()) return;
-      const int row_head = row - tok * P.group;
-      sm.store(live, split == 1 ? nullptr : reinterpret_cast<float*>(base + L::o), TILE, row,
-               P.out + (c0 + tok0 + (live ? tok : 0)) * P.ot + (static_cast<int64_t>(head) * P.group + row_head) * P.oh);
+    Softmax<D> sm(tmem, warp, lane, base + L::p, reinterpret_cast<float*>(base + L::scratch), s_full, s_free, p_full, pv_done,
+                  P.scale_log2);
+    const int row = sm.row, tok = row / P.group;
+    const bool live = tok < tokens;
+    const int sees = static_cast<int>(pos0) + tok + 1;  // keys, of the pages its token lists
+    const uint32_t bit = live ? 1u << tok : 0u;
+    const int block0 = k0 * 8;
+    auto keys = [&](int j, int block) {
+      const int i = block0 + j * 8 + block;
+      const int2 e = s_entry[i >> block_shift];
+      const int left = min(max(sees - ((e.x + (i & in_page)) << 4), 0), BLOCK);
+      return e.y & bit ? left : 0;
     };
-    if (copies == 4) work(std::integral_constant<int, 8>());
-    else if (copies == 2) work(std::integral_constant<int, 4>());
-    else work(std::integral_constant<int, 2>());
+    const bool ok = count == 0 || sm.run(count, live, keys);
+    if (ok && lane == 0) atomicAdd(&s_well, 1);
+    if (ok && count > 0) {
+      const int row_head = row - tok * P.group;
+      sm.store(live, split == 1 ? nullptr : reinterpret_cast<float*>(base + L::o),
+               P.out + (c0 + tok0 + (live ? tok : 0)) * P.ot + (static_cast<int64_t>(head) * P.group + row_head) * P.oh);
+    }
   }
   __syncthreads();
-  if (warp == 18) {
+  if (warp == PRODUCTS) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
@@ -503,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   bool all = true;
   int parts = 0;  // bit k: CTA k had key tiles
   for (int k = 0; k < split; ++k) {
-    all = all && cluster_load_int(mapa_shared(smem_addr(&s_well), k)) == 8;
+    all = all && cluster_load_int(mapa_shared(smem_addr(&s_well), k)) == SOFTMAX_WARPS;
     if (static_cast<int64_t>(tiles) * (k + 1) / split > static_cast<int64_t>(tiles) * k / split) parts |= 1 << k;
   }
   for (int i = tid + THREADS * rank; i < rows * (D / 4); i += THREADS * split) {
@@ -534,15 +577,12 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
 template <int NG>
 static int launch(const Params& P, int64_t heads, void* stream) {
   constexpr int D = 64 * NG;
-  QMaps maps;
+  CUtensorMap map_q;
   const uint64_t dims[3] = {D, static_cast<uint64_t>(heads), static_cast<uint64_t>(P.total)};
   const uint64_t str[2] = {static_cast<uint64_t>(P.qh) * 2, static_cast<uint64_t>(P.qt) * 2};
-  int rc = FAQ_OK;
-  for (int i = 0; i < 3; ++i) {
-    const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(std::max((TILE >> i) / P.group, 1))};
-    rc = make_tmap(&maps.q[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-  }
+  const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(tile_tokens(P.group))};
+  int rc = make_tmap(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
   auto kern = sparse_tile_kernel<NG>;
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
   rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
@@ -553,7 +593,7 @@ static int launch(const Params& P, int64_t heads, void* stream) {
   int split = 1;
   while (split < 8 && units * split * 2 <= num_sms() && tiles >= 4 * split) split *= 2;
   FAQ_CHECK_ARG(units * split < (int64_t(1) << 31), "too many tokens for one call");
-  FAQ_CUDA(launch_clusters(kern, units * split, THREADS, Smem<NG>::bytes, split, stream, maps, P, split));
+  FAQ_CUDA(launch_clusters(kern, units * split, THREADS, Smem<NG>::bytes, split, stream, map_q, P, split));
   return launch_status("sparse_tile_kernel");
 }
 
