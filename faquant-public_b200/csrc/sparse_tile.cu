@@ -490,13 +490,13 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
         };
       };
       if (!mbar_wait_warp(smem_addr(&k_empty[st]), ((step >> 1) & 1) ^ 1, 96, step)) break;
-      kb.template each<1>(expand, lane, write(base + L::k + st * L::tile));
+      kb.template each<2>(expand, lane, write(base + L::k + st * L::tile));
       fence_proxy_async_smem();  // the tensor core reads it through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
       if (src) kb.load(src, lane);
       if (!mbar_wait_warp(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 97, step)) break;
-      vb.template each<1>(expand, lane, write(base + L::v + st * L::tile));
+      vb.template each<2>(expand, lane, write(base + L::v + st * L::tile));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));

@@ -707,19 +707,17 @@ def _ragged(pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, lens: to
         raise TypeError("pages must be a uint8 tensor [num_pages, ...]")
     if len(shape) == 4 and (shape[1] != 2 or shape[2] != kv_heads):
         raise ValueError("pages of four dimensions are [num_pages, 2, kv_heads, bytes]")
-    page_stride = inner = 1
-    for n in shape[1:]:
-        inner *= n
-    whole = inner == size
     if pages.is_contiguous():
         page_stride = size
+        whole = pages.numel() == shape[0] * size
     else:
         stride = pages.stride()
         page_stride = stride[0] if shape[0] > 1 else size
-        inner = 1
+        whole, inner = True, 1
         for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
             whole = whole and (st == inner or n == 1)
             inner *= n
+        whole = whole and inner == size
     if not whole:
         raise ValueError("a page must be hif4_page_bytes(kv_heads, head_dim, page_size) contiguous bytes")
     return ((pages.data_ptr(), shape[0], page_stride, page_size), _batch(table, cu, lens))
@@ -731,10 +729,11 @@ def _batch(table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor) -> tuple:
     int32 = torch.int32
     if table.dtype is not int32 or cu.dtype is not int32 or lens.dtype is not int32:
         raise TypeError("table, cu and lens must be int32")
-    batch = lens.shape[0] if lens.dim() == 1 else -1
-    if table.dim() != 2 or table.shape[0] != batch or cu.shape != (batch + 1,):
+    shape, rows = table.shape, lens.shape
+    if len(rows) != 1 or len(shape) != 2 or shape[0] != rows[0] or cu.shape != (rows[0] + 1,):
         raise ValueError("table must be [batch, columns], cu [batch + 1] and lens [batch]")
-    columns = ld = table.shape[1]
+    batch, columns = shape
+    ld = columns
     if not table.is_contiguous():
         ld, unit = table.stride()
         if unit != 1 and columns > 1:
@@ -890,18 +889,16 @@ def hif4_paged_attention(
     return out
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call_on(device: torch.device, name: str, *args) -> None:
-    """A C call for ``device``'s tensors, whichever device is the current one."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args)
+    """A C call for ``device``'s tensors on its current stream, whichever device is the current one."""
+    if device.index == _current_device():
+        _lib.call(name, *args, _stream(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args)
-
-
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with unit stride in its last dimension."""
-    return t if t.stride(-1) == 1 else t.contiguous()
+            _lib.call(name, *args, _stream(device))
 
 
 def hif4_kv_append(
@@ -940,50 +937,74 @@ def hif4_kv_append(
     zero, or beyond the tables, which sets ``FAQ_STATUS_BAD_BOUND``) is not written, its row of q is zero;
     rows beyond ``cu[B]`` stay as they are."""
     device = _require_cuda(q, k, v, pages, table, cu, lens, cos, sin, q_norm, k_norm, smooth_scale, key_offset, out)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[0] != ks[0] or qs[2] != ks[2]:
         raise ValueError("q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("q, k and v must have one dtype")
-    total, heads, d = q.shape
-    h = k.shape[1]
+    total, heads, d = qs
+    h = ks[1]
     pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
     if h == 0 or heads % h or heads == 0:
         raise ValueError("query heads must be divisible by key/value heads")
-    q, k, v = _unit(q), _unit(k), _unit(v)
-    norms = [n for n in (q_norm, k_norm) if n is not None]
-    for n in norms:
-        if n.shape != (d,) or n.dtype != norms[0].dtype:
-            raise ValueError("q_norm and k_norm must be [head_dim] tensors of one dtype")
-    norm_dtype = _dtype_code(norms[0]) if norms else _lib.FAQ_F32
-    q_norm, k_norm = (None if n is None else n.contiguous() for n in (q_norm, k_norm))
-    rope_dtype, rope_ld, rope_rows = _lib.FAQ_F32, 0, 0
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    if cos is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] not in (d // 2, d) or cos.dtype != sin.dtype:
+    q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+    if q_st[2] != 1:
+        q = q.contiguous()
+        q_st = q.stride()
+    if k_st[2] != 1:
+        k = k.contiguous()
+        k_st = k.stride()
+    if v_st[2] != 1:
+        v = v.contiguous()
+        v_st = v.stride()
+    q_norm_ptr = k_norm_ptr = cos_ptr = sin_ptr = smooth_ptr = offset_ptr = None
+    norm_dtype = rope_dtype = _lib.FAQ_F32
+    rope_ld = rope_rows = smooth_stride = 0
+    if q_norm is not None or k_norm is not None:
+        norm_type = (k_norm if q_norm is None else q_norm).dtype
+        for n in (q_norm, k_norm):
+            if n is not None and (n.shape != (d,) or n.dtype is not norm_type):
+                raise ValueError("q_norm and k_norm must be [head_dim] tensors of one dtype")
+        norm_dtype = _dtype_code(k_norm if q_norm is None else q_norm)
+        if q_norm is not None:
+            q_norm = q_norm.contiguous()
+            q_norm_ptr = q_norm.data_ptr()
+        if k_norm is not None:
+            k_norm = k_norm.contiguous()
+            k_norm_ptr = k_norm.data_ptr()
+    if cos is not None and sin is not None:
+        shape = cos.shape
+        if len(shape) != 2 or sin.shape != shape or shape[1] not in (d // 2, d) or sin.dtype is not cos.dtype:
             raise ValueError("cos and sin must be [positions, head_dim / 2] or [positions, head_dim], of one dtype")
-        if cos.stride(1) != 1 or cos.stride() != sin.stride() or cos.stride(0) < d // 2:
+        if not (cos.is_contiguous() and sin.is_contiguous()):
             cos, sin = cos.contiguous(), sin.contiguous()
-        rope_dtype, rope_ld, rope_rows = _dtype_code(cos), max(cos.stride(0), d // 2), cos.shape[0]
-    smooth_stride = 0
+        rope_rows, rope_ld = shape
+        rope_dtype, cos_ptr, sin_ptr = _dtype_code(cos), cos.data_ptr(), sin.data_ptr()
+    elif cos is not None or sin is not None:
+        raise ValueError("cos and sin go together")
     if smooth_scale is not None:
         if smooth_scale.shape not in ((d,), (h, d)):
             raise ValueError("smooth_scale must be [head_dim] or [kv_heads, head_dim]")
         smooth_stride = d if smooth_scale.dim() == 2 else 0
         smooth_scale = smooth_scale.to(torch.float32).contiguous()
+        smooth_ptr = smooth_scale.data_ptr()
     if key_offset is not None:
         if key_offset.shape != (h, d):
             raise ValueError("key_offset must be [kv_heads, head_dim]")
         key_offset = key_offset.to(torch.float32).contiguous()
+        offset_ptr = key_offset.data_ptr()
     if out is None:
-        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
-    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
-        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-    _call_on(device, "faq_hif4_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), total, heads, h, d, qs[0],
-             qs[1], ks[0], ks[1], vs[0], vs[1], _ptr(q_norm), _ptr(k_norm), norm_dtype, float(eps), _ptr(cos), _ptr(sin),
-             rope_dtype, rope_ld, rope_rows, _ptr(key_offset), _ptr(smooth_scale), smooth_stride, int(rotate),
-             out.data_ptr(), os_[0], os_[1], *pool, *ragged, levels_code(levels[0]), levels_code(levels[1]), _stream(device))
+        out = q.new_empty(qs, dtype=torch.bfloat16)
+        out_st = (heads * d, d)
+    else:
+        if out.shape != qs or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+            raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+        out_st = out.stride()
+    k_levels, v_levels = levels
+    _call_on(device, "faq_hif4_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), total, heads, h, d,
+             q_st[0], q_st[1], k_st[0], k_st[1], v_st[0], v_st[1], q_norm_ptr, k_norm_ptr, norm_dtype, eps, cos_ptr, sin_ptr,
+             rope_dtype, rope_ld, rope_rows, offset_ptr, smooth_ptr, smooth_stride, rotate, out.data_ptr(), out_st[0],
+             out_st[1], *pool, *ragged, levels_code(k_levels), levels_code(v_levels))
     return out
 
 
@@ -1014,17 +1035,18 @@ def hif4_key_bounds(
     pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
     if bounds.shape[0] != pool[1]:
         raise ValueError("pages and bounds must have one number of pages")
-    _call_on(device, "faq_hif4_key_bounds", *pool, h, d, *ragged, total, bounds.data_ptr(), _stream(device))
+    _call_on(device, "faq_hif4_key_bounds", *pool, h, d, *ragged, total, bounds.data_ptr())
 
 
 def _bounds_shape(bounds: torch.Tensor) -> tuple[int, int]:
     """``(kv_heads, head_dim)`` of a bounds tensor."""
-    if bounds.dtype is not torch.uint8 or bounds.dim() != 3 or not bounds.is_contiguous():
+    shape = bounds.shape
+    if bounds.dtype is not torch.uint8 or len(shape) != 3 or not bounds.is_contiguous():
         raise TypeError("bounds must be a contiguous uint8 tensor [num_pages, kv_heads, hif4_bounds_bytes(head_dim)]")
-    d = (bounds.shape[2] - 16) // 2
-    if d not in (64, 128) or bounds.shape[2] != hif4_bounds_bytes(d):
+    d = (shape[2] - 16) // 2
+    if d not in (64, 128) or shape[2] != 2 * d + 16:
         raise ValueError("bounds must be [num_pages, kv_heads, hif4_bounds_bytes(head_dim)]")
-    return bounds.shape[1], d
+    return shape[1], d
 
 
 def hif4_select_pages(
@@ -1053,25 +1075,29 @@ def hif4_select_pages(
     ``want_scores`` returns ``(selected, scores)``, scores fp32 of the same shape, -inf behind the pages. Rows
     beyond ``cu[B]`` stay as they are. At most 32768 columns and 128 query heads per kv head."""
     device = _require_cuda(q, bounds, table, cu, lens, out)
-    if q.dtype is not torch.bfloat16 or q.dim() != 3:
+    qs = q.shape
+    if q.dtype is not torch.bfloat16 or len(qs) != 3:
         raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
-    total, heads, d = q.shape
-    h, bd = _bounds_shape(bounds)
-    if bd != d or h == 0 or heads % h or heads == 0:
+    total, heads, d = qs
+    h, bounds_d = _bounds_shape(bounds)
+    if bounds_d != d or h == 0 or heads % h or heads == 0:
         raise ValueError("q's heads must be divisible by the kv heads of the bounds, of one head_dim")
     hif4_page_bytes(h, d, page_size)
     ragged = _batch(table, cu, lens)
-    q = _unit(q)
+    st = q.stride()
+    if st[2] != 1:
+        q = q.contiguous()
+        st = q.stride()
     shape = (total, h, count)
     if out is None:
         if count < 1:
             raise ValueError("count must be positive")
-        out = torch.empty(shape, dtype=torch.int32, device=device)
+        out = q.new_empty(shape, dtype=torch.int32)
     elif out.shape != shape or out.dtype is not torch.int32 or not out.is_contiguous():
         raise ValueError("out must be a contiguous int32 tensor [tokens, kv_heads, count]")
-    scores = torch.empty(shape, dtype=torch.float32, device=device) if want_scores else None
-    _call_on(device, "faq_hif4_select_pages", q.data_ptr(), total, heads, q.stride(0), q.stride(1), bounds.data_ptr(),
-             bounds.shape[0], page_size, h, d, *ragged, count, first, last, out.data_ptr(), _ptr(scores), _stream(device))
+    scores = q.new_empty(shape, dtype=torch.float32) if want_scores else None
+    _call_on(device, "faq_hif4_select_pages", q.data_ptr(), total, heads, st[0], st[1], bounds.data_ptr(), bounds.shape[0],
+             page_size, h, d, *ragged, count, first, last, out.data_ptr(), _ptr(scores))
     return (out, scores) if want_scores else out
 
 
@@ -1095,29 +1121,32 @@ def hif4_sparse_attention(
     A row without a key is zero; rows beyond ``cu[B]`` stay as they are; pages that the table does not hold are
     left out and set ``FAQ_STATUS_BAD_PAGE``."""
     device = _require_cuda(q, pages, table, cu, lens, selected, out)
-    if q.dtype is not torch.bfloat16 or q.dim() != 3:
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or len(shape) != 3:
         raise TypeError("q must be bfloat16 [tokens, heads, head_dim]")
-    total, heads, d = q.shape
+    total, heads, d = shape
     h = _kv_heads(pages, d, page_size)
     pool, ragged = _ragged(pages, table, cu, lens, h, d, page_size)
     if heads % h or heads == 0:
         raise ValueError("query heads must be divisible by key/value heads")
-    if selected.dtype is not torch.int32 or selected.dim() != 3 or selected.shape[:2] != (total, h):
+    lists = selected.shape
+    if selected.dtype is not torch.int32 or len(lists) != 3 or lists[0] != total or lists[1] != h:
         raise ValueError("selected must be int32 [tokens, kv_heads, count]")
-    selected = selected.contiguous()
-    qs = q.stride()
-    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] < 8 or qs[1] < 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-        if q.data_ptr() % 16:
-            q = q.clone()
-        qs = (heads * d, d)
+    if not selected.is_contiguous():
+        selected = selected.contiguous()
+    st = q.stride()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or st[0] < 8 or st[1] < 8 or q.data_ptr() % 16:
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+        st = (heads * d, d)
     if out is None:
-        out = torch.empty((total, heads, d), dtype=torch.bfloat16, device=device)
-    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
-        raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
-    _call_on(device, "faq_hif4_sparse_attention", q.data_ptr(), total, heads, qs[0], qs[1], *pool, h, d, *ragged,
-             selected.data_ptr(), selected.shape[2], d**-0.5 if scale is None else float(scale), out.data_ptr(),
-             out.stride(0), out.stride(1), _stream(device))
+        out = q.new_empty(shape)
+        out_st = (heads * d, d)
+    else:
+        if out.shape != shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+            raise ValueError("out must be a bfloat16 tensor of q's shape with unit channel stride")
+        out_st = out.stride()
+    _call_on(device, "faq_hif4_sparse_attention", q.data_ptr(), total, heads, st[0], st[1], *pool, h, d, *ragged,
+             selected.data_ptr(), lists[2], d**-0.5 if scale is None else scale, out.data_ptr(), out_st[0], out_st[1])
     return out
 
 
