@@ -49,81 +49,97 @@ struct AppendParams {
   int64_t kv_blocks; // blocks of the grid that write K and V
 };
 
-// Eight consecutive entries of a table, fp32 or bf16 (any alignment of its type).
+// Eight consecutive entries of a table, fp32 or bf16.
 __device__ __forceinline__ void load8(const void* base, bool f32, int64_t at, float (&v)[8]) {
   if (f32) {
     const float* p = static_cast<const float*>(base) + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p[i];
+    Raw<float> r;
+    r.load(p, (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+    r.values(v);
   } else {
     const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+    Raw<__nv_bfloat16> r;
+    r.load(p, (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+    r.values(v);
   }
 }
-
-__device__ __forceinline__ float rsqrt_of(float x) { return rsqrtf(x); }
-__device__ __forceinline__ double rsqrt_of(double x) { return rsqrt(x); }
 
 // A row's position-dependent entries of one lane.
 struct Angles {
   float c[8], s[8];
-  __device__ __forceinline__ void load(const TurnParams& t, int64_t pos, int lane_of_row, int ng) {
-    const int64_t at = pos * t.rope_ld + 8 * (ng == 2 ? lane_of_row : lane_of_row & 3);
+  __device__ __forceinline__ void load(const TurnParams& t, int64_t pos, int s_, int ng) {
+    const int64_t at = pos * t.rope_ld + 8 * (ng == 2 ? s_ : s_ & 3);
     load8(t.cos, t.rope_f32, at, c);
     load8(t.sin, t.rope_f32, at, s);
   }
 };
 
-// norm, rotation, offset, smoothing and transform of the lane's part of a row; all lanes take part.
-// `divide`: a key's smoothing; `head` is the kv head.
-template <typename R, int NG, bool KEY>
-__device__ __forceinline__ void turn_row(R (&x)[NG][8], const TurnParams& t, const void* norm, const Angles& a, int head,
-                                         int s) {
+// x / w in fp64 to 2^-46: a Newton's step from the fp32 reciprocal (the result is rounded to 2^-24).
+__device__ __forceinline__ double quotient(double x, float w) {
+  const double r = __frcp_rn(w), y = x * r;
+  return fma(fma(-static_cast<double>(w), y, x), r, y);
+}
+
+// A key: norm, rotation, offset, smoothing and transform of the lane's part of a row in fp64; all
+// lanes take part.
+template <int NG>
+__device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t, const Angles& a, bool bf16, int head, int s) {
   constexpr int D = 64 * NG;
-  if (norm != nullptr) {
-    R sum = 0;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[g][i] * x[g][i];
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const R r = rsqrt_of(sum * (R(1) / D) + static_cast<R>(t.eps));
+  double x[NG][8], factor = 1.0;  // the norm's, which waits for the transform's: the steps between are linear
+  if (t.k_norm != nullptr) {
+    double sum = 0;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float w[8];
-      load8(norm, t.norm_f32, 64 * g + 8 * s, w);
+      load8(t.k_norm, t.norm_f32, 64 * g + 8 * s, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[g][i] = x[g][i] * r * static_cast<R>(w[i]);
+      for (int i = 0; i < 8; ++i) {
+        const double y = v[g][i];
+        sum = fma(y, y, sum);
+        x[g][i] = bf16 ? static_cast<double>(v[g][i] * w[i]) : y * w[i];  // exact in fp32 for two bf16
+      }
     }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    factor = rsqrt(sum * (1.0 / D) + t.eps);
+  } else {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] = v[g][i];
   }
   if (t.cos != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const R c = a.c[i], n = a.s[i];
+      const double c = a.c[i], n = a.s[i];
       if constexpr (NG == 2) {
-        const R u = x[0][i], v = x[1][i];
+        const double u = x[0][i], v = x[1][i];
         x[0][i] = u * c - v * n;
         x[1][i] = v * c + u * n;
       } else {
-        const R other = __shfl_xor_sync(0xffffffffu, x[0][i], 4);
+        const double other = __shfl_xor_sync(0xffffffffu, x[0][i], 4);
         x[0][i] = x[0][i] * c + (s & 4 ? other : -other) * n;
       }
     }
   }
-  if (KEY && t.offset != nullptr) {
+  if (t.offset != nullptr) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
+    for (int g = 0; g < NG; ++g) {
+      float w[8];
+      load8(t.offset, true, head * D + 64 * g + 8 * s, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[g][i] -= t.offset[head * D + 64 * g + 8 * s + i];
+      for (int i = 0; i < 8; ++i) x[g][i] = fma(x[g][i], factor, -static_cast<double>(w[i]));
+    }
+    factor = 1.0;
   }
   if (t.smooth != nullptr) {
-    const float* m = t.smooth + head * t.smooth_head_stride + 8 * s;
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
+    for (int g = 0; g < NG; ++g) {
+      float w[8];
+      load8(t.smooth, true, head * t.smooth_head_stride + 64 * g + 8 * s, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[g][i] = KEY ? x[g][i] / static_cast<R>(m[64 * g + i]) : x[g][i] * m[64 * g + i];
+      for (int i = 0; i < 8; ++i) x[g][i] = quotient(x[g][i], w[i]);
+    }
   }
   if (t.rotate) {
 #pragma unroll
@@ -133,31 +149,152 @@ __device__ __forceinline__ void turn_row(R (&x)[NG][8], const TurnParams& t, con
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if ((i & d) == 0) {
-            const R u = x[g][i], v = x[g][i + d];
+            const double u = x[g][i], v = x[g][i + d];
             x[g][i] = u + v;
             x[g][i + d] = u - v;
           }
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1)
+      for (int o = 1; o < 8; o <<= 1) {
+        const double sign = (s & o) ? -1.0 : 1.0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const R other = __shfl_xor_sync(0xffffffffu, x[g][i], o);
-          x[g][i] = (s & o) ? other - x[g][i] : x[g][i] + other;
-        }
-    }
-    const R unit = NG == 2 ? static_cast<R>(0.08838834764831843) : static_cast<R>(0.125);  // 1 / sqrt(d)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (NG == 2) {
-        const R u = x[0][i], v = x[1][i];
-        x[0][i] = (u + v) * unit;
-        x[1][i] = (u - v) * unit;
-      } else {
-        x[0][i] *= unit;
+        for (int i = 0; i < 8; ++i) x[g][i] = fma(x[g][i], sign, __shfl_xor_sync(0xffffffffu, x[g][i], o));
       }
     }
+    if constexpr (NG == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double u = x[0][i], w = x[1][i];
+        x[0][i] = u + w;
+        x[1][i] = u - w;
+      }
+    }
+    factor *= NG == 2 ? 0.08838834764831843 : 0.125;  // 1 / sqrt(d)
   }
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[g][i] = __double2float_rn(x[g][i] * factor);
 }
+
+// A query: what a token's rows have in common is multiplied together once, weight times cosine or sine
+// times smoothing (where that is one for all heads): out = x * own + partner * other, partner the same
+// channel of the other half. The norm's factor waits for the transform's, both linear.
+template <int NG>
+struct QueryTurn {
+  float2 own[NG][4], other[NG][4];
+  __device__ __forceinline__ void make(const TurnParams& t, int64_t pos, int s) {
+    Angles a;
+    if (t.cos != nullptr) a.load(t, pos, s, NG);
+    float w[NG][8], m[NG][8];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[g][i] = m[g][i] = 1.0f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      if (t.q_norm != nullptr) load8(t.q_norm, t.norm_f32, 64 * g + 8 * s, w[g]);
+      if (t.smooth != nullptr && t.smooth_head_stride == 0) load8(t.smooth, true, 64 * g + 8 * s, m[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool low = NG == 2 ? g == 0 : s < 4;
+        float partner;  // its weight
+        if constexpr (NG == 2) partner = w[1 - g][i]; else partner = __shfl_xor_sync(0xffffffffu, w[0][i], 4);
+        const float c = t.cos != nullptr ? a.c[i] : 1.0f, n = t.cos != nullptr ? a.s[i] : 0.0f;
+        const float x = w[g][i] * c * m[g][i], y = (low ? -partner : partner) * n * m[g][i];
+        if (i & 1) {
+          own[g][i >> 1].y = x;
+          other[g][i >> 1].y = y;
+        } else {
+          own[g][i >> 1].x = x;
+          other[g][i >> 1].x = y;
+        }
+      }
+  }
+  __device__ __forceinline__ void apply(float2 (&x)[NG][4], const TurnParams& t, int h, int group, int s) const {
+    constexpr int D = 64 * NG;
+    float r = 1.0f;
+    if (t.q_norm != nullptr) {
+      float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = __ffma2_rn(x[g][i], x[g][i], sum);
+      float ss = sum.x + sum.y;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      r = rsqrtf(ss * (1.0f / D) + static_cast<float>(t.eps));
+    }
+    if (t.cos != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (NG == 2) {
+          const float2 u = x[0][i], v = x[1][i];
+          x[0][i] = __ffma2_rn(u, own[0][i], __fmul2_rn(v, other[0][i]));
+          x[1][i] = __ffma2_rn(v, own[1][i], __fmul2_rn(u, other[1][i]));
+        } else {
+          const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, x[0][i].x, 4), __shfl_xor_sync(0xffffffffu, x[0][i].y, 4));
+          x[0][i] = __ffma2_rn(x[0][i], own[0][i], __fmul2_rn(v, other[0][i]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[g][i] = __fmul2_rn(x[g][i], own[g][i]);
+    }
+    if (t.smooth_head_stride != 0) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float m[8];
+        load8(t.smooth, true, h / group * t.smooth_head_stride + 64 * g + 8 * s, m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[g][i] = __fmul2_rn(x[g][i], make_float2(m[2 * i], m[2 * i + 1]));
+      }
+    }
+    if (t.rotate) {
+      const float2 minus = make_float2(-1.0f, -1.0f);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[g][i] = make_float2(x[g][i].x + x[g][i].y, x[g][i].x - x[g][i].y);
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((i & d) == 0) {
+              const float2 u = x[g][i], v = x[g][i + d];
+              x[g][i] = __fadd2_rn(u, v);
+              x[g][i + d] = __ffma2_rn(v, minus, u);
+            }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const float sign = (s & o) ? -1.0f : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, x[g][i].x, o), __shfl_xor_sync(0xffffffffu, x[g][i].y, o));
+            x[g][i] = __ffma2_rn(x[g][i], make_float2(sign, sign), v);
+          }
+        }
+      }
+      if constexpr (NG == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 u = x[0][i], v = x[1][i];
+          x[0][i] = __fadd2_rn(u, v);
+          x[1][i] = __ffma2_rn(v, minus, u);
+        }
+      }
+      r *= NG == 2 ? 0.08838834764831843f : 0.125f;  // 1 / sqrt(d)
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[g][i] = __fmul2_rn(x[g][i], make_float2(r, r));
+  }
+};
 
 template <typename T, int NG>
 __global__ void __launch_bounds__(32 * WRITE_WARPS) kv_append_kernel(AppendParams a, bool vec, bool out_vec) {
@@ -188,18 +325,9 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) kv_append_kernel(AppendParam
                             [&](float (&v)[NG][8], int r) {
                               if (t.k_norm == nullptr && t.cos == nullptr && t.offset == nullptr && t.smooth == nullptr && !t.rotate)
                                 return;
-                              double y[NG][8];
                               Angles ang;
                               if (t.cos != nullptr) ang.load(t, x.pos + min(max(r, x.from), x.to - 1), s, NG);
-#pragma unroll
-                              for (int g = 0; g < NG; ++g)
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) y[g][i] = v[g][i];
-                              turn_row<double, NG, true>(y, t, t.k_norm, ang, head, s);
-#pragma unroll
-                              for (int g = 0; g < NG; ++g)
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) v[g][i] = __double2float_rn(y[g][i]);
+                              turn_key<NG>(v, t, ang, sizeof(T) == 2 && !t.norm_f32, head, s);
                             });
     return;
   }
@@ -213,30 +341,46 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) kv_append_kernel(AppendParam
   if (!find_token(p, token, w.total, b, pos)) return;  // reported where its keys would be written
   const int h_begin = static_cast<int>(item - token * items) * a.hpw, h_end = min(h_begin + a.hpw, a.heads);
   const bool placed = pos >= 0 && (t.cos == nullptr || pos < t.rope_rows);
-  Angles ang;
-  if (t.cos != nullptr && placed) ang.load(t, pos, s, NG);
-  for (int h0 = h_begin; h0 < h_end; h0 += 4) {
-    const bool live = h0 + (lane >> 3) < h_end;
-    const int h = live ? h0 + (lane >> 3) : h_begin;  // idle rows redo a live one, unstored
-    const T* src = static_cast<const T*>(a.q) + token * a.qt + h * a.qh + 8 * s;
-    Raw<T> raw[NG];
-    float x[NG][8];
+  __nv_bfloat16* out_row = a.out + token * a.ot + 8 * s;
+  if (!placed) {
+    const uint32_t zero[4] = {0, 0, 0, 0};
+    for (int h = h_begin + (lane >> 3); h < h_end; h += 4)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) store_pairs(out_row + h * a.oh + 64 * g, out_vec, zero);
+    return;
+  }
+  QueryTurn<NG> turn;
+  turn.make(t, pos, s);
+  const T* row = static_cast<const T*>(a.q) + token * a.qt + 8 * s;
+  Raw<T> raw[NG];
+  auto load = [&](int h0) {  // rows past the last head repeat it, unstored
+    const T* src = row + min(h0 + (lane >> 3), h_end - 1) * a.qh;
 #pragma unroll
     for (int g = 0; g < NG; ++g) raw[g].load(src + 64 * g, vec);
+  };
+  load(h_begin);
+  for (int h0 = h_begin; h0 < h_end; h0 += 4) {
+    const int h = min(h0 + (lane >> 3), h_end - 1);
+    float2 x[NG][4];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) raw[g].values(x[g]);
-    turn_row<float, NG, false>(x, t, t.q_norm, ang, h / a.group, s);
-    if (!live) continue;
-    __nv_bfloat16* dst = a.out + token * a.ot + h * a.oh + 8 * s;
+    for (int g = 0; g < NG; ++g) {
+      float v[8];
+      raw[g].values(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[g][i] = make_float2(v[2 * i], v[2 * i + 1]);
+    }
+    if (h0 + 4 < h_end) load(h0 + 4);
+    turn.apply(x, t, h, a.group, s);
+    if (h0 + (lane >> 3) >= h_end) continue;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint32_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x[g][2 * i], x[g][2 * i + 1]);
-        o[i] = placed ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[g][i].x, x[g][i].y);
+        o[i] = *reinterpret_cast<const uint32_t*>(&v);
       }
-      store_pairs(dst + 64 * g, out_vec, o);
+      store_pairs(out_row + h * a.oh + 64 * g, out_vec, o);
     }
   }
 }
@@ -285,7 +429,7 @@ extern "C" int faq_hif4_kv_append(const void* q, const void* k, const void* v, i
   w.k_levels = k_levels;
   w.v_levels = v_levels;
   a.t = {q_norm, k_norm, norm_dtype == FAQ_F32, eps, cos, sin, rope_dtype == FAQ_F32, rope_ld, rope_rows,
-         key_offset, smooth, smooth_head_stride, rotate != 0};
+         key_offset, smooth, smooth ? smooth_head_stride : 0, rotate != 0};
   a.q = q;
   a.qt = q_token_stride;
   a.qh = q_head_stride;

@@ -12,6 +12,14 @@ A step is: :meth:`PagedKVCache.extend` (host: pages for the new tokens), then pe
 runs a Hugging Face Qwen3 on it (``qwen3.attention_forward``); the first layer of a forward
 call opens the step.
 
+:meth:`append` stands for the steps between the projections and :meth:`write` too (per-head norm,
+rotation of each token's position, Smooth-QK, Hadamard) and returns the attention's queries.
+
+With ``sparse_pages`` the attention of a long context reads that many pages per token and kv head: the
+first ones, the last ones, and those whose keys' bounds allow the greatest products
+(``ops.hif4_select_pages``). The bounds are kept beside the pages, 2 * head_dim + 16 bytes per page
+and kv head, and made anew for the pages that a step writes to.
+
 A step is not to be captured in a CUDA graph: :meth:`extend` makes the step's device arrays anew, and
 :meth:`attend` gives the step's own lengths as bounds. What a graph needs -- arrays that stay in
 their place, bounds of its last replay, one workspace -- the operators take (``ops.hif4_kv_write``,
@@ -30,16 +38,31 @@ class PagedKVCache:
     ``max_length`` tokens on ``layers`` attention layers."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, *, max_sequences: int = 1, max_length: int,
-                 num_pages: int | None = None, page_size: int = 64, device: torch.device | str = "cuda") -> None:
+                 num_pages: int | None = None, page_size: int = 64, device: torch.device | str = "cuda",
+                 sparse_pages: int | None = None, sparse_first: int = 1, sparse_last: int = 2,
+                 sparse_max_new: int | None = None) -> None:
+        """``sparse_pages``: the pages that a token attends to per kv head, among them the
+        ``sparse_first`` first and ``sparse_last`` last ones; None: all. Steps in which a sequence has more
+        than ``sparse_max_new`` new tokens (prompts) attend to all pages all the same (None: no step does)."""
+        if sparse_pages is not None and (sparse_first < 0 or sparse_last < 1 or sparse_first + sparse_last > sparse_pages):
+            raise ValueError("sparse_pages must hold the first pages and the last ones, of which there is at least one")
         if layers < 1 or max_sequences < 1 or max_length < 1:
             raise ValueError("layers, max_sequences and max_length must be positive")
         columns = -(-max_length // page_size)
+        if sparse_pages is not None and columns > 32768:
+            raise ValueError("the selection of pages takes sequences of at most 32768 pages")
         self.layers, self.kv_heads, self.head_dim, self.page_size = layers, kv_heads, head_dim, page_size
         self.max_length, self.device = max_length, torch.device(device)
         num_pages = columns * max_sequences if num_pages is None else num_pages
         size = ops.hif4_page_bytes(kv_heads, head_dim, page_size)
         self.pages = torch.empty((layers, num_pages, 2, kv_heads, size // (2 * kv_heads)), dtype=torch.uint8,
                                  device=self.device)
+        self.sparse_pages, self.sparse_first, self.sparse_last = sparse_pages, sparse_first, sparse_last
+        self.sparse_max_new = sparse_max_new
+        self.bounds = None
+        if sparse_pages is not None:
+            self.bounds = torch.zeros((layers, num_pages, kv_heads, ops.hif4_bounds_bytes(head_dim)), dtype=torch.uint8,
+                                      device=self.device)
         self.table = torch.full((max_sequences, columns), -1, dtype=torch.int32, device=self.device)
         self._free = list(range(num_pages - 1, -1, -1))
         self._held: list[list[int]] = [[] for _ in range(max_sequences)]
@@ -111,6 +134,26 @@ class PagedKVCache:
             raise ValueError(f"the step has {sum(self._new)} new tokens, got {k.shape[0]}")
         ops.hif4_kv_write(k, v, self.pages[layer], self.table, self._cu, self._lens, page_size=self.page_size,
                           levels=(ops.default_levels("k"), ops.default_levels("v")))
+        self._refresh(layer)
+
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, **transform) -> torch.Tensor:
+        """From the projections of the step's tokens, ``q [tokens, heads, head_dim]`` and ``k``/``v [tokens,
+        kv_heads, head_dim]``, to the layer's cache and the queries of :meth:`attend`: norms, position
+        rotation, smoothing and Hadamard transform as ``transform`` asks (``ops.hif4_kv_append``: ``cos``,
+        ``sin``, ``q_norm``, ``k_norm``, ``eps``, ``rotate``, ``smooth_scale``, ``key_offset``, ``out``)."""
+        self._open()
+        if q.shape[0] != sum(self._new):
+            raise ValueError(f"the step has {sum(self._new)} new tokens, got {q.shape[0]}")
+        q = ops.hif4_kv_append(q, k, v, self.pages[layer], self.table, self._cu, self._lens, page_size=self.page_size,
+                               levels=(ops.default_levels("k"), ops.default_levels("v")), **transform)
+        self._refresh(layer)
+        return q
+
+    def _refresh(self, layer: int) -> None:
+        """The bounds of the pages that the step wrote to."""
+        if self.bounds is not None:
+            ops.hif4_key_bounds(self.pages[layer], self.bounds[layer], self.table, self._cu, self._lens,
+                                page_size=self.page_size, total=sum(self._new))
 
     def attend(self, layer: int, q: torch.Tensor, scale: float | None = None) -> torch.Tensor:
         """Attention of the step's ``q [tokens, heads, head_dim]`` over the layer's cache."""
@@ -118,8 +161,17 @@ class PagedKVCache:
         if q.shape[0] != sum(self._new):
             raise ValueError(f"the step has {sum(self._new)} new tokens, got {q.shape[0]}")
         lengths = [n for n, new in zip(self.lengths, self._new) if new]  # of those that take part
+        max_new, max_len = max(self._new), max(lengths, default=0)
+        # where no sequence has more pages than are taken, all of them are: the dense kernels'
+        if self.sparse_pages is not None and max_len > self.sparse_pages * self.page_size and (
+                self.sparse_max_new is None or max_new <= self.sparse_max_new):
+            selected = ops.hif4_select_pages(q, self.bounds[layer], self.table, self._cu, self._lens,
+                                             page_size=self.page_size, count=self.sparse_pages, first=self.sparse_first,
+                                             last=self.sparse_last)
+            return ops.hif4_sparse_attention(q, self.pages[layer], self.table, self._cu, self._lens, selected,
+                                             page_size=self.page_size, scale=scale)
         return ops.hif4_paged_attention(q, self.pages[layer], self.table, self._cu, self._lens,
-                                        page_size=self.page_size, max_new=max(self._new), max_len=max(lengths, default=0),
+                                        page_size=self.page_size, max_new=max_new, max_len=max_len,
                                         total_len=sum(lengths), scale=scale)
 
     def read(self, layer: int, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:

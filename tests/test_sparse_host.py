@@ -81,3 +81,17 @@ def test_operators_refuse_cpu_tensors() -> None:
     assert ops.hif4_bounds_bytes(128) == 272 and ops.hif4_bounds_bytes(64) == 144
     with pytest.raises(ValueError):
         ops.hif4_bounds_bytes(96)
+
+
+def test_sparse_caches_are_checked_when_made() -> None:
+    from faquant_b200.kv_cache import PagedKVCache
+
+    for bad in (dict(sparse_pages=2, sparse_first=1, sparse_last=2), dict(sparse_pages=3, sparse_last=0),
+                dict(sparse_pages=3, sparse_first=-1)):
+        with pytest.raises(ValueError, match="sparse_pages"):
+            PagedKVCache(1, 1, 64, max_length=100, page_size=16, device="cpu", **bad)
+    with pytest.raises(ValueError, match="32768 pages"):
+        PagedKVCache(1, 1, 64, max_length=1 << 20, num_pages=4, page_size=16, device="cpu", sparse_pages=4)
+    cache = PagedKVCache(2, 3, 64, max_length=100, page_size=16, device="cpu", sparse_pages=4)
+    assert cache.bounds.shape == (2, 7, 3, 144)
+    assert PagedKVCache(2, 3, 64, max_length=100, page_size=16, device="cpu").bounds is None
