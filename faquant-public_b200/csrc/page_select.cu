@@ -266,33 +266,64 @@ struct PageRows {
       e[h] = static_cast<int8_t>(src[2 * D]);
     }
   }
-  // key(slot, c, value) is called, by one lane each, for the columns below `columns` and the tokens' slots
-  // (0 .. 7 >> slots) of `q` with the greatest score of the token's heads, 0 for a page that is not there.
-  template <typename F>
-  __device__ __forceinline__ void score(const SelectParams& w, const Query<NG>& q, int c0, int columns, int lane,
+  // key(k, slot, c, value) is called, by one lane each, for the columns below `columns` and the tokens' slots
+  // (0 .. 7 >> slots) of q[k] with the greatest score of the token's heads, 0 for a page that is not there.
+  // Two sums per product, so that its steps do not all wait for one another; the lanes of a page that hold a
+  // token's columns halve what they hold at each exchange of their maxima.
+  template <int K, typename F>
+  __device__ __forceinline__ void score(const SelectParams& w, const Query<NG> (&q)[K], int c0, int columns, int lane,
                                         F&& key) const {
     const int g = lane >> 2, t = lane & 3;
-    int acc[4] = {0, 0, 0, 0};
+    int v[K][2][2];  // [product][row lane / 4 or 8 further][column 2 t or the next]
 #pragma unroll
-    for (int j = 0; j < 2 * NG; ++j) {
-      mma_s8_16832(acc, a[0][j].x, a[1][j].x, a[0][j].y, a[1][j].y, q.b[j].x, q.b[j].y);
-      mma_s8_16832(acc, a[0][j].z, a[1][j].z, a[0][j].w, a[1][j].w, q.b[j].z, q.b[j].w);
-    }
+    for (int k = 0; k < K; ++k) {
+      int acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + g + 8 * h;
-      const float unit = pow2f(min(max(e[h], -100), 100));
-      int v0 = acc[2 * h], v1 = acc[2 * h + 1];
-      if (w.slots > 0) v0 = max(v0, v1);
-      if (w.slots > 1) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
-      if (w.slots > 2) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
-      if (c >= columns) continue;
-      if (w.slots == 0) {
-        key(2 * t, c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
-        key(2 * t + 1, c, ok[h] ? order_key(static_cast<float>(v1) * unit) : 0u);
-      } else if ((t & ((1 << (w.slots - 1)) - 1)) == 0) {
-        key(t >> (w.slots - 1), c, ok[h] ? order_key(static_cast<float>(v0) * unit) : 0u);
+      for (int j = 0; j < 2 * NG; ++j) {
+        mma_s8_16832(acc[0], a[0][j].x, a[1][j].x, a[0][j].y, a[1][j].y, q[k].b[j].x, q[k].b[j].y);
+        mma_s8_16832(acc[1], a[0][j].z, a[1][j].z, a[0][j].w, a[1][j].w, q[k].b[j].z, q[k].b[j].w);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k][i >> 1][i & 1] = acc[0][i] + acc[1][i];
+    }
+    auto give = [&](int k, int slot, int h, int value) {
+      const int c = c0 + g + 8 * h;
+      const float unit = pow2f(min(max(h ? e[1] : e[0], -100), 100));
+      if (c < columns) key(k, slot, c, (h ? ok[1] : ok[0]) ? order_key(static_cast<float>(value) * unit) : 0u);
+    };
+    if (w.slots == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) give(k, 2 * t + (i & 1), i >> 1, v[k][i >> 1][i & 1]);
+      return;
+    }
+    int x[K][2], y[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[k][h] = max(v[k][h][0], v[k][h][1]);
+    if (w.slots == 1) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) give(k, t, h, x[k][h]);
+      return;
+    }
+    const int h = t & 1;  // the lane keeps this row
+#pragma unroll
+    for (int k = 0; k < K; ++k) y[k] = max(h ? x[k][1] : x[k][0], __shfl_xor_sync(0xffffffffu, h ? x[k][0] : x[k][1], 1));
+    if (w.slots == 2) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) give(k, t >> 1, h, y[k]);
+      return;
+    }
+    if constexpr (K == 2) {
+      const int k = t >> 1;  // and this product
+      give(k, 0, h, max(k ? y[1] : y[0], __shfl_xor_sync(0xffffffffu, k ? y[0] : y[1], 2)));
+    } else {
+      const int z = max(y[0], __shfl_xor_sync(0xffffffffu, y[0], 2));
+      if (t < 2) give(0, 0, h, z);
     }
   }
   // A page that the table does not hold is reported, once per row of it.
@@ -335,23 +366,20 @@ __device__ __forceinline__ void take(const uint32_t* keys, const Wanted& w, int 
   };
   uint32_t held[HELD], top = 0, low = 0xFFFFFFFFu;  // of the choices
   int always = 0, others = 0;
-  auto choice = [&](int c) -> uint32_t {  // 0: none
-    return c < w.columns && !w.forced(c) ? keys[c] : 0;
+  auto key_at = [&](int c) -> uint32_t { return c < w.columns ? keys[c] : 0; };
+  auto count_in = [&](uint32_t key, bool forced) -> uint32_t {  // the key as a choice, 0: it is none
+    always += key != 0 && forced;
+    if (key == 0 || forced) return 0;
+    ++others;
+    top = max(top, key);
+    low = min(low, key);
+    return key;
   };
   if (few) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i] = i < rounds ? choice(c0 + 32 * i) : 0;
-  }
-  for (int i = 0; i < rounds; ++i) {
-    const int c = c0 + 32 * i;
-    const uint32_t key = c < w.columns ? keys[c] : 0;
-    if (key && w.forced(c)) {
-      ++always;
-    } else if (key) {
-      ++others;
-      top = max(top, key);
-      low = min(low, key);
-    }
+    for (int i = 0; i < HELD; ++i) held[i] = i < rounds ? count_in(key_at(c0 + 32 * i), w.forced(c0 + 32 * i)) : 0;
+  } else {
+    for (int i = 0; i < rounds; ++i) count_in(key_at(c0 + 32 * i), w.forced(c0 + 32 * i));
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
@@ -389,7 +417,7 @@ __device__ __forceinline__ void take(const uint32_t* keys, const Wanted& w, int 
 #pragma unroll
         for (int i = 0; i < HELD; ++i) n += held[i] >= at;
       } else {
-        for (int i = 0; i < rounds; ++i) n += choice(c0 + 32 * i) >= at;
+        for (int i = 0; i < rounds; ++i) n += !w.forced(c0 + 32 * i) && key_at(c0 + 32 * i) >= at;
       }
       n = all(n);
       if (n >= need) found = at; else above = n;
@@ -404,7 +432,7 @@ __device__ __forceinline__ void take(const uint32_t* keys, const Wanted& w, int 
     int sure = 0, same = 0;
     for (int i = 0; i < rounds; ++i) {
       const int c = c0 + 32 * i;
-      const uint32_t key = c < w.columns ? keys[c] : 0;
+      const uint32_t key = key_at(c);
       const bool f = w.forced(c);
       sure += key != 0 && (f || key > limit);
       same += key != 0 && !f && key == limit;
@@ -425,18 +453,22 @@ __device__ __forceinline__ void take(const uint32_t* keys, const Wanted& w, int 
   const uint32_t below = (1u << lane) - 1;
   for (int i = 0; i < rounds; ++i) {
     const int c = c0 + 32 * i;
-    const uint32_t key = c < w.columns ? keys[c] : 0;
-    const bool f = w.forced(c), same = key != 0 && !f && key == limit;
-    const uint32_t vs = __ballot_sync(0xffffffffu, same);
-    const bool taken = key != 0 && (f || key > limit || (same && equal + __popc(vs & below) < ties));
+    const uint32_t key = key_at(c);
+    const bool f = w.forced(c), same = ties > 0 && !f && key == limit;
+    bool taken = key != 0 && (f || key > limit);
+    if (ties > 0) {
+      const uint32_t vs = __ballot_sync(0xffffffffu, same);
+      taken = taken || (same && equal + __popc(vs & below) < ties);
+      equal += __popc(vs);
+    }
     const uint32_t vt = __ballot_sync(0xffffffffu, taken);
+    if (vt == 0) continue;
     const int mine = at + __popc(vt & below);
     if (taken && mine < w.count) {
       out[mine] = c;
       if (scores != nullptr) scores[mine] = ldexpf(number_of(key), eq);
     }
     at += __popc(vt);
-    equal += __popc(vs);
   }
   const int listed = min(always + min(others, need), w.count);
   for (int i = listed + (WARPS > 1 ? static_cast<int>(threadIdx.x) : lane); i < w.count; i += 32 * WARPS) {
@@ -487,10 +519,10 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_cta_kernel(Sel
   PageRows<NG> rows;  // the first pages' loads fly while q is rounded
   rows.load(w, head, PageRows<NG>::entry(row, begin, want.columns, lane), lane);
   int entry = PageRows<NG>::entry(row, begin + step, want.columns, lane);
-  Query<NG> q;
-  q.e = query_exponent(q, w, heads, min(lane >> 2, w.group - 1), lane);
+  Query<NG> q[1];
+  q[0].e = query_exponent(q[0], w, heads, min(lane >> 2, w.group - 1), lane);
   for (int h = 0; h < w.group; h += 8) {
-    q.round(heads + min(h + (lane >> 2), w.group - 1) * w.qh, lane, w.vec);
+    q[0].round(heads + min(h + (lane >> 2), w.group - 1) * w.qh, lane, w.vec);
     if (h > 0) {
       rows.load(w, head, PageRows<NG>::entry(row, begin, want.columns, lane), lane);
       entry = PageRows<NG>::entry(row, begin + step, want.columns, lane);
@@ -500,7 +532,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_cta_kernel(Sel
       if (c0 + step < want.columns) rows.load(w, head, entry, lane);
       entry = PageRows<NG>::entry(row, c0 + 2 * step, want.columns, lane);
       now.report(c0, want.columns, lane);
-      now.score(w, q, c0, want.columns, lane, [&](int, int c, uint32_t key) {
+      now.score(w, q, c0, want.columns, lane, [&](int, int, int c, uint32_t key) {
         const uint32_t at = dst + 4 * c;  // a column's passes are one lane's
         if (h > 0) {
           uint32_t old;
@@ -517,9 +549,9 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_cta_kernel(Sel
   int32_t* out = w.out + list;
   float* scores = w.scores == nullptr ? nullptr : w.scores + list;
   if (want.columns > WARP_COLUMNS)
-    take<SELECT_WARPS>(s_keys, want, q.e, out, scores, &s_search);
+    take<SELECT_WARPS>(s_keys, want, q[0].e, out, scores, &s_search);
   else if (warp == 0)
-    take<1>(s_keys, want, q.e, out, scores, nullptr);
+    take<1>(s_keys, want, q[0].e, out, scores, nullptr);
 }
 
 // Many rows: a warp per kv head and two products' columns, 16 >> slots tokens: the heads of several tokens
@@ -563,20 +595,24 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) select_pages_warp_kernel(Se
     for (int h = 0; h < w.group; h += 8) {
 #pragma unroll
       for (int k = 0; k < PRODUCTS; ++k) q[k].round(heads[k] + min(h + column, w.group - 1) * w.qh, lane, w.vec);
-      PageRows<NG> rows;
-      rows.load(w, head, PageRows<NG>::entry(row, 0, columns, lane), lane);
+      auto step = [&](const PageRows<NG>& rows, int c0) {
+        rows.report(c0, columns, lane);
+        rows.score(w, q, c0, columns, lane, [&](int k, int slot, int c, uint32_t key) {
+          uint32_t* at = keys + static_cast<int64_t>(k * each + slot) * w.key_ld + c;
+          *at = h > 0 ? max(key, *at) : key;
+        });
+      };
+      PageRows<NG> rows[2];  // the next 16 pages' are loaded while these are multiplied
       int entry = PageRows<NG>::entry(row, 16, columns, lane);
-      for (int c0 = 0; c0 < columns; c0 += 16) {
-        const PageRows<NG> now = rows;
-        if (c0 + 16 < columns) rows.load(w, head, entry, lane);
+      rows[0].load(w, head, PageRows<NG>::entry(row, 0, columns, lane), lane);
+      for (int c0 = 0; c0 < columns; c0 += 32) {
+        if (c0 + 16 < columns) rows[1].load(w, head, entry, lane);
         entry = PageRows<NG>::entry(row, c0 + 32, columns, lane);
-        now.report(c0, columns, lane);
-#pragma unroll
-        for (int k = 0; k < PRODUCTS; ++k)
-          now.score(w, q[k], c0, columns, lane, [&](int slot, int c, uint32_t key) {
-            uint32_t* at = keys + static_cast<int64_t>(k * each + slot) * w.key_ld + c;
-            *at = h > 0 ? max(key, *at) : key;
-          });
+        step(rows[0], c0);
+        if (c0 + 16 >= columns) break;
+        if (c0 + 32 < columns) rows[0].load(w, head, entry, lane);
+        entry = PageRows<NG>::entry(row, c0 + 48, columns, lane);
+        step(rows[1], c0 + 16);
       }
     }
     __syncwarp();

@@ -448,10 +448,13 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   P.scale_log2 = scale * 1.4426950408889634f;
   // Tokens of a sequence mostly want the same pages: from eight of them to a sequence on (or fewer, with more than eight
   // query heads to a kv head) a tile of them is taken together.
-  const int tokens = P.group <= pre::TILE ? spt::tile_tokens(P.group) : 0;
-  if (tokens && total * P.passes >= 8 * batch && std::min(tokens * count, table_cols) <= spt::MAX_UNION &&
-      table_cols <= spt::columns(d) && q_token_stride >= 8 && q_head_stride >= 8)
-    return d == 64 ? spt::launch<1>(P, heads, stream) : spt::launch<2>(P, heads, stream);
+  if (total * P.passes >= 8 * batch && q_token_stride >= 8 && q_head_stride >= 8 && spt::fits(P, d, 1)) {
+    // two tiles to a CTA, which share the expansion, where that leaves no SM idle: (XXX)
+    const int64_t pairs = total / (2 * spt::tile_tokens(P.group)) * kv_heads;
+    if (spt::fits(P, d, 2) && pairs * 4 >= 3 * num_sms())
+      return d == 64 ? spt::launch<1, 2>(P, heads, stream) : spt::launch<2, 2>(P, heads, stream);
+    return d == 64 ? spt::launch<1, 1>(P, heads, stream) : spt::launch<2, 1>(P, heads, stream);
+  }
   const int64_t units = total * kv_heads * P.passes, blocks = count << (P.p.page_shift - 4);
   int split = 1;
   while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > W * split) split *= 2;

@@ -471,6 +471,13 @@ SHAPES = [  # heads, kv_heads, d, page, lens, new, count
     (16, 2, 128, 16, [40] * 10, [20] * 10, 3),
     (8, 1, 128, 16, [3500], [16], 100),
     (4, 4, 64, 32, [3000, 2, 700], [90, 2, 1], 60),
+    # two tiles of them to a CTA, the second full, in part there or not at all
+    (128, 16, 128, 16, [900, 300], [180, 77], 9),
+    (128, 16, 64, 64, [1500, 40, 8], [230, 17, 8], 12),
+    (64, 16, 128, 32, [500, 70], [400, 66], 5),
+    (320, 8, 128, 16, [130], [97], 4),
+    (16, 16, 64, 16, [460], [460], 6),
+    (144, 16, 64, 128, [1000], [203], 2),
 ]
 
 
