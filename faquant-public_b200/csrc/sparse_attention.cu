@@ -10,9 +10,17 @@
 // entry, table entry, address), drops those that are not there or lie behind the token, and streams the rest
 // through a ring of bulk copies.
 //
+// A column counts once: where a list is not ascending, entries that an earlier one repeats are dropped.
+//
 // Work split: a unit's blocks are dealt out to the warps of a cluster of 1, 2, 4 or 8 CTAs, as many as fill the
 // SMs once; the CTAs' results meet through distributed shared memory, so there is no second
 // kernel and no workspace. The order of every sum is fixed by the list and the cluster's size.
+//
+// Measured (one B200, 32 query heads on 8 kv heads of 128, one new token): 32 pages of 64 of a context
+// of 32768 in 8.0 us, 64 pages of 16 of 32 sequences of 1 .. 16000 tokens in 16.6 us. The first is a chain of
+// loads (cu and lens, the list, the table, the pages), two blocks per warp and the two joins; the second
+// some 10700 blocks at 190 cycles of an SM each (see paged_attention.cu: 118 of issue), as 256 CTAs
+// of unequal length in one wave; clusters of two there took 20.3 us, of four 31.2.
 #include "kv_pages.cuh"
 
 namespace faq {
@@ -448,13 +456,10 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   P.scale_log2 = scale * 1.4426950408889634f;
   // Tokens of a sequence mostly want the same pages: from eight of them to a sequence on (or fewer, with more than eight
   // query heads to a kv head) a tile of them is taken together.
-  if (total * P.passes >= 8 * batch && q_token_stride >= 8 && q_head_stride >= 8 && spt::fits(P, d, 1)) {
-    // two tiles to a CTA, which share the expansion, where that leaves no SM idle: (XXX)
-    const int64_t pairs = total / (2 * spt::tile_tokens(P.group)) * kv_heads;
-    if (spt::fits(P, d, 2) && pairs * 4 >= 3 * num_sms())
-      return d == 64 ? spt::launch<1, 2>(P, heads, stream) : spt::launch<2, 2>(P, heads, stream);
-    return d == 64 ? spt::launch<1, 1>(P, heads, stream) : spt::launch<2, 1>(P, heads, stream);
-  }
+  const int tokens = P.group <= pre::TILE ? spt::tile_tokens(P.group) : 0;
+  if (tokens && total * P.passes >= 8 * batch && std::min(tokens * count, table_cols) <= spt::MAX_UNION &&
+      table_cols <= spt::columns(d) && q_token_stride >= 8 && q_head_stride >= 8)
+    return d == 64 ? spt::launch<1>(P, heads, stream) : spt::launch<2>(P, heads, stream);
   const int64_t units = total * kv_heads * P.passes, blocks = count << (P.p.page_shift - 4);
   int split = 1;
   while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > W * split) split *= 2;

@@ -8,11 +8,18 @@
 // marked columns in order: page, column, tokens. A column counts once, however often it is listed.
 // Key tiles are 8 blocks of 16 tokens, as they come in that order.
 //
-// One CTA per (sequence, kv head, one or two tiles of tokens), or a cluster of 2, 4 or 8 that share the union's
-// key tiles and add up their rows through distributed shared memory. With two tiles the expansion serves both:
-// the sixteen softmax warps take their steps in turn, P and V have one buffer.
+// One CTA per (sequence, kv head, tile of tokens), or a cluster of 2, 4 or 8 that share the union's key tiles
+// and add up their rows through distributed shared memory.
 //
-// Measured (one B200): 512 tokens of 32768 with 64 query heads on 8 kv heads of 128, 32 pages of 64 each, XXX
+// Measured (one B200): 512 tokens of 32768 with 64 query heads on 8 kv heads of 128 and 32 pages of 64
+// tokens each, 164 us (359 with the kernel of single tokens): 9000 key tiles (the lists of 16 neighbours
+// hold some 75 pages) at 4300 cycles, two waves of CTAs. The expansion is what the others wait for: a warp
+// takes 1100 cycles for its block of K and 1300 for one of V, at one instruction in five cycles, then come waits
+// for its slots. Dropped: eight softmax warps with 64 keys a thread (186 us; read twice from
+// tensor memory, with sixteen expanding warps, 173: then the softmax is), two tiles of rows to a CTA that share the
+// expansion (173: their sixteen softmax warps move in step, and the exponentials' unit idles between),
+// twelve expanding warps (175, with 64 registers and loads one block ahead), two places for S and a warp of their
+// own for the products with V (167).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -85,30 +92,27 @@ using spa::Params;
 constexpr int SOFTMAX_WARPS = 16, EXPAND_WARPS = 8;
 constexpr int THREADS = 32 * (SOFTMAX_WARPS + EXPAND_WARPS + 4);  // and a warpgroup for Q and the products
 constexpr int PRODUCTS = SOFTMAX_WARPS + EXPAND_WARPS;  // the warp that issues them
-constexpr int MAX_TOKENS = 64;   // of a CTA: bits of a mark
-constexpr int MAX_UNION = 1024;  // columns of a CTA's union
-// the table's columns whose marks fit where K, V and P will be
-__host__ __device__ constexpr int columns(int d) { return d / 64 * 4 * CHUNK / 8; }
-__host__ __device__ constexpr int tile_tokens(int group) { return TILE / group < MAX_TOKENS / 2 ? TILE / group : MAX_TOKENS / 2; }
+constexpr int MAX_UNION = 1536;  // columns of a tile's union
+// the table's columns whose marks fit where K and V will be
+__host__ __device__ constexpr int columns(int d) { return d / 64 * 4 * CHUNK / 4; }
+__host__ __device__ constexpr int tile_tokens(int group) { return TILE / group < 32 ? TILE / group : 32; }
 
-template <int NG, int TILES>
+template <int NG>
 struct Smem {
-  static constexpr int tile = NG * CHUNK, v_stages = TILES == 1 ? 2 : 1;
+  static constexpr int tile = NG * CHUNK;
   static constexpr int q = 0;
-  static constexpr int k = q + TILES * tile;  // [2 stages]
+  static constexpr int k = q + tile;
   static constexpr int v = k + 2 * tile;
-  static constexpr int p = v + v_stages * tile;
+  static constexpr int p = v + 2 * tile;
   static constexpr int page = p + 2 * CHUNK;          // [MAX_UNION]
   static constexpr int entry = page + 8 * MAX_UNION;  // [MAX_UNION + 8], the last ones' tokens none
-  static constexpr int scratch = entry + 16 * (MAX_UNION + 8);  // [4][TILE]
+  static constexpr int scratch = entry + 8 * (MAX_UNION + 8);  // [4][TILE]
   static constexpr int bar = scratch + 16 * TILE;
   static constexpr int bytes = 1024 + bar + 256;
   // at the end, where K and V were: O [TILE][D], m and l [TILE]
   static constexpr int o = k;
-  static constexpr int marks = k;  // at the start: [columns] of 64 bits
-  static_assert(p + 2 * CHUNK - marks >= 8 * columns(64 * NG), "marks");
 };
-static_assert(Smem<2, 1>::bytes <= 227 * 1024 && Smem<2, 2>::bytes <= 227 * 1024, "shared memory");
+static_assert(Smem<2>::bytes <= 227 * 1024, "shared memory");
 
 // As the slots of blocks (kv_cache.cu): n tokens are at most n / T + 1 tiles of T, so sequence b's
 // tiles get the slots from cu[b] / T + b on.
@@ -132,16 +136,15 @@ __device__ __forceinline__ void tmem_stf(uint32_t taddr, const float* v) {
 // The softmax of a tile's rows, of which each sees some of a key tile's blocks only, by sixteen warps.
 // TMEM lets a warp read the lanes of its own quarter (warp % 4), so the four warps of a quarter share
 // its 32 rows: part warp / 4 has the keys 32 part .. of every key tile and that quarter of O's channels.
-// (Eight warps with 64 keys a thread spilled their registers and took XXX us instead of YYY.)
+// Eight warps with 64 keys a thread spilled their registers.
 template <int D>
 struct Softmax {
   static constexpr int KEYS = TILE / 4, BLOCKS = KEYS / BLOCK, CHANNELS = D / 4;
   int lane, quarter, part, row;
-  uint32_t s_addr, o_addr, p_row;  // of the first tile
+  uint32_t s_addr, o_addr, p_row;
   float* scratch;  // [4][TILE]
-  uint32_t s_full, s_free, p_full, pv_done;  // the first two per tile
-  float scale_log2, m, l;  // the reference maximum (log2) and the row's sum, of the tile at hand
-  float m_other, l_other;  // of the other one
+  uint32_t s_full, s_free, p_full, pv_done;
+  float scale_log2, m, l;  // the reference maximum (log2) and, after run(), the row's sum
 
   __device__ __forceinline__ Softmax(uint32_t tmem, int warp, int lane_, uint8_t* p, float* x, uint64_t* full, uint64_t* free_,
                                      uint64_t* pfull, uint64_t* pv, float scale)
@@ -164,38 +167,27 @@ struct Softmax {
     return pre::bar_and(1 + quarter, 128, well);  // read: it may be written again
   }
 
-  __device__ __forceinline__ void turn() {  // to the other tile
-    const float x = m, y = l;
-    m = m_other;
-    l = l_other;
-    m_other = x;
-    l_other = y;
-  }
-
-  // `count` key tiles for `tiles` tiles of rows in turn; keys(t, j, block) is how many keys of block `block`
-  // (0 .. 7) of key tile j the row of tile t sees, there(t) whether it is one of the unit's. A block that none
-  // of the warp's rows sees costs nothing but its zeros. False: a wait ran out.
-  template <int TILES, typename F, typename G>
-  __device__ __forceinline__ bool run(int count, int tiles, F&& there, G&& keys) {
-    m = there(0) ? LOWEST : INFINITY;  // rows that are not there never raise the others' maxima
-    m_other = TILES > 1 && there(1) ? LOWEST : INFINITY;
-    l = l_other = 0.0f;
+  // `count` key tiles; keys(j, block) is how many keys of block `block` (0 .. 7) of key tile j the row
+  // sees. A block that none of the warp's rows sees costs nothing but its zeros. False: a wait ran out.
+  template <typename F>
+  __device__ __forceinline__ bool run(int count, bool there, F&& keys) {
+    m = there ? LOWEST : INFINITY;  // rows that are not there never raise the others' maxima
+    l = 0.0f;
     bool ok = true;
-    int t = 0, j = 0;
-    for (int n = 0; n < count * tiles; ++n) {
+    for (int j = 0; j < count; ++j) {
       int seen[BLOCKS];
 #pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) seen[c] = keys(t, j, part * BLOCKS + c);
-      ok = ok && mbar_wait_warp(s_full + 8 * t, j & 1, 98, n);
+      for (int c = 0; c < BLOCKS; ++c) seen[c] = keys(j, part * BLOCKS + c);
+      ok = ok && mbar_wait_warp(s_full, j & 1, 98, j);
       tc_fence_after();
       float f[KEYS];
-      tmem_ld32f(s_addr + (TILES > 1 ? s_col(1) * t : 0), f);
+      tmem_ld32f(s_addr, f);
       tc_wait_ld();
       reg_fence32f(f);
       // S is in registers: the tensor core may write the next one
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free + 8 * t);
+      if (lane == 0) mbar_arrive(s_free);
       float mine = -INFINITY;
 #pragma unroll
       for (int c = 0; c < BLOCKS; ++c) {
@@ -215,7 +207,7 @@ struct Softmax {
       float a = 1.0f;
       const bool raise = pre::bar_or(1 + quarter, 128, __fmul_rn(mine, scale_log2) > m + pat::RAISE || !ok);
       if (raise) {
-        if (n > 0) ok = ok && mbar_wait_warp(pv_done, (n - 1) & 1, 99, n);
+        if (j > 0) ok = ok && mbar_wait_warp(pv_done, (j - 1) & 1, 99, j);
         float all[4];
         if (!exchange(ok, mine, all)) return false;
         const float top = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3]));
@@ -245,8 +237,8 @@ struct Softmax {
           for (int x = 0; x < BLOCK / 2; ++x) w[BLOCK / 2 * c + x] = 0u;
         }
       }
-      // the product of the step before has read P; so has the tile's last one, and O is its
-      if (n > 0) ok = mbar_wait_warp(pv_done, (n - 1) & 1, 99, n);
+      // the product of the step before has read P, and O is its
+      if (j > 0) ok = mbar_wait_warp(pv_done, (j - 1) & 1, 99, j);
 #pragma unroll
       for (int u = 0; u < KEYS / 8; ++u)  // key chunk, row, unit at unit ^ (row % 8), as TMA would lay it out
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + ((((part & 1) * 4 + u) ^ (row & 7)) << 4)),
@@ -256,43 +248,32 @@ struct Softmax {
       tc_fence_after();
       if (raise && j > 0) {
         float o[CHANNELS];
-        const uint32_t at = o_addr + (TILES > 1 ? s_col(1) * t : 0);
-        pre::tmem_ldf<CHANNELS>(at, o);
+        pre::tmem_ldf<CHANNELS>(o_addr, o);
         tc_wait_ld();
         pre::reg_fencef<CHANNELS>(o);
 #pragma unroll
         for (int x = 0; x < CHANNELS; ++x) o[x] = o[x] * a * a;
-        tmem_stf<CHANNELS>(at, o);
+        tmem_stf<CHANNELS>(o_addr, o);
         tc_wait_st();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
-      if (TILES > 1 && tiles > 1) {
-        turn();
-        t ^= 1;
-        j += t == 0;
-      } else {
-        ++j;
-      }
     }
-    ok = ok && mbar_wait_warp(pv_done, (count * tiles - 1) & 1, 99, count);
+    ok = ok && mbar_wait_warp(pv_done, (count - 1) & 1, 99, count);
     tc_fence_after();
-    for (int i = 0; i < tiles; ++i) {
-      float all[4];
-      if (!exchange(ok, l, all)) return false;
-      l = (all[0] + all[1]) + (all[2] + all[3]);
-      if (TILES > 1 && tiles > 1) turn();
-    }
+    float all[4];
+    if (!exchange(ok, l, all)) return false;
+    l = (all[0] + all[1]) + (all[2] + all[3]);
     return true;
   }
 
-  // O of the row of tile t, the one at hand: to dst (bf16, normalized) or, unnormalized with m and l, to the
-  // rows `o` of a partial. Whole warps take part; only live ones store.
-  __device__ __forceinline__ void store(int t, bool live, float* o, __nv_bfloat16* dst) {
+  // O of the row: to dst (bf16, normalized) or, unnormalized with m and l, to the rows `o` of a
+  // partial. Whole warps take part; only live ones store.
+  __device__ __forceinline__ void store(bool live, float* o, __nv_bfloat16* dst) {
     const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);  // NaN stays
     float v[CHANNELS];
-    pre::tmem_ldf<CHANNELS>(o_addr + s_col(1) * t, v);
+    pre::tmem_ldf<CHANNELS>(o_addr, v);
     tc_wait_ld();
     pre::reg_fencef<CHANNELS>(v);
     if (live && o) {
@@ -314,25 +295,25 @@ struct Softmax {
   }
 };
 
-template <int NG, int TILES>
+template <int NG>
 __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_constant__ CUtensorMap map_q, Params P, int split) {
-  using L = Smem<NG, TILES>;
+  using L = Smem<NG>;
   constexpr int D = 64 * NG, WARPS = THREADS / 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::bar);
   uint64_t* q_full = bars + 0;
-  uint64_t* pv_done = bars + 1;
   uint64_t* k_full = bars + 2;  // [2 stages]
   uint64_t* k_empty = bars + 4;
   uint64_t* v_full = bars + 6;
   uint64_t* v_empty = bars + 8;
-  uint64_t* s_full = bars + 10;  // [tile of rows]
-  uint64_t* s_free = bars + 12;
-  uint64_t* p_full = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* s_full = bars + 10;
+  uint64_t* s_free = bars + 11;
+  uint64_t* p_full = bars + 12;
+  uint64_t* pv_done = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   int64_t* s_page = reinterpret_cast<int64_t*>(base + L::page);  // offset of a page's K of this head
-  int4* s_entry = reinterpret_cast<int4*>(base + L::entry);      // its first block in the sequence, its tokens (64 bits)
+  int2* s_entry = reinterpret_cast<int2*>(base + L::entry);  // a page's first block in the sequence, its tokens
   __shared__ int64_t s_scan[WARPS];
   __shared__ int s_well;  // softmax warps that came to their end
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -341,27 +322,29 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   allow_dependent_launch();
 
   // ---- the unit
-  const int T = tile_tokens(P.group), TT = TILES * T;  // tokens of a tile, of the CTA
+  const int T = tile_tokens(P.group);
   const int rank = static_cast<int>(blockIdx.x % split);
   const int64_t unit = blockIdx.x / split, slot = unit / p.kv_heads;
   const int head = static_cast<int>(unit - slot * p.kv_heads);
   if (blockIdx.x == 0) check_batch(p, P.total, tid, THREADS);
-  const int b = last_of(p.batch, [&](int i) { return p.cu[i] / TT + static_cast<int64_t>(i) <= slot; });
+  const int b = last_of(p.batch, [&](int i) { return p.cu[i] / T + static_cast<int64_t>(i) <= slot; });
   const int64_t c0 = p.cu[b], n = p.cu[b + 1] - c0;
-  const int64_t u = slot - (c0 / TT + b);
-  if (c0 < 0 || n <= 0 || c0 + n > P.total || u < 0 || u * TT >= n) return;  // the whole cluster
-  const int64_t tok0 = u * TT;
-  const int tokens = static_cast<int>(std::min<int64_t>(TT, n - tok0)), row_tiles = TILES > 1 && tokens > T ? 2 : 1;
-  const int64_t pos0 = p.lens[b] - n + tok0;  // of the first token
+  const int64_t u = slot - (c0 / T + b);
+  if (c0 < 0 || n <= 0 || c0 + n > P.total || u < 0 || u * T >= n) return;  // the whole cluster
+  const int64_t tok0 = u * T;
+  const int tokens = static_cast<int>(std::min<int64_t>(T, n - tok0));
+  const int64_t pos0 = p.lens[b] - n + tok0;  // of the tile's first token
   const int64_t last_pos = pos0 + tokens - 1;
 
   // ---- which of the tokens list a column
-  uint64_t* marks = reinterpret_cast<uint64_t*>(base + L::marks);
+  uint32_t* marks = reinterpret_cast<uint32_t*>(base + L::k);
   const int seen = last_pos < 0 ? 0 : static_cast<int>(std::min<int64_t>((last_pos >> p.page_shift) + 1, p.table_cols));
   for (int c = tid; c < seen; c += THREADS) marks[c] = 0;
   if (tid == 0) {
     s_well = 0;
     mbar_init(smem_addr(q_full), 1);
+    mbar_init(smem_addr(s_full), 1);
+    mbar_init(smem_addr(s_free), SOFTMAX_WARPS);
     mbar_init(smem_addr(p_full), SOFTMAX_WARPS);
     mbar_init(smem_addr(pv_done), 1);
     for (int i = 0; i < 2; ++i) {
@@ -369,8 +352,6 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
       mbar_init(smem_addr(&k_empty[i]), 1);
       mbar_init(smem_addr(&v_full[i]), EXPAND_WARPS);
       mbar_init(smem_addr(&v_empty[i]), 1);
-      mbar_init(smem_addr(&s_full[i]), 1);
-      mbar_init(smem_addr(&s_free[i]), SOFTMAX_WARPS);
     }
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
@@ -388,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     const int col = P.list[((c0 + tok0 + tok) * p.kv_heads + head) * P.count + (i - tok * P.count)];
     if (col >= 0 && static_cast<int64_t>(col) << p.page_shift <= pos0 + tok) {
       if (col < seen)
-        atomicOr(reinterpret_cast<uint32_t*>(&marks[col]) + (tok >> 5), 1u << (tok & 31));
+        atomicOr(&marks[col], 1u << tok);
       else
         atomicOr(&g_status, FAQ_STATUS_BAD_PAGE);  // beyond the table
     }
@@ -413,9 +394,9 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     for (int c = begin; c < end; ++c)
       if (marks[c]) {
         s_page[i] = p.table[b * p.table_ld + c] * p.page_stride + block_in_page<NG>(p, 0, head, 0);
-        s_entry[i++] = make_int4(c << (p.page_shift - 4), static_cast<int>(marks[c]), static_cast<int>(marks[c] >> 32), 0);
+        s_entry[i++] = make_int2(c << (p.page_shift - 4), static_cast<int>(marks[c]));
       }
-    if (tid < 8) s_entry[found + tid] = make_int4(0, 0, 0, 0);
+    if (tid < 8) s_entry[found + tid] = make_int2(0, 0);
   }
   __syncthreads();
   const int block_shift = p.page_shift - 4, in_page = (1 << block_shift) - 1;
@@ -432,10 +413,10 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n" ::: "memory");
     if (warp == PRODUCTS + 1) {
       if (lane == 0 && count > 0) {
-        mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(row_tiles * T * P.group) * 128 * NG);
-        for (int c = 0; c < NG * row_tiles; ++c)
-          tma_load_3d(smem_addr(base + L::q + c * CHUNK), &map_q, smem_addr(q_full), c % NG * 64, head * P.group,
-                      static_cast<int>(c0 + tok0 + c / NG * T));
+        mbar_arrive_expect_tx(smem_addr(q_full), static_cast<uint32_t>(T * P.group) * 128 * NG);
+        for (int c = 0; c < NG; ++c)
+          tma_load_3d(smem_addr(base + L::q + c * CHUNK), &map_q, smem_addr(q_full), c * 64, head * P.group,
+                      static_cast<int>(c0 + tok0));
         mbar_wait_site(smem_addr(q_full), 0, 90, 0);  // (bounded) it is there before the CTA's end
       }
     } else if (warp == PRODUCTS) {
@@ -448,46 +429,41 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
       auto wait = [&](uint64_t* bar, uint32_t parity, int site, int step) {
         return mbar_wait_warp(smem_addr(bar), parity & 1, site, step);
       };
-      // the scores of tile t with key tile j, whose K is done with after the last tile of rows
-      auto issue_qk = [&](int t, uint32_t st, bool last) {
+      auto issue_qk = [&](auto stage) {
+        constexpr int st = decltype(stage)::value;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
-          mma_ss(tmem + s_col(t), q_desc + t * TILE_D + off, k_desc + st * TILE_D + off, IDESC_QK, kk != 0);
+          mma_ss(tmem + s_col(0), q_desc + off, k_desc + st * TILE_D + off, IDESC_QK, kk != 0);
         }
-        commit(smem_addr(&s_full[t]));
-        if (last) commit(smem_addr(&k_empty[st]));
+        commit(smem_addr(s_full));
+        commit(smem_addr(&k_empty[st]));
       };
-      auto issue_pv = [&](int t, uint32_t st, bool add, bool last) {
+      auto issue_pv = [&](auto stage, bool add) {
+        constexpr int st = decltype(stage)::value;
 #pragma unroll
         for (int kk = 0; kk < TILE / 16; ++kk) {
           const uint32_t off = static_cast<uint32_t>((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4;
-          mma_ss(tmem + o_col(t), p_desc + off, v_desc + st * TILE_D + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
+          mma_ss(tmem + o_col(0), p_desc + off, v_desc + st * TILE_D + ((kk * 2048) >> 4), idesc_pv(D), add || kk != 0);
         }
         commit(smem_addr(pv_done));
-        if (last) commit(smem_addr(&v_empty[st]));
+        commit(smem_addr(&v_empty[st]));
       };
-      auto scores = [&](int t, uint32_t j) {
-        if (t == 0 && !wait(&k_full[j & 1], j >> 1, 91, j)) return false;
-        if (j > 0 && !wait(&s_free[t], j - 1, 92, j)) return false;
+      const std::integral_constant<int, 0> st0;
+      const std::integral_constant<int, 1> st1;
+      auto scores = [&](uint32_t step) {
+        if (!wait(&k_full[step & 1], step >> 1, 91, step)) return false;
+        if (step > 0 && !wait(s_free, step - 1, 92, step)) return false;
         tc_fence_after();
-        issue_qk(t, j & 1, t == row_tiles - 1);
+        if (step & 1) issue_qk(st1); else issue_qk(st0);
         return true;
       };
-      bool ok = count > 0 && wait(q_full, 0, 93, 0) && scores(0, 0);
-      if (row_tiles > 1) ok = ok && scores(1, 0);
+      const bool ok = count > 0 && wait(q_full, 0, 93, 0) && scores(0);
       for (int j = 0; j < count && ok; ++j) {
-        const uint32_t st = L::v_stages == 2 ? j & 1 : 0;
-        for (int t = 0; t < row_tiles && ok; ++t) {
-          // one tile: the next scores run under this step's exponentials; two: under the other tile's
-          if (row_tiles == 1 && j + 1 < count) ok = scores(0, j + 1);
-          ok = ok && (t > 0 || wait(&v_full[st], L::v_stages == 2 ? j >> 1 : j, 94, j)) &&
-               wait(p_full, j * row_tiles + t, 95, j);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, st, j != 0, t == row_tiles - 1);
-          if (row_tiles > 1 && j + 1 < count) ok = scores(t, j + 1);
-        }
+        if (j + 1 < count && !scores(j + 1)) break;
+        if (!wait(&v_full[j & 1], j >> 1, 94, j) || !wait(p_full, j, 95, j)) break;
+        tc_fence_after();
+        if (j & 1) issue_pv(st1, j != 0); else issue_pv(st0, j != 0);
       }
     }
     __syncwarp();
@@ -529,39 +505,33 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
       if (src) kb.load(src, lane);
-      const int vs = L::v_stages == 2 ? st : 0, v_phase = L::v_stages == 2 ? step >> 1 : step;
-      if (!mbar_wait_warp(smem_addr(&v_empty[vs]), (v_phase & 1) ^ 1, 97, step)) break;
-      vb.template each<2>(expand, lane, write(base + L::v + vs * L::tile));
+      if (!mbar_wait_warp(smem_addr(&v_empty[st]), ((step >> 1) & 1) ^ 1, 97, step)) break;
+      vb.template each<2>(expand, lane, write(base + L::v + st * L::tile));
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&v_full[vs]));
+      if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
       if (src) vb.load(src + v_off, lane);
     }
   } else {
     Softmax<D> sm(tmem, warp, lane, base + L::p, reinterpret_cast<float*>(base + L::scratch), s_full, s_free, p_full, pv_done,
                   P.scale_log2);
-    // the row's token of the first tile; that of the second is T further
-    const int row = sm.row, tok = row / P.group, row_head = row - tok * P.group;
-    auto there = [&](int t) { return tok < T && t * T + tok < tokens; };
+    const int row = sm.row, tok = row / P.group;
+    const bool live = tok < tokens;
     const int sees = static_cast<int>(pos0) + tok + 1;  // keys, of the pages its token lists
-    const uint64_t bit0 = there(0) ? 1ull << tok : 0, bit1 = TILES > 1 && there(1) ? 1ull << (T + tok) : 0;
+    const uint32_t bit = live ? 1u << tok : 0u;
     const int block0 = k0 * 8;
-    auto keys = [&](int t, int j, int block) {
+    auto keys = [&](int j, int block) {
       const int i = block0 + j * 8 + block;
-      const int4 e = s_entry[i >> block_shift];
-      const int left = min(max(sees + (TILES > 1 ? t * T : 0) - ((e.x + (i & in_page)) << 4), 0), BLOCK);
-      const uint64_t bit = TILES > 1 && t ? bit1 : bit0;
-      return (static_cast<uint32_t>(e.y) & static_cast<uint32_t>(bit)) | (static_cast<uint32_t>(e.z) & static_cast<uint32_t>(bit >> 32))
-                 ? left
-                 : 0;
+      const int2 e = s_entry[i >> block_shift];
+      const int left = min(max(sees - ((e.x + (i & in_page)) << 4), 0), BLOCK);
+      return e.y & bit ? left : 0;
     };
-    const bool ok = count == 0 || sm.template run<TILES>(count, row_tiles, there, keys);
+    const bool ok = count == 0 || sm.run(count, live, keys);
     if (ok && lane == 0) atomicAdd(&s_well, 1);
-    for (int t = 0; ok && count > 0 && t < row_tiles; ++t) {
-      const bool live = there(t);
-      sm.store(t, live, split == 1 ? nullptr : reinterpret_cast<float*>(base + L::o),
-               P.out + (c0 + tok0 + (live ? t * T + tok : 0)) * P.ot + (static_cast<int64_t>(head) * P.group + row_head) * P.oh);
-      sm.turn();
+    if (ok && count > 0) {
+      const int row_head = row - tok * P.group;
+      sm.store(live, split == 1 ? nullptr : reinterpret_cast<float*>(base + L::o),
+               P.out + (c0 + tok0 + (live ? tok : 0)) * P.ot + (static_cast<int64_t>(head) * P.group + row_head) * P.oh);
     }
   }
   __syncthreads();
@@ -614,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   cluster_sync();  // the others have read this CTA's rows
 }
 
-template <int NG, int TILES>
+template <int NG>
 static int launch(const Params& P, int64_t heads, void* stream) {
   constexpr int D = 64 * NG;
   CUtensorMap map_q;
@@ -623,24 +593,18 @@ static int launch(const Params& P, int64_t heads, void* stream) {
   const uint32_t box[3] = {64, static_cast<uint32_t>(P.group), static_cast<uint32_t>(tile_tokens(P.group))};
   int rc = make_tmap(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, P.q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  auto kern = sparse_tile_kernel<NG, TILES>;
+  auto kern = sparse_tile_kernel<NG>;
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
-  rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG, TILES>::bytes, set);
+  rc = allow_smem(reinterpret_cast<const void*>(kern), Smem<NG>::bytes, set);
   if (rc) return rc;
-  const int64_t units = slots_of(P.total, P.p.batch, TILES * tile_tokens(P.group)) * P.p.kv_heads;
+  const int64_t units = slots_of(P.total, P.p.batch, tile_tokens(P.group)) * P.p.kv_heads;
   // as many CTAs as fill the SMs once, of some key tiles each
   const int64_t tiles = (static_cast<int64_t>(P.count) << (P.p.page_shift - 4)) / 8;
   int split = 1;
-  while (TILES == 1 && split < 8 && units * split * 2 <= num_sms() && tiles >= 4 * split) split *= 2;
+  while (split < 8 && units * split * 2 <= num_sms() && tiles >= 4 * split) split *= 2;
   FAQ_CHECK_ARG(units * split < (int64_t(1) << 31), "too many tokens for one call");
-  FAQ_CUDA(launch_clusters(kern, units * split, THREADS, Smem<NG, TILES>::bytes, split, stream, map_q, P, split));
+  FAQ_CUDA(launch_clusters(kern, units * split, THREADS, Smem<NG>::bytes, split, stream, map_q, P, split));
   return launch_status("sparse_tile_kernel");
-}
-
-// Whether tiles can take the call: the marks and the union of a CTA's tokens' lists fit.
-static bool fits(const Params& P, int d, int tiles) {
-  return P.group <= TILE && P.p.table_cols <= columns(d) &&
-         std::min<int64_t>(static_cast<int64_t>(tiles * tile_tokens(P.group)) * P.count, P.p.table_cols) <= MAX_UNION;
 }
 
 }  // namespace spt
