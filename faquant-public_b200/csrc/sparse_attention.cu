@@ -435,6 +435,7 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   FAQ_CHECK_ARG(total >= 0 && total < (int64_t(1) << 31), "bad token count");
   FAQ_CHECK_ARG(heads > 0 && heads < (int64_t(1) << 24) && heads % kv_heads == 0,
                 "query heads must be divisible by key/value heads");
+  FAQ_CHECK_ARG(total * heads < (int64_t(1) << 31), "too many tokens for one call");
   FAQ_CHECK_ARG(count > 0 && count < (int64_t(1) << 24), "bad page count");
   FAQ_CHECK_ARG(scale > 0.0f && scale < 1e30f, "scale must be positive");
   if (total == 0) return FAQ_OK;
@@ -454,13 +455,22 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   P.list = selected;
   P.count = static_cast<int>(count);
   P.scale_log2 = scale * 1.4426950408889634f;
-  // Tokens of a sequence mostly want the same pages: from eight of them to a sequence on (or fewer, with more than eight
-  // query heads to a kv head) a tile of them is taken together.
+  const int64_t units = total * kv_heads * P.passes, blocks = std::min(count, table_cols) << (P.p.page_shift - 4);
+  // Tokens of a sequence mostly want the same pages. Tiles of them (sparse_tile.cu) take a call where a sequence has
+  // eight tokens, or blocks of eight query heads of them, on average, and the kernel of single tokens would
+  // expand 440 blocks or more per SM, some 50 us. Both kernels, us, where neighbours' lists differ in about a third
+  // of the pages (the tiles' also where they are the same, and have nothing in common), 32 pages of 64, heads of 128:
+  //   16 sequences, 4 tokens, 32 / 8 heads (443 blocks per SM)  55   59 (48, 104)
+  //   the same, 8 tokens (886)                                  94   66 (52, 134)
+  //   1 sequence, 8 tokens, 64 / 8 heads (55)                   14   26 (23, 41)
+  //   4 sequences, 8 tokens, 8 / 8 heads (221)                  29   40 (32, 70)
+  //   the same, 32 tokens (886)                                 92   45 (36, 77)
+  //   1 sequence, 512 tokens, 64 / 8 heads (3542)              359  169 (110, 598)
   const int tokens = P.group <= pre::TILE ? spt::tile_tokens(P.group) : 0;
-  if (tokens && total * P.passes >= 8 * batch && std::min(tokens * count, table_cols) <= spt::MAX_UNION &&
-      table_cols <= spt::columns(d) && q_token_stride >= 8 && q_head_stride >= 8)
+  if (tokens && total * P.passes >= 8 * batch && units * blocks >= 440 * static_cast<int64_t>(num_sms()) &&
+      std::min(tokens * count, table_cols) <= spt::MAX_UNION && table_cols <= spt::columns(d) && q_token_stride >= 8 &&
+      q_head_stride >= 8)
     return d == 64 ? spt::launch<1>(P, heads, stream) : spt::launch<2>(P, heads, stream);
-  const int64_t units = total * kv_heads * P.passes, blocks = count << (P.p.page_shift - 4);
   int split = 1;
   while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > W * split) split *= 2;
   FAQ_CHECK_ARG(units * split < (int64_t(1) << 31), "too many tokens for one call");

@@ -333,6 +333,30 @@ def test_selection_matches_the_definition(shape) -> None:
     _no_status()
 
 
+def test_selection_of_strided_and_unaligned_operands() -> None:
+    from faquant_b200 import ops
+
+    lens, new = [300, 90, 1200], [1, 2, 1]
+    pool = Pool(lens, 2, 64, 16, DEV)
+    k = _randn(sum(lens), 2, 64, seed=41)
+    pool.write(k, k)
+    bounds = _bounds(pool)
+    _refresh(pool, bounds)
+    wide = _randn(4, 6 * 64 + 8, seed=42)[:, 3 : 3 + 6 * 64].unflatten(1, (6, 64))  # not 16-byte aligned
+    turned = _randn(64, 6, 4, seed=43).permute(2, 1, 0)                            # channels outermost
+    table = torch.full((3, pool.table.shape[1] + 5), -1, dtype=torch.int32, device=DEV)[:, 2:-3]
+    table.copy_(pool.table)
+    for q in (wide, turned):
+        got = ops.hif4_select_pages(q, bounds, table, pool.cu(new), pool.lens, page_size=16, count=9)
+        assert torch.equal(got.cpu(), ref.select(q, k, lens, new, 16, 9, 1, 2)[0])
+        lists = torch.empty(4, 2, 12, dtype=torch.int32, device=DEV)[..., :9]
+        lists.copy_(got)  # a list that is a slice
+        out = ops.hif4_sparse_attention(q, pool.pages, table, pool.cu(new), pool.lens, lists, page_size=16)
+        want, size = ref.attention(q, quantized(k), quantized(k), lens, new, 16, got.cpu())
+        assert bool(((out.double().cpu() - want).abs() <= BOUND * size).all())
+    _no_status()
+
+
 def test_scores_bound_the_products() -> None:
     """A page's score is at least the product of the 8-bit query with every key of the page."""
     from faquant_b200 import ops
@@ -460,24 +484,22 @@ SHAPES = [  # heads, kv_heads, d, page, lens, new, count
     (16, 8, 128, 16, [600], [300], 6),
     (7, 7, 64, 4096, [5000], [1], 2),
     (1, 1, 128, 16, [4000], [1], 250),
-    # tokens taken together: one to 32 of them, all ratios of heads, one CTA or a cluster
-    (1, 1, 128, 16, [700], [200], 9),
-    (3, 1, 64, 16, [300, 5, 90], [100, 5, 33], 4),
-    (5, 1, 128, 64, [2000, 100], [64, 30], 6),
     (33, 1, 64, 32, [200], [20], 3),
     (100, 1, 128, 16, [150], [9], 5),
-    (64, 8, 128, 64, [1500], [130], 10),
-    (8, 1, 64, 4096, [9000], [16], 3),
-    (16, 2, 128, 16, [40] * 10, [20] * 10, 3),
     (8, 1, 128, 16, [3500], [16], 100),
-    (4, 4, 64, 32, [3000, 2, 700], [90, 2, 1], 60),
-    # two tiles of them to a CTA, the second full, in part there or not at all
-    (128, 16, 128, 16, [900, 300], [180, 77], 9),
-    (128, 16, 64, 64, [1500, 40, 8], [230, 17, 8], 12),
-    (64, 16, 128, 32, [500, 70], [400, 66], 5),
-    (320, 8, 128, 16, [130], [97], 4),
-    (16, 16, 64, 16, [460], [460], 6),
-    (144, 16, 64, 128, [1000], [203], 2),
+    # enough of them to be taken together: tiles of one to 32 tokens, all ratios of heads, one CTA or a cluster
+    (8, 8, 128, 16, [700], [200], 41),
+    (6, 2, 64, 64, [900, 5, 300], [400, 5, 200], 27),
+    (20, 4, 128, 32, [2000, 100], [180, 60], 36),
+    (132, 4, 64, 32, [400], [150], 13),
+    (100, 1, 128, 16, [600], [150], 38),
+    (64, 8, 128, 64, [1500], [130], 16),
+    (8, 1, 64, 4096, [9000], [100], 3),
+    (16, 2, 128, 16, [400] * 10, [200] * 10, 17),
+    (8, 1, 128, 1024, [33000], [32], 32),
+    (4, 4, 64, 32, [3000, 2, 700], [150, 2, 1], 60),
+    (128, 1, 128, 64, [1300], [60], 21),
+    (16, 16, 64, 16, [460], [460], 9),
 ]
 
 
@@ -501,7 +523,7 @@ def test_attention_over_listed_pages_matches_fp64(shape) -> None:
     assert _status() in (0, 2)
 
 
-@pytest.mark.parametrize("n", [1, 5, 8, 90])
+@pytest.mark.parametrize("n", [1, 5, 90, 300])
 def test_every_page_listed_is_the_dense_attention(n) -> None:
     lens, page = [1000, 300], 32
     pool = Pool(lens, 2, 128, page, DEV)
@@ -515,7 +537,7 @@ def test_every_page_listed_is_the_dense_attention(n) -> None:
     _no_status()
 
 
-@pytest.mark.parametrize("heads", [3, 17])  # the kernel of single tokens, that of tiles
+@pytest.mark.parametrize("heads", [3, 17])
 def test_rows_without_a_key_and_rows_left_alone(heads) -> None:
     from faquant_b200 import _lib
 
@@ -548,18 +570,50 @@ def test_rows_without_a_key_and_rows_left_alone(heads) -> None:
     assert _status() == _lib.FAQ_STATUS_BAD_PAGE and bool(((out.double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
 
 
-@pytest.mark.parametrize("n", [6, 20])
-def test_peaked_scores_ranges_and_not_a_number(n) -> None:
-    lens, new, page = [900], [n], 16
+def test_tiles_of_rows_without_a_key_and_rows_left_alone() -> None:
+    from faquant_b200 import _lib, ops
+
+    lens, new, count = [100, 900], [300, 400], 50
+    pool = Pool(lens, 2, 64, 16, DEV)
+    k, v = _randn(1000, 2, 64, seed=65), _randn(1000, 2, 64, seed=66)
+    pool.write(k, v)
+    q = _randn(720, 8, 64, seed=67)
+    lists = torch.full((720, 2, count), -1, dtype=torch.int32)
+    lists[:700] = _lists(lens, new, 2, 16, count, 68)
+    lists[300:310] = -1  # tokens without a list
+    args = (pool.pages, pool.table)
+    kw = dict(page_size=16)
+    out = torch.full_like(q, 7.0)
+    ops.hif4_sparse_attention(q, *args, pool.cu(new), pool.lens, lists.to(DEV), out=out, **kw)
+    want, size = ref.attention(q[:700], quantized(k), quantized(v), lens, new, 16, lists)
+    assert not out[:200].any() and not out[300:310].any() and bool((out[700:] == 7.0).all())
+    assert bool(((out[:700].double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
+    _status()
+    for bounds in ((0, 300, 721), (0, 300, 299)):
+        out = torch.full_like(q, 7.0)
+        ops.hif4_sparse_attention(q, *args, _int32(*bounds), pool.lens, lists.to(DEV), out=out, **kw)
+        assert _status() == _lib.FAQ_STATUS_BAD_BOUND and bool((out[300:] == 7.0).all())
+        assert bool(((out[:300].double().cpu() - want[:300]).abs() <= BOUND * size[:300] + 2.0**-126).all())
+    pool.table[1, 2], pool.table[1, 40] = -1, 10**6
+    out = ops.hif4_sparse_attention(q, *args, pool.cu(new), pool.lens, lists.to(DEV), **kw)
+    want, size = ref.attention(q[:700], quantized(k), quantized(v), lens, new, 16, lists, missing={(1, 2), (1, 40)})
+    assert _status() == _lib.FAQ_STATUS_BAD_PAGE
+    assert bool(((out[:700].double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
+
+
+@pytest.mark.parametrize("n, length", [(6, 900), (530, 2000)])
+def test_peaked_scores_ranges_and_not_a_number(n, length) -> None:
+    lens, new, page = [length], [n], 16
     pool = Pool(lens, 1, 128, page, DEV)
-    k, v = _randn(900, 1, 128, seed=59), _randn(900, 1, 128, seed=60)
+    k, v = _randn(length, 1, 128, seed=59), _randn(length, 1, 128, seed=60)
     k[700] *= 30.0  # one key far above the others, found late
     v[3] *= 1e6     # and a value row of another magnitude
     v[600:] *= 1e-20
     pool.write(k, v)
     q = _randn(n, 4, 128, seed=61)
     q[1] = 0
-    lists = torch.arange(57, dtype=torch.int32).expand(n, 1, 57)
+    pages = -(-length // page)
+    lists = torch.arange(pages, dtype=torch.int32).expand(n, 1, pages)
     for scale in (None, 0.002, 0.5):
         out = _attend(pool, q, new, lists, scale=scale)
         want, size = ref.attention(q, quantized(k), quantized(v), lens, new, page, lists, scale)
