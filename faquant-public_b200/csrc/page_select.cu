@@ -16,6 +16,12 @@
 // [negative | positive entries of q], whose lanes load 16 bytes of a page's row each.
 // Selection. The first pages and the token's last ones, then the greatest scores, ties to the
 // lowest column: a search for the count-th greatest key, then one pass in order.
+//
+// Measured (one B200): bounds of a step's pages 2.6 to 3.8 us. Selection for one token of 8 kv heads among 512 pages 7.6 us
+// and for 32 sequences of 1 .. 1000 pages 13.7, both chains of loads that wait for one another (cu, lens, table,
+// bounds), then the search; for 512 tokens of 64 query heads on 8 kv heads among 512 pages 62 us: some 7300
+// instructions per token and kv head at 14 warps an SM (the scores take 37 us, the search 16). With dp4a in
+// place of the 8-bit products they took 17.6, 32 and 227.
 #include "kv_pages.cuh"
 
 namespace faq {
@@ -690,12 +696,15 @@ extern "C" int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads
   w.vec = aligned16(q) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   const int64_t units = total * kv_heads;
   static std::atomic<uint64_t> set[4];  // devices on which the kernels' shared memory is set
-  // Many rows, and room for the keys of a CTA's warps: a warp each, whose heads of several tokens share a
-  // product.
+  // Many rows, and room for the keys of a CTA's warps: a warp for the heads of 16 >> slots tokens, the more of them the later
+  // (they are searched one after the other). A CTA each and a warp each, us, 32 of 512 pages where not said otherwise:
+  //   512 tokens, 64 / 8 heads (4096 rows)  141   62;   128 tokens (1024)    41   47
+  //   256 tokens, 32 / 8 heads (2048)        42   31;   128 tokens (1024)    23   29  (of 128 pages)
+  //   800 tokens, 8 / 8 heads (6400)        100   62;   256 tokens (2048)    41   74  (of 125, 128)
   int slots = 0;
   while (slots < 3 && (1 << slots) < w.group) ++slots;
   const int64_t tokens = SELECT_WARPS * PRODUCTS * 8 >> slots, keys = tokens * table_cols;  // of a CTA
-  if (units << slots >= 8 * SELECT_WARPS * static_cast<int64_t>(num_sms()) && 4 * keys <= SELECT_KEY_BYTES) {
+  if (units >= (8 + (16 >> slots)) * static_cast<int64_t>(num_sms()) && 4 * keys <= SELECT_KEY_BYTES) {
     w.slots = slots;
     w.key_ld = static_cast<int>(table_cols);
     auto kern = d == 64 ? select_pages_warp_kernel<1> : select_pages_warp_kernel<2>;

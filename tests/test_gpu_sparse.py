@@ -301,12 +301,12 @@ SELECTIONS = [  # heads, kv_heads, d, page, lens, new, count, first, last
     (128, 1, 128, 32, [1500], [2], 20, 1, 2),
     (2, 2, 128, 16, [20000], [2], 700, 2, 2),
     # many rows, one to eight tokens of a warp, at sequences' ends and starts
-    (8, 1, 128, 16, [700, 30, 500, 3], [690, 3, 500, 3], 9, 1, 2),
-    (40, 4, 64, 32, [330, 100], [300, 50], 4, 1, 1),
+    (16, 2, 128, 16, [700, 30, 500, 3], [690, 3, 500, 3], 9, 1, 2),
+    (50, 5, 64, 32, [330, 100], [300, 50], 4, 1, 1),
     (24, 8, 64, 16, [200, 150, 7], [150, 150, 7], 5, 2, 1),
     (16, 8, 64, 16, [9, 9, 9, 600, 20], [9, 1, 1, 570, 20], 6, 0, 1),
     (8, 8, 128, 16, [8, 1, 2, 1190, 5], [8, 1, 2, 1170, 5], 3, 1, 2),
-    (32, 4, 64, 16, [17000], [300], 80, 1, 2),
+    (40, 5, 64, 16, [17000], [300], 80, 1, 2),
 ]
 
 
