@@ -80,10 +80,11 @@ struct Angles {
   }
 };
 
-// x / w in fp64 to 2^-46: a Newton's step from the fp32 reciprocal (the result is rounded to 2^-24).
-__device__ __forceinline__ double quotient(double x, float w) {
-  const double r = __frcp_rn(w), y = x * r;
-  return fma(fma(-static_cast<double>(w), y, x), r, y);
+// 1 / w in fp64 to 2^-47, w a normal number: a Newton's step from the fp32 reciprocal (a key is rounded to 2^-24).
+// The step is on the reciprocal, not on a quotient, so that an infinite key stays infinite.
+__device__ __forceinline__ double reciprocal(float w) {
+  const double r = __frcp_rn(w);
+  return fma(fma(-static_cast<double>(w), r, 1.0), r, r);
 }
 
 // A key: norm, rotation, offset, smoothing and transform of the lane's part of a row in fp64; all
@@ -102,7 +103,7 @@ __device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t,
       for (int i = 0; i < 8; ++i) {
         const double y = v[g][i];
         sum = fma(y, y, sum);
-        x[g][i] = bf16 ? static_cast<double>(v[g][i] * w[i]) : y * w[i];  // exact in fp32 for two bf16
+        x[g][i] = bf16 ? static_cast<double>(v[g][i] * w[i]) : y * w[i];  // exact in fp32 for two bf16 within its range
       }
     }
 #pragma unroll
@@ -144,7 +145,7 @@ __device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t,
       float w[8];
       load8(t.smooth, true, head * t.smooth_head_stride + 64 * g + 8 * s, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[g][i] = quotient(x[g][i], w[i]);
+      for (int i = 0; i < 8; ++i) x[g][i] *= reciprocal(w[i]);
     }
   }
   if (t.rotate) {

@@ -222,6 +222,56 @@ def test_append_not_a_number_stays_in_its_row() -> None:
     assert torch.equal(a[torch.arange(20) != 7], b[torch.arange(20) != 7]) and torch.equal(a[7, 0], b[7, 0])
 
 
+def test_append_infinite_keys_scale_their_group() -> None:
+    """Where no step mixes the channels, an infinite key divided by its smoothing is infinite, as it would
+    be written without the step; its group of 64 channels takes the greatest scale, the others keep their bits."""
+    from faquant_b200 import ops
+
+    pools = [Pool([3], 2, 128, 16, DEV, fill=0) for _ in range(2)]
+    q, k, v = (_randn(3, x, 128, seed=19 + i, dtype=torch.float32) for i, x in enumerate((2, 2, 2)))
+    k[0, 0, 3], k[1, 1, 70], k[2, 0, 127] = math.inf, -math.inf, math.inf
+    smooth = torch.full((128,), 2.0, device=DEV)  # the division is exact
+    ops.hif4_kv_append(q, k, v, pools[0].pages, pools[0].table, pools[0].cu([3]), _int32(3), page_size=16, smooth_scale=smooth)
+    ops.hif4_kv_write(k / 2, v, pools[1].pages, pools[1].table, pools[1].cu([3]), _int32(3), page_size=16)
+    assert torch.equal(pools[0].store, pools[1].store)
+    _no_status()
+
+
+def test_steps_without_a_token_and_two_streams_at_once() -> None:
+    from faquant_b200 import ops
+
+    pools = [Pool([1500], 2, 128, 16, DEV, fill=0) for _ in range(2)]
+    k, v, q = (_randn(1500, x, 128, seed=23 + i) for i, x in enumerate((2, 2, 8)))
+    bounds = [_bounds(p) for p in pools]
+
+    def step(pool, bounds, lens, new):
+        args = (pool.table, pool.cu([new]), _int32(lens))
+        part = slice(lens - new, lens)
+        x = ops.hif4_kv_append(q[part], k[part], v[part], pool.pages, *args, page_size=16, rotate=True)
+        ops.hif4_key_bounds(pool.pages, bounds, *args, page_size=16, total=new)
+        lists = ops.hif4_select_pages(x, bounds, *args, page_size=16, count=9)
+        return x, lists, ops.hif4_sparse_attention(x, pool.pages, *args, lists, page_size=16)
+
+    before = [p.store.clone() for p in pools]
+    x, lists, out = step(pools[0], bounds[0], 0, 0)
+    assert x.shape == out.shape == (0, 8, 128) and lists.shape == (0, 2, 9) and torch.equal(pools[0].store, before[0])
+    cuts = [(1200, 1200), (1203, 3), (1500, 297)]
+    want = [step(pools[0], bounds[0], *c) for c in cuts]
+    torch.cuda.synchronize()
+    # the same on another stream, while this one repeats its last step
+    other = torch.cuda.Stream(DEV)
+    got = []
+    for c in cuts:
+        with torch.cuda.stream(other):
+            got.append(step(pools[1], bounds[1], *c))
+        again = step(pools[0], bounds[0], *cuts[-1])
+        assert all(torch.equal(a, b) for a, b in zip(again, want[-1]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    assert torch.equal(pools[0].store, pools[1].store) and torch.equal(bounds[0], bounds[1])
+    _no_status()
+
+
 # ------------------------------------------------------------------ bounds
 def _refresh(pool, bounds, new=None, lens=None):
     from faquant_b200 import ops
@@ -521,6 +571,22 @@ def test_attention_over_listed_pages_matches_fp64(shape) -> None:
     assert torch.equal(_attend(pool, wide[..., :d], new, lists, out=into), out)
     # columns beyond the table set the status, others do not
     assert _status() in (0, 2)
+
+
+@pytest.mark.parametrize("heads", [4, 9])
+def test_long_lists_in_any_order(heads) -> None:
+    """Entries that repeat an earlier one far before them are dropped: the list once through, in its order."""
+    pool = Pool([9000], 1, 128, 16, DEV, fill=0xFF)
+    k, v = _randn(9000, 1, 128, seed=61), _randn(9000, 1, 128, seed=62, scale=0.5)
+    pool.write(k, v)
+    q = _randn(1, heads, 128, seed=63, scale=2.0)
+    g = torch.Generator().manual_seed(64)
+    once = torch.randperm(563, generator=g)[:400]
+    lists = torch.cat((once, once[torch.randint(400, (900,), generator=g)]))[torch.randperm(1300, generator=g)].to(torch.int32)
+    want, size = ref.attention(q, quantized(k), quantized(v), [9000], [1], 16, lists.reshape(1, 1, -1))
+    out = _attend(pool, q, [1], lists.reshape(1, 1, -1))
+    assert bool(((out.double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
+    _no_status()
 
 
 @pytest.mark.parametrize("n", [1, 5, 90, 300])
