@@ -10,7 +10,8 @@
 // entry, table entry, address), drops those that are not there or lie behind the token, and streams the rest
 // through a ring of bulk copies.
 //
-// A column counts once: where a list is not ascending, entries that an earlier one repeats are dropped.
+// A column counts once: where a list is not ascending, entries that an earlier one repeats are dropped, by a look at
+// all the earlier ones (hence a list's most entries).
 //
 // Work split: a unit's blocks are dealt out to the warps of a cluster of 1, 2, 4 or 8 CTAs, as many as fill the
 // SMs once; the CTAs' results meet through distributed shared memory, so there is no second
@@ -37,6 +38,7 @@ using pat::transpose8x8;
 constexpr int W = 8;   // warps of a CTA, two CTAs per SM: 128 registers a thread
 constexpr int THREADS = 32 * W;
 constexpr int S = 4;   // blocks in flight per warp
+constexpr int MAX_COUNT = 32768;  // entries of a list, as many as the selection has columns
 
 // shared memory: the warps' rings, then in their place the warps' O (rows padded) | the CTA's O | (m, l) of
 // warps and CTA | the ring slots' first keys | mbarriers
@@ -436,7 +438,8 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   FAQ_CHECK_ARG(heads > 0 && heads < (int64_t(1) << 24) && heads % kv_heads == 0,
                 "query heads must be divisible by key/value heads");
   FAQ_CHECK_ARG(total * heads < (int64_t(1) << 31), "too many tokens for one call");
-  FAQ_CHECK_ARG(count > 0 && count < (int64_t(1) << 24), "bad page count");
+  FAQ_CHECK_ARG(count > 0, "bad page count");
+  if (count > MAX_COUNT) return fail(FAQ_ERR_UNSUPPORTED, "more than 32768 listed pages");
   FAQ_CHECK_ARG(scale > 0.0f && scale < 1e30f, "scale must be positive");
   if (total == 0) return FAQ_OK;
   FAQ_CHECK_ARG(q && out && selected, "null pointer");

@@ -925,7 +925,7 @@ def hif4_kv_append(
     """From the projections' ``q [T, H, D]`` and ``k``/``v [T, Hkv, D]`` (bf16 or fp32, D 64 or 128, any token
     and head strides) to the cache and the attention's queries in one pass
     (``faq_hif4_kv_append``): per-head RMSNorm (``q_norm``/``k_norm [D]``), the rotation of each token's
-    position, Smooth-QK (``q * smooth_scale``, ``(k - key_offset) / smooth_scale``; ``[D]`` or ``[Hkv, D]``, ``key_offset
+    position, Smooth-QK (``q * smooth_scale``, ``(k - key_offset) / smooth_scale``, normal numbers; ``[D]`` or ``[Hkv, D]``, ``key_offset
     [Hkv, D]``), the Hadamard transform over D (``rotate``), each where given. K and V are quantized and written to
     their ``pages`` as :func:`hif4_kv_write` does (``table``, ``cu``, ``lens``, ``levels`` as there); the queries
     are returned in bf16 ``[T, H, D]`` (in ``out`` where given; it may be ``q`` itself).
@@ -1117,7 +1117,7 @@ def hif4_sparse_attention(
     ``[T, H, D]`` bf16 (``faq_hif4_sparse_attention``). ``selected`` int32 ``[T, Hkv, count]``
     (:func:`hif4_select_pages`) holds columns of the sequence's row of ``table``, in any order; entries below zero and
     pages behind the token are passed over, a column listed twice counts once, and no token sees keys behind
-    itself. With every visible page listed this is :func:`hif4_paged_attention`, up to the rounding of its sums.
+    itself (at most 32768 entries; lists that ascend are read fastest). With every visible page listed this is :func:`hif4_paged_attention`, up to the rounding of its sums.
     A row without a key is zero; rows beyond ``cu[B]`` stay as they are; pages that the table does not hold are
     left out and set ``FAQ_STATUS_BAD_PAGE``."""
     device = _require_cuda(q, pages, table, cu, lens, selected, out)

@@ -47,7 +47,8 @@ extern "C" {
 /* device status word bits */
 #define FAQ_STATUS_TIMEOUT 1u
 #define FAQ_STATUS_BAD_PAGE 2u  /* a page table entry or a length outside the pool or the table */
-#define FAQ_STATUS_BAD_BOUND 4u /* a ragged batch beyond the bounds the host gave (total, max_new, max_len, total_len) */
+#define FAQ_STATUS_BAD_BOUND 4u /* a ragged batch beyond the bounds the host gave (total, max_new, max_len,
+                                   total_len), or a position beyond the rows of a table (K11) */
 
 /* element types */
 #define FAQ_BF16 0
@@ -495,7 +496,7 @@ int faq_verify_drafts(const int64_t* draft_tokens, const void* target_probs, con
  * strides in elements, d contiguous); q_norm, k_norm [d] (norm_dtype; null: no norm); cos, sin
  * [rope_rows, >= d / 2] with row stride rope_ld (rope_dtype; null: no rotation), row p of
  * position p; key_offset fp32 [kv_heads, d] or null; smooth fp32 [d] (smooth_head_stride 0) or
- * [kv_heads, d] (smooth_head_stride d) or null: q heads times it, keys divided by it; rotate:
+ * [kv_heads, d] (smooth_head_stride d) or null, normal numbers: q heads times it, keys divided by it; rotate:
  * the Hadamard transform. out bf16 [total, heads, d]; it may be q. q is computed in fp32 and rounded
  * once; K in fp64 and rounded to fp32, which faq_hif4_kv_write's fit takes: a key's bits are those of
  * the formula, whatever the batch. The batch, the pages and their errors are as in
@@ -545,7 +546,8 @@ int faq_hif4_select_pages(const void* q, int64_t total, int64_t heads, int64_t q
  * of the token's sequence's row of the table, one list per kv head, in any order. Entries below zero and
  * pages behind the token are passed over, a column listed twice counts once, keys behind the token are not
  * seen; an entry whose page is missing is left out and sets FAQ_STATUS_BAD_PAGE. q, out and scale as in
- * faq_hif4_paged_attention (which a list of every page equals, up to the rounding of the sums). A row without a key is
+ * faq_hif4_paged_attention (which a list of every page equals, up to the rounding of the sums). At most 32768 entries
+ * (FAQ_ERR_UNSUPPORTED); lists that do not ascend are read more slowly. A row without a key is
  * zero; rows beyond cu[batch] are not written. No workspace. A row's bits depend on its own queries,
  * keys and list, scale, and through the choice of the kernel and the split of the work on the call's sizes; where
  * tokens are taken together, on cu and the lists of its neighbours.

@@ -58,6 +58,7 @@ def test_c_entry_points_refuse_bad_arguments() -> None:
 
     assert attend(q=None) == 1 and attend(out=None) == 1 and attend(lists=None) == 1
     assert attend(heads=3) == 1 and attend(count=0) == 1 and attend(qs=12) == 1 and "strides" in _lib.last_error()
+    assert attend(count=32769) == 3 and "32768" in _lib.last_error()
     assert attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1 and attend(scale=float("inf")) == 1
     assert attend(q=ctypes.c_void_p(264)) == 1 and "aligned" in _lib.last_error()
     assert attend(total=0) == 0
