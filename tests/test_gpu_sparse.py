@@ -450,6 +450,32 @@ def test_ties_missing_pages_and_what_is_not_finite() -> None:
     assert bool((ops.hif4_select_pages(q, *args, **kw) == -1).all()) and _status() == _lib.FAQ_STATUS_BAD_PAGE
 
 
+@pytest.mark.parametrize("behind", [0, 3])
+@pytest.mark.parametrize("heads, h, d", [(24, 12, 64), (99, 9, 128), (12, 12, 128)])
+def test_many_rows_missing_pages_and_what_is_not_finite(heads, h, d, behind) -> None:
+    """Tokens of one sequence taken together and others, pages that are not there, tokens below position zero."""
+    from faquant_b200 import _lib, ops
+
+    lens, new, count = [900, 50, 333], [200, 80, 70], 6
+    pool = Pool(lens, h, d, 16, DEV)
+    k = _randn(sum(lens), h, d, seed=44)
+    pool.write(k, k)
+    bounds = _bounds(pool)
+    _refresh(pool, bounds)
+    q = _randn(sum(new) + behind, heads, d, seed=45, scale=2.0)
+    q[5, 0, 3], q[6, 1, 4], q[270, heads - 1, 0], q[340] = math.nan, math.inf, -math.inf, 0.0
+    missing = [(0, 0), (0, 17), (0, 55), (1, 1), (2, 20)]
+    for b, c in missing:
+        pool.table[b, c] = -1 if c else 10**6
+    out = torch.full((sum(new) + behind, h, count), -7, dtype=torch.int32, device=DEV)
+    _, scores = ops.hif4_select_pages(q, bounds, pool.table, pool.cu(new), pool.lens, page_size=16, count=count, want_scores=True,
+                                      out=out)
+    n = sum(new)
+    want, want_scores = ref.select(q[:n], k, lens, new, 16, count, 1, 2, set(missing))
+    assert torch.equal(out[:n].cpu(), want) and torch.equal(scores[:n].double().cpu(), want_scores) and bool((out[n:] == -7).all())
+    assert _status() == _lib.FAQ_STATUS_BAD_PAGE
+
+
 def test_selection_of_tokens_without_a_place_and_bad_batches() -> None:
     from faquant_b200 import _lib, ops
 
