@@ -21,7 +21,8 @@
 // of 32768 in 8.0 us, 64 pages of 16 of 32 sequences of 1 .. 16000 tokens in 16.6 us. The first is a chain of
 // loads (cu and lens, the list, the table, the pages), two blocks per warp and the two joins; the second
 // some 10700 blocks at 190 cycles of an SM each (see paged_attention.cu: 118 of issue), as 256 CTAs
-// of unequal length in one wave; clusters of two there took 20.3 us, of four 31.2.
+// of unequal length in one wave; clusters of two there took 20.3 us, of four 31.2. 128 such sequences of 2000 tokens
+// take 54 us, with four warps to a unit.
 #include "kv_pages.cuh"
 
 namespace faq {
@@ -35,14 +36,13 @@ using pat::pack_bf16;
 using pat::RAISE;
 using pat::transpose8x8;
 
-constexpr int W = 8;   // warps of a CTA, two CTAs per SM: 128 registers a thread
-constexpr int THREADS = 32 * W;
+constexpr int SM_WARPS = 16;  // in CTAs of 4 or 8: 128 registers a thread
 constexpr int S = 4;   // blocks in flight per warp
 constexpr int MAX_COUNT = 32768;  // entries of a list, as many as the selection has columns
 
 // shared memory: the warps' rings, then in their place the warps' O (rows padded) | the CTA's O | (m, l) of
 // warps and CTA | the ring slots' first keys | mbarriers
-template <int NG>
+template <int NG, int W>
 struct Smem {
   static constexpr int old = 64 * NG + 8;  // floats of an O row
   static constexpr int stage = 2 * block_bytes(NG);
@@ -56,10 +56,10 @@ struct Smem {
   static constexpr int bytes = bar + W * S * 8;
 };
 
-template <int NG>
-__global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, int split) {
-  using L = Smem<NG>;
-  constexpr int D = 64 * NG, OLD = L::old, UNIT = block_bytes(NG), STAGE = L::stage;
+template <int NG, int W>
+__global__ void __launch_bounds__(32 * W, SM_WARPS / W) sparse_attention_kernel(Params P, int split) {
+  using L = Smem<NG, W>;
+  constexpr int THREADS = 32 * W, D = 64 * NG, OLD = L::old, UNIT = block_bytes(NG), STAGE = L::stage;
   extern __shared__ __align__(128) unsigned char smem[];
   float* s_o = reinterpret_cast<float*>(smem);            // [W][RB][OLD], over the rings
   float* s_part = reinterpret_cast<float*>(smem + L::o);  // [RB][D]
@@ -408,14 +408,14 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_attention_kernel(Params P, 
   cluster_sync();  // the others have read this CTA's part
 }
 
-template <int NG>
+template <int NG, int W>
 static int launch(const Params& P, int split, void* stream) {
-  constexpr int bytes = Smem<NG>::bytes;
-  auto kern = sparse_attention_kernel<NG>;
+  constexpr int bytes = Smem<NG, W>::bytes;
+  auto kern = sparse_attention_kernel<NG, W>;
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory is set
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), bytes, set);
   if (rc) return rc;
-  FAQ_CUDA(launch_clusters(kern, P.total * P.p.kv_heads * P.passes * split, THREADS, bytes, split, stream, P, split));
+  FAQ_CUDA(launch_clusters(kern, P.total * P.p.kv_heads * P.passes * split, 32 * W, bytes, split, stream, P, split));
   return launch_status("sparse_attention_kernel");
 }
 
@@ -463,19 +463,27 @@ extern "C" int faq_hif4_sparse_attention(const void* q, int64_t total, int64_t h
   // eight tokens, or blocks of eight query heads of them, on average, and the kernel of single tokens would
   // expand 440 blocks or more per SM, some 50 us. Both kernels, us, where neighbours' lists differ in about a third
   // of the pages (the tiles' also where they are the same, and have nothing in common), 32 pages of 64, heads of 128:
-  //   16 sequences, 4 tokens, 32 / 8 heads (443 blocks per SM)  55   59 (48, 104)
-  //   the same, 8 tokens (886)                                  94   66 (52, 134)
-  //   1 sequence, 8 tokens, 64 / 8 heads (55)                   14   26 (23, 41)
-  //   4 sequences, 8 tokens, 8 / 8 heads (221)                  29   40 (32, 70)
-  //   the same, 32 tokens (886)                                 92   45 (36, 77)
-  //   1 sequence, 512 tokens, 64 / 8 heads (3542)              359  169 (110, 598)
+  //   16 sequences, 4 tokens, 32 / 8 heads (443 blocks per SM)  52   59 (48, 104)
+  //   the same, 8 tokens (886)                                  88   65 (52, 134)
+  //   1 sequence, 8 tokens, 64 / 8 heads (55)                   13   26 (23, 41)
+  //   4 sequences, 8 tokens, 8 / 8 heads (221)                  28   40 (32, 70)
+  //   the same, 32 tokens (886)                                 87   46 (36, 77)
+  //   1 sequence, 512 tokens, 64 / 8 heads (3542)              329  164 (110, 598)
   const int tokens = P.group <= pre::TILE ? spt::tile_tokens(P.group) : 0;
   if (tokens && total * P.passes >= 8 * batch && units * blocks >= 440 * static_cast<int64_t>(num_sms()) &&
       std::min(tokens * count, table_cols) <= spt::MAX_UNION && table_cols <= spt::columns(d) && q_token_stride >= 8 &&
       q_head_stride >= 8)
     return d == 64 ? spt::launch<1>(P, heads, stream) : spt::launch<2>(P, heads, stream);
-  int split = 1;
-  while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > W * split) split *= 2;
+  // Units that fill the SMs more than once take four warps each: the waits at a unit's beginning and end are then those of
+  // half as many waves. Eight and four warps, us, 64 pages of 16, one token, 32 / 8 heads of 128:
+  //   32 sequences (256 units)  17.1  18.5;   40 (320)  25.8  28.3;   64 (512)  33.2  29.7;   128 (1024)  60.7  53.3
+  //   128 sequences, heads of 64 42.1  34.8;   64, 8 pages of 64  20.5  16.8
+  int split = 1, warps = 8;
+  if (units > 3 * static_cast<int64_t>(num_sms()))
+    warps = 4;
+  else
+    while (split < 8 && units * split * 2 <= 2 * num_sms() && blocks > warps * split) split *= 2;
   FAQ_CHECK_ARG(units * split < (int64_t(1) << 31), "too many tokens for one call");
-  return d == 64 ? launch<1>(P, split, stream) : launch<2>(P, split, stream);
+  if (warps == 4) return d == 64 ? launch<1, 4>(P, split, stream) : launch<2, 4>(P, split, stream);
+  return d == 64 ? launch<1, 8>(P, split, stream) : launch<2, 8>(P, split, stream);
 }

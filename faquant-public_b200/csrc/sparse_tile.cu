@@ -12,7 +12,7 @@
 // and add up their rows through distributed shared memory.
 //
 // Measured (one B200): 512 tokens of 32768 with 64 query heads on 8 kv heads of 128 and 32 pages of 64
-// tokens each, 164 us (359 with the kernel of single tokens): 9000 key tiles (the lists of 16 neighbours
+// tokens each, 164 us (329 with the kernel of single tokens): 9000 key tiles (the lists of 16 neighbours
 // hold some 75 pages) at 4300 cycles, two waves of CTAs. The expansion is what the others wait for: a warp
 // takes 1100 cycles for its block of K and 1300 for one of V, at one instruction in five cycles, then come waits
 // for its slots. Dropped: eight softmax warps with 64 keys a thread (186 us; read twice from

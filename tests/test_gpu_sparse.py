@@ -563,6 +563,10 @@ SHAPES = [  # heads, kv_heads, d, page, lens, new, count
     (33, 1, 64, 32, [200], [20], 3),
     (100, 1, 128, 16, [150], [9], 5),
     (8, 1, 128, 16, [3500], [16], 100),
+    # more units than the SMs hold at once
+    (16, 8, 64, 16, [50 + 37 * i for i in range(60)], [1] * 60, 12),
+    (20, 4, 128, 32, [90 + 31 * i for i in range(40)], [3] * 40, 5),
+    (16, 16, 128, 64, [4 + 19 * i for i in range(33)], [0, 1, 2] * 11, 4),
     # enough of them to be taken together: tiles of one to 32 tokens, all ratios of heads, one CTA or a cluster
     (8, 8, 128, 16, [700], [200], 41),
     (6, 2, 64, 64, [900, 5, 300], [400, 5, 200], 27),
