@@ -994,7 +994,8 @@ def hif4_kv_append(
         key_offset = key_offset.to(torch.float32).contiguous()
         offset_ptr = key_offset.data_ptr()
     if out is None:
-        out = q.new_empty(qs, dtype=torch.bfloat16)
+        # of a contiguous tensor the like is made sooner
+        out = torch.empty_like(q) if dtype is torch.bfloat16 and q.is_contiguous() else q.new_empty(qs, dtype=torch.bfloat16)
         out_st = (heads * d, d)
     else:
         if out.shape != qs or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
@@ -1139,7 +1140,7 @@ def hif4_sparse_attention(
         q = q.contiguous() if not q.is_contiguous() else q.clone()
         st = (heads * d, d)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         out_st = (heads * d, d)
     else:
         if out.shape != shape or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
