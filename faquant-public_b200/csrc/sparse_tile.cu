@@ -319,7 +319,6 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Pages& p = P.p;
   grid_dependency_wait();
-  allow_dependent_launch();
 
   // ---- the unit
   const int T = tile_tokens(P.group);
@@ -364,6 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_tile_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  allow_dependent_launch();  // not before: a CTA of the next kernel that took this SM's columns would wait for this one's end
   for (int i = tid; i < tokens * P.count; i += THREADS) {
     const int tok = i / P.count;
     const int col = P.list[((c0 + tok0 + tok) * p.kv_heads + head) * P.count + (i - tok * P.count)];
