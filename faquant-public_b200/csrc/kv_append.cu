@@ -90,7 +90,7 @@ __device__ __forceinline__ double reciprocal(float w) {
 // A key: norm, rotation, offset, smoothing and transform of the lane's part of a row in fp64; all
 // lanes take part.
 template <int NG>
-__device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t, const Angles& a, bool bf16, int head, int s) {
+__device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t, const Angles& a, int head, int s) {
   constexpr int D = 64 * NG;
   double x[NG][8], factor = 1.0;  // the norm's, which waits for the transform's: the steps between are linear
   if (t.k_norm != nullptr) {
@@ -103,7 +103,7 @@ __device__ __forceinline__ void turn_key(float (&v)[NG][8], const TurnParams& t,
       for (int i = 0; i < 8; ++i) {
         const double y = v[g][i];
         sum = fma(y, y, sum);
-        x[g][i] = bf16 ? static_cast<double>(v[g][i] * w[i]) : y * w[i];  // exact in fp32 for two bf16 within its range
+        x[g][i] = y * w[i];  // in fp64 for bf16 too: the product of two may leave fp32's range, and the norm bring it back
       }
     }
 #pragma unroll
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) kv_append_kernel(AppendParam
                                 return;
                               Angles ang;
                               if (t.cos != nullptr) ang.load(t, x.pos + min(max(r, x.from), x.to - 1), s, NG);
-                              turn_key<NG>(v, t, ang, sizeof(T) == 2 && !t.norm_f32, head, s);
+                              turn_key<NG>(v, t, ang, head, s);
                             });
     return;
   }
