@@ -8,7 +8,7 @@ import torch
 
 import sparse_reference as ref
 from paged_reference import Pool, quantized
-from test_gpu_sparse import DEV, _int32, _no_status, _pos, _randn, _tables
+from test_gpu_sparse import DEV, _int32, _no_status, _pos, _randn, _status, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -97,13 +97,110 @@ def test_repeated_columns_of_a_context_of_many(heads, h, d, tokens) -> None:
     for row in lists.view(-1, 700):
         row[:500] = once[torch.randint(len(once), (500,), generator=g)].to(torch.int32)
         row[:] = row[torch.randperm(700, generator=g)]
-    out = ops.hif4_sparse_attention(q, pool.pages, table, cu, lens, lists.to(DEV), page_size=page).double().cpu()
-    group = heads // h
-    for t in range(tokens):
-        for j in range(h):
+    out = ops.hif4_sparse_attention(q, pool.pages, table, cu, lens, lists.to(DEV), page_size=page)
+    _check(out, q, k, v, at, lists)
+    _no_status()
+
+
+def _check(out, q, k, v, at, lists):
+    """Of whole pages, all visible: ``k``, ``v`` fp64 ``[pages, page, H, D]``, ``at`` the page of each column."""
+    out, q, (h, d) = out.double().cpu(), q.double().cpu(), k.shape[2:]
+    for t in range(q.shape[0]):
+        for j, heads in enumerate(torch.arange(q.shape[1]).chunk(h)):
             mine = at[torch.tensor(sorted(set(lists[t, j].tolist()) - {-1}))]
             keys, values = (x[mine, :, j].reshape(-1, d) for x in (k, v))
-            p = torch.softmax(q[t, j * group : (j + 1) * group].double().cpu() @ keys.T * d**-0.5, -1)
-            error = (out[t, j * group : (j + 1) * group] - p @ values).abs()
-            assert bool((error <= BOUND * (p @ values.abs()) + 2.0**-126).all())
+            p = torch.softmax(q[t, heads] @ keys.T * d**-0.5, -1)
+            assert bool(((out[t, heads] - p @ values).abs() <= BOUND * (p @ values.abs()) + 2.0**-126).all())
+
+
+# ------------------------------------------------------------------ both kernels at their ends
+def _tokens_of_tiles(h, blocks):
+    """New tokens of a call that the kernel of tiles takes for certain: half as many again as its rule asks for."""
+    sms = torch.cuda.get_device_properties(DEV).multi_processor_count
+    return -(-3 * 440 * sms // (2 * h * blocks))
+
+
+@pytest.mark.parametrize("heads, h, d, columns, apart", [
+    (8, 2, 64, 1875, True),     # a tile's union holds the most columns that there may be
+    (8, 2, 64, 1875, False),    # more columns than a tile has threads
+    (12, 4, 64, 16384, False),  # the most columns whose marks fit
+    (12, 4, 64, 16385, False),  # and one more, which single tokens take
+    (10, 2, 128, 32768, False),
+    (10, 2, 128, 32769, False),
+])
+def test_tiles_among_many_columns(heads, h, d, columns, apart) -> None:
+    from faquant_b200 import ops
+
+    page, held = 16, 40
+    tile = min(32, 128 // (heads // h))
+    count = 1536 // tile
+    tokens = _tokens_of_tiles(h, count)
+    pool = Pool([held * page], h, d, page, DEV, fill=0xFF)
+    k, v = _randn(held * page, h, d, seed=120), _randn(held * page, h, d, seed=121, scale=0.5)
+    pool.write(k, v)
+    k, v = (quantized(x).double().reshape(held, page, h, d) for x in (k, v))
+    g = torch.Generator().manual_seed(122)
+    at = torch.randint(held, (columns,), generator=g)
+    table = pool.table[0][at.to(DEV)][None].contiguous()
+    seen = columns - -(-tokens // page)
+    q = _randn(tokens, heads, d, seed=123, scale=2.0)
+    if apart:
+        order = torch.stack([torch.randperm(seen, generator=g)[:1536] for _ in range(-(-tokens // tile) * h)])
+        lists = order.reshape(-1, h, tile, count).transpose(1, 2).reshape(-1, h, count)[:tokens]
+    else:
+        lists = torch.randint(seen, (tokens, h, count), generator=g)
+        lists[:, :, 0], lists[:, :, 1] = 0, seen - 1
+    lists = lists.to(torch.int32).contiguous()
+    out = ops.hif4_sparse_attention(q, pool.pages, table, _int32(0, tokens), _int32(columns * page), lists.to(DEV), page_size=page)
+    _check(out, q, k, v, at, lists)
+    _no_status()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_columns_behind_the_token_set_no_status_and_those_beyond_the_table_do(tiles) -> None:
+    from faquant_b200 import _lib, ops
+
+    heads, h, d, page, count = 8, 2, 128, 64, 24
+    tokens = _tokens_of_tiles(h, count * page // 16) if tiles else 5
+    length = 60 * page
+    pool = Pool([length], h, d, page, DEV, fill=0xFF)  # a table of 61 columns, the last one without a page
+    k, v = _randn(length, h, d, seed=124), _randn(length, h, d, seed=125)
+    pool.write(k, v)
+    q = _randn(tokens, heads, d, seed=126, scale=2.0)
+    g = torch.Generator().manual_seed(127)
+    lists = torch.stack([torch.randperm(90, generator=g)[:count] for _ in range(tokens * h)]).reshape(tokens, h, count).to(torch.int32)
+    args = (pool.pages, pool.table, pool.cu([tokens]))
+    # all of a column's tokens behind the queries, or no column at all
+    out = ops.hif4_sparse_attention(q, *args, pool.lens, lists.to(DEV), page_size=page)
+    want, size = ref.attention(q, quantized(k), quantized(v), [length], [tokens], page, lists)
+    assert bool(((out.double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
+    _no_status()
+    # a sequence that is longer than its row of the table: columns that the tokens see, and no page for them
+    longer = length + 12 * page + tokens
+    out = ops.hif4_sparse_attention(q, *args, _int32(longer), lists.to(DEV), page_size=page)
+    assert _status() == _lib.FAQ_STATUS_BAD_PAGE
+    want, size = ref.attention(q, quantized(k), quantized(v), [longer], [tokens], page, lists, missing={(0, c) for c in range(60, 90)})
+    assert bool(((out.double().cpu() - want).abs() <= BOUND * size + 2.0**-126).all())
+
+
+@pytest.mark.parametrize("heads, h, d, lens, new", [(32, 8, 128, [3000], [700]), (8, 8, 64, [2000, 900], [400, 500]), (8, 2, 128, [700], [3])])
+def test_selection_with_a_table_far_wider_than_the_lengths(heads, h, d, lens, new) -> None:
+    """The kernel and its split are chosen by the table's columns; the lists are the same."""
+    from faquant_b200 import ops
+
+    pool = Pool(lens, h, d, 16, DEV)
+    k = _randn(sum(lens), h, d, seed=130)
+    pool.write(k, k)
+    bounds = torch.zeros(pool.pages.shape[0], h, ops.hif4_bounds_bytes(d), dtype=torch.uint8, device=DEV)
+    wide = torch.full((len(lens), 8192), -1, dtype=torch.int32, device=DEV)
+    wide[:, : pool.table.shape[1]] = pool.table
+    ops.hif4_key_bounds(pool.pages, bounds, wide, pool.cu(lens), pool.lens, page_size=16, total=sum(lens))
+    q = _randn(sum(new), heads, d, seed=131)
+    lists = [ops.hif4_select_pages(q, bounds, table, pool.cu(new), pool.lens, page_size=16, count=20, want_scores=True)
+             for table in (pool.table, wide, wide[:, : pool.table.shape[1]])]
+    for other in lists[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(lists[0], other))
+    out = [ops.hif4_sparse_attention(q, pool.pages, table, pool.cu(new), pool.lens, lists[0][0], page_size=16)
+           for table in (pool.table, wide)]
+    assert torch.equal(*out)
     _no_status()
