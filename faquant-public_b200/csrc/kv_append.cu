@@ -21,10 +21,10 @@
 // kv_write_kernel does, the others one token's rows of q, four at a time.
 //
 // Measured (one B200, 64 query heads on 8 kv heads of 128, norm, rotation, smoothing and transform):
-// 8192 tokens in 100 us, 311 MB at 3.1 TB/s, half the issue slots active with 16 warps on an SM. Alone
+// 8192 tokens in 99 us, 311 MB at 3.1 TB/s, half the issue slots active with 16 warps on an SM. Alone
 // q takes 58 us (its bytes' time is 41) and the keys and values 44, of which fp64 some 25. Dropped: two
 // launches, the queries' with fewer registers (101 to 113 us); blocks of keys spread among those of queries (105);
-// 96 registers a thread (99, with spills). One token: 4.1 us, a launch and a chain of loads.
+// 96 registers a thread (no gain, with spills). One token: 4.1 us, a launch and a chain of loads.
 #include "kv_pages.cuh"
 
 namespace faq {

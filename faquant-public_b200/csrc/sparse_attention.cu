@@ -5,10 +5,11 @@
 // per token, kv head and its G = heads / kv_heads query heads, which share a list. A unit is
 // (token, kv head, 8 query heads). The arithmetic of a block of 16 tokens is K9's kernel of few rows
 // (paged_attention.cu): codes to bf16 fragments in registers, S^T = K Q^T and O^T = V^T P^T on
-// mma.sync, one reference maximum per row and warp, P rounded to bf16 after its product with V's
-// scale. What differs is where the blocks come from: a warp looks up 32 of its blocks at once (list
-// entry, table entry, address), drops those that are not there or lie behind the token, and streams the rest
-// through a ring of bulk copies.
+// mma.sync, one reference maximum per row and warp, P rounded to bf16, the type of the products with V, after its product
+// with V's scale: at most 2^-8 of a term, as in the dense kernels. Sums are fp32; that rounding and the output's own put
+// the output 0.001 to 0.003 of its norm from one whose P stays in fp32. What differs is where the blocks come from: a warp
+// looks up 32 of its blocks at once (list entry, table entry, address), drops those that are not there or lie behind the
+// token, and streams the rest through a ring of bulk copies.
 //
 // A column counts once: where a list is not ascending, a warp first goes through it once, 32 entries at a time, with a
 // bit per column and one per entry that is the first of its column (hence a list's most entries). 32 entries cost 0.8 us,
@@ -19,7 +20,7 @@
 // kernel and no workspace. The order of every sum is fixed by the list and the cluster's size.
 //
 // Measured (one B200, 32 query heads on 8 kv heads of 128, one new token): 32 pages of 64 of a context
-// of 32768 in 8.0 us, 64 pages of 16 of 32 sequences of 1 .. 16000 tokens in 16.6 us. The first is a chain of
+// of 32768 in 8.3 us, 64 pages of 16 of 32 sequences of 1 .. 16000 tokens in 16.6 us. The first is a chain of
 // loads (cu and lens, the list, the table, the pages), two blocks per warp and the two joins; the second
 // some 10700 blocks at 190 cycles of an SM each (see paged_attention.cu: 118 of issue), as 256 CTAs
 // of unequal length in one wave; clusters of two there took 20.3 us, of four 31.2. 128 such sequences of 2000 tokens

@@ -14,8 +14,9 @@
 // Measured (one B200): 512 tokens of 32768 with 64 query heads on 8 kv heads of 128 and 32 pages of 64
 // tokens each, 164 us (329 with the kernel of single tokens): 9000 key tiles (the lists of 16 neighbours
 // hold some 75 pages) at 4300 cycles, two waves of CTAs. The expansion is what the others wait for: a warp
-// takes 1100 cycles for its block of K and 1300 for one of V, at one instruction in five cycles, then come waits
-// for its slots. Dropped: eight softmax warps with 64 keys a thread (186 us; read twice from
+// takes 960 cycles for its block of K and 880 for one of V, 460 for the next block's address, 290 for its loads' issue, then come
+// waits for its slots. P is rounded to bf16, as in the kernel of single tokens.
+// Dropped: eight softmax warps with 64 keys a thread (186 us; read twice from
 // tensor memory, with sixteen expanding warps, 173: then the softmax is), two tiles of rows to a CTA that share the
 // expansion (173: their sixteen softmax warps move in step, and the exponentials' unit idles between),
 // twelve expanding warps (175, with 64 registers and loads one block ahead), two places for S and a warp of their

@@ -17,7 +17,8 @@ rotation of each token's position, Smooth-QK, Hadamard) and returns the attentio
 
 With ``sparse_pages`` the attention of a long context reads that many pages per token and kv head: the
 first ones, the last ones, and those whose keys' bounds allow the greatest products
-(``ops.hif4_select_pages``). The bounds are kept beside the pages, 2 * head_dim + 16 bytes per page
+(``ops.hif4_select_pages``). It pays in steps that read hundreds of thousands of keys; below, the dense step is
+faster, and exact. The bounds are kept beside the pages, 2 * head_dim + 16 bytes per page
 and kv head, and made anew for the pages that a step writes to.
 
 A step is not to be captured in a CUDA graph: :meth:`extend` makes the step's device arrays anew, and

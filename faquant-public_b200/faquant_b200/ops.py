@@ -1074,7 +1074,8 @@ def hif4_select_pages(
     least one), then those of the greatest scores, ties to the lowest column. Pages that the table does not hold
     are not taken and set ``FAQ_STATUS_BAD_PAGE``; entries of q that are not finite count as zero. With
     ``want_scores`` returns ``(selected, scores)``, scores fp32 of the same shape, -inf behind the pages. Rows
-    beyond ``cu[B]`` stay as they are. At most 32768 columns and 128 query heads per kv head."""
+    beyond ``cu[B]`` stay as they are. At most 32768 columns and 128 query heads per kv head; the columns choose the
+    kernel, so give no more of them than the longest sequence has (a slice of a wider table)."""
     device = _require_cuda(q, bounds, table, cu, lens, out)
     qs = q.shape
     if q.dtype is not torch.bfloat16 or len(qs) != 3:
